@@ -40,6 +40,7 @@ def lfm3_plan(cfg: Lfm3Config) -> ModelPlan:
                 "position": PartSpec("rope", {"rope_dim": cfg.rope_dim, "theta": theta, "style": "neox",
                                               "freq_factors": not sliding}),
                 "window": cfg.sliding_window if sliding else 0,
+                "first": cfg.sliding_window_first if sliding else 0,
                 "output_gate": cfg.attn_output_gate})
             mixer_name = "self_attn"
         if cfg.layer_is_moe(l):

@@ -3,11 +3,12 @@
 A sequence gets a slot when it starts and gives it back when it ends; slots and pages are
 reused.  Layers are grouped by what they need:
 
-* a KV group per distinct (kv heads, key head size, value head size, window, chunk): pools of pages of
+* a KV group per distinct (kv heads, key head size, value head size, window, chunk, first positions): pools of pages of
   `page_size` positions, keys `[entry, page, kv_head, position in page, head_dim]` and values
   `[entry, page, kv_head, value_dim, position in page]`, with a page pool and a page list per
   sequence of its own.  A windowed group gives pages back once every position in
-  them has left the window, or lies in a chunk before the next position's.
+  them has left the window, or lies in a chunk before the next position's; pages with one of the sequence's first
+  positions that stay visible (`first`) are kept.
   A group whose spec pools blocks of positions has a second pair of pools of the same layout, one row per
   complete block, with pages and a page list per sequence of their own; they are never given back before
   the sequence ends.
@@ -110,8 +111,9 @@ class KVGroup:
         if self.pool > 0:                 # the block that is still filling is pooled from its cached rows
             first_needed = min(first_needed, length // self.pool * self.pool)
         lst = self.seq_pages.get(slot, [])
+        kept = -(-getattr(self.spec, "first", 0) // self.page_size)      # pages of the first positions that stay visible
         for j, p in enumerate(lst):
-            if p >= 0 and (j + 1) * self.page_size - 1 < first_needed:
+            if j >= kept and p >= 0 and (j + 1) * self.page_size - 1 < first_needed:
                 self.pages.free(p)
                 lst[j] = -1
 

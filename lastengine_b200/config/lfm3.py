@@ -61,6 +61,7 @@ class Lfm3Config:
     sandwich_norms: bool
     attn_output_gate: bool
     sliding_window: int
+    sliding_window_first: int      # a sequence's first positions that the windowed layers go on seeing
     # generation defaults
     eos_token_ids: tuple[int, ...]
     bos_token_id: int | None
@@ -186,6 +187,7 @@ class Lfm3Config:
             for i, p in enumerate(pat):
                 if p in (1, True) and kinds[i] == ATTENTION:
                     kinds[i] = SLIDING  # the reference's per-layer flag, src/dense.rs:60-63
+        first = r.integer("sliding_window_first", default=0, minimum=0)
         if any(k_ == SLIDING for k_ in kinds) and window <= 0:
             raise ConfigError(f"{where}: a layer is '{SLIDING}' but 'sliding_window' is not set")
 
@@ -209,4 +211,4 @@ class Lfm3Config:
             num_experts_per_tok=k, moe_intermediate_size=fe, num_dense_layers=nd,
             norm_topk_prob=norm_topk, use_expert_bias=use_bias, routed_scaling_factor=scale,
             tie_embedding=tie, sandwich_norms=sandwich, attn_output_gate=gate,
-            sliding_window=window, eos_token_ids=eos_ids, bos_token_id=bos, raw=dict(raw))
+            sliding_window=window, sliding_window_first=first, eos_token_ids=eos_ids, bos_token_id=bos, raw=dict(raw))

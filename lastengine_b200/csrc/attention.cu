@@ -11,7 +11,8 @@
 // An optional per-head gate multiplies the head's output by sigmoid(gate) (src/dense.rs:147-150); it may also be
 // given per dimension of the head.  Instead of a window a layer may cut its positions into chunks (t0 = the start
 // of pos's chunk).  `slopes` [nh]: slope_h (pos - t) is taken off the score of key t; `sinks` [nh]: one more logit per head in
-// the softmax's denominator, without a key and without a value (each or null).
+// the softmax's denominator, without a key and without a value (each or null).  `first` > 0: beside its window (or chunk) a row reads
+// the sequence's first `first` positions.
 // Scores, maximum, exponentials, sums and the value accumulation are float.  The reference's
 // GPU kernels keep the same running (max, sum, acc) per warp and merge them
 // (src/cuda/dense.cu:94-123 whole range, :152-183 split range, :238-247 merge); this kernel lets
@@ -30,7 +31,9 @@
 #define ATT_RPW 8  // query vectors per warp at most: 32 / 4
 #define ATT_NEG (-1e30f)
 
-template <typename T, typename CT, int HDL>  // value head size <= 32 * HDL (the key head size is free)
+// value head size <= 32 * HDL (the key head size is free).  FIRST: a row also reads the sequence's first `first` positions
+// (first_tiles in common.cuh).
+template <typename T, typename CT, int HDL, bool FIRST>
 __global__ void __launch_bounds__(32 * ATT_WARPS)
 attention_kernel(T* __restrict__ out, float* __restrict__ part, const T* __restrict__ q,
                  const CT* __restrict__ k_pool, const CT* __restrict__ v_pool,
@@ -38,7 +41,7 @@ attention_kernel(T* __restrict__ out, float* __restrict__ part, const T* __restr
                  const int* __restrict__ seq_slot, const int* __restrict__ seq_pos0,
                  const int* __restrict__ seq_qstart, const int* __restrict__ seq_qlen,
                  const T* __restrict__ gate, int gate_stride, int gate_elem, int nh, int nkv, int hd, int vd,
-                 int page_size, int window, int chunk, float scale, const float* __restrict__ slopes,
+                 int page_size, int window, int chunk, int first, float scale, const float* __restrict__ slopes,
                  const float* __restrict__ sinks, int QT, int HC, int n_splits) {
   extern __shared__ __align__(16) float sm[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -94,7 +97,8 @@ attention_kernel(T* __restrict__ out, float* __restrict__ part, const T* __restr
   const int kv_len = pos0 + qlen;  // keys the cache holds for this sequence after this step's writes
   const int pos_lo = pos0 + row_lo, pos_hi = pos0 + row_lo + nrows - 1;
   const int key_lo = first_key(pos_lo, window, chunk);
-  const int tile_first = key_lo / 32, tile_last = pos_hi / 32;
+  const int n_first = FIRST ? first_tiles(first, key_lo, 32) : 0, shift = key_lo / 32 - n_first;
+  const int tile_first = FIRST ? 0 : key_lo / 32, tile_last = pos_hi / 32 - (FIRST ? shift : 0);
   const int n_tiles = tile_last - tile_first + 1;
   const int per_split = (n_tiles + n_splits - 1) / n_splits;
   const int t_lo = tile_first + split * per_split;
@@ -113,7 +117,9 @@ attention_kernel(T* __restrict__ out, float* __restrict__ part, const T* __restr
   const int kk_step4 = 128 * ATT_WARPS / hd, d_step4 = 128 * ATT_WARPS % hd;
   const bool wide = (hd & 3) == 0 && (((uintptr_t)k_pool | (uintptr_t)v_pool) & 15) == 0;      // (pages are multiples of 32 positions)
   for (int tile = t_lo; tile < t_hi; tile++) {
-    const int key0 = tile * 32;
+    const int key0 = (FIRST && tile >= n_first ? tile + shift : tile) * 32;
+    // what no row of the block reads between the first positions and key_lo does not enter the sums, whatever it holds
+    const int gap_lo = FIRST ? max(0, first - key0) : 32, gap_hi = FIRST ? key_lo - key0 : 0;
     const int page = block_table[(size_t)b * bt_width + key0 / page_size];
     const size_t base = (((size_t)(page < 0 ? 0 : page) * nkv + kvh) * page_size + key0 % page_size) * hd;
     const size_t vbase = ((size_t)(page < 0 ? 0 : page) * nkv + kvh) * vd * page_size + key0 % page_size;
@@ -137,6 +143,9 @@ attention_kernel(T* __restrict__ out, float* __restrict__ part, const T* __restr
         const float4 vv = left > 0 ? load4(v_pool + vbase + (size_t)dim * page_size + k4) : make_float4(0.f, 0.f, 0.f, 0.f);
         float* vs = v_s + k4 * vd + dim;
         vs[0] = left > 0 ? vv.x : 0.f, vs[vd] = left > 1 ? vv.y : 0.f, vs[2 * vd] = left > 2 ? vv.z : 0.f, vs[3 * vd] = left > 3 ? vv.w : 0.f;
+        if (FIRST && gap_lo < gap_hi)
+          for (int e = 0; e < 4; e++)
+            if (k4 + e >= gap_lo && k4 + e < gap_hi) vs[e * vd] = 0.f;
       }
     } else {
       int kk = kk0, d = d0;      // idx / hd and idx % hd, kept up without dividing
@@ -153,7 +162,7 @@ attention_kernel(T* __restrict__ out, float* __restrict__ part, const T* __restr
       for (int idx = threadIdx.x; idx < 32 * vd; idx += 32 * ATT_WARPS) {
         int dim = idx / 32, pos = idx - dim * 32;                         // values are stored [dim][position]
         float vv = 0.f;
-        if (page >= 0 && key0 + pos < kv_len) vv = to_f32(v_pool[vbase + (size_t)dim * page_size + pos]);
+        if (page >= 0 && key0 + pos < kv_len && !(FIRST && pos >= gap_lo && pos < gap_hi)) vv = to_f32(v_pool[vbase + (size_t)dim * page_size + pos]);
         v_s[pos * vd + dim] = vv;
       }
     }
@@ -198,12 +207,12 @@ attention_kernel(T* __restrict__ out, float* __restrict__ part, const T* __restr
       const int qpos = pos0 + row_lo + i;
       const int lo = first_key(qpos, window, chunk);
       // an idle vector, or the whole tile lies after this row or before what it reads
-      if (i >= nrows || j >= nheads || key0 > qpos || key0 + 31 < lo) continue;
+      if (i >= nrows || j >= nheads || key0 > qpos || (key0 + 31 < lo && !(FIRST && key0 < first))) continue;
       live |= 1u << ri;
       float sc = s[ri] * scale;
       const int kp = key0 + lane;
       if (slopes) sc -= slopes[kvh * G + hc * HC + j] * (float)(qpos - kp);
-      const bool valid = kp <= qpos && kp >= lo;
+      const bool valid = kp <= qpos && (kp >= lo || (FIRST && kp < first));
       sc = valid ? sc : ATT_NEG;
       const float mn = fmaxf(mx[ri], warp_max(sc));
       const float p = valid ? expf(sc - mn) : 0.f;
@@ -318,12 +327,12 @@ __global__ void attention_merge_kernel(T* __restrict__ out, const float* __restr
   }
 }
 
-template <typename T, typename CT, int HDL>
+template <typename T, typename CT, int HDL, bool FIRST>
 static int launch_attention(void* out, float* part, const void* q, const void* k_pool,
                             const void* v_pool, const int* block_table, int bt_width,
                             const int* seq_slot, const int* seq_pos0, const int* seq_qstart,
                             const int* seq_qlen, const void* gate, int gate_stride, int gate_elem, int B, int nh,
-                            int nkv, int hd, int vd, int page_size, int window, int chunk, float scale,
+                            int nkv, int hd, int vd, int page_size, int window, int chunk, int first, float scale,
                             const float* slopes, const float* sinks, int max_qlen, int n_splits, cudaStream_t st) {
   const int G = nh / nkv;
   const int HC = G < 8 ? G : 8;
@@ -332,7 +341,7 @@ static int launch_attention(void* out, float* part, const void* q, const void* k
   const int R = QT * HC;
   const int n_hc = ceil_div(G, HC);
   size_t smem = ((size_t)R * hd + 32 * (hd + 1) + 32 * vd + ATT_WARPS * ATT_RPW * 32) * sizeof(float);
-  constexpr auto kern = attention_kernel<T, CT, HDL>;
+  constexpr auto kern = attention_kernel<T, CT, HDL, FIRST>;
   if (smem > 48 * 1024) {
     const cudaError_t e = leb_allow_smem<kern>();
     if (e != cudaSuccess) return leb_fail("leb_attention: shared memory %zu: %s", smem, cudaGetErrorString(e));
@@ -342,7 +351,7 @@ static int launch_attention(void* out, float* part, const void* q, const void* k
   kern<<<grid, 32 * ATT_WARPS, smem, st>>>(
       (T*)out, part, (const T*)q, (const CT*)k_pool, (const CT*)v_pool, block_table, bt_width,
       seq_slot, seq_pos0, seq_qstart, seq_qlen, (const T*)gate, gate_stride, gate_elem, nh, nkv, hd, vd, page_size,
-      window, chunk, scale, slopes, sinks, QT, HC, n_splits);
+      window, chunk, first, scale, slopes, sinks, QT, HC, n_splits);
   LEB_CHECK_LAUNCH("leb_attention");
   return 0;
 }
@@ -354,7 +363,7 @@ LEB_API int leb_attention(void* out, float* part, const void* q, const void* k_p
                           const void* v_pool, int dtype, const int* block_table, int bt_width,
                           const int* seq_slot, const int* seq_pos0, const int* seq_qstart,
                           const int* seq_qlen, const void* gate, int gate_stride, int gate_elem, int M, int B,
-                          int nh, int nkv, int hd, int page_size, int window, int chunk, float scale,
+                          int nh, int nkv, int hd, int page_size, int window, int chunk, int first, float scale,
                           const float* slopes, const float* sinks, int max_qlen, int n_splits, int vd, cudaStream_t st) {
   if (M <= 0 || B <= 0) return 0;
   if (vd <= 0) vd = hd;
@@ -364,9 +373,10 @@ LEB_API int leb_attention(void* out, float* part, const void* q, const void* k_p
   LEB_REQUIRE(page_size % 32 == 0, "leb_attention: page size %d is not a multiple of 32", page_size);
   LEB_REQUIRE(n_splits >= 1 && (n_splits == 1 || (max_qlen == 1 && part)), "leb_attention: splits need single-row sequences and scratch");
   int rc;
-#define LEB_ATT_W(T, CT, HDL)                                                                                           \
-  launch_attention<T, CT, HDL>(out, part, q, k_pool, v_pool, block_table, bt_width, seq_slot, seq_pos0, seq_qstart,      \
-                               seq_qlen, gate, gate_stride, gate_elem, B, nh, nkv, hd, vd, page_size, window, chunk, scale, \
+#define LEB_ATT_W(T, CT, HDL) (first > 0 ? LEB_ATT_F(T, CT, HDL, true) : LEB_ATT_F(T, CT, HDL, false))
+#define LEB_ATT_F(T, CT, HDL, F)                                                                                           \
+  launch_attention<T, CT, HDL, F>(out, part, q, k_pool, v_pool, block_table, bt_width, seq_slot, seq_pos0, seq_qstart,      \
+                               seq_qlen, gate, gate_stride, gate_elem, B, nh, nkv, hd, vd, page_size, window, chunk, first, scale, \
                                slopes, sinks, max_qlen, n_splits, st)
 #define LEB_ATT(T, CT) \
   (vd <= 32 ? LEB_ATT_W(T, CT, 1) : vd <= 64 ? LEB_ATT_W(T, CT, 2) : vd <= 128 ? LEB_ATT_W(T, CT, 4) : LEB_ATT_W(T, CT, 8))
@@ -378,6 +388,7 @@ LEB_API int leb_attention(void* out, float* part, const void* q, const void* k_p
     return leb_fail("leb_attention: unknown dtype %d", dtype);
 #undef LEB_ATT
 #undef LEB_ATT_W
+#undef LEB_ATT_F
   if (rc) return rc;
   if (n_splits > 1) {
     dim3 grid(M, nh);

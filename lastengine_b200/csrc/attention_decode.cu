@@ -163,15 +163,16 @@ __device__ __forceinline__ void atd_prep_head(const bf16* __restrict__ src, cons
 }
 
 // HD: head_dim, a multiple of 32; S: stages of a warp's ring; WIDE: the softmax weights enter the second product as two
-// bfloat16 terms, p = hi + lo (16 significant bits; the row sum is of the float p either way)
-template <int HD, int S, bool WIDE>
+// bfloat16 terms, p = hi + lo (16 significant bits; the row sum is of the float p either way); FIRST: the row also reads the
+// sequence's first `first` positions, whose blocks come before the window's in the walk (first_tiles in common.cuh)
+template <int HD, int S, bool WIDE, bool FIRST>
 __global__ void __launch_bounds__(32 * ATD_WARPS)
 attention_decode_kernel(bf16* __restrict__ out, float* __restrict__ part, const bf16* __restrict__ q,
                         const bf16* __restrict__ k_pool, const bf16* __restrict__ v_pool,
                         const int* __restrict__ block_table, int bt_width,
                         const int* __restrict__ seq_slot, const int* __restrict__ seq_pos0,
                         const int* __restrict__ seq_qstart, const bf16* __restrict__ gate,
-                        int gate_stride, int gate_elem, int nh, int nkv, int page_size, int window, int chunk,
+                        int gate_stride, int gate_elem, int nh, int nkv, int page_size, int window, int chunk, int first,
                         float scale, const float* __restrict__ slopes, const float* __restrict__ sinks, int n_splits,
                         AtdPrep prep) {
   constexpr int KB = HD / 32;  // 32-wide pieces of head_dim
@@ -228,7 +229,9 @@ attention_decode_kernel(bf16* __restrict__ out, float* __restrict__ part, const 
   const int qpos = seq_pos0[b];
   const int kv_len = qpos + 1;
   const int key_lo = first_key(qpos, window, chunk);
-  const int blk_first = key_lo / 32, blk_last = (kv_len - 1) / 32;
+  // blocks are numbered as they lie; with FIRST as they are walked (block number `blk` lies at `blk` or `blk + shift`)
+  const int n_first = FIRST ? first_tiles(first, key_lo, 32) : 0, shift = FIRST ? key_lo / 32 - n_first : 0;
+  const int blk_first = FIRST ? 0 : key_lo / 32, blk_last = (kv_len - 1) / 32 - shift;
   const int n_blk = blk_last - blk_first + 1;
   const int per_split = (n_blk + n_splits - 1) / n_splits;
   const int blk_lo = blk_first + split * per_split;
@@ -239,7 +242,7 @@ attention_decode_kernel(bf16* __restrict__ out, float* __restrict__ part, const 
   int p_blk = blk_lo + warp, p_q = 0;      // the next block to ask for and its stage number
   auto issue = [&]() {
     if (p_blk < blk_hi) {
-      const int key0 = p_blk * 32;
+      const int key0 = (FIRST && p_blk >= n_first ? p_blk + shift : p_blk) * 32;
       const int page = table[key0 / page_size];
       const int off = key0 % page_size;
       const bf16* kbase = k_pool + (((size_t)page * nkv + kvh) * page_size + off) * HD;   // 32 rows of HD, contiguous
@@ -345,7 +348,7 @@ attention_decode_kernel(bf16* __restrict__ out, float* __restrict__ part, const 
   uint4 kf[4][KB], vf[NT];      // the block being multiplied
   int q_stage = 0;
   for (int blk = blk_lo + warp; blk < blk_hi; blk += ATD_WARPS, q_stage++) {
-    const int key0 = blk * 32;
+    const int key0 = (FIRST && blk >= n_first ? blk + shift : blk) * 32;
     asm volatile("cp.async.wait_group %0;" ::"n"(S - 2) : "memory");
     __syncwarp();     // every lane's pieces of this stage have landed; everyone is done with the stage before
     issue();
@@ -365,8 +368,21 @@ attention_decode_kernel(bf16* __restrict__ out, float* __restrict__ part, const 
     }
     const bool partial = key0 < key_lo || key0 + 32 > kv_len;
     if (partial) {
+      if (FIRST && key0 < first) {       // the row reads [0, first) and [key_lo, kv_len) of this block
+        if (first < key_lo && key0 + 32 > first) {
 #pragma unroll
-      for (int n = 0; n < NT; n++) vf[n] = mask_positions(vf[n], key0 + 8 * c, key_lo, kv_len);
+          for (int n = 0; n < NT; n++) {
+            const uint4 head = mask_positions(vf[n], key0 + 8 * c, 0, first), rest = mask_positions(vf[n], key0 + 8 * c, key_lo, kv_len);
+            vf[n] = make_uint4(head.x | rest.x, head.y | rest.y, head.z | rest.z, head.w | rest.w);
+          }
+        } else if (key0 + 32 > kv_len) {
+#pragma unroll
+          for (int n = 0; n < NT; n++) vf[n] = mask_positions(vf[n], key0 + 8 * c, 0, kv_len);
+        }
+      } else {
+#pragma unroll
+        for (int n = 0; n < NT; n++) vf[n] = mask_positions(vf[n], key0 + 8 * c, key_lo, kv_len);
+      }
     }
 
     float s[4][4];
@@ -387,7 +403,7 @@ attention_decode_kernel(bf16* __restrict__ out, float* __restrict__ part, const 
 #pragma unroll
       for (int e = 0; e < 4; e++) {
         const int kp = key0 + 8 * c + 2 * t + (e & 1);
-        const bool valid = kp >= key_lo && kp < kv_len;
+        const bool valid = (kp >= key_lo || (FIRST && kp < first)) && kp < kv_len;
         s[t][e] = valid ? fmaf(s[t][e], scale2, slope2[e >> 1] * (float)(kp - qpos)) : ATD_NEG;
         tmax[e >> 1] = fmaxf(tmax[e >> 1], s[t][e]);
       }
@@ -495,7 +511,7 @@ static int attention_decode_launch(void* out, float* part, const void* q, const 
                                    const void* v_pool, const int* block_table, int bt_width,
                                    const int* seq_slot, const int* seq_pos0, const int* seq_qstart,
                                    const void* gate, int gate_stride, int gate_elem, int B, int nh, int nkv, int hd,
-                                   int page_size, int window, int chunk, int wide, float scale, const float* slopes,
+                                   int page_size, int window, int chunk, int first, int wide, float scale, const float* slopes,
                                    const float* sinks, int n_splits, AtdPrep prep, cudaStream_t st) {
   if (B <= 0) return 0;
   LEB_REQUIRE(leb_attention_decode_supported(nh, nkv, hd, page_size),
@@ -503,19 +519,24 @@ static int attention_decode_launch(void* out, float* part, const void* q, const 
   LEB_REQUIRE(n_splits >= 1 && (n_splits == 1 || part), "leb_attention_decode: splits need scratch");
   dim3 grid(nkv, B, n_splits);
   LEB_REQUIRE(grid.y <= 65535 && grid.z <= 65535, "leb_attention_decode: grid too large");
-#define LEB_ATD_W(HD_, S_, W_)                                                                    \
+#define LEB_ATD_F(HD_, S_, W_, F_)                                                                \
   {                                                                                               \
     constexpr int smem = ATD_WARPS * S_ * 2 * 32 * HD_ * 2;                                        \
     static bool set = false;                                                                      \
     if (!set) {                                                                                   \
-      if (cudaFuncSetAttribute(attention_decode_kernel<HD_, S_, W_>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) \
+      if (cudaFuncSetAttribute(attention_decode_kernel<HD_, S_, W_, F_>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) \
         return leb_fail("leb_attention_decode: %d bytes of shared memory per block refused", smem); \
       set = true;                                                                                 \
     }                                                                                             \
-    leb_launch(attention_decode_kernel<HD_, S_, W_>, grid, dim3(32 * ATD_WARPS), smem, st,             \
+    leb_launch(attention_decode_kernel<HD_, S_, W_, F_>, grid, dim3(32 * ATD_WARPS), smem, st,             \
         (bf16*)out, part, (const bf16*)q, (const bf16*)k_pool, (const bf16*)v_pool, block_table,  \
         bt_width, seq_slot, seq_pos0, seq_qstart, (const bf16*)gate, gate_stride, gate_elem, nh, nkv, \
-        page_size, window, chunk, scale, slopes, sinks, n_splits, prep);                          \
+        page_size, window, chunk, first, scale, slopes, sinks, n_splits, prep);                   \
+  }
+#define LEB_ATD_W(HD_, S_, W_)                       \
+  {                                                  \
+    if (first > 0) LEB_ATD_F(HD_, S_, W_, true)      \
+    else LEB_ATD_F(HD_, S_, W_, false)               \
   }
 #define LEB_ATD(HD_, S_)                    \
   {                                         \
@@ -531,6 +552,7 @@ static int attention_decode_launch(void* out, float* part, const void* q, const 
   }
 #undef LEB_ATD
 #undef LEB_ATD_W
+#undef LEB_ATD_F
   LEB_CHECK_LAUNCH("leb_attention_decode");
   return 0;
 }
@@ -539,10 +561,10 @@ LEB_API int leb_attention_decode(void* out, float* part, const void* q, const vo
                                  const void* v_pool, const int* block_table, int bt_width,
                                  const int* seq_slot, const int* seq_pos0, const int* seq_qstart,
                                  const void* gate, int gate_stride, int gate_elem, int B, int nh, int nkv, int hd,
-                                 int page_size, int window, int chunk, int wide, float scale, const float* slopes,
+                                 int page_size, int window, int chunk, int first, int wide, float scale, const float* slopes,
                                  const float* sinks, int n_splits, cudaStream_t st) {
   return attention_decode_launch(out, part, q, k_pool, v_pool, block_table, bt_width, seq_slot, seq_pos0, seq_qstart, gate,
-                                 gate_stride, gate_elem, B, nh, nkv, hd, page_size, window, chunk, wide, scale, slopes, sinks,
+                                 gate_stride, gate_elem, B, nh, nkv, hd, page_size, window, chunk, first, wide, scale, slopes, sinks,
                                  n_splits, AtdPrep{}, st);
 }
 
@@ -562,7 +584,7 @@ LEB_API int leb_attention_decode_prep(void* out, float* part, const void* q_raw,
                                       const int* seq_pos0, const int* seq_qstart, const float* q_norm_w,
                                       const float* k_norm_w, float eps, const float* inv_freq, int rope_dim,
                                       int neox, int row_norm, const void* gate, int gate_stride, int gate_elem, int B, int nh, int nkv,
-                                      int hd, int page_size, int window, int chunk, int wide, float scale, const float* slopes,
+                                      int hd, int page_size, int window, int chunk, int first, int wide, float scale, const float* slopes,
                                       const float* sinks, float temp_coef, float temp_every, int n_splits, cudaStream_t st) {
   LEB_REQUIRE(leb_attention_decode_prep_supported(nh, nkv, hd, page_size, rope_dim, neox),
               "leb_attention_decode_prep: sizes not taken (head_dim %d, rope_dim %d, split-half %d)", hd, rope_dim, neox);
@@ -573,7 +595,7 @@ LEB_API int leb_attention_decode_prep(void* out, float* part, const void* q_raw,
                (bf16*)v_pool, q_norm_w, k_norm_w, rope_dim ? inv_freq : nullptr, eps, neox != 0, row_norm != 0, temp_coef,
                temp_every};
   return attention_decode_launch(out, part, nullptr, k_pool, v_pool, block_table, bt_width, seq_slot, seq_pos0, seq_qstart,
-                                 gate, gate_stride, gate_elem, B, nh, nkv, hd, page_size, window, chunk, wide, scale, slopes, sinks,
+                                 gate, gate_stride, gate_elem, B, nh, nkv, hd, page_size, window, chunk, first, wide, scale, slopes, sinks,
                                  n_splits, prep, st);
 }
 
@@ -618,7 +640,7 @@ LEB_API int leb_attention_decode_static(void* out, const void* q, const void* k_
     scratch = g_static_scratch_ptr[dev];
   }
   int rc = leb_attention_decode(out, scratch, q, k_pool, v_pool, block_table, bt_width, seq_slot, seq_pos0,
-                                seq_qstart, gate, gate_stride, 0, B, nh, nkv, hd, page_size, window, 0, 0, scale, nullptr, nullptr,
+                                seq_qstart, gate, gate_stride, 0, B, nh, nkv, hd, page_size, window, 0, 0, 0, scale, nullptr, nullptr,
                                 n_splits, st);
   if (rc) return rc;
   if (n_splits > 1)

@@ -49,8 +49,9 @@ __device__ __forceinline__ uint4 mask_tail(uint4 v, int first, int hi) {
 }
 
 // HD: head_dim (multiple of 32); MT: 16-row tiles per warp.  WIDE: the softmax weights enter the second product as two
-// bfloat16 terms, p = hi + lo (16 significant bits; the row sum is of the float p either way).
-template <int HD, int MT, bool WIDE>
+// bfloat16 terms, p = hi + lo (16 significant bits; the row sum is of the float p either way).  FIRST: a row also reads the
+// sequence's first `first` positions, whose blocks come before the window's in the walk (first_tiles in common.cuh).
+template <int HD, int MT, bool WIDE, bool FIRST>
 __global__ void __launch_bounds__(32 * ATP_WARPS)
 attention_prefill_kernel(bf16* __restrict__ out, const bf16* __restrict__ q,
                          const bf16* __restrict__ k_pool, const bf16* __restrict__ v_pool,
@@ -58,7 +59,7 @@ attention_prefill_kernel(bf16* __restrict__ out, const bf16* __restrict__ q,
                          const int* __restrict__ seq_slot, const int* __restrict__ seq_pos0,
                          const int* __restrict__ seq_qstart, const int* __restrict__ seq_qlen,
                          const bf16* __restrict__ gate, int gate_stride, int gate_elem, int nh, int nkv,
-                         int page_size, int window, int chunk, float scale, const float* __restrict__ slopes,
+                         int page_size, int window, int chunk, int first, float scale, const float* __restrict__ slopes,
                          const float* __restrict__ sinks, int QT) {
   constexpr int KB = HD / 32, NT = HD / 8;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -156,11 +157,13 @@ attention_prefill_kernel(bf16* __restrict__ out, const bf16* __restrict__ q,
   qmin = min(qmin, __shfl_xor_sync(0xffffffffu, qmin, 8));
   qmin = min(qmin, __shfl_xor_sync(0xffffffffu, qmin, 16));
 
-  const int blk_first = key_lo / 32, blk_last = key_hi / 32;
+  // blocks are numbered as they lie; with FIRST as they are walked (block number `blk` lies at `blk` or `blk + shift`)
+  const int n_first = FIRST ? first_tiles(first, key_lo, 32) : 0, shift = FIRST ? key_lo / 32 - n_first : 0;
+  const int blk_first = FIRST ? 0 : key_lo / 32, blk_last = key_hi / 32 - shift;
   uint4 kf[4][KB], vf[NT];      // the block being multiplied
   uint4 kn[4][KB], vn[NT];      // the next block, in flight meanwhile
   auto load_block = [&](int blk, uint4 (&kd)[4][KB], uint4 (&vd)[NT]) {
-    const int key0 = blk * 32;
+    const int key0 = (FIRST && blk >= n_first ? blk + shift : blk) * 32;
     const int page = table[key0 / page_size];
     const int off = key0 % page_size;
     const bf16* kbase = k_pool + (((size_t)page * nkv + kvh) * page_size + off) * HD;
@@ -179,7 +182,16 @@ attention_prefill_kernel(bf16* __restrict__ out, const bf16* __restrict__ q,
   constexpr bool PREFETCH = HD <= 64;   // larger heads have no registers to spare for a second block
   // one block of 32 positions against this warp's rows
   auto compute = [&](uint4 (&kf)[4][KB], uint4 (&vf)[NT], int blk) {
-    const int key0 = blk * 32;
+    const int key0 = (FIRST && blk >= n_first ? blk + shift : blk) * 32;
+    if (FIRST && key0 < key_lo && key0 + 32 > first) {
+      // what no row of this warp reads, between the first positions and key_lo, does not enter the sums, whatever it holds
+#pragma unroll
+      for (int n = 0; n < NT; n++) {
+        const uint4 head = mask_tail(vf[n], key0 + 8 * c, first), rest = mask_tail(vf[n], key0 + 8 * c, key_lo);   // kept | zeroed below
+        vf[n] = make_uint4(head.x | (vf[n].x & ~rest.x), head.y | (vf[n].y & ~rest.y), head.z | (vf[n].z & ~rest.z),
+                           head.w | (vf[n].w & ~rest.w));
+      }
+    }
     if (key0 + 32 > kv_len) {
 #pragma unroll
       for (int n = 0; n < NT; n++) vf[n] = mask_tail(vf[n], key0 + 8 * c, kv_len);
@@ -209,7 +221,7 @@ attention_prefill_kernel(bf16* __restrict__ out, const bf16* __restrict__ q,
             const int hh = e >> 1;
             const int kp = key0 + 8 * c + 2 * t + (e & 1);
             const int qp = pos0 + rpos[mt][hh];
-            const bool valid = kp <= qp && kp >= rlo[hh];
+            const bool valid = kp <= qp && (kp >= rlo[hh] || (FIRST && kp < first));
             s[t][e] = valid ? fmaf(s[t][e], scale2, slope2[mt][hh] * (float)(kp - qp)) : ATP_NEG;
             tmax[hh] = fmaxf(tmax[hh], s[t][e]);
           }
@@ -335,7 +347,7 @@ LEB_API int leb_attention_prefill(void* out, const void* q, const void* k_pool, 
                                   const int* block_table, int bt_width, const int* seq_slot,
                                   const int* seq_pos0, const int* seq_qstart, const int* seq_qlen,
                                   const void* gate, int gate_stride, int gate_elem, int B, int nh, int nkv, int hd,
-                                  int page_size, int window, int chunk, int wide, float scale, const float* slopes,
+                                  int page_size, int window, int chunk, int first, int wide, float scale, const float* slopes,
                                   const float* sinks, int max_qlen, cudaStream_t st) {
   if (B <= 0 || max_qlen <= 0) return 0;
   LEB_REQUIRE(leb_attention_prefill_supported(nh, nkv, hd, page_size),
@@ -347,11 +359,16 @@ LEB_API int leb_attention_prefill(void* out, const void* q, const void* k_pool, 
   if (QT < 1) QT = 1;
   dim3 grid(ceil_div(max_qlen, QT), nkv, B);
   LEB_REQUIRE(grid.y <= 65535 && grid.z <= 65535, "leb_attention_prefill: grid too large");
-#define LEB_ATP_W(HD_, MT_, W_)                                                                      \
-  attention_prefill_kernel<HD_, MT_, W_><<<grid, 32 * ATP_WARPS, 0, st>>>(                               \
+#define LEB_ATP_F(HD_, MT_, W_, F_)                                                                  \
+  attention_prefill_kernel<HD_, MT_, W_, F_><<<grid, 32 * ATP_WARPS, 0, st>>>(                               \
       (bf16*)out, (const bf16*)q, (const bf16*)k_pool, (const bf16*)v_pool, block_table, bt_width,   \
       seq_slot, seq_pos0, seq_qstart, seq_qlen, (const bf16*)gate, gate_stride, gate_elem, nh, nkv,  \
-      page_size, window, chunk, scale, slopes, sinks, QT)
+      page_size, window, chunk, first, scale, slopes, sinks, QT)
+#define LEB_ATP_W(HD_, MT_, W_)                       \
+  do {                                                \
+    if (first > 0) LEB_ATP_F(HD_, MT_, W_, true);     \
+    else LEB_ATP_F(HD_, MT_, W_, false);              \
+  } while (0)
 #define LEB_ATP(HD_, MT_)                \
   if (wide) LEB_ATP_W(HD_, MT_, true);   \
   else LEB_ATP_W(HD_, MT_, false)
@@ -363,6 +380,7 @@ LEB_API int leb_attention_prefill(void* out, const void* q, const void* k_pool, 
   }
 #undef LEB_ATP
 #undef LEB_ATP_W
+#undef LEB_ATP_F
   LEB_CHECK_LAUNCH("leb_attention_prefill");
   return 0;
 }

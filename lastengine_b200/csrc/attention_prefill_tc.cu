@@ -140,7 +140,9 @@ __device__ __forceinline__ int atc_blocks_seen(int qpos, int window, int pool) {
 // WIDE: the weights as two terms as POOLED has them, for layers without pooled blocks too.
 // GS query heads per kv head (1, 2, 4, 8): a tile is GS heads x 128/GS positions; VD: width of a value head (64 or 32)
 // DEEP: two blocks per SM, two buffers of S, P over the S it came from (WIDE always).
-template <int GS, bool POOLED, bool WIDE, bool DEEP, int VD>
+// FIRST (not POOLED): a row also reads the sequence's first `first` positions; their pages come before the window's in the walk
+// (first_tiles in common.cuh).
+template <int GS, bool POOLED, bool WIDE, bool DEEP, int VD, bool FIRST>
 __global__ void __launch_bounds__(ATC_THREADS, AtcShape<DEEP>::BLOCKS)
 attention_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                             const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_pk,
@@ -149,7 +151,7 @@ attention_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __g
                             int pt_width, const int* __restrict__ seq_slot,
                             const int* __restrict__ seq_pos0, const int* __restrict__ seq_qstart,
                             const int* __restrict__ seq_qlen, const bf16* __restrict__ gate, int gate_stride, int gate_elem,
-                            int nh, int nkv, int window, int chunk, int pool, float scale, const float* __restrict__ head_scale,
+                            int nh, int nkv, int window, int chunk, int first, int pool, float scale, const float* __restrict__ head_scale,
                             const float* __restrict__ freq_v, const float* __restrict__ slopes,
                             const float* __restrict__ sinks, int* __restrict__ status) {
   constexpr int HD = 64, PAGE = 64, TP = 128 / GS, NS = AtcShape<DEEP>::STAGES, SB = AtcShape<DEEP>::S_BUFS;
@@ -191,7 +193,8 @@ attention_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __g
   const int q_lo = pos0 + row0;                  // position of the tile's first query
   const int key_hi = q_lo + rows;                // keys [.., key_hi) exist for this tile
   const int key_lo_tile = first_key(q_lo, window, chunk);
-  const int jb0 = key_lo_tile / PAGE, nblk = (key_hi - 1) / PAGE - jb0 + 1;
+  const int nf = FIRST ? first_tiles(first, key_lo_tile, PAGE) : 0;             // pages of first positions, walked first
+  const int jb0 = key_lo_tile / PAGE, nblk = (key_hi - 1) / PAGE - jb0 + 1 + nf;
   const int* table = block_table + (size_t)b * bt_width;
   const int nb_tile = POOLED ? atc_blocks_seen(key_hi - 1, window, pool) : 0;   // pooled blocks the tile's last row sees
   const int npp = (nb_tile + PAGE - 1) / PAGE;                                  // pages of them, walked first
@@ -240,7 +243,7 @@ attention_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __g
       mbar_expect_tx(&q_full, Q_BYTES);
       for (int g = 0; g < GS; g++)
         tma_load_2d(sq + g * (TP * HD * 2), &map_q, &q_full, (h0 + g) * HD, (int)m_base);
-      auto page_of = [&](int i) { return (POOLED && i < npp) ? ptable[i] : table[jb0 + i - npp]; };
+      auto page_of = [&](int i) { return (POOLED && i < npp) ? ptable[i] : table[FIRST && i < nf ? i : jb0 + i - npp - nf]; };
       int next_page = page_of(0);
       for (int i = 0; i < n_it && ok; i++) {
         const int s = i % NS;
@@ -325,7 +328,7 @@ attention_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __g
     float m_used = ATC_NEG, l = 0.f;
     for (int i = 0; i < n_it && ok; i++) {
       const bool pooled = POOLED && i < npp;
-      const int key0 = pooled ? i * PAGE : (jb0 + i - npp) * PAGE, bsel = i & (SB - 1), s = i % NS;
+      const int key0 = (pooled || (FIRST && i < nf) ? i : jb0 + i - npp - nf) * PAGE, bsel = i & (SB - 1), s = i % NS;
       if (!mbar_wait(&s_full[bsel], (i / SB) & 1, abort_flag)) { atomicExch(status, 16); ok = false; break; }
       tc_fence_after();
       const uint32_t t_s = t_s0 + 64 * bsel + lane_base;
@@ -348,10 +351,11 @@ attention_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __g
         for (int c = 0; c < PAGE; c++)
           v[c] = __float_as_uint(fmaf(__uint_as_float(v[c]), scale2, fmaf(slope2, (float)c, at0)));
       }
-      if (c_lo > 0 || c_hi < PAGE - 1) {
+      const int c_first = FIRST ? first - key0 : 0;      // columns below this one are first positions
+      if ((c_lo > 0 && !(FIRST && c_first >= min(c_lo, PAGE))) || c_hi < PAGE - 1) {
 #pragma unroll
         for (int c = 0; c < PAGE; c++)
-          if (c < c_lo || c > c_hi) v[c] = __float_as_uint(ATC_NEG);
+          if ((c < c_lo && !(FIRST && c < c_first)) || c > c_hi) v[c] = __float_as_uint(ATC_NEG);
       }
       float rm[2] = {ATC_NEG, ATC_NEG};
 #pragma unroll
@@ -414,6 +418,16 @@ attention_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __g
       const float2 sums = halves(add_f2(ps[0], ps[1]));
       l += sums.x + sums.y;
       const int key_end = pooled ? nb_tile : key_hi;
+      if (FIRST && max(c_first, 0) < min(key_lo_tile - key0, PAGE)) {
+        // value columns that no row of the tile reads, between the first positions and the tile's window, become zero
+        if (!mbar_wait(&v_full[s], (i / NS) & 1, abort_flag)) { atomicExch(status, 19); ok = false; break; }
+        if (r < VD) {
+          uint8_t* vrow = sv + s * V_BYTES + r * 128;
+          for (int e = max(c_first, 0); e < min(key_lo_tile - key0, PAGE); e++)
+            reinterpret_cast<bf16*>(vrow + (((e >> 3) ^ (r & 7)) << 4))[e & 7] = __float2bfloat16_rn(0.f);
+        }
+        if (DEEP) fence_proxy_async_smem();
+      }
       if (key0 + PAGE > key_end) {
         // the page with the end of the sequence (or of the pooled blocks): its value columns beyond it become zero
         if (!mbar_wait(&v_full[s], (i / NS) & 1, abort_flag)) { atomicExch(status, 19); ok = false; break; }
@@ -518,13 +532,13 @@ static bool atc_few_tiles(int M, int B, int nh, int nkv, int max_qlen) {
   return (per_head < by_rows ? per_head : by_rows) * nkv * 2 <= 5ll * sm_count();
 }
 
-template <bool POOLED, bool WIDE, bool DEEP, int VD>
+template <bool POOLED, bool WIDE, bool DEEP, int VD, bool FIRST>
 static int launch_attention_prefill_tc(const char* who, void* out, const void* q, int q_stride, int M, const void* k_pool,
                                        const void* v_pool, int n_pages, const int* block_table, int bt_width,
                                        const void* pk_pool, const void* pv_pool, int n_pooled_pages, const int* pool_table,
                                        int pt_width, const int* seq_slot, const int* seq_pos0, const int* seq_qstart,
                                        const int* seq_qlen, const void* gate, int gate_stride, int gate_elem, int B, int nh, int nkv,
-                                       int hd, int page_size, int window, int chunk, int pool, float scale, const float* head_scale,
+                                       int hd, int page_size, int window, int chunk, int first, int pool, float scale, const float* head_scale,
                                        const float* freq_v, const float* slopes, const float* sinks, int max_qlen, int* status,
                                        cudaStream_t st) {
   if (B <= 0 || max_qlen <= 0 || M <= 0) return 0;
@@ -555,13 +569,13 @@ static int launch_attention_prefill_tc(const char* who, void* out, const void* q
   {                                                                                                               \
     static bool set = false;                                                                                      \
     if (!set) {                                                                                                   \
-      if (cudaFuncSetAttribute(attention_prefill_tc_kernel<GS_, POOLED, WIDE, DEEP, VD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) \
+      if (cudaFuncSetAttribute(attention_prefill_tc_kernel<GS_, POOLED, WIDE, DEEP, VD, FIRST>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) \
         return leb_fail("%s: %zu bytes of shared memory per block refused", who, smem);                         \
       set = true;                                                                                                 \
     }                                                                                                             \
-    leb_launch(attention_prefill_tc_kernel<GS_, POOLED, WIDE, DEEP, VD>, grid, dim3(ATC_THREADS), smem, st,                       \
+    leb_launch(attention_prefill_tc_kernel<GS_, POOLED, WIDE, DEEP, VD, FIRST>, grid, dim3(ATC_THREADS), smem, st,                       \
         mq, mk, mv, mpk, mpv, (bf16*)out, block_table, bt_width, pool_table, pt_width, seq_slot, seq_pos0, seq_qstart, \
-        seq_qlen, (const bf16*)gate, gate_stride, gate_elem, nh, nkv, window, chunk, pooled ? pool : 0, scale, head_scale, freq_v, slopes, \
+        seq_qlen, (const bf16*)gate, gate_stride, gate_elem, nh, nkv, window, chunk, first, pooled ? pool : 0, scale, head_scale, freq_v, slopes, \
         sinks, status); \
   }
   switch (G) {
@@ -584,14 +598,17 @@ LEB_API int leb_attention_prefill_tc(void* out, const void* q, int q_stride, int
                                      const void* v_pool, int n_pages, const int* block_table, int bt_width,
                                      const int* seq_slot, const int* seq_pos0, const int* seq_qstart,
                                      const int* seq_qlen, const void* gate, int gate_stride, int gate_elem, int B, int nh,
-                                     int nkv, int hd, int page_size, int window, int chunk, int wide, float scale,
+                                     int nkv, int hd, int page_size, int window, int chunk, int first, int wide, float scale,
                                      const float* slopes, const float* sinks, int max_qlen, int* status, cudaStream_t st) {
 #define LEB_ATC_ARGS "leb_attention_prefill_tc", out, q, q_stride, M, k_pool, v_pool, n_pages, block_table, bt_width, nullptr, \
                      nullptr, 0, nullptr, 0, seq_slot, seq_pos0, seq_qstart, seq_qlen, gate, gate_stride, gate_elem, B, nh, nkv, \
-                     hd, page_size, window, chunk, 0, scale, nullptr, nullptr, slopes, sinks, max_qlen, status, st
-  if (wide) return launch_attention_prefill_tc<false, true, true, 64>(LEB_ATC_ARGS);
-  return atc_few_tiles(M, B, nh, nkv, max_qlen) ? launch_attention_prefill_tc<false, false, true, 64>(LEB_ATC_ARGS)
-                                                : launch_attention_prefill_tc<false, false, false, 64>(LEB_ATC_ARGS);
+                     hd, page_size, window, chunk, first, 0, scale, nullptr, nullptr, slopes, sinks, max_qlen, status, st
+#define LEB_ATC_FORM(FIRST)                                                                                                   \
+  (wide ? launch_attention_prefill_tc<false, true, true, 64, FIRST>(LEB_ATC_ARGS)                                             \
+        : atc_few_tiles(M, B, nh, nkv, max_qlen) ? launch_attention_prefill_tc<false, false, true, 64, FIRST>(LEB_ATC_ARGS)   \
+                                                 : launch_attention_prefill_tc<false, false, false, 64, FIRST>(LEB_ATC_ARGS))
+  return first > 0 ? LEB_ATC_FORM(true) : LEB_ATC_FORM(false);
+#undef LEB_ATC_FORM
 #undef LEB_ATC_ARGS
 }
 
@@ -609,8 +626,8 @@ LEB_API int leb_attention_pooled_tc(void* out, const void* q, int q_stride, int 
   LEB_REQUIRE(vd == 64 || vd == 32, "leb_attention_pooled_tc: value heads of %d numbers (64 or 32)", vd);
 #define LEB_APT_ARGS "leb_attention_pooled_tc", out, q, q_stride, M, k_pool, v_pool, n_pages, block_table, bt_width, pk_pool, \
                      pv_pool, n_pooled_pages, pool_table, pt_width, seq_slot, seq_pos0, seq_qstart, seq_qlen, nullptr, 0, 0, B, nh, \
-                     nkv, hd, page_size, window, 0, pool, 1.0f, head_scale, freq_v, nullptr, nullptr, max_qlen, status, st
-  const int rc = vd == 64 ? launch_attention_prefill_tc<true, true, true, 64>(LEB_APT_ARGS) : launch_attention_prefill_tc<true, true, true, 32>(LEB_APT_ARGS);
+                     nkv, hd, page_size, window, 0, 0, pool, 1.0f, head_scale, freq_v, nullptr, nullptr, max_qlen, status, st
+  const int rc = vd == 64 ? launch_attention_prefill_tc<true, true, true, 64, false>(LEB_APT_ARGS) : launch_attention_prefill_tc<true, true, true, 32, false>(LEB_APT_ARGS);
 #undef LEB_APT_ARGS
   return rc;
 }

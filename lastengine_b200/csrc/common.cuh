@@ -178,6 +178,11 @@ __device__ __forceinline__ int first_key(int pos, int window, int chunk) {
   return lo;
 }
 
+// First positions that stay visible: beside the positions from its first_key on a row reads positions [0, first).  Tiles of T
+// positions that rows from `key_lo` (the earliest one's first_key) on read: how many there are of the first positions before the
+// tile that holds key_lo.  Those come first in the walk, numbered 0 on; the tiles from key_lo / T on follow them.
+__device__ __forceinline__ int first_tiles(int first, int key_lo, int T) { return min((first + T - 1) / T, key_lo / T); }
+
 // The factor sigmoid(gate) of a head's result: one per (row, head), or with `elem` one per dimension of the head
 // (gate [rows, heads, width]).
 template <typename T>

@@ -257,7 +257,7 @@ def _declare(L) -> None:
         "leb_add": [P, P, S, P],
         "leb_shortconv": [P, P, I, P, P, P, P, P, P, P, I, I, I, I, P],
         "leb_qk_rope_store": [P, P, I, P, P, I, P, P, I, P, I, P, P, P, P, P, F, P, I, I, I, I, I, I, I, I, I, I, I, F, F, P],
-        "leb_attention": [P, P, P, P, P, I, P, I, P, P, P, P, P, I, I, I, I, I, I, I, I, I, I, F, P, P, I, I, I, P],
+        "leb_attention": [P, P, P, P, P, I, P, I, P, P, P, P, P, I, I, I, I, I, I, I, I, I, I, I, F, P, P, I, I, I, P],
         "leb_gated_act": [P, I, P, I, I, I, I, F, F, P],
         "leb_layernorm": [P, I, P, P, P, I, I, F, P],
         "leb_scaled_residual": [P, P, F, P, I, P, F, I, I, P],
@@ -301,16 +301,20 @@ def _declare(L) -> None:
         "leb_penalties_slots": [P, P, P, P, I, I, I, F, F, P],
         "leb_history_append": [P, P, P, P, I, I, P],
         "leb_attention_decode_supported": [I, I, I, I],
-        "leb_attention_decode": [P, P, P, P, P, P, I, P, P, P, P, I, I, I, I, I, I, I, I, I, I, F, P, P, I, P],
+        "leb_attention_decode": [P, P, P, P, P, P, I, P, P, P, P, I, I, I, I, I, I, I, I, I, I, I, F, P, P, I, P],
         "leb_attention_merge": [P, P, I, P, I, I, P, I, I, I, I, P],
         "leb_attention_decode_prep_supported": [I, I, I, I, I, I],
-        "leb_attention_decode_prep": [P, P, P, I, P, P, I, P, P, P, I, P, P, P, P, P, F, P, I, I, I, P, I, I, I, I, I, I, I, I, I, I, F, P, P, F, F, I, P],
+        "leb_attention_decode_prep": [P, P, P, I, P, P, I, P, P, P, I, P, P, P, P, P, F, P, I, I, I, P, I, I, I, I, I, I, I, I, I, I, I, F, P, P, F, F, I, P],
         "leb_attention_prefill_supported": [I, I, I, I],
         "leb_attention_prefill_tc_supported": [I, I, I, I],
-        "leb_attention_prefill_tc": [P, P, I, I, P, P, I, P, I, P, P, P, P, P, I, I, I, I, I, I, I, I, I, I, F, P, P, I, P, P],
+        "leb_attention_prefill_tc": [P, P, I, I, P, P, I, P, I, P, P, P, P, P, I, I, I, I, I, I, I, I, I, I, I, F, P, P, I, P, P],
         "leb_attention_pooled_tc": [P, P, I, I, P, P, I, P, I, P, P, I, P, I, P, P, P, P, P, P, I, I, I, I, I, I, I, I, I, P, P],
         "leb_attention_pooled_tc_value_dim": [I],
-        "leb_attention_prefill": [P, P, P, P, P, I, P, P, P, P, P, I, I, I, I, I, I, I, I, I, I, F, P, P, I, P],
+        "leb_attention_prefill": [P, P, P, P, P, I, P, P, P, P, P, I, I, I, I, I, I, I, I, I, I, I, F, P, P, I, P],
+        "leb_stream_tables": [P, I, P, P, P, P, P, P, P, P, P, P, I, P, I, P, I, P, I, I, I, P],
+        "leb_stream_advance": [P, P, P, I, P, P, I, P, I, P, I, I, I, I, P],
+        "leb_stream_release": [P, P, I, P, P, I, P, I, P, I, I, I, P],
+        "leb_store_rows": [P, P, P, I, P, I, I, P, I, I, I, I, I, I, P],
         "leb_gemm_bf16_skinny_slices": [I, I],
         "leb_gemm_bf16_skinny_supported": [P, P, I, I, I],
         "leb_gemm_bf16_skinny": [P, I, P, P, I, I, I, I, I, I, P, I, P, I, I, F, P, P, P, P, P],
@@ -1511,14 +1515,14 @@ def set_latent_mma(on: bool) -> None:
     lib().leb_set_latent_mma(1 if on else 0)
 
 
-def _read_length(max_kvlen: int, window: int = 0, chunk: int = 0) -> int:
-    """The most cached positions a row reads: its sequence, its window or its chunk."""
+def _read_length(max_kvlen: int, window: int = 0, chunk: int = 0, first: int = 0) -> int:
+    """The most cached positions a row reads: its sequence, its window or its chunk, with the sequence's first positions beside them."""
     n = max_kvlen
     if window > 0:
         n = min(n, window)
     if chunk > 0:
         n = min(n, chunk)
-    return n
+    return min(max_kvlen, n + first)
 
 
 @functools.lru_cache(maxsize=256)
@@ -1587,7 +1591,7 @@ def sm_count() -> int:
 
 
 def attention_splits(batch, nkv: int, G: int, sm_count: int | None = None, hd: int = 64, chunk: int = 0, window: int = 0,
-                     general: bool = False) -> int:
+                     general: bool = False, first: int = 0) -> int:
     """How many blocks share one sequence's key range in a decode step (1 for prompts).
 
     Measured on B200 (head size 64, 8 kv heads, times with the merge of the splits): a block has a
@@ -1606,7 +1610,7 @@ def attention_splits(batch, nkv: int, G: int, sm_count: int | None = None, hd: i
         return 1
     if sm_count is None:
         sm_count = globals()["sm_count"]()
-    kv = max(_read_length(int(batch.max_kvlen), window, chunk), 1)
+    kv = max(_read_length(int(batch.max_kvlen), window, chunk, first), 1)
     per = max(batch.n_seqs * nkv * ((G + 15) // 16), 1)
     stage_bytes = 2 * 32 * hd * 2 * (3 if hd <= 32 else 2) * 4          # a block's rings: 4 warps, keys and values
     slots = sm_count * max(1, min(3, (227 * 1024) // stage_bytes))      # blocks that run at once
@@ -1660,7 +1664,7 @@ def attention(out: torch.Tensor, q: torch.Tensor | None, k_pool: torch.Tensor, v
               window: int, scale: float, gate: torch.Tensor | None = None,
               n_splits: int = 1, scratch: torch.Tensor | None = None, raw: RawQKV | None = None,
               vd: int | None = None, chunk: int = 0, wide: bool = False, slopes: torch.Tensor | None = None,
-              sinks: torch.Tensor | None = None) -> None:
+              sinks: torch.Tensor | None = None, first: int = 0) -> None:
     """Causal attention of the step's rows over the paged cache (which already holds their keys;
     with `raw`, the kernel puts the step's keys and values there itself and `q` is not used).
     `vd`: width of a value head where it differs from the key head's (the general kernel then).
@@ -1668,7 +1672,13 @@ def attention(out: torch.Tensor, q: torch.Tensor | None, k_pool: torch.Tensor, v
     `chunk` > 0: a row reads its own chunk of that many positions only, counted from the sequence's first.
     `wide`: the softmax weights enter the bfloat16 product with the values as two terms (16 significant bits).
     `slopes` [heads]: slope_h (i - j) is taken off the scaled score of query i and key j.  `sinks` [heads]: one more logit
-    per head in the softmax's denominator, without a key and without a value, not scaled."""
+    per head in the softmax's denominator, without a key and without a value, not scaled.
+    `first` > 0: beside its window (or chunk) a row reads the sequence's first `first` positions, whose pages the cache then
+    keeps; without either it reads every position anyway.  What lies in the cache between those positions and the window of the step's first
+    row of a sequence reaches no result, whatever it is."""
+    if first < 0:
+        raise KernelError(f"attention: {first} first positions")
+    first = int(first) if window > 0 or chunk > 0 else 0
     _cuda(out, "attention.out")
     for name, t in (("slopes", slopes), ("sinks", sinks)):
         if t is not None:
@@ -1676,10 +1686,10 @@ def attention(out: torch.Tensor, q: torch.Tensor | None, k_pool: torch.Tensor, v
             assert t.numel() == nh
     if vd is not None and vd != hd:
         return _attention_general(out, q, k_pool, v_pool, block_table, batch, nh, nkv, hd, int(vd), page_size, window,
-                                  scale, gate, n_splits, scratch, chunk, slopes, sinks)
+                                  scale, gate, n_splits, scratch, chunk, slopes, sinks, first)
     if raw is not None:
         return _attention_decode_raw(out, raw, k_pool, v_pool, block_table, batch, nh, nkv, hd, page_size, window,
-                                     scale, gate, n_splits, scratch, chunk, wide, slopes, sinks)
+                                     scale, gate, n_splits, scratch, chunk, wide, slopes, sinks, first)
     _cuda(q, "attention.q", out.dtype)
     _cuda(k_pool, "attention.k_pool", out.dtype)
     _cuda(v_pool, "attention.v_pool", out.dtype)
@@ -1700,7 +1710,7 @@ def attention(out: torch.Tensor, q: torch.Tensor | None, k_pool: torch.Tensor, v
         _check(L.leb_attention_decode(
             _ptr(out), _ptr(scratch), _ptr(q), _ptr(k_pool), _ptr(v_pool), _ptr(block_table),
             block_table.shape[1], _ptr(batch.seq_slot), _ptr(batch.seq_pos0), _ptr(batch.seq_qstart),
-            _ptr(gate), gate_stride, gate_elem, batch.n_seqs, nh, nkv, hd, page_size, window, chunk, int(wide), float(scale),
+            _ptr(gate), gate_stride, gate_elem, batch.n_seqs, nh, nkv, hd, page_size, window, chunk, first, int(wide), float(scale),
             _ptr(slopes), _ptr(sinks), n_splits, _stream()))
         if n_splits > 1:
             _check(L.leb_attention_merge(_ptr(out), _ptr(scratch), BF16, _ptr(gate), gate_stride, gate_elem, _ptr(sinks), M,
@@ -1713,7 +1723,7 @@ def attention(out: torch.Tensor, q: torch.Tensor | None, k_pool: torch.Tensor, v
             _ptr(out), _ptr(q), q.stride(0), M, _ptr(k_pool), _ptr(v_pool), k_pool.shape[0], _ptr(block_table),
             block_table.shape[1], _ptr(batch.seq_slot), _ptr(batch.seq_pos0), _ptr(batch.seq_qstart),
             _ptr(batch.seq_qlen), _ptr(gate), gate_stride, gate_elem, batch.n_seqs, nh, nkv, hd, page_size, window, chunk,
-            int(wide), float(scale), _ptr(slopes), _ptr(sinks), batch.max_qlen, _ptr(_status_word(out.device)), _stream()))
+            first, int(wide), float(scale), _ptr(slopes), _ptr(sinks), batch.max_qlen, _ptr(_status_word(out.device)), _stream()))
         return
     if (out.dtype == torch.bfloat16 and n_splits == 1
             and L.leb_attention_prefill_supported(nh, nkv, hd, page_size)):
@@ -1721,18 +1731,18 @@ def attention(out: torch.Tensor, q: torch.Tensor | None, k_pool: torch.Tensor, v
         _check(L.leb_attention_prefill(
             _ptr(out), _ptr(q), _ptr(k_pool), _ptr(v_pool), _ptr(block_table), block_table.shape[1],
             _ptr(batch.seq_slot), _ptr(batch.seq_pos0), _ptr(batch.seq_qstart), _ptr(batch.seq_qlen),
-            _ptr(gate), gate_stride, gate_elem, batch.n_seqs, nh, nkv, hd, page_size, window, chunk, int(wide), float(scale),
+            _ptr(gate), gate_stride, gate_elem, batch.n_seqs, nh, nkv, hd, page_size, window, chunk, first, int(wide), float(scale),
             _ptr(slopes), _ptr(sinks), batch.max_qlen, _stream()))
         return
     _check(L.leb_attention(
         _ptr(out), _ptr(scratch), _ptr(q), _ptr(k_pool), _ptr(v_pool), _dt(out, "attention"),
         _ptr(block_table), block_table.shape[1], _ptr(batch.seq_slot), _ptr(batch.seq_pos0),
         _ptr(batch.seq_qstart), _ptr(batch.seq_qlen), _ptr(gate), gate_stride, gate_elem, M, batch.n_seqs, nh, nkv,
-        hd, page_size, window, chunk, float(scale), _ptr(slopes), _ptr(sinks), batch.max_qlen, n_splits, hd, _stream()))
+        hd, page_size, window, chunk, first, float(scale), _ptr(slopes), _ptr(sinks), batch.max_qlen, n_splits, hd, _stream()))
 
 
 def _attention_general(out, q, k_pool, v_pool, block_table, batch, nh, nkv, hd, vd, page_size, window, scale, gate,
-                       n_splits, scratch, chunk=0, slopes=None, sinks=None) -> None:
+                       n_splits, scratch, chunk=0, slopes=None, sinks=None, first=0) -> None:
     """The general kernel with value heads of their own width."""
     _cuda(q, "attention.q", out.dtype)
     _cuda(k_pool, "attention.k_pool", out.dtype)
@@ -1750,11 +1760,11 @@ def _attention_general(out, q, k_pool, v_pool, block_table, batch, nh, nkv, hd, 
         _ptr(out), _ptr(scratch), _ptr(q), _ptr(k_pool), _ptr(v_pool), _dt(out, "attention"),
         _ptr(block_table), block_table.shape[1], _ptr(batch.seq_slot), _ptr(batch.seq_pos0),
         _ptr(batch.seq_qstart), _ptr(batch.seq_qlen), _ptr(gate), gate_stride, gate_elem, M, batch.n_seqs, nh, nkv,
-        hd, page_size, window, chunk, float(scale), _ptr(slopes), _ptr(sinks), batch.max_qlen, n_splits, vd, _stream()))
+        hd, page_size, window, chunk, first, float(scale), _ptr(slopes), _ptr(sinks), batch.max_qlen, n_splits, vd, _stream()))
 
 
 def _attention_decode_raw(out, raw: RawQKV, k_pool, v_pool, block_table, batch, nh, nkv, hd, page_size, window,
-                          scale, gate, n_splits, scratch, chunk=0, wide=False, slopes=None, sinks=None) -> None:
+                          scale, gate, n_splits, scratch, chunk=0, wide=False, slopes=None, sinks=None, first=0) -> None:
     M = out.shape[0]
     if not decode_attention_takes_raw(out.dtype, batch, M, nh, nkv, hd, page_size, raw.inv_freq, raw.rope_dim, raw.neox):
         raise KernelError("attention: this step's q, k and v must be normed, rotated and stored before the call")
@@ -1787,10 +1797,99 @@ def _attention_decode_raw(out, raw: RawQKV, k_pool, v_pool, block_table, batch, 
         _ptr(k_pool), _ptr(v_pool), _ptr(block_table), block_table.shape[1], _ptr(batch.seq_slot), _ptr(batch.seq_pos0),
         _ptr(batch.seq_qstart), _ptr(raw.q_norm_w), _ptr(raw.k_norm_w), raw.eps, _ptr(raw.inv_freq), raw.rope_dim,
         1 if raw.neox else 0, int(raw.row_norm), _ptr(gate), gate_stride, gate_elem, batch.n_seqs, nh, nkv, hd, page_size, window,
-        chunk, int(wide), float(scale), _ptr(slopes), _ptr(sinks), *_temperature(raw.temperature), n_splits, _stream()))
+        chunk, first, int(wide), float(scale), _ptr(slopes), _ptr(sinks), *_temperature(raw.temperature), n_splits, _stream()))
     if n_splits > 1:
         _check(L.leb_attention_merge(_ptr(out), _ptr(scratch), BF16, _ptr(gate), gate_stride, gate_elem, _ptr(sinks), M, nh, hd,
                                      n_splits, _stream()))
+
+
+# ----------------------------------------------------------------------------------------------
+def _words(name: str, **tensors: torch.Tensor) -> None:
+    for what, t in tensors.items():
+        _cuda(t, f"{name}.{what}", torch.int32)
+
+
+def _stream_state(name: str, lens: torch.Tensor, pages: torch.Tensor, free: torch.Tensor, counts: torch.Tensor, page_size: int) -> None:
+    if pages.dim() != 2 or pages.shape[0] != lens.numel() or counts.numel() != 2 or lens.numel() < 1 or pages.shape[1] < 1:
+        raise KernelError(f"{name}: page lists {tuple(pages.shape)} of {lens.numel()} slots, {counts.numel()} counts (2)")
+    if page_size < 1 or free.numel() * page_size > 2 ** 31:
+        raise KernelError(f"{name}: {free.numel()} pages of {page_size} positions (2^31 positions at most)")
+
+
+def stream_tables(table: torch.Tensor, slot_map: torch.Tensor, row_seq: torch.Tensor, row_pos: torch.Tensor, step_slot: torch.Tensor,
+                  step_qlen: torch.Tensor, pos0: torch.Tensor, qstart: torch.Tensor, seq_slot: torch.Tensor, seq_qlen: torch.Tensor,
+                  lens: torch.Tensor, pages: torch.Tensor, free: torch.Tensor, counts: torch.Tensor, page_size: int) -> None:
+    """A step's tables from its sequences' slots and row counts (`seq_slot`, `seq_qlen` [B]; slot -1 is padding), all int32 on the device.
+
+    State: `lens` [slots] positions held, `pages` [slots, width] page lists (-1: nothing held), `free` [pages] a stack of
+    page numbers of which counts[0] are on it.  Written: `table` [B, width of the step's tables] (-1 beyond what is held),
+    per row `slot_map` (page * page_size + place, -1 for padding), `row_seq`, `row_pos`; per sequence `step_slot`,
+    `step_qlen`, `pos0`, `qstart`; pages new to a sequence are entered in `pages`.  Lengths and stack stay as they were until
+    `stream_advance`: a step may be laid out again.  The rows are as many as slot_map has.
+
+    counts[1] is 0, or why the step is refused: how many pages it is short of, -1 a sequence longer than its tables, -2 rows
+    that are not as many as seq_qlen says, -3 a slot or row count that cannot be.  A refused step changes no state, and all of its
+    sequences are padding without rows.  Every slot may be named once.
+    (Kernels may read a step's tables ahead of the wait for the kernel launched before: `stream_advance`, a copy or a
+    graph's launch lies between this call and them.)"""
+    _words("stream_tables", table=table, slot_map=slot_map, row_seq=row_seq, row_pos=row_pos, step_slot=step_slot, step_qlen=step_qlen,
+           pos0=pos0, qstart=qstart, seq_slot=seq_slot, seq_qlen=seq_qlen, lens=lens, pages=pages, free=free, counts=counts)
+    _stream_state("stream_tables", lens, pages, free, counts, page_size)
+    B, M = seq_slot.numel(), slot_map.numel()
+    if table.dim() != 2 or table.shape[0] != B or table.shape[1] < 1 or row_seq.numel() != M or row_pos.numel() != M \
+            or any(t.numel() != B for t in (seq_qlen, step_slot, step_qlen, pos0, qstart)):
+        raise KernelError(f"stream_tables: outputs do not fit {B} sequences and {M} rows")
+    _check(lib().leb_stream_tables(
+        _ptr(table), table.shape[1], _ptr(slot_map), _ptr(row_seq), _ptr(row_pos), _ptr(step_slot), _ptr(step_qlen), _ptr(pos0),
+        _ptr(qstart), _ptr(seq_slot), _ptr(seq_qlen), _ptr(lens), lens.numel(), _ptr(pages), pages.shape[1], _ptr(free), free.numel(),
+        _ptr(counts), M, B, page_size, _stream()))
+
+
+def stream_advance(seq_slot: torch.Tensor, seq_qlen: torch.Tensor, lens: torch.Tensor, kept: torch.Tensor, pages: torch.Tensor,
+                   free: torch.Tensor, counts: torch.Tensor, page_size: int, window: int = 0, first: int = 0) -> None:
+    """After `stream_tables` laid a step out: the sequences are longer, the pages they took leave the stack, and with a `window` the
+    pages that no later row reads go back on it, in the order of sequences and pages; those with one of the `first` positions stay.
+    Takes the step's `step_slot` and `step_qlen` (a refused step then changes nothing).  `kept` [slots]: a sequence's first
+    page, behind those of its first positions, that is still held (at the start: ceil(first / page_size)).
+    May be called before the step's kernels are: what goes back is given out by the next step's tables at the earliest."""
+    _words("stream_advance", seq_slot=seq_slot, seq_qlen=seq_qlen, lens=lens, kept=kept, pages=pages, free=free, counts=counts)
+    _stream_state("stream_advance", lens, pages, free, counts, page_size)
+    if seq_slot.numel() != seq_qlen.numel() or kept.numel() != lens.numel() or window < 0 or first < 0:
+        raise KernelError(f"stream_advance: {seq_slot.numel()} slots and {seq_qlen.numel()} row counts, window {window}, first {first}")
+    _check(lib().leb_stream_advance(
+        _ptr(seq_slot), _ptr(seq_qlen), _ptr(lens), lens.numel(), _ptr(kept), _ptr(pages), pages.shape[1], _ptr(free), free.numel(),
+        _ptr(counts), seq_slot.numel(), page_size, window, first, _stream()))
+
+
+def stream_release(seq_slot: torch.Tensor, lens: torch.Tensor, kept: torch.Tensor, pages: torch.Tensor, free: torch.Tensor,
+                   counts: torch.Tensor, page_size: int, first: int = 0) -> None:
+    """The sequences in `seq_slot` (each named once; -1: none) end: their pages go back on the stack, their lengths are 0."""
+    _words("stream_release", seq_slot=seq_slot, lens=lens, kept=kept, pages=pages, free=free, counts=counts)
+    _stream_state("stream_release", lens, pages, free, counts, page_size)
+    if kept.numel() != lens.numel() or first < 0:
+        raise KernelError(f"stream_release: {kept.numel()} of {lens.numel()} slots, first {first}")
+    _check(lib().leb_stream_release(_ptr(seq_slot), _ptr(lens), lens.numel(), _ptr(kept), _ptr(pages), pages.shape[1], _ptr(free),
+                                    free.numel(), _ptr(counts), seq_slot.numel(), page_size, first, _stream()))
+
+
+def store_rows(k_pool: torch.Tensor, v_pool: torch.Tensor, k: torch.Tensor, v: torch.Tensor, slot_map: torch.Tensor) -> None:
+    """Keys `k` [M, kv heads * width] and values `v` [M, kv heads * value width] into the paged cache: row m at place
+    slot_map[m] % page size of page slot_map[m] / page size, -1 nowhere (int32 [M]; no place is named twice).  k and v may be
+    column slices of one fused projection; k_pool [page, kv head, place, width], v_pool [page, kv head, value width, place]."""
+    _cuda(k_pool, "store_rows.k_pool")
+    dt = _dt(k_pool, "store_rows")
+    _cuda(v_pool, "store_rows.v_pool", k_pool.dtype)
+    _cuda(k, "store_rows.k", k_pool.dtype, contiguous=False)
+    _cuda(v, "store_rows.v", k_pool.dtype, contiguous=False)
+    _cuda(slot_map, "store_rows.slot_map", torch.int32)
+    n_pages, nkv, P, hd = k_pool.shape
+    vd, M = v_pool.shape[2], slot_map.numel()
+    if v_pool.shape != (n_pages, nkv, vd, P) or k.shape != (M, nkv * hd) or v.shape != (M, nkv * vd):
+        raise KernelError(f"store_rows: {M} rows of {tuple(k.shape)} and {tuple(v.shape)} into pools {tuple(k_pool.shape)} and {tuple(v_pool.shape)}")
+    if M > 0 and (k.stride(1) != 1 or v.stride(1) != 1):
+        raise KernelError("store_rows: the numbers of a row must lie one behind the other")
+    _check(lib().leb_store_rows(_ptr(k_pool), _ptr(v_pool), _ptr(k), k.stride(0), _ptr(v), v.stride(0), dt, _ptr(slot_map), n_pages, M,
+                                nkv, hd, vd, P, _stream()))
 
 
 # ----------------------------------------------------------------------------------------------

@@ -19,7 +19,8 @@ the tensors under the part's prefix.
 q and k may also be normed over their whole projected row, before heads are cut out of it, with weights over the row
 (`qk_norm="row"`); the output gate may be a factor per number of every head, sigmoid(Wg h) with Wg [heads * v_head_dim,
 hidden] (`output_gate="numbers"`); instead of a window the positions may be cut into chunks of `chunk`, counted from the
-sequence's first: a row reads its own chunk up to itself.  `wide_weights`: the softmax weights enter the bfloat16
+sequence's first: a row reads its own chunk up to itself.  `first`: beside its window or chunk a row reads the sequence's
+first `first` positions, which then stay in the cache.  `wide_weights`: the softmax weights enter the bfloat16
 product with the values as two bfloat16 terms (16 significant bits) instead of one.
 
 More options: `values="keys"`: there is no value projection, a position's value is its key as it leaves the convolution
@@ -55,7 +56,7 @@ class AttentionMixer(Mixer):
                  scale: float | None = None, v_head_dim: int | None = None, conv_taps: int = 0,
                  v_norm: bool = False, names: dict[str, str] | None = None, chunk: int = 0, wide_weights: bool = False,
                  values: str = "own", slopes: list[float] | None = None, sink: str | None = None,
-                 query_temperature: tuple[float, float] | None = None, widen: bool = False):
+                 query_temperature: tuple[float, float] | None = None, widen: bool = False, first: int = 0):
         if values not in ("own", "keys") or sink not in (None, "zero", "learned"):
             raise ValueError(f"values {values!r} ('own', 'keys') / sink {sink!r} (None, 'zero', 'learned')")
         if qk_norm not in (True, False, "unit", "row") or output_gate not in (True, False, "numbers"):
@@ -99,6 +100,9 @@ class AttentionMixer(Mixer):
                   "q_conv": "q_conv.weight", "k_conv": "k_conv.weight", "v_conv": "v_conv.weight", "sink": "sink"}
         self.n.update(names or {})
         self.window, self.chunk, self.wide = int(window), int(chunk), bool(wide_weights)
+        if first < 0:
+            raise ValueError(f"{first} first positions")
+        self.first = int(first) if self.window > 0 or self.chunk > 0 else 0      # (without either a row reads them anyway)
         self.output_gate, self.gate_numbers = bool(output_gate), output_gate == "numbers"
         if self.qk_row and (self.v_norm or not own_kv):
             raise NotImplementedError("norms over whole rows beside normed values or a layer that reads another's cache")
@@ -137,7 +141,7 @@ class AttentionMixer(Mixer):
         return t
 
     def cache_spec(self):
-        kv = KVSpec(self.nkv, self.khd, self.window, None if self.kvd == self.khd else self.kvd, chunk=self.chunk)
+        kv = KVSpec(self.nkv, self.khd, self.window, None if self.kvd == self.khd else self.kvd, chunk=self.chunk, first=self.first)
         if self.taps <= 1:       # a single tap looks at the current row only
             return kv
         # the convolution's memory: the last taps-1 projected values of every q, k and v channel
@@ -273,12 +277,12 @@ class AttentionMixer(Mixer):
                                   None, 0, True, nh, nkv, hd, cache.page_size)
         o = ws.get("attn.o", (M, nh * kvd), env.dtype)
         n_splits = kernels.attention_splits(batch, nkv, nh // nkv, hd=khd, chunk=self.chunk, window=self.window,
-                                            general=env.is_float32)
+                                            general=env.is_float32, first=self.first)
         scratch = None
         if n_splits > 1:
             scratch = ws.get("attn.part", (M * nh * n_splits * (max(khd, kvd) + 2),), torch.float32)
         kernels.attention(o, None if raw is not None else q, cache.k, cache.v, cache.block_table, batch, nh, nkv, khd,
                           cache.page_size, self.window, self.scale, gate=gate, n_splits=n_splits, scratch=scratch, raw=raw,
-                          vd=kvd, chunk=self.chunk, wide=self.wide, slopes=self.slopes, sinks=self.sinks)
+                          vd=kvd, chunk=self.chunk, wide=self.wide, slopes=self.slopes, sinks=self.sinks, first=self.first)
         kernels.linear(out, o, self.w_out, kernels.ACCUMULATE if accumulate else kernels.STORE,
                        emit=emit if accumulate else None)

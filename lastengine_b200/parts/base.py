@@ -76,13 +76,15 @@ class KVSpec:
     of the chunk of that many positions (counted from the sequence's first) the next position lies in.
     `v_head_dim`: width of a value head where it differs from a key head's (None: the same).
     `pool` > 0: beside them one pooled key and value row for every complete block of `pool` positions,
-    in pages of their own (block b in row b); they stay when the window has let the block's positions go."""
+    in pages of their own (block b in row b); they stay when the window has let the block's positions go.
+    `first` > 0: beside the window (or chunk) a sequence's first positions stay."""
     n_kv_heads: int
     head_dim: int
     window: int = 0
     v_head_dim: int | None = None
     pool: int = 0
     chunk: int = 0
+    first: int = 0
 
     @property
     def value_dim(self) -> int:
