@@ -1,0 +1,430 @@
+// Prompt attention of streams on the fifth-generation tensor cores: a window and a sequence's first positions, heads of 64 or 128.
+//
+// A row at position p reads positions j <= p with j >= first_key(p) or j < first.  A block owns a tile of 128 rows: the G query heads
+// of one kv head times TP = 128 / G consecutive positions (a multiple of 8; the rows that are left are idle).  It walks a list of
+// pages, those of first positions and then those from its first row's window to its last row, two pages (128 keys) at a time:
+//
+//   S[128, 128] = Q[128, HD] . K[128, HD]^T       operands in shared memory, S in tensor memory
+//   P           = exp2(S * scale * log2 e - m)     two threads per row, one a page, P (bfloat16) to tensor memory
+//   O[128, HD] += P[128, 128] . V[128, HD]         P from tensor memory, V from shared memory
+//
+// Warps: eight for the softmax, one that brings Q and pages by TMA, one that issues the products, two that fill their warpgroup
+// (registers move between warpgroups).  Two blocks share an SM, so that one's products run under the other's exponentials, and a
+// scheduler has four softmax warps: what bounds the loop is the chain from a row's scores to its weights, not a pipe.
+// With heads of 64, P has columns beside S and the next scores are issued as soon as a row of S is in registers; with heads of 128, O
+// takes those columns, P lies over S and the next scores follow the product that reads P.
+//
+// Bounds: 128 keys of a tile are 1,024 cycles of the SM's special function unit (16 exponentials a cycle) and 512 (heads of 64) or 1,024
+// of its tensor cores, 512 or 1,280 of shared memory's 128 bytes a cycle; a tile alone takes some 2,400, two blocks on an SM 1,250 each.
+// 8,191 rows, window 4,096, 128 first positions, 32 heads over 8: heads of 64 308 us (683 TFLOP/s; the form with pages of 64 keys and
+// three blocks an SM, attention_prefill_tc.cu, 390), heads of 128 408 us (1,031); turns of 100 to 2,047 rows, 16 heads of 128 over 4,
+// window 2,048: 67 us (mma.sync 190).  Measured beside it: one thread a row 311 to 317 and 77 us on 12 streams' turns (71 now), two tiles
+// a block (one block an SM) 329, 64 keys at a time with two buffers of S 323 (heads of 128: 442), an eighth to a half of the
+// exponentials as polynomials on the multiply-add pipes 304 to 365 (heads of 128: 428 to 515).
+//
+// Every wait on an mbarrier is bounded; a wait that gives up sets the status word, all roles leave their loops, tensor memory is freed
+// and the block returns.
+#include "attention_tc.cuh"
+
+#define AST_NEG (-1e30f)
+
+template <int HD>
+struct AstShape {
+  static constexpr int THREADS = 384;
+  // registers a thread: at the launch, then of the softmax warps and of the other four (as many in all)
+  static constexpr int REGS = 80, REGS_SOFTMAX = 96, REGS_OTHER = 48;
+  static_assert(2 * REGS_SOFTMAX + REGS_OTHER <= 3 * REGS, "more registers than the block is launched with");
+  static constexpr int STAGES = HD == 64 ? 2 : 1;                     // iterations' keys and values on their way
+  static constexpr int Q_BYTES = 128 * HD * 2;
+  static constexpr int KV_BYTES = 128 * HD * 2;                       // of an iteration's keys (or values)
+  static constexpr int SMEM = 1024 + Q_BYTES + STAGES * 2 * KV_BYTES;
+  static constexpr bool OWN_P = HD == 64;                             // P beside S (else over it)
+  static constexpr int COLUMNS = 256;                                 // S, P and O
+};
+
+// The lowest n bits (none for n <= 0, all from 32 on).
+__device__ __forceinline__ uint32_t ast_below(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; }
+
+template <int HD>
+__global__ void __launch_bounds__(AstShape<HD>::THREADS, 2)
+attention_stream_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                           const __grid_constant__ CUtensorMap map_v, bf16* __restrict__ out, const int* __restrict__ block_table,
+                           int bt_width, const int* __restrict__ seq_slot, const int* __restrict__ seq_pos0,
+                           const int* __restrict__ seq_qstart, const int* __restrict__ seq_qlen, const bf16* __restrict__ gate,
+                           int gate_stride, int gate_elem, int nh, int nkv, int G, int TP, int window, int chunk, int first,
+                           float scale, const float* __restrict__ slopes, const float* __restrict__ sinks, int* __restrict__ status) {
+  using Shape = AstShape<HD>;
+  constexpr int PAGE = 64, NS = Shape::STAGES, HALVES = HD / 64;
+  constexpr int Q_BYTES = Shape::Q_BYTES, KV_BYTES = Shape::KV_BYTES;
+  constexpr bool OWN_P = Shape::OWN_P;
+  constexpr uint32_t COL_S = 0, COL_P = OWN_P ? 128 : 0, COL_O = OWN_P ? 192 : 128;
+  extern __shared__ uint8_t ast_raw[];
+  uint8_t* smem = (uint8_t*)(((uintptr_t)ast_raw + 1023) & ~(uintptr_t)1023);   // swizzled tiles want 1024
+  uint8_t* sq = smem;                         // [64 dimensions][128 rows][128 bytes]
+  uint8_t* sk = sq + Q_BYTES;                 // [stage][64 dimensions][128 keys][128 bytes]
+  uint8_t* sv = sk + NS * KV_BYTES;           // [stage][page][dimension][64 positions]
+  __shared__ uint64_t q_full, k_full[NS], v_full[NS], k_empty[NS], v_empty[NS], s_full, s_free, p_full, pv_done;
+  __shared__ float row_s[2][2][128];          // what the two threads of a row tell each other: [iteration's parity][thread][row]
+  __shared__ uint32_t tmem_slot;
+  __shared__ int abort_s;
+  volatile int* abort_flag = &abort_s;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // kv heads, then sequences vary fastest; the tiles with the longest key range come first
+  const int kvh = blockIdx.x, b = blockIdx.y;
+  const int row0 = (int)(gridDim.z - 1 - blockIdx.z) * TP;
+  const int qlen = seq_qlen[b];      // step data: written long before the kernel before this one
+  if (row0 >= qlen) {
+    pdl_wait();   // a kernel counts as complete when its blocks are: none may finish before its predecessor has
+    return;
+  }
+  const int rows = min(TP, qlen - row0);
+  const int pos0 = seq_pos0[b];
+  const size_t m_base = (size_t)seq_qstart[b] + row0;
+  const int h0 = kvh * G;
+  if (seq_slot[b] < 0) {   // a padding sequence: its rows are zero
+    pdl_wait();
+    for (int idx = threadIdx.x; idx < rows * G * (HD / 8); idx += blockDim.x) {
+      const int i = idx / (G * (HD / 8)), rest = idx % (G * (HD / 8));
+      reinterpret_cast<uint4*>(out + ((m_base + i) * nh + h0) * HD)[rest] = make_uint4(0, 0, 0, 0);
+    }
+    return;
+  }
+  const int q_lo = pos0 + row0, key_hi = q_lo + rows;      // keys [.., key_hi) exist for the tile
+  const int key_lo = first_key(q_lo, window, chunk);
+  const int nf = first_tiles(first, key_lo, PAGE), jb0 = key_lo / PAGE;
+  const int n_pages = nf + (key_hi - 1) / PAGE - jb0 + 1, n_it = (n_pages + 1) / 2;
+  const int* table = block_table + (size_t)b * bt_width;
+
+  if (threadIdx.x == 0) {
+    abort_s = 0;
+    mbar_init(&q_full, 1);
+    for (int s = 0; s < NS; s++) {
+      mbar_init(&k_full[s], 1);
+      mbar_init(&v_full[s], 1);
+      mbar_init(&k_empty[s], 1);
+      mbar_init(&v_empty[s], 1);
+    }
+    mbar_init(&s_full, 1);
+    mbar_init(&s_free, 8);
+    mbar_init(&p_full, 8);
+    mbar_init(&pv_done, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 8) {
+    tmem_alloc(&tmem_slot, Shape::COLUMNS);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  pdl_wait();      // barriers and tensor memory are set up; now q and the cache must be complete
+  const uint32_t tmem = tmem_slot;
+  // instruction descriptors: float accumulate, bfloat16 operands, both K-major, M = 128; N = 128 keys, N = HD
+  constexpr uint32_t IDESC = (1u << 4) | (1u << 7) | (1u << 10) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
+  constexpr uint32_t IDESC_PV = (1u << 4) | (1u << 7) | (1u << 10) | (((uint32_t)HD >> 3) << 17) | ((128u >> 4) << 24);
+  bool ok = true;
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Shape::REGS_OTHER));
+    if (warp == 8) {
+      // ---- TMA producer ----
+      if (lane == 0) {
+        mbar_expect_tx(&q_full, G * HALVES * TP * 128);
+        for (int g = 0; g < G; g++)
+          for (int h = 0; h < HALVES; h++)
+            tma_load_2d(sq + h * (128 * 128) + g * (TP * 128), &map_q, &q_full, (h0 + g) * HD + h * 64, (int)m_base);
+        auto page_of = [&](int v) { return v < n_pages ? max(table[v < nf ? v : jb0 + v - nf], 0) : -1; };   // (a page given back: every key of it is masked)
+        int p0 = page_of(0), p1 = page_of(1);
+        for (int i = 0; i < n_it; i++) {
+          const int s = i % NS, a = p0, c = p1;
+          p0 = page_of(2 * i + 2), p1 = page_of(2 * i + 3);      // asked for before the waits below
+          const uint32_t bytes = c >= 0 ? KV_BYTES : KV_BYTES / 2;
+          if (!mbar_wait(&k_empty[s], ((i / NS) & 1) ^ 1, abort_flag)) { atomicExch(status, 31); break; }
+          mbar_expect_tx(&k_full[s], bytes);
+          for (int h = 0; h < HALVES; h++) {
+            tma_load_2d(sk + s * KV_BYTES + h * (128 * 128), &map_k, &k_full[s], h * 64, (a * nkv + kvh) * PAGE);
+            if (c >= 0) tma_load_2d(sk + s * KV_BYTES + h * (128 * 128) + 64 * 128, &map_k, &k_full[s], h * 64, (c * nkv + kvh) * PAGE);
+          }
+          if (!mbar_wait(&v_empty[s], ((i / NS) & 1) ^ 1, abort_flag)) { atomicExch(status, 32); break; }
+          mbar_expect_tx(&v_full[s], bytes);
+          tma_load_2d(sv + s * KV_BYTES, &map_v, &v_full[s], 0, (a * nkv + kvh) * HD);
+          if (c >= 0) tma_load_2d(sv + s * KV_BYTES + HD * 128, &map_v, &v_full[s], 0, (c * nkv + kvh) * HD);
+        }
+      }
+    } else if (warp == 9) {
+      // ---- MMA issuer: the whole warp walks the loop, one lane issues ----
+      const int n = __shfl_sync(0xffffffffu, n_it, 0), odd = __shfl_sync(0xffffffffu, n_pages & 1, 0);
+      const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+      const uint64_t q_desc = make_desc(smem_u32(sq)), k_desc = make_desc(smem_u32(sk)), v_desc = make_desc(smem_u32(sv));
+      auto arrived = [&](uint64_t* bar, uint32_t parity, int code) -> bool {
+        const bool in = mbar_wait_warp(bar, parity, abort_flag);
+        if (!in && lane == 0) atomicExch(status, code);
+        return in;
+      };
+      auto scores = [&](int i) -> bool {
+        const int s = i % NS;
+        if (!arrived(&k_full[s], (i / NS) & 1, 33)) return false;
+        tc_fence_after();
+        if (elect_lane()) {
+#pragma unroll
+          for (int kk = 0; kk < HD / 16; kk++)
+            umma_bf16(tm + COL_S, q_desc + (kk >> 2) * 1024 + (kk & 3) * 2, k_desc + s * (KV_BYTES / 16) + (kk >> 2) * 1024 + (kk & 3) * 2, IDESC, kk > 0);
+          umma_commit(&k_empty[s]);
+          umma_commit(&s_full);
+        }
+        __syncwarp();
+        return true;
+      };
+      ok = arrived(&q_full, 0, 34) && scores(0);
+      for (int i = 0; i < n && ok; i++) {
+        const int s = i % NS, steps = i == n - 1 && odd ? 4 : 8;
+        // P beside S: the next scores wait until every softmax warp holds its rows of these
+        if (OWN_P && i + 1 < n && !(arrived(&s_free, i & 1, 35) && scores(i + 1))) break;
+        if (!arrived(&v_full[s], (i / NS) & 1, 36) || !arrived(&p_full, i & 1, 37)) break;
+        tc_fence_after();
+        if (elect_lane()) {
+          for (int kk = 0; kk < steps; kk++)
+            umma_bf16_ts(tm + COL_O, tm + COL_P + kk * 8, v_desc + s * (KV_BYTES / 16) + (kk >> 2) * (HD * 128 / 16) + (kk & 3) * 2, IDESC_PV, (i > 0 || kk > 0));
+          umma_commit(&v_empty[s]);
+          umma_commit(&pv_done);
+        }
+        __syncwarp();
+        // P over S: the tensor pipe runs the product that reads it before the one that overwrites it
+        if (!OWN_P && i + 1 < n && !scores(i + 1)) break;
+      }
+    }
+  } else {
+    // ---- softmax: two threads own row r = (head r / TP, position r % TP), `half` 0 the first page of an iteration, 1 the second ----
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Shape::REGS_SOFTMAX));
+    const int half = warp >> 2, r = threadIdx.x & 127, g = r / TP, pi = r % TP;
+    const bool row_valid = g < G && pi < rows;
+    const int qpos = q_lo + pi;
+    const int key_lo_row = first_key(qpos, window, chunk);
+    const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t t_s = tmem + COL_S + half * 64 + lane_base, t_p = tmem + COL_P + half * 32 + lane_base;
+    const uint32_t t_o = tmem + COL_O + half * (HD / 2) + lane_base;      // the half of a row of O that this thread rescales and stores
+    const float scale2 = scale * 1.4426950408889634f;
+    // With slopes the scores are finished (scaled, less slope (qpos - key), times log2 e) as they come out of tensor memory,
+    // and what follows multiplies them by one.
+    const float slope2 = slopes && g < G ? slopes[h0 + g] * 1.4426950408889634f : 0.f;
+    const float scale_after = slopes ? 1.f : scale2;
+    float m_used = AST_NEG, l = 0.f;
+    // The two warps of 32 rows meet once an iteration.  One that leaves the loop early has to let the other go.
+    auto meet = [&]() { asm volatile("bar.sync %0, 64;" ::"r"(1 + (warp & 3)) : "memory"); };
+    // Pages that every row of the tile reads whole need no look at single keys: those that end at or before the tile's first
+    // row and begin at or behind the last row's window, or hold first positions only.  (Idle rows read what comes: they are never written.)
+    const int lo_last = first_key(key_hi - 1, window, chunk);
+    for (int i = 0; i < n_it; i++) {
+      const int s = i % NS, vp = 2 * i + half, key0 = (vp < nf ? vp : jb0 + vp - nf) * PAGE;
+      const bool there = vp < n_pages;
+      const bool whole = there && key0 + PAGE - 1 <= q_lo && (key0 >= lo_last || key0 + PAGE <= first);
+      if (!mbar_wait_warp(&s_full, i & 1, abort_flag)) { atomicExch(status, 38); ok = false; break; }
+      tc_fence_after();
+      uint32_t v[PAGE];
+      tmem_ld32(t_s, v);
+      tmem_ld32(t_s + 32, v + 32);
+      tmem_ld_wait();
+      if (OWN_P) {      // the next scores may come
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s_free);
+      }
+      if (slopes) {
+        const float at0 = slope2 * (float)(key0 - qpos);
+#pragma unroll
+        for (int c = 0; c < PAGE; c++) v[c] = __float_as_uint(fmaf(__uint_as_float(v[c]), scale2, fmaf(slope2, (float)c, at0)));
+      }
+      if (!whole) {
+        // columns [0, c_first) and [c_lo, c_end) of this page are keys this row reads
+        const int c_lo = key_lo_row - key0, c_first = first - key0, c_end = there ? qpos - key0 + 1 : 0;
+#pragma unroll
+        for (int h = 0; h < PAGE; h += 32) {
+          const uint32_t seen = (ast_below(c_first - h) | ~ast_below(c_lo - h)) & ast_below(c_end - h);
+#pragma unroll
+          for (int c = 0; c < 32; c++)
+            if (!(seen & (1u << c))) v[h + c] = __float_as_uint(AST_NEG);
+        }
+        // value columns that no row of the tile reads become zero before the product reads them, whatever they hold: those between
+        // the first positions and the tile's window, and those beyond the last row
+        if (there && ((key_lo > key0 && c_first < min(key_lo - key0, PAGE)) || key_hi < key0 + PAGE)) {
+          if (!mbar_wait_warp(&v_full[s], (i / NS) & 1, abort_flag)) { atomicExch(status, 39); ok = false; break; }
+          if (r < HD) {
+            uint8_t* vrow = sv + s * KV_BYTES + half * (HD * 128) + r * 128;   // dimension r: 64 positions, 16-byte pieces swizzled by r & 7
+#pragma unroll 1
+            for (int e = 0; e < 8; e++) {
+              const int at = 8 * e;
+              const uint32_t keep = (ast_below(c_first - at) | ~ast_below(key_lo - key0 - at)) & ast_below(key_hi - key0 - at) & 255u;
+              uint4* piece = reinterpret_cast<uint4*>(vrow + ((e ^ (r & 7)) << 4));
+              if (keep == 255u) continue;
+              uint4 x = make_uint4(0, 0, 0, 0);
+              if (keep) {
+                auto pair = [&](uint32_t w, int j) { return w & ((keep >> j & 1 ? 0xffffu : 0u) | (keep >> (j + 1) & 1 ? 0xffff0000u : 0u)); };
+                x = *piece;
+                x = make_uint4(pair(x.x, 0), pair(x.y, 2), pair(x.z, 4), pair(x.w, 6));
+              }
+              *piece = x;
+            }
+          }
+          fence_proxy_async_smem();
+        }
+      }
+      float rm[2] = {AST_NEG, AST_NEG};
+#pragma unroll
+      for (int c = 0; c < PAGE; c += 4)
+#pragma unroll
+        for (int e = 0; e < 2; e++) rm[e] = max3(rm[e], __uint_as_float(v[c + 2 * e]), __uint_as_float(v[c + 2 * e + 1]));
+      const float mine = fmaxf(rm[0], rm[1]);
+      row_s[i & 1][half][r] = mine;
+      meet();      // (with P over S: from here on both have their scores in registers)
+      const float top = fmaxf(mine, row_s[i & 1][half ^ 1][r]);
+      // maxima are kept times scale * log2(e); a row with no key in these pages keeps what it had
+      const float m_new = top > 0.5f * AST_NEG ? fmaxf(m_used, top * scale_after) : m_used;
+      bool move = false;
+      if (m_used < 0.5f * AST_NEG) m_used = m_new;  // nothing accumulated for this row yet: O's row is zero
+      else if (m_new > m_used + 8.f) move = true;   // the reference maximum has to follow
+      // P beside S: the last one has to have been read, and O to hold the pages before these; P over S: that product came before these scores
+      if (OWN_P && i > 0 && !mbar_wait_warp(&pv_done, (i - 1) & 1, abort_flag)) { atomicExch(status, 40); ok = false; break; }
+      if (__any_sync(0xffffffffu, move)) {
+        tc_fence_after();
+        const float f = move ? ex2(m_used - m_new) : 1.f;
+#pragma unroll 1
+        for (int hcol = 0; hcol < HD / 2; hcol += 16) {
+          uint32_t o[16];
+          tmem_ld16(t_o + hcol, o);
+          tmem_ld_wait();
+#pragma unroll
+          for (int c = 0; c < 16; c++) o[c] = __float_as_uint(__uint_as_float(o[c]) * f);
+          tmem_st16(t_o + hcol, o);
+        }
+        l *= f;
+        if (move) m_used = m_new;
+      }
+      const float m_ref = m_used > 0.5f * AST_NEG ? m_used : 0.f;
+      const uint64_t scale_pair = f2(scale_after, scale_after), ref_pair = f2(-m_ref, -m_ref);
+      uint64_t ps[2] = {f2(0.f, 0.f), f2(0.f, 0.f)};
+#pragma unroll
+      for (int c0 = 0; c0 < PAGE; c0 += 32) {
+        uint32_t pk[16];
+#pragma unroll
+        for (int c = 0; c < 32; c += 2) {
+          // a masked score is -1e30: 2^(that * scale - m_ref) is exactly zero
+          const float2 x = halves(fma_f2(f2(__uint_as_float(v[c0 + c]), __uint_as_float(v[c0 + c + 1])), scale_pair, ref_pair));
+          const float p0 = ex2(x.x), p1 = ex2(x.y);
+          ps[(c >> 1) & 1] = add_f2(ps[(c >> 1) & 1], f2(p0, p1));
+          __nv_bfloat162 pp = __floats2bfloat162_rn(p0, p1);
+          pk[c >> 1] = *reinterpret_cast<uint32_t*>(&pp);
+        }
+        tmem_st16(t_p + c0 / 2, pk);
+      }
+      tmem_st_wait();
+      const float2 sums = halves(add_f2(ps[0], ps[1]));
+      l += sums.x + sums.y;
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&p_full);   // one arrival per softmax warp
+    }
+    if (ok && !mbar_wait_warp(&pv_done, (n_it - 1) & 1, abort_flag)) { atomicExch(status, 41); ok = false; }
+    if (!ok) {
+      asm volatile("bar.arrive %0, 64;" ::"r"(1 + (warp & 3)) : "memory");
+    } else {
+      row_s[n_it & 1][half][r] = l;
+      meet();
+      l += row_s[n_it & 1][half ^ 1][r];
+      tc_fence_after();
+      float inv = l > 0.f ? 1.0f / l : 0.f;
+      if (sinks && row_valid) inv = sink_quotient(m_used * 0.6931471805599453f, l, sinks[h0 + g]);
+      if (gate && !gate_elem && row_valid) inv *= head_gate(gate, m_base + pi, gate_stride, h0 + g, 0, HD, 0);
+#pragma unroll
+      for (int d0 = 0; d0 < HD / 2; d0 += 32) {
+        __syncwarp();      // idle rows left the branch below early: the loads take the whole warp
+        uint32_t o[32];
+        tmem_ld32(t_o + d0, o);
+        tmem_ld_wait();
+        if (row_valid) {
+          const int d = half * (HD / 2) + d0;
+          uint4* orow = reinterpret_cast<uint4*>(out + ((m_base + pi) * nh + h0 + g) * HD + d);
+#pragma unroll
+          for (int c = 0; c < 32; c++) {
+            float x = __uint_as_float(o[c]) * inv;
+            if (gate && gate_elem) x *= head_gate(gate, m_base + pi, gate_stride, h0 + g, d + c, HD, 1);
+            o[c] = __float_as_uint(x);
+          }
+#pragma unroll
+          for (int c = 0; c < 32; c += 8) {
+            uint32_t w[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+              __nv_bfloat162 pp = __floats2bfloat162_rn(__uint_as_float(o[c + 2 * e]), __uint_as_float(o[c + 2 * e + 1]));
+              w[e] = *reinterpret_cast<uint32_t*>(&pp);
+            }
+            orow[c / 8] = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 8) tmem_dealloc(tmem, Shape::COLUMNS);
+}
+
+// Positions of a tile: as many as fit 128 rows with all heads of a kv head, in eights (a head's rows start on a group of eight
+// rows of the swizzled tile).
+static int ast_positions(int G) { return (128 / G) & ~7; }
+
+// Returns 1 when the sizes are ones this kernel takes.
+LEB_API int leb_attention_stream_tc_supported(int nh, int nkv, int hd, int page_size) {
+  return (hd == 64 || hd == 128) && page_size == 64 && nkv > 0 && nh % nkv == 0 && nh / nkv <= 16;
+}
+
+template <int HD>
+static int launch_attention_stream_tc(void* out, const void* q, int q_stride, int M, const void* k_pool, const void* v_pool, int n_pages,
+                                      const int* block_table, int bt_width, const int* seq_slot, const int* seq_pos0,
+                                      const int* seq_qstart, const int* seq_qlen, const void* gate, int gate_stride, int gate_elem,
+                                      int B, int nh, int nkv, int window, int chunk, int first, float scale, const float* slopes,
+                                      const float* sinks, int max_qlen, int* status, cudaStream_t st) {
+  using Shape = AstShape<HD>;
+  const int G = nh / nkv, TP = ast_positions(G);
+  CUtensorMap mq, mk, mv;
+  if (tensor_map(&mq, q, M, nh * HD, q_stride, TP)) return 1;
+  if (tensor_map(&mk, k_pool, n_pages * nkv * 64, HD, HD, 64)) return 1;
+  if (tensor_map(&mv, v_pool, n_pages * nkv * HD, 64, 64, HD)) return 1;
+  dim3 grid(nkv, B, ceil_div(max_qlen, TP));
+  LEB_REQUIRE(grid.y <= 65535 && grid.z <= 65535, "leb_attention_stream_tc: grid too large (%u, %u)", grid.y, grid.z);
+  constexpr auto kern = attention_stream_tc_kernel<HD>;
+  // The warpgroups share out the registers of the launch: with fewer than REGS a thread they would wait for ever.
+  static std::atomic<int> regs{0};
+  if (regs.load(std::memory_order_relaxed) == 0) {
+    cudaFuncAttributes a;
+    if (cudaFuncGetAttributes(&a, kern) != cudaSuccess) return leb_fail("leb_attention_stream_tc: no attributes of the kernel");
+    regs.store(a.numRegs, std::memory_order_relaxed);
+  }
+  LEB_REQUIRE(regs.load(std::memory_order_relaxed) >= Shape::REGS, "leb_attention_stream_tc: built with %d registers a thread, %d are shared out",
+              regs.load(std::memory_order_relaxed), Shape::REGS);
+  const cudaError_t e = leb_allow_smem<kern, Shape::SMEM>();
+  if (e != cudaSuccess) return leb_fail("leb_attention_stream_tc: shared memory %d: %s", Shape::SMEM, cudaGetErrorString(e));
+  leb_launch(kern, grid, dim3(Shape::THREADS), Shape::SMEM, st, mq, mk, mv, (bf16*)out, block_table, bt_width, seq_slot, seq_pos0, seq_qstart,
+             seq_qlen, (const bf16*)gate, gate_stride, gate_elem, nh, nkv, G, TP, window, chunk, first, scale, slopes, sinks, status);
+  LEB_CHECK_LAUNCH("leb_attention_stream_tc");
+  return 0;
+}
+
+// Prompt attention of the step's rows over the paged cache (which already holds their keys and values).  q: [M, nh*hd] with row
+// stride q_stride; k_pool [n_pages][nkv][64][hd], v_pool [n_pages][nkv][hd][64]; out [M, nh*hd].  status: device int, set non-zero by a
+// block whose bounded wait gave up.  slopes, sinks [nh] or null as in leb_attention.
+LEB_API int leb_attention_stream_tc(void* out, const void* q, int q_stride, int M, const void* k_pool, const void* v_pool, int n_pages,
+                                    const int* block_table, int bt_width, const int* seq_slot, const int* seq_pos0,
+                                    const int* seq_qstart, const int* seq_qlen, const void* gate, int gate_stride, int gate_elem, int B,
+                                    int nh, int nkv, int hd, int page_size, int window, int chunk, int first, float scale,
+                                    const float* slopes, const float* sinks, int max_qlen, int* status, cudaStream_t st) {
+  if (B <= 0 || max_qlen <= 0 || M <= 0) return 0;
+  LEB_REQUIRE(leb_attention_stream_tc_supported(nh, nkv, hd, page_size),
+              "leb_attention_stream_tc: sizes not taken (heads %d, kv heads %d, head_dim %d, page %d)", nh, nkv, hd, page_size);
+  LEB_REQUIRE(status != nullptr, "leb_attention_stream_tc: a status word is required");
+  LEB_REQUIRE(((uintptr_t)q & 15) == 0 && q_stride % 8 == 0 && ((uintptr_t)out & 15) == 0,
+              "leb_attention_stream_tc: q and out must be 16-byte aligned, q's row stride a multiple of 8");
+#define LEB_AST_ARGS out, q, q_stride, M, k_pool, v_pool, n_pages, block_table, bt_width, seq_slot, seq_pos0, seq_qstart, seq_qlen, gate, \
+                     gate_stride, gate_elem, B, nh, nkv, window, chunk, first, scale, slopes, sinks, max_qlen, status, st
+  return hd == 64 ? launch_attention_stream_tc<64>(LEB_AST_ARGS) : launch_attention_stream_tc<128>(LEB_AST_ARGS);
+#undef LEB_AST_ARGS
+}
