@@ -1814,16 +1814,20 @@ def _attention_decode_raw(out, raw: RawQKV, k_pool, v_pool, block_table, batch, 
 
 
 # ----------------------------------------------------------------------------------------------
-def _words(name: str, **tensors: torch.Tensor) -> None:
-    for what, t in tensors.items():
-        _cuda(t, f"{name}.{what}", torch.int32)
+def _words(name: str, *tensors: torch.Tensor) -> None:
+    for t in tensors:
+        if t.dtype is not torch.int32 or not t.is_cuda or not t.is_contiguous():
+            raise KernelError(f"{name}: contiguous int32 tensors on a CUDA device, got {t.dtype} {tuple(t.shape)} on {t.device}")
 
 
-def _stream_state(name: str, lens: torch.Tensor, pages: torch.Tensor, free: torch.Tensor, counts: torch.Tensor, page_size: int) -> None:
-    if pages.dim() != 2 or pages.shape[0] != lens.numel() or counts.numel() != 2 or lens.numel() < 1 or pages.shape[1] < 1:
-        raise KernelError(f"{name}: page lists {tuple(pages.shape)} of {lens.numel()} slots, {counts.numel()} counts (2)")
-    if page_size < 1 or free.numel() * page_size > 2 ** 31:
-        raise KernelError(f"{name}: {free.numel()} pages of {page_size} positions (2^31 positions at most)")
+def _stream_state(name: str, lens: torch.Tensor, pages: torch.Tensor, free: torch.Tensor, counts: torch.Tensor, page_size: int) -> tuple[int, int, int]:
+    """(slots, places of a page list, pages) of a stream cache's state."""
+    n_slots, n_pages, shape = lens.numel(), free.numel(), pages.shape
+    if len(shape) != 2 or shape[0] != n_slots or counts.numel() != 2 or n_slots < 1 or shape[1] < 1:
+        raise KernelError(f"{name}: page lists {tuple(shape)} of {n_slots} slots, {counts.numel()} counts (2)")
+    if page_size < 1 or n_pages * page_size > 2 ** 31:
+        raise KernelError(f"{name}: {n_pages} pages of {page_size} positions (2^31 positions at most)")
+    return n_slots, shape[1], n_pages
 
 
 def stream_tables(table: torch.Tensor, slot_map: torch.Tensor, row_seq: torch.Tensor, row_pos: torch.Tensor, step_slot: torch.Tensor,
@@ -1842,17 +1846,16 @@ def stream_tables(table: torch.Tensor, slot_map: torch.Tensor, row_seq: torch.Te
     sequences are padding without rows.  Every slot may be named once.
     (Kernels may read a step's tables ahead of the wait for the kernel launched before: `stream_advance`, a copy or a
     graph's launch lies between this call and them.)"""
-    _words("stream_tables", table=table, slot_map=slot_map, row_seq=row_seq, row_pos=row_pos, step_slot=step_slot, step_qlen=step_qlen,
-           pos0=pos0, qstart=qstart, seq_slot=seq_slot, seq_qlen=seq_qlen, lens=lens, pages=pages, free=free, counts=counts)
-    _stream_state("stream_tables", lens, pages, free, counts, page_size)
-    B, M = seq_slot.numel(), slot_map.numel()
-    if table.dim() != 2 or table.shape[0] != B or table.shape[1] < 1 or row_seq.numel() != M or row_pos.numel() != M \
-            or any(t.numel() != B for t in (seq_qlen, step_slot, step_qlen, pos0, qstart)):
+    _words("stream_tables", table, slot_map, row_seq, row_pos, step_slot, step_qlen, pos0, qstart, seq_slot, seq_qlen, lens, pages, free, counts)
+    n_slots, width, n_pages = _stream_state("stream_tables", lens, pages, free, counts, page_size)
+    B, M, shape = seq_slot.numel(), slot_map.numel(), table.shape
+    if (len(shape) != 2 or shape[0] != B or shape[1] < 1 or row_seq.numel() != M or row_pos.numel() != M or seq_qlen.numel() != B
+            or step_slot.numel() != B or step_qlen.numel() != B or pos0.numel() != B or qstart.numel() != B):
         raise KernelError(f"stream_tables: outputs do not fit {B} sequences and {M} rows")
     _check(lib().leb_stream_tables(
-        _ptr(table), table.shape[1], _ptr(slot_map), _ptr(row_seq), _ptr(row_pos), _ptr(step_slot), _ptr(step_qlen), _ptr(pos0),
-        _ptr(qstart), _ptr(seq_slot), _ptr(seq_qlen), _ptr(lens), lens.numel(), _ptr(pages), pages.shape[1], _ptr(free), free.numel(),
-        _ptr(counts), M, B, page_size, _stream()))
+        table.data_ptr(), shape[1], slot_map.data_ptr(), row_seq.data_ptr(), row_pos.data_ptr(), step_slot.data_ptr(), step_qlen.data_ptr(),
+        pos0.data_ptr(), qstart.data_ptr(), seq_slot.data_ptr(), seq_qlen.data_ptr(), lens.data_ptr(), n_slots, pages.data_ptr(), width,
+        free.data_ptr(), n_pages, counts.data_ptr(), M, B, page_size, _stream()))
 
 
 def stream_advance(seq_slot: torch.Tensor, seq_qlen: torch.Tensor, lens: torch.Tensor, kept: torch.Tensor, pages: torch.Tensor,
@@ -1862,24 +1865,24 @@ def stream_advance(seq_slot: torch.Tensor, seq_qlen: torch.Tensor, lens: torch.T
     Takes the step's `step_slot` and `step_qlen` (a refused step then changes nothing).  `kept` [slots]: a sequence's first
     page, behind those of its first positions, that is still held (at the start: ceil(first / page_size)).
     May be called before the step's kernels are: what goes back is given out by the next step's tables at the earliest."""
-    _words("stream_advance", seq_slot=seq_slot, seq_qlen=seq_qlen, lens=lens, kept=kept, pages=pages, free=free, counts=counts)
-    _stream_state("stream_advance", lens, pages, free, counts, page_size)
+    _words("stream_advance", seq_slot, seq_qlen, lens, kept, pages, free, counts)
+    n_slots, width, n_pages = _stream_state("stream_advance", lens, pages, free, counts, page_size)
     if seq_slot.numel() != seq_qlen.numel() or kept.numel() != lens.numel() or window < 0 or first < 0:
         raise KernelError(f"stream_advance: {seq_slot.numel()} slots and {seq_qlen.numel()} row counts, window {window}, first {first}")
     _check(lib().leb_stream_advance(
-        _ptr(seq_slot), _ptr(seq_qlen), _ptr(lens), lens.numel(), _ptr(kept), _ptr(pages), pages.shape[1], _ptr(free), free.numel(),
-        _ptr(counts), seq_slot.numel(), page_size, window, first, _stream()))
+        seq_slot.data_ptr(), seq_qlen.data_ptr(), lens.data_ptr(), n_slots, kept.data_ptr(), pages.data_ptr(), width, free.data_ptr(), n_pages,
+        counts.data_ptr(), seq_slot.numel(), page_size, window, first, _stream()))
 
 
 def stream_release(seq_slot: torch.Tensor, lens: torch.Tensor, kept: torch.Tensor, pages: torch.Tensor, free: torch.Tensor,
                    counts: torch.Tensor, page_size: int, first: int = 0) -> None:
     """The sequences in `seq_slot` (each named once; -1: none) end: their pages go back on the stack, their lengths are 0."""
-    _words("stream_release", seq_slot=seq_slot, lens=lens, kept=kept, pages=pages, free=free, counts=counts)
-    _stream_state("stream_release", lens, pages, free, counts, page_size)
+    _words("stream_release", seq_slot, lens, kept, pages, free, counts)
+    n_slots, width, n_pages = _stream_state("stream_release", lens, pages, free, counts, page_size)
     if kept.numel() != lens.numel() or first < 0:
         raise KernelError(f"stream_release: {kept.numel()} of {lens.numel()} slots, first {first}")
-    _check(lib().leb_stream_release(_ptr(seq_slot), _ptr(lens), lens.numel(), _ptr(kept), _ptr(pages), pages.shape[1], _ptr(free),
-                                    free.numel(), _ptr(counts), seq_slot.numel(), page_size, first, _stream()))
+    _check(lib().leb_stream_release(seq_slot.data_ptr(), lens.data_ptr(), n_slots, kept.data_ptr(), pages.data_ptr(), width,
+                                    free.data_ptr(), n_pages, counts.data_ptr(), seq_slot.numel(), page_size, first, _stream()))
 
 
 def store_rows(k_pool: torch.Tensor, v_pool: torch.Tensor, k: torch.Tensor, v: torch.Tensor, slot_map: torch.Tensor) -> None:
