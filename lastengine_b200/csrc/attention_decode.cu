@@ -162,9 +162,23 @@ __device__ __forceinline__ void atd_prep_head(const bf16* __restrict__ src, cons
   for (int e = 0; e < EPL; e++) dst[lane + 32 * e] = __float2bfloat16_rn(x[e] * factor);
 }
 
+// All threads of the cluster's blocks; what they wrote to their shared memory is visible to the others.
+__device__ __forceinline__ void atd_cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+}
+// The number at this address of block `rank`'s shared memory.
+__device__ __forceinline__ float atd_remote(const float* p, int rank) {
+  uint32_t a;
+  float v;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(rank));
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
+  return v;
+}
+
 // HD: head_dim, a multiple of 32; S: stages of a warp's ring; WIDE: the softmax weights enter the second product as two
 // bfloat16 terms, p = hi + lo (16 significant bits; the row sum is of the float p either way); FIRST: the row also reads the
-// sequence's first `first` positions, whose blocks come before the window's in the walk (first_tiles in common.cuh)
+// sequence's first `first` positions, whose blocks come before the window's in the walk (first_tiles in common.cuh), and without
+// `part` the splits of a sequence are a cluster of blocks, which join their sums through shared memory instead of a second kernel
 template <int HD, int S, bool WIDE, bool FIRST>
 __global__ void __launch_bounds__(32 * ATD_WARPS)
 attention_decode_kernel(bf16* __restrict__ out, float* __restrict__ part, const bf16* __restrict__ q,
@@ -196,8 +210,9 @@ attention_decode_kernel(bf16* __restrict__ out, float* __restrict__ part, const 
   pdl_trigger();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int r = lane >> 2, c = lane & 3;
-  const int kvh = blockIdx.x, b = blockIdx.y, split = blockIdx.z;
+  const int kvh = blockIdx.x, b = blockIdx.y, split = blockIdx.z;      // (of a cluster's blocks `split` is the rank)
   const int G = nh / nkv;
+  const bool joined = FIRST && n_splits > 1 && !part, partial_out = n_splits > 1 && !joined;
   const int slot = seq_slot[b];
   const size_t m_row = seq_qstart[b];
   const int h0 = kvh * G;
@@ -213,12 +228,12 @@ attention_decode_kernel(bf16* __restrict__ out, float* __restrict__ part, const 
     pdl_wait();
     for (int idx = threadIdx.x; idx < G * HD; idx += blockDim.x) {
       int hh = idx / HD, d = idx % HD;
-      if (n_splits == 1)
+      if (!partial_out)
         out[(m_row * nh + h0 + hh) * HD + d] = __float2bfloat16_rn(0.f);
       else
         part[((m_row * nh + h0 + hh) * n_splits + split) * (size_t)(HD + 2) + 2 + d] = 0.f;
     }
-    if (n_splits > 1 && threadIdx.x < G) {
+    if (partial_out && threadIdx.x < G) {
       float* pp = part + ((m_row * nh + h0 + threadIdx.x) * n_splits + split) * (size_t)(HD + 2);
       pp[0] = ATD_NEG;
       pp[1] = 0.f;
@@ -471,6 +486,9 @@ attention_decode_kernel(bf16* __restrict__ out, float* __restrict__ part, const 
     l_s[warp][r + 8] = l[1];
   }
   __syncthreads();
+  // (FIRST, several splits) this block's rows, for the cluster's blocks to read: [head][HD], then maxima and sums
+  float* const mine = reinterpret_cast<float*>(l_s + ATD_WARPS);
+  static_assert(sizeof(float) * (ATD_WARPS * 16 * (HD + 4 + 2) + 16 * (HD + 2)) <= (size_t)ATD_WARPS * S * STAGE, "results must fit the rings");
   for (int idx = threadIdx.x; idx < G * HD; idx += blockDim.x) {
     const int hh = idx / HD, d = idx % HD;
     float M = ATD_NEG;
@@ -484,7 +502,10 @@ attention_decode_kernel(bf16* __restrict__ out, float* __restrict__ part, const 
       a += o_s[w][hh][d] * f;
     }
     const int h = h0 + hh;
-    if (n_splits == 1) {
+    if (joined) {
+      mine[idx] = a;
+      if (d == 0) mine[16 * HD + hh] = M, mine[16 * HD + 16 + hh] = L;
+    } else if (n_splits == 1) {
       float g = 1.f;
       if (gate) g = head_gate(gate, m_row, gate_stride, h, d, HD, gate_elem);
       const float o = sinks ? a * sink_quotient(M * 0.6931471805599453f, L, sinks[h]) : (L > 0.f ? a / L : 0.f);
@@ -495,6 +516,43 @@ attention_decode_kernel(bf16* __restrict__ out, float* __restrict__ part, const 
       pp[2 + d] = a;
     }
   }
+  if (joined) {
+    atd_cluster_sync();
+    const int share = (G * HD + n_splits - 1) / n_splits, end = min(G * HD, (split + 1) * share);
+    for (int idx = split * share + threadIdx.x; idx < end; idx += blockDim.x) {
+      const int hh = idx / HD, d = idx % HD, h = h0 + hh;
+      float M = ATD_NEG, L = 0.f, a = 0.f;
+      for (int s0 = 0; s0 < n_splits; s0 += 8) {      // eight blocks' numbers are asked for together
+        float ms[8], ls[8], as[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+          const int rank = min(s0 + j, n_splits - 1);
+          ms[j] = atd_remote(mine + 16 * HD + hh, rank);
+          ls[j] = atd_remote(mine + 16 * HD + 16 + hh, rank);
+          as[j] = atd_remote(mine + idx, rank);
+        }
+        float cm = M;
+#pragma unroll
+        for (int j = 0; j < 8; j++)
+          if (s0 + j < n_splits) cm = fmaxf(cm, ms[j]);
+        const float f = exp2f(M - cm);
+        L *= f;
+        a *= f;
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+          const float e = s0 + j < n_splits ? exp2f(ms[j] - cm) : 0.f;
+          L += ls[j] * e;
+          a += as[j] * e;
+        }
+        M = cm;
+      }
+      float g = 1.f;
+      if (gate) g = head_gate(gate, m_row, gate_stride, h, d, HD, gate_elem);
+      const float o = sinks ? a * sink_quotient(M * 0.6931471805599453f, L, sinks[h]) : (L > 0.f ? a / L : 0.f);
+      out[(m_row * nh + h) * HD + d] = __float2bfloat16_rn(o * g);
+    }
+    atd_cluster_sync();      // no block ends while others read its memory
+  }
 }
 
 // Returns 1 when the sizes are ones this kernel takes (the caller then uses the general kernel).
@@ -502,6 +560,19 @@ LEB_API int leb_attention_decode_supported(int nh, int nkv, int hd, int page_siz
   if (nkv <= 0 || nh % nkv != 0 || nh / nkv > 16) return 0;
   if (hd != 32 && hd != 64 && hd != 96 && hd != 128) return 0;
   return page_size % 32 == 0;
+}
+
+// Blocks that share a sequence and kv head with first positions: as many as run at once, with `least` positions or more for each; a
+// portable cluster at most.
+static int atd_cluster_blocks(int B, int nkv, int G, int hd, int window, int chunk, int first, int max_kvlen) {
+  long long keys = window > 0 ? window : max_kvlen;
+  if (chunk > 0 && chunk < keys) keys = chunk;
+  keys = keys + first < max_kvlen ? keys + first : max_kvlen;
+  const long long per = (long long)B * nkv * ((G + 15) / 16);
+  const int stage = ATD_WARPS * ATD_STAGES(hd) * 2 * 32 * hd * 2, fit = 227 * 1024 / stage;
+  const long long slots = (long long)sm_count() * (fit < 1 ? 1 : fit > 3 ? 3 : fit), least = per * 8 <= sm_count() ? 128 : 256;
+  long long n = slots / per < keys / least ? slots / per : keys / least;
+  return (int)(n < 1 ? 1 : n > 8 ? 8 : n);
 }
 
 // The first stage of a decode step's attention: every sequence brings one row.  With
@@ -512,11 +583,17 @@ static int attention_decode_launch(void* out, float* part, const void* q, const 
                                    const int* seq_slot, const int* seq_pos0, const int* seq_qstart,
                                    const void* gate, int gate_stride, int gate_elem, int B, int nh, int nkv, int hd,
                                    int page_size, int window, int chunk, int first, int wide, float scale, const float* slopes,
-                                   const float* sinks, int n_splits, AtdPrep prep, cudaStream_t st) {
+                                   const float* sinks, int n_splits, int max_kvlen, int blocks, AtdPrep prep, cudaStream_t st) {
   if (B <= 0) return 0;
   LEB_REQUIRE(leb_attention_decode_supported(nh, nkv, hd, page_size),
               "leb_attention_decode: sizes not taken (heads %d, kv heads %d, head_dim %d, page %d)", nh, nkv, hd, page_size);
-  LEB_REQUIRE(n_splits >= 1 && (n_splits == 1 || part), "leb_attention_decode: splits need scratch");
+  // with first positions and without splits of the caller's: a cluster of as many blocks as suit the step, or of `blocks`
+  const bool joined = first > 0 && n_splits == 1;
+  if (joined) {
+    n_splits = blocks > 0 ? (blocks < 8 ? blocks : 8) : atd_cluster_blocks(B, nkv, nh / nkv, hd, window, chunk, first, max_kvlen);
+    part = nullptr;
+  }
+  LEB_REQUIRE(n_splits >= 1 && (n_splits == 1 || part || joined), "leb_attention_decode: splits need scratch");
   dim3 grid(nkv, B, n_splits);
   LEB_REQUIRE(grid.y <= 65535 && grid.z <= 65535, "leb_attention_decode: grid too large");
 #define LEB_ATD_F(HD_, S_, W_, F_)                                                                \
@@ -528,7 +605,7 @@ static int attention_decode_launch(void* out, float* part, const void* q, const 
         return leb_fail("leb_attention_decode: %d bytes of shared memory per block refused", smem); \
       set = true;                                                                                 \
     }                                                                                             \
-    leb_launch(attention_decode_kernel<HD_, S_, W_, F_>, grid, dim3(32 * ATD_WARPS), smem, st,             \
+    leb_launch_cluster(F_ && joined ? n_splits : 1, attention_decode_kernel<HD_, S_, W_, F_>, grid, dim3(32 * ATD_WARPS), smem, st, \
         (bf16*)out, part, (const bf16*)q, (const bf16*)k_pool, (const bf16*)v_pool, block_table,  \
         bt_width, seq_slot, seq_pos0, seq_qstart, (const bf16*)gate, gate_stride, gate_elem, nh, nkv, \
         page_size, window, chunk, first, scale, slopes, sinks, n_splits, prep);                   \
@@ -562,10 +639,10 @@ LEB_API int leb_attention_decode(void* out, float* part, const void* q, const vo
                                  const int* seq_slot, const int* seq_pos0, const int* seq_qstart,
                                  const void* gate, int gate_stride, int gate_elem, int B, int nh, int nkv, int hd,
                                  int page_size, int window, int chunk, int first, int wide, float scale, const float* slopes,
-                                 const float* sinks, int n_splits, cudaStream_t st) {
+                                 const float* sinks, int n_splits, int max_kvlen, int blocks, cudaStream_t st) {
   return attention_decode_launch(out, part, q, k_pool, v_pool, block_table, bt_width, seq_slot, seq_pos0, seq_qstart, gate,
                                  gate_stride, gate_elem, B, nh, nkv, hd, page_size, window, chunk, first, wide, scale, slopes, sinks,
-                                 n_splits, AtdPrep{}, st);
+                                 n_splits, max_kvlen, blocks, AtdPrep{}, st);
 }
 
 // Returns 1 when the kernel can norm, rotate and store the step's q, k and v itself: head size 64 or
@@ -585,7 +662,7 @@ LEB_API int leb_attention_decode_prep(void* out, float* part, const void* q_raw,
                                       const float* k_norm_w, float eps, const float* inv_freq, int rope_dim,
                                       int neox, int row_norm, const void* gate, int gate_stride, int gate_elem, int B, int nh, int nkv,
                                       int hd, int page_size, int window, int chunk, int first, int wide, float scale, const float* slopes,
-                                      const float* sinks, float temp_coef, float temp_every, int n_splits, cudaStream_t st) {
+                                      const float* sinks, float temp_coef, float temp_every, int n_splits, int max_kvlen, int blocks, cudaStream_t st) {
   LEB_REQUIRE(leb_attention_decode_prep_supported(nh, nkv, hd, page_size, rope_dim, neox),
               "leb_attention_decode_prep: sizes not taken (head_dim %d, rope_dim %d, split-half %d)", hd, rope_dim, neox);
   LEB_REQUIRE(q_raw && (inv_freq || rope_dim == 0), "leb_attention_decode_prep: q and the frequencies are required");
@@ -596,7 +673,7 @@ LEB_API int leb_attention_decode_prep(void* out, float* part, const void* q_raw,
                temp_every};
   return attention_decode_launch(out, part, nullptr, k_pool, v_pool, block_table, bt_width, seq_slot, seq_pos0, seq_qstart,
                                  gate, gate_stride, gate_elem, B, nh, nkv, hd, page_size, window, chunk, first, wide, scale, slopes, sinks,
-                                 n_splits, prep, st);
+                                 n_splits, max_kvlen, blocks, prep, st);
 }
 
 // ---- the same step for callers that cannot allocate (see leb_no_alloc.h) ---------------------------
@@ -641,7 +718,7 @@ LEB_API int leb_attention_decode_static(void* out, const void* q, const void* k_
   }
   int rc = leb_attention_decode(out, scratch, q, k_pool, v_pool, block_table, bt_width, seq_slot, seq_pos0,
                                 seq_qstart, gate, gate_stride, 0, B, nh, nkv, hd, page_size, window, 0, 0, 0, scale, nullptr, nullptr,
-                                n_splits, st);
+                                n_splits, 0, 0, st);
   if (rc) return rc;
   if (n_splits > 1)
     return leb_attention_merge(out, scratch, LEB_BF16, gate, gate_stride, 0, nullptr, B, nh, hd, n_splits, st);

@@ -529,12 +529,12 @@ LEB_API int leb_attention_prefill_tc(void* out, const void* q, int q_stride, int
 #define LEB_ATC_ARGS "leb_attention_prefill_tc", out, q, q_stride, M, k_pool, v_pool, n_pages, block_table, bt_width, nullptr, \
                      nullptr, 0, nullptr, 0, seq_slot, seq_pos0, seq_qstart, seq_qlen, gate, gate_stride, gate_elem, B, nh, nkv, \
                      hd, page_size, window, chunk, first, 0, scale, nullptr, nullptr, slopes, sinks, max_qlen, status, st
-#define LEB_ATC_FORM(FIRST)                                                                                                   \
-  (wide ? launch_attention_prefill_tc<false, true, true, 64, FIRST>(LEB_ATC_ARGS)                                             \
-        : atc_few_tiles(M, B, nh, nkv, max_qlen) ? launch_attention_prefill_tc<false, false, true, 64, FIRST>(LEB_ATC_ARGS)   \
-                                                 : launch_attention_prefill_tc<false, false, false, 64, FIRST>(LEB_ATC_ARGS))
-  return first > 0 ? LEB_ATC_FORM(true) : LEB_ATC_FORM(false);
-#undef LEB_ATC_FORM
+  // (with first positions only the weights of two terms come here: leb_attention_stream_tc takes the others)
+  LEB_REQUIRE(first <= 0 || wide, "leb_attention_prefill_tc: first positions with weights of one term");
+  if (wide) return first > 0 ? launch_attention_prefill_tc<false, true, true, 64, true>(LEB_ATC_ARGS)
+                             : launch_attention_prefill_tc<false, true, true, 64, false>(LEB_ATC_ARGS);
+  return atc_few_tiles(M, B, nh, nkv, max_qlen) ? launch_attention_prefill_tc<false, false, true, 64, false>(LEB_ATC_ARGS)
+                                                : launch_attention_prefill_tc<false, false, false, 64, false>(LEB_ATC_ARGS);
 #undef LEB_ATC_ARGS
 }
 

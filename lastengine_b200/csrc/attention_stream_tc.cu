@@ -11,6 +11,7 @@
 // Warps: eight for the softmax, one that brings Q and pages by TMA, one that issues the products, two that fill their warpgroup
 // (registers move between warpgroups).  Two blocks share an SM, so that one's products run under the other's exponentials, and a
 // scheduler has four softmax warps: what bounds the loop is the chain from a row's scores to its weights, not a pipe.
+// Where there are few tiles, a cluster of n_splits blocks shares the pages of one and joins its sums through shared memory.
 // With heads of 64, P has columns beside S and the next scores are issued as soon as a row of S is in registers; with heads of 128, O
 // takes those columns, P lies over S and the next scores follow the product that reads P.
 //
@@ -27,6 +28,7 @@
 #include "attention_tc.cuh"
 
 #define AST_NEG (-1e30f)
+#define AST_MOST_SPLITS 8      // blocks that share a tile's keys: a portable cluster
 
 template <int HD>
 struct AstShape {
@@ -42,17 +44,40 @@ struct AstShape {
   static constexpr int COLUMNS = 256;                                 // S, P and O
 };
 
+// All threads of the cluster's blocks; what they wrote to their shared memory is visible to the others.
+__device__ __forceinline__ void ast_cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+}
+// The number at this address of block `rank`'s shared memory.
+__device__ __forceinline__ uint32_t ast_map(const void* p, int rank) {
+  uint32_t a;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
+  return a;
+}
+__device__ __forceinline__ float ast_remote(const float* p, int rank) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(ast_map(p, rank)) : "memory");
+  return v;
+}
+__device__ __forceinline__ float4 ast_remote4(const float* p, int rank) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(ast_map(p, rank)) : "memory");
+  return v;
+}
+
 // The lowest n bits (none for n <= 0, all from 32 on).
 __device__ __forceinline__ uint32_t ast_below(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; }
 
-template <int HD>
+// SHARED: a cluster of n_splits blocks shares a tile's keys (else n_splits is 1).
+template <int HD, bool SHARED>
 __global__ void __launch_bounds__(AstShape<HD>::THREADS, 2)
 attention_stream_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                            const __grid_constant__ CUtensorMap map_v, bf16* __restrict__ out, const int* __restrict__ block_table,
                            int bt_width, const int* __restrict__ seq_slot, const int* __restrict__ seq_pos0,
                            const int* __restrict__ seq_qstart, const int* __restrict__ seq_qlen, const bf16* __restrict__ gate,
                            int gate_stride, int gate_elem, int nh, int nkv, int G, int TP, int window, int chunk, int first,
-                           float scale, const float* __restrict__ slopes, const float* __restrict__ sinks, int* __restrict__ status) {
+                           float scale, const float* __restrict__ slopes, const float* __restrict__ sinks, int n_blocks, int* __restrict__ status) {
+  const int n_splits = SHARED ? n_blocks : 1;
   using Shape = AstShape<HD>;
   constexpr int PAGE = 64, NS = Shape::STAGES, HALVES = HD / 64;
   constexpr int Q_BYTES = Shape::Q_BYTES, KV_BYTES = Shape::KV_BYTES;
@@ -65,6 +90,7 @@ attention_stream_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gr
   uint8_t* sv = sk + NS * KV_BYTES;           // [stage][page][dimension][64 positions]
   __shared__ uint64_t q_full, k_full[NS], v_full[NS], k_empty[NS], v_empty[NS], s_full, s_free, p_full, pv_done;
   __shared__ float row_s[2][2][128];          // what the two threads of a row tell each other: [iteration's parity][thread][row]
+  __shared__ float last_s[2][SHARED ? 128 : 1], join_s[AST_MOST_SPLITS][SHARED ? 64 : 1];      // maxima and sums of this block's rows; factors of the rows it joins
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_s;
   volatile int* abort_flag = &abort_s;
@@ -72,7 +98,7 @@ attention_stream_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gr
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   // kv heads, then sequences vary fastest; the tiles with the longest key range come first
   const int kvh = blockIdx.x, b = blockIdx.y;
-  const int row0 = (int)(gridDim.z - 1 - blockIdx.z) * TP;
+  const int split = blockIdx.z % n_splits, row0 = (int)(gridDim.z / n_splits - 1 - blockIdx.z / n_splits) * TP;
   const int qlen = seq_qlen[b];      // step data: written long before the kernel before this one
   if (row0 >= qlen) {
     pdl_wait();   // a kernel counts as complete when its blocks are: none may finish before its predecessor has
@@ -82,18 +108,21 @@ attention_stream_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gr
   const int pos0 = seq_pos0[b];
   const size_t m_base = (size_t)seq_qstart[b] + row0;
   const int h0 = kvh * G;
-  if (seq_slot[b] < 0) {   // a padding sequence: its rows are zero
+  const bool live = seq_slot[b] >= 0;
+  const int q_lo = pos0 + row0, key_hi = q_lo + rows;      // keys [.., key_hi) exist for the tile
+  const int key_lo = first_key(q_lo, window, chunk);
+  const int nf = first_tiles(first, key_lo, PAGE), jb0 = key_lo / PAGE;
+  const int n_pages = nf + (key_hi - 1) / PAGE - jb0 + 1, n_all = (n_pages + 1) / 2;
+  if (!live) {   // a padding sequence: its rows are zero
     pdl_wait();
-    for (int idx = threadIdx.x; idx < rows * G * (HD / 8); idx += blockDim.x) {
+    for (int idx = split * blockDim.x + threadIdx.x; idx < rows * G * (HD / 8); idx += n_splits * blockDim.x) {
       const int i = idx / (G * (HD / 8)), rest = idx % (G * (HD / 8));
       reinterpret_cast<uint4*>(out + ((m_base + i) * nh + h0) * HD)[rest] = make_uint4(0, 0, 0, 0);
     }
     return;
   }
-  const int q_lo = pos0 + row0, key_hi = q_lo + rows;      // keys [.., key_hi) exist for the tile
-  const int key_lo = first_key(q_lo, window, chunk);
-  const int nf = first_tiles(first, key_lo, PAGE), jb0 = key_lo / PAGE;
-  const int n_pages = nf + (key_hi - 1) / PAGE - jb0 + 1, n_it = (n_pages + 1) / 2;
+  // this block's share of the iterations (none for the last ones where they do not go round)
+  const int per_split = (n_all + n_splits - 1) / n_splits, it0 = split * per_split, n_it = max(0, min(n_all - it0, per_split));
   const int* table = block_table + (size_t)b * bt_width;
 
   if (threadIdx.x == 0) {
@@ -129,11 +158,11 @@ attention_stream_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gr
     if (warp == 8) {
       // ---- TMA producer ----
       if (lane == 0) {
-        mbar_expect_tx(&q_full, G * HALVES * TP * 128);
-        for (int g = 0; g < G; g++)
+        if (n_it > 0) mbar_expect_tx(&q_full, G * HALVES * TP * 128);
+        for (int g = 0; g < G && n_it > 0; g++)
           for (int h = 0; h < HALVES; h++)
             tma_load_2d(sq + h * (128 * 128) + g * (TP * 128), &map_q, &q_full, (h0 + g) * HD + h * 64, (int)m_base);
-        auto page_of = [&](int v) { return v < n_pages ? max(table[v < nf ? v : jb0 + v - nf], 0) : -1; };   // (a page given back: every key of it is masked)
+        auto page_of = [&](int v) { v += 2 * it0; return v < n_pages ? max(table[v < nf ? v : jb0 + v - nf], 0) : -1; };   // (a page given back: every key of it is masked)
         int p0 = page_of(0), p1 = page_of(1);
         for (int i = 0; i < n_it; i++) {
           const int s = i % NS, a = p0, c = p1;
@@ -153,7 +182,7 @@ attention_stream_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gr
       }
     } else if (warp == 9) {
       // ---- MMA issuer: the whole warp walks the loop, one lane issues ----
-      const int n = __shfl_sync(0xffffffffu, n_it, 0), odd = __shfl_sync(0xffffffffu, n_pages & 1, 0);
+      const int n = __shfl_sync(0xffffffffu, n_it, 0), odd = __shfl_sync(0xffffffffu, it0 + n_it == n_all ? n_pages & 1 : 0, 0);      // the sequence's last page may be alone
       const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
       const uint64_t q_desc = make_desc(smem_u32(sq)), k_desc = make_desc(smem_u32(sk)), v_desc = make_desc(smem_u32(sv));
       auto arrived = [&](uint64_t* bar, uint32_t parity, int code) -> bool {
@@ -175,7 +204,7 @@ attention_stream_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gr
         __syncwarp();
         return true;
       };
-      ok = arrived(&q_full, 0, 34) && scores(0);
+      ok = n > 0 && arrived(&q_full, 0, 34) && scores(0);
       for (int i = 0; i < n && ok; i++) {
         const int s = i % NS, steps = i == n - 1 && odd ? 4 : 8;
         // P beside S: the next scores wait until every softmax warp holds its rows of these
@@ -192,6 +221,10 @@ attention_stream_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gr
         // P over S: the tensor pipe runs the product that reads it before the one that overwrites it
         if (!OWN_P && i + 1 < n && !scores(i + 1)) break;
       }
+    }
+    if (SHARED) {
+      ast_cluster_sync();
+      ast_cluster_sync();
     }
   } else {
     // ---- softmax: two threads own row r = (head r / TP, position r % TP), `half` 0 the first page of an iteration, 1 the second ----
@@ -215,7 +248,7 @@ attention_stream_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gr
     // row and begin at or behind the last row's window, or hold first positions only.  (Idle rows read what comes: they are never written.)
     const int lo_last = first_key(key_hi - 1, window, chunk);
     for (int i = 0; i < n_it; i++) {
-      const int s = i % NS, vp = 2 * i + half, key0 = (vp < nf ? vp : jb0 + vp - nf) * PAGE;
+      const int s = i % NS, vp = 2 * (it0 + i) + half, key0 = (vp < nf ? vp : jb0 + vp - nf) * PAGE;
       const bool there = vp < n_pages;
       const bool whole = there && key0 + PAGE - 1 <= q_lo && (key0 >= lo_last || key0 + PAGE <= first);
       if (!mbar_wait_warp(&s_full, i & 1, abort_flag)) { atomicExch(status, 38); ok = false; break; }
@@ -323,44 +356,104 @@ attention_stream_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gr
       __syncwarp();
       if (lane == 0) mbar_arrive(&p_full);   // one arrival per softmax warp
     }
-    if (ok && !mbar_wait_warp(&pv_done, (n_it - 1) & 1, abort_flag)) { atomicExch(status, 41); ok = false; }
+    if (ok && n_it > 0 && !mbar_wait_warp(&pv_done, (n_it - 1) & 1, abort_flag)) { atomicExch(status, 41); ok = false; }
     if (!ok) {
       asm volatile("bar.arrive %0, 64;" ::"r"(1 + (warp & 3)) : "memory");
     } else {
       row_s[n_it & 1][half][r] = l;
       meet();
       l += row_s[n_it & 1][half ^ 1][r];
-      tc_fence_after();
-      float inv = l > 0.f ? 1.0f / l : 0.f;
-      if (sinks && row_valid) inv = sink_quotient(m_used * 0.6931471805599453f, l, sinks[h0 + g]);
-      if (gate && !gate_elem && row_valid) inv *= head_gate(gate, m_base + pi, gate_stride, h0 + g, 0, HD, 0);
+    }
+    tc_fence_after();
+    if (!SHARED) {
+      if (ok) {
+        float inv = l > 0.f ? 1.0f / l : 0.f;
+        if (sinks && row_valid) inv = sink_quotient(m_used * 0.6931471805599453f, l, sinks[h0 + g]);
+        if (gate && !gate_elem && row_valid) inv *= head_gate(gate, m_base + pi, gate_stride, h0 + g, 0, HD, 0);
 #pragma unroll
-      for (int d0 = 0; d0 < HD / 2; d0 += 32) {
-        __syncwarp();      // idle rows left the branch below early: the loads take the whole warp
-        uint32_t o[32];
-        tmem_ld32(t_o + d0, o);
-        tmem_ld_wait();
-        if (row_valid) {
-          const int d = half * (HD / 2) + d0;
-          uint4* orow = reinterpret_cast<uint4*>(out + ((m_base + pi) * nh + h0 + g) * HD + d);
+        for (int d0 = 0; d0 < HD / 2; d0 += 32) {
+          __syncwarp();      // idle rows left the branch below early: the loads take the whole warp
+          uint32_t o[32];
+          tmem_ld32(t_o + d0, o);
+          tmem_ld_wait();
+          if (row_valid) {
+            const int d = half * (HD / 2) + d0;
+            uint4* orow = reinterpret_cast<uint4*>(out + ((m_base + pi) * nh + h0 + g) * HD + d);
 #pragma unroll
-          for (int c = 0; c < 32; c++) {
-            float x = __uint_as_float(o[c]) * inv;
-            if (gate && gate_elem) x *= head_gate(gate, m_base + pi, gate_stride, h0 + g, d + c, HD, 1);
-            o[c] = __float_as_uint(x);
-          }
-#pragma unroll
-          for (int c = 0; c < 32; c += 8) {
-            uint32_t w[4];
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-              __nv_bfloat162 pp = __floats2bfloat162_rn(__uint_as_float(o[c + 2 * e]), __uint_as_float(o[c + 2 * e + 1]));
-              w[e] = *reinterpret_cast<uint32_t*>(&pp);
+            for (int c = 0; c < 32; c++) {
+              float x = __uint_as_float(o[c]) * inv;
+              if (gate && gate_elem) x *= head_gate(gate, m_base + pi, gate_stride, h0 + g, d + c, HD, 1);
+              o[c] = __float_as_uint(x);
             }
-            orow[c / 8] = make_uint4(w[0], w[1], w[2], w[3]);
+#pragma unroll
+            for (int c = 0; c < 32; c += 8) {
+              uint32_t w[4];
+#pragma unroll
+              for (int e = 0; e < 4; e++) {
+                __nv_bfloat162 pp = __floats2bfloat162_rn(__uint_as_float(o[c + 2 * e]), __uint_as_float(o[c + 2 * e + 1]));
+                w[e] = *reinterpret_cast<uint32_t*>(&pp);
+              }
+              orow[c / 8] = make_uint4(w[0], w[1], w[2], w[3]);
+            }
           }
         }
       }
+    } else {
+      // The blocks of a tile (a cluster) lay their rows of O, their maxima and sums out in their shared memory (keys and values are done
+      // with); each then joins 128 / n_splits rows, reading from all of them, in the blocks' order.
+      float* so = reinterpret_cast<float*>(sk);      // [row][16-byte pieces moved by row & 7]
+      const bool any = ok && n_it > 0;
+      if (half == 0) {
+        last_s[0][r] = any ? m_used : AST_NEG;
+        last_s[1][r] = any ? l : 0.f;
+      }
+      if (any) {
+#pragma unroll
+        for (int d0 = 0; d0 < HD / 2; d0 += 32) {
+          uint32_t o[32];
+          tmem_ld32(t_o + d0, o);
+          tmem_ld_wait();
+#pragma unroll
+          for (int c = 0; c < 32; c += 4) {
+            const int piece = (half * (HD / 2) + d0 + c) / 4;
+            *reinterpret_cast<uint4*>(so + r * HD + ((piece ^ (r & 7)) << 2)) = make_uint4(o[c], o[c + 1], o[c + 2], o[c + 3]);
+          }
+        }
+      }
+      ast_cluster_sync();
+      const int share = (128 + n_splits - 1) / n_splits, r0 = split * share, n_rows = min(share, 128 - r0);
+      for (int i = threadIdx.x; i < n_rows; i += 256) {      // a row's factors, one per block
+        const int row = r0 + i, gg = row / TP, ii = row % TP;
+        float top = AST_NEG, sum = 0.f;
+        for (int j = 0; j < n_splits; j++) top = fmaxf(top, ast_remote(&last_s[0][row], j));
+        for (int j = 0; j < n_splits; j++) sum += ast_remote(&last_s[1][row], j) * ex2(ast_remote(&last_s[0][row], j) - top);
+        float inv = sum > 0.f ? 1.0f / sum : 0.f;
+        if (gg < G && ii < rows) {
+          if (sinks) inv = sink_quotient(top * 0.6931471805599453f, sum, sinks[h0 + gg]);
+          if (gate && !gate_elem) inv *= head_gate(gate, m_base + ii, gate_stride, h0 + gg, 0, HD, 0);
+        }
+        for (int j = 0; j < n_splits; j++)
+          join_s[j][i] = ast_remote(&last_s[1][row], j) > 0.f ? inv * ex2(ast_remote(&last_s[0][row], j) - top) : 0.f;
+      }
+      asm volatile("bar.sync 9, 256;" ::: "memory");
+      for (int idx = threadIdx.x; idx < n_rows * (HD / 4); idx += 256) {
+        const int i = idx / (HD / 4), piece = idx % (HD / 4), row = r0 + i, gg = row / TP, ii = row % TP;
+        if (gg >= G || ii >= rows) continue;
+        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int j = 0; j < n_splits; j++) {
+          const float f = join_s[j][i];
+          if (f == 0.f) continue;      // (that block read nothing for this row: its numbers may be anything)
+          const float4 y = ast_remote4(so + row * HD + ((piece ^ (row & 7)) << 2), j);
+          x.x += f * y.x, x.y += f * y.y, x.z += f * y.z, x.w += f * y.w;
+        }
+        const size_t m = m_base + ii;
+        if (gate && gate_elem) {
+          x.x *= head_gate(gate, m, gate_stride, h0 + gg, 4 * piece, HD, 1), x.y *= head_gate(gate, m, gate_stride, h0 + gg, 4 * piece + 1, HD, 1);
+          x.z *= head_gate(gate, m, gate_stride, h0 + gg, 4 * piece + 2, HD, 1), x.w *= head_gate(gate, m, gate_stride, h0 + gg, 4 * piece + 3, HD, 1);
+        }
+        store4(out + (m * nh + h0 + gg) * HD + 4 * piece, x);
+      }
+      ast_cluster_sync();      // no block ends while others read its memory
     }
   }
   tc_fence_before();
@@ -372,26 +465,40 @@ attention_stream_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gr
 // rows of the swizzled tile).
 static int ast_positions(int G) { return (128 / G) & ~7; }
 
+// Blocks that share a tile's keys: as many as there is room for on the SMs (two each), with two iterations of 128 keys or more for each.
+static int ast_splits(int M, int B, int nh, int nkv, int window, int chunk, int first, int max_qlen, int max_kvlen) {
+  const int TP = ast_positions(nh / nkv);
+  const long long per_head = (long long)ceil_div(max_qlen, TP) * B, by_rows = (long long)M / TP + B;
+  const long long tiles = (per_head < by_rows ? per_head : by_rows) * nkv, room = 2ll * sm_count() / tiles;
+  long long keys = (long long)(window > 0 ? window : max_kvlen);
+  if (chunk > 0 && chunk < keys) keys = chunk;
+  keys += first + (TP < max_qlen ? TP : max_qlen);
+  if (keys > max_kvlen) keys = max_kvlen;
+  const long long most = (keys + 127) / 128 / 2;
+  long long n = room < most ? room : most;
+  return (int)(n < 1 ? 1 : n > AST_MOST_SPLITS ? AST_MOST_SPLITS : n);
+}
+
 // Returns 1 when the sizes are ones this kernel takes.
 LEB_API int leb_attention_stream_tc_supported(int nh, int nkv, int hd, int page_size) {
   return (hd == 64 || hd == 128) && page_size == 64 && nkv > 0 && nh % nkv == 0 && nh / nkv <= 16;
 }
 
-template <int HD>
+template <int HD, bool SHARED>
 static int launch_attention_stream_tc(void* out, const void* q, int q_stride, int M, const void* k_pool, const void* v_pool, int n_pages,
                                       const int* block_table, int bt_width, const int* seq_slot, const int* seq_pos0,
                                       const int* seq_qstart, const int* seq_qlen, const void* gate, int gate_stride, int gate_elem,
                                       int B, int nh, int nkv, int window, int chunk, int first, float scale, const float* slopes,
-                                      const float* sinks, int max_qlen, int* status, cudaStream_t st) {
+                                      const float* sinks, int max_qlen, int n_splits, int* status, cudaStream_t st) {
   using Shape = AstShape<HD>;
   const int G = nh / nkv, TP = ast_positions(G);
   CUtensorMap mq, mk, mv;
   if (tensor_map(&mq, q, M, nh * HD, q_stride, TP)) return 1;
   if (tensor_map(&mk, k_pool, n_pages * nkv * 64, HD, HD, 64)) return 1;
   if (tensor_map(&mv, v_pool, n_pages * nkv * HD, 64, 64, HD)) return 1;
-  dim3 grid(nkv, B, ceil_div(max_qlen, TP));
+  dim3 grid(nkv, B, ceil_div(max_qlen, TP) * n_splits);
   LEB_REQUIRE(grid.y <= 65535 && grid.z <= 65535, "leb_attention_stream_tc: grid too large (%u, %u)", grid.y, grid.z);
-  constexpr auto kern = attention_stream_tc_kernel<HD>;
+  constexpr auto kern = attention_stream_tc_kernel<HD, SHARED>;
   // The warpgroups share out the registers of the launch: with fewer than REGS a thread they would wait for ever.
   static std::atomic<int> regs{0};
   if (regs.load(std::memory_order_relaxed) == 0) {
@@ -403,28 +510,34 @@ static int launch_attention_stream_tc(void* out, const void* q, int q_stride, in
               regs.load(std::memory_order_relaxed), Shape::REGS);
   const cudaError_t e = leb_allow_smem<kern, Shape::SMEM>();
   if (e != cudaSuccess) return leb_fail("leb_attention_stream_tc: shared memory %d: %s", Shape::SMEM, cudaGetErrorString(e));
-  leb_launch(kern, grid, dim3(Shape::THREADS), Shape::SMEM, st, mq, mk, mv, (bf16*)out, block_table, bt_width, seq_slot, seq_pos0, seq_qstart,
-             seq_qlen, (const bf16*)gate, gate_stride, gate_elem, nh, nkv, G, TP, window, chunk, first, scale, slopes, sinks, status);
+  leb_launch_cluster(SHARED ? n_splits : 1, kern, grid, dim3(Shape::THREADS), Shape::SMEM, st, mq, mk, mv, (bf16*)out, block_table, bt_width,
+                     seq_slot, seq_pos0, seq_qstart, seq_qlen, (const bf16*)gate, gate_stride, gate_elem, nh, nkv, G, TP, window, chunk, first,
+                     scale, slopes, sinks, n_splits, status);
   LEB_CHECK_LAUNCH("leb_attention_stream_tc");
   return 0;
 }
 
 // Prompt attention of the step's rows over the paged cache (which already holds their keys and values).  q: [M, nh*hd] with row
 // stride q_stride; k_pool [n_pages][nkv][64][hd], v_pool [n_pages][nkv][hd][64]; out [M, nh*hd].  status: device int, set non-zero by a
-// block whose bounded wait gave up.  slopes, sinks [nh] or null as in leb_attention.
+// block whose bounded wait gave up.  slopes, sinks [nh] or null as in leb_attention.  max_kvlen: the most positions a sequence of the step holds.
+// n_splits: blocks that share a tile's keys (0: as many as suit the step).
 LEB_API int leb_attention_stream_tc(void* out, const void* q, int q_stride, int M, const void* k_pool, const void* v_pool, int n_pages,
                                     const int* block_table, int bt_width, const int* seq_slot, const int* seq_pos0,
                                     const int* seq_qstart, const int* seq_qlen, const void* gate, int gate_stride, int gate_elem, int B,
                                     int nh, int nkv, int hd, int page_size, int window, int chunk, int first, float scale,
-                                    const float* slopes, const float* sinks, int max_qlen, int* status, cudaStream_t st) {
+                                    const float* slopes, const float* sinks, int max_qlen, int max_kvlen, int n_splits,
+                                    int* status, cudaStream_t st) {
   if (B <= 0 || max_qlen <= 0 || M <= 0) return 0;
   LEB_REQUIRE(leb_attention_stream_tc_supported(nh, nkv, hd, page_size),
               "leb_attention_stream_tc: sizes not taken (heads %d, kv heads %d, head_dim %d, page %d)", nh, nkv, hd, page_size);
   LEB_REQUIRE(status != nullptr, "leb_attention_stream_tc: a status word is required");
   LEB_REQUIRE(((uintptr_t)q & 15) == 0 && q_stride % 8 == 0 && ((uintptr_t)out & 15) == 0,
               "leb_attention_stream_tc: q and out must be 16-byte aligned, q's row stride a multiple of 8");
+  LEB_REQUIRE(n_splits >= 0 && n_splits <= AST_MOST_SPLITS, "leb_attention_stream_tc: %d blocks for a tile's keys, %d at most", n_splits, AST_MOST_SPLITS);
+  if (n_splits == 0) n_splits = ast_splits(M, B, nh, nkv, window, chunk, first, max_qlen, max_kvlen);
 #define LEB_AST_ARGS out, q, q_stride, M, k_pool, v_pool, n_pages, block_table, bt_width, seq_slot, seq_pos0, seq_qstart, seq_qlen, gate, \
-                     gate_stride, gate_elem, B, nh, nkv, window, chunk, first, scale, slopes, sinks, max_qlen, status, st
-  return hd == 64 ? launch_attention_stream_tc<64>(LEB_AST_ARGS) : launch_attention_stream_tc<128>(LEB_AST_ARGS);
+                     gate_stride, gate_elem, B, nh, nkv, window, chunk, first, scale, slopes, sinks, max_qlen, n_splits, status, st
+  if (n_splits > 1) return hd == 64 ? launch_attention_stream_tc<64, true>(LEB_AST_ARGS) : launch_attention_stream_tc<128, true>(LEB_AST_ARGS);
+  return hd == 64 ? launch_attention_stream_tc<64, false>(LEB_AST_ARGS) : launch_attention_stream_tc<128, false>(LEB_AST_ARGS);
 #undef LEB_AST_ARGS
 }

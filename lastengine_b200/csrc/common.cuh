@@ -49,6 +49,25 @@ static inline cudaError_t leb_launch(void (*kern)(KArgs...), dim3 grid, dim3 blo
   cfg.numAttrs = g_leb_pdl ? 1 : 0;
   return cudaLaunchKernelEx(&cfg, kern, static_cast<KArgs>(args)...);
 }
+// The same as clusters of `cluster` blocks along z (1: none).
+template <typename... KArgs, typename... Args>
+static inline cudaError_t leb_launch_cluster(int cluster, void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, Args... args) {
+  if (cluster <= 1) return leb_launch(kern, grid, block, smem, st, args...);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = cluster;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = g_leb_pdl ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kern, static_cast<KArgs>(args)...);
+}
 // Launches of a scope without programmatic dependent launch (strictly after their predecessor).
 struct LebPlainLaunches {
   int saved;

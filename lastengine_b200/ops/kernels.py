@@ -301,10 +301,10 @@ def _declare(L) -> None:
         "leb_penalties_slots": [P, P, P, P, I, I, I, F, F, P],
         "leb_history_append": [P, P, P, P, I, I, P],
         "leb_attention_decode_supported": [I, I, I, I],
-        "leb_attention_decode": [P, P, P, P, P, P, I, P, P, P, P, I, I, I, I, I, I, I, I, I, I, I, F, P, P, I, P],
+        "leb_attention_decode": [P, P, P, P, P, P, I, P, P, P, P, I, I, I, I, I, I, I, I, I, I, I, F, P, P, I, I, I, P],
         "leb_attention_merge": [P, P, I, P, I, I, P, I, I, I, I, P],
         "leb_attention_decode_prep_supported": [I, I, I, I, I, I],
-        "leb_attention_decode_prep": [P, P, P, I, P, P, I, P, P, P, I, P, P, P, P, P, F, P, I, I, I, P, I, I, I, I, I, I, I, I, I, I, I, F, P, P, F, F, I, P],
+        "leb_attention_decode_prep": [P, P, P, I, P, P, I, P, P, P, I, P, P, P, P, P, F, P, I, I, I, P, I, I, I, I, I, I, I, I, I, I, I, F, P, P, F, F, I, I, I, P],
         "leb_attention_prefill_supported": [I, I, I, I],
         "leb_attention_prefill_tc_supported": [I, I, I, I],
         "leb_attention_prefill_tc": [P, P, I, I, P, P, I, P, I, P, P, P, P, P, I, I, I, I, I, I, I, I, I, I, I, F, P, P, I, P, P],
@@ -312,7 +312,7 @@ def _declare(L) -> None:
         "leb_attention_pooled_tc_value_dim": [I],
         "leb_attention_prefill": [P, P, P, P, P, I, P, P, P, P, P, I, I, I, I, I, I, I, I, I, I, I, F, P, P, I, P],
         "leb_attention_stream_tc_supported": [I, I, I, I],
-        "leb_attention_stream_tc": [P, P, I, I, P, P, I, P, I, P, P, P, P, P, I, I, I, I, I, I, I, I, I, I, F, P, P, I, P, P],
+        "leb_attention_stream_tc": [P, P, I, I, P, P, I, P, I, P, P, P, P, P, I, I, I, I, I, I, I, I, I, I, F, P, P, I, I, I, P, P],
         "leb_stream_tables": [P, I, P, P, P, P, P, P, P, P, P, P, I, P, I, P, I, P, I, I, I, P],
         "leb_stream_advance": [P, P, P, I, P, P, I, P, I, P, I, I, I, I, P],
         "leb_stream_release": [P, P, I, P, P, I, P, I, P, I, I, I, P],
@@ -1618,10 +1618,21 @@ def attention_splits(batch, nkv: int, G: int, sm_count: int | None = None, hd: i
     slots = sm_count * max(1, min(3, (227 * 1024) // stage_bytes))      # blocks that run at once
     if per >= 2 * sm_count:
         return 1 if kv < 2048 else min(4, kv // 1024)
+    if first > 0 and (window > 0 or chunk > 0) and not general and hd in (32, 64, 96, 128) and G <= 16:
+        return 1      # the blocks of a sequence join their sums by themselves, without a second kernel
     least = 128 if per * 8 <= sm_count else 256       # one or two sequences: latency counts, shorter blocks pay
     if general and kv > 128:
         least //= 2
     return max(1, min(slots // per, kv // least, 32))
+
+
+_stream_splits = 0          # blocks that share a tile's keys in the streams' prompt attention (0: as many as suit the step)
+
+
+def set_stream_attention_splits(n: int) -> None:
+    """For tests and timing: how many blocks (1 to 8) share a row's keys, a cluster, in attention with first positions; 0: chosen."""
+    global _stream_splits
+    _stream_splits = int(n)
 
 
 TC_ATTENTION_MIN_ROWS = 8   # longest row count of a sequence from which prompts go to the tcgen05 attention
@@ -1713,18 +1724,18 @@ def attention(out: torch.Tensor, q: torch.Tensor | None, k_pool: torch.Tensor, v
             _ptr(out), _ptr(scratch), _ptr(q), _ptr(k_pool), _ptr(v_pool), _ptr(block_table),
             block_table.shape[1], _ptr(batch.seq_slot), _ptr(batch.seq_pos0), _ptr(batch.seq_qstart),
             _ptr(gate), gate_stride, gate_elem, batch.n_seqs, nh, nkv, hd, page_size, window, chunk, first, int(wide), float(scale),
-            _ptr(slopes), _ptr(sinks), n_splits, _stream()))
+            _ptr(slopes), _ptr(sinks), n_splits, batch.max_kvlen, _stream_splits, _stream()))
         if n_splits > 1:
             _check(L.leb_attention_merge(_ptr(out), _ptr(scratch), BF16, _ptr(gate), gate_stride, gate_elem, _ptr(sinks), M,
                                          nh, hd, n_splits, _stream()))
         return
-    if (first > 0 and not wide and out.dtype == torch.bfloat16 and n_splits == 1 and batch.max_qlen >= TC_ATTENTION_MIN_ROWS
+    if (first > 0 and not wide and out.dtype == torch.bfloat16 and batch.max_qlen > 1
             and q.stride(0) % 8 == 0 and L.leb_attention_stream_tc_supported(nh, nkv, hd, page_size)):
         _check(L.leb_attention_stream_tc(
             _ptr(out), _ptr(q), q.stride(0), M, _ptr(k_pool), _ptr(v_pool), k_pool.shape[0], _ptr(block_table),
             block_table.shape[1], _ptr(batch.seq_slot), _ptr(batch.seq_pos0), _ptr(batch.seq_qstart),
             _ptr(batch.seq_qlen), _ptr(gate), gate_stride, gate_elem, batch.n_seqs, nh, nkv, hd, page_size, window, chunk,
-            first, float(scale), _ptr(slopes), _ptr(sinks), batch.max_qlen, _ptr(_status_word(out.device)), _stream()))
+            first, float(scale), _ptr(slopes), _ptr(sinks), batch.max_qlen, batch.max_kvlen, _stream_splits, _ptr(_status_word(out.device)), _stream()))
         return
     if (out.dtype == torch.bfloat16 and n_splits == 1 and batch.max_qlen >= TC_ATTENTION_MIN_ROWS
             and q.stride(0) % 8 == 0 and L.leb_attention_prefill_tc_supported(nh, nkv, hd, page_size)):
@@ -1807,7 +1818,7 @@ def _attention_decode_raw(out, raw: RawQKV, k_pool, v_pool, block_table, batch, 
         _ptr(k_pool), _ptr(v_pool), _ptr(block_table), block_table.shape[1], _ptr(batch.seq_slot), _ptr(batch.seq_pos0),
         _ptr(batch.seq_qstart), _ptr(raw.q_norm_w), _ptr(raw.k_norm_w), raw.eps, _ptr(raw.inv_freq), raw.rope_dim,
         1 if raw.neox else 0, int(raw.row_norm), _ptr(gate), gate_stride, gate_elem, batch.n_seqs, nh, nkv, hd, page_size, window,
-        chunk, first, int(wide), float(scale), _ptr(slopes), _ptr(sinks), *_temperature(raw.temperature), n_splits, _stream()))
+        chunk, first, int(wide), float(scale), _ptr(slopes), _ptr(sinks), *_temperature(raw.temperature), n_splits, batch.max_kvlen, _stream_splits, _stream()))
     if n_splits > 1:
         _check(L.leb_attention_merge(_ptr(out), _ptr(scratch), BF16, _ptr(gate), gate_stride, gate_elem, _ptr(sinks), M, nh, hd,
                                      n_splits, _stream()))

@@ -125,8 +125,14 @@ def test_single_tokens(dtype, nh, nkv, hd, vd, page, window, first):
     c = Case(DECODE, nh, nkv, hd, vd, page, window, first, dtype, seed=window + first, padding=[4])
     a = c.run()
     c.check(a)
-    for n in (1, 2, 5):
+    for n in (2, 5):
         c.check(c.run(n_splits=n))
+    try:
+        for n in (1, 2, 3, 8):
+            K().set_stream_attention_splits(n)
+            c.check(c.run(n_splits=1))
+    finally:
+        K().set_stream_attention_splits(0)
     assert torch.equal(a, c.run())
 
 
@@ -141,6 +147,41 @@ def test_chunks_of_tokens(dtype, nh, nkv, hd, vd, page, window, first):
     a = c.run()
     c.check(a)
     assert torch.equal(a, c.run())
+
+
+@pytest.mark.parametrize("nh,nkv,hd", [(8, 2, 64), (3, 3, 64), (8, 2, 128), (5, 1, 128)])
+@pytest.mark.parametrize("window,first", [(1, 1), (64, 64), (300, 33), (33, 1000), (900, 4)])
+def test_blocks_that_share_a_tile_s_keys(nh, nkv, hd, window, first):
+    """1 to 8 blocks for the keys of a tile, also where some of them get none; with sinks and gates, which the join takes."""
+    c = Case(CHUNKS + [(1500, 20), (0, 3)], nh, nkv, hd, hd, 64, window, first, BF16, seed=window, padding=[5])
+    g = torch.Generator().manual_seed(1)
+    sinks, gate = torch.randn(nh, generator=g), torch.randn(c.rows, nh, generator=g).to(BF16)
+    numbers = torch.randn(c.rows, nh * hd, generator=g).to(BF16)
+    try:
+        for n in (1, 2, 3, 5, 8):
+            K().set_stream_attention_splits(n)
+            a = c.run()
+            c.check(a)
+            assert torch.equal(a, c.run())
+            c.check(c.run(sinks=sinks.to(DEV), gate=gate.to(DEV)), sinks=sinks.double(), factor=torch.sigmoid(gate.double())[:, :, None])
+            c.check(c.run(gate=numbers.to(DEV)), factor=torch.sigmoid(numbers.double()).view(c.rows, nh, hd))
+    finally:
+        K().set_stream_attention_splits(0)
+
+
+@pytest.mark.parametrize("seqs", [DECODE, CHUNKS])
+def test_weights_of_two_terms_beside_first_positions(seqs):
+    """Nearer to the 64-bit result than weights of one term: 2^-16 of a weight where that is 2^-8, but for the rounding of the result."""
+    for hd in (64, 128, 32):
+        c = Case(seqs, 4, 2, hd, hd, 64, 70, 40, BF16, seed=11)
+        wide = c.run(wide=True)
+        c.check(wide)
+        out, row = wide.double().cpu().view(c.rows, 4, hd), 0
+        for (h, n), q, (k, v) in zip(c.seqs, c.q, c.kv):
+            want, mass, size = S.attention(q.double(), k.double(), v.double(), torch.arange(h, h + n), 70, 40, c.scale)
+            bound = 2 ** -8 * (1 + 2 ** -6) * want.abs() + 2 * mass * (2 ** -16 + hd * 2 ** -22 * size + 110 * 2 ** -24 + 2 ** -18)
+            assert bool(((out[row:row + n] - want).abs() <= bound).all()), (hd, h, n)
+            row += n
 
 
 @pytest.mark.parametrize("nh,nkv,hd", [(8, 2, 64), (8, 2, 128), (4, 4, 32)])
