@@ -313,6 +313,8 @@ def _declare(L) -> None:
         "leb_attention_prefill": [P, P, P, P, P, I, P, P, P, P, P, I, I, I, I, I, I, I, I, I, I, I, F, P, P, I, P],
         "leb_attention_stream_tc_supported": [I, I, I, I],
         "leb_attention_stream_tc": [P, P, I, I, P, P, I, P, I, P, P, P, P, P, I, I, I, I, I, I, I, I, I, I, F, P, P, I, I, I, P, P],
+        "leb_attention_stream_f32_supported": [I, I, I, I, I],
+        "leb_attention_stream_f32": [P, P, P, P, P, I, P, P, P, P, I, I, I, I, I, I, I, I, I, I, I, F, P, P, I, I, P],
         "leb_stream_tables": [P, I, P, P, P, P, P, P, P, P, P, P, I, P, I, P, I, P, I, I, I, P],
         "leb_stream_advance": [P, P, P, I, P, P, I, P, I, P, I, I, I, I, P],
         "leb_stream_release": [P, P, I, P, P, I, P, I, P, I, I, I, P],
@@ -1697,6 +1699,10 @@ def attention(out: torch.Tensor, q: torch.Tensor | None, k_pool: torch.Tensor, v
         if t is not None:
             _cuda(t, f"attention.{name}", torch.float32)
             assert t.numel() == nh
+    if (first > 0 and raw is None and out.dtype == torch.float32 and batch.max_qlen == 1 and out.shape[0] == batch.n_seqs
+            and (k_pool.data_ptr() | v_pool.data_ptr()) & 15 == 0 and lib().leb_attention_stream_f32_supported(nh, nkv, hd, vd or hd, page_size)):
+        return _attention_stream_f32(out, q, k_pool, v_pool, block_table, batch, nh, nkv, hd, int(vd or hd), page_size, window, scale, gate,
+                                     chunk, slopes, sinks, first)
     if vd is not None and vd != hd:
         return _attention_general(out, q, k_pool, v_pool, block_table, batch, nh, nkv, hd, int(vd), page_size, window,
                                   scale, gate, n_splits, scratch, chunk, slopes, sinks, first)
@@ -1760,6 +1766,23 @@ def attention(out: torch.Tensor, q: torch.Tensor | None, k_pool: torch.Tensor, v
         _ptr(block_table), block_table.shape[1], _ptr(batch.seq_slot), _ptr(batch.seq_pos0),
         _ptr(batch.seq_qstart), _ptr(batch.seq_qlen), _ptr(gate), gate_stride, gate_elem, M, batch.n_seqs, nh, nkv,
         hd, page_size, window, chunk, first, float(scale), _ptr(slopes), _ptr(sinks), batch.max_qlen, n_splits, hd, _stream()))
+
+
+def _attention_stream_f32(out, q, k_pool, v_pool, block_table, batch, nh, nkv, hd, vd, page_size, window, scale, gate, chunk, slopes, sinks,
+                          first) -> None:
+    """A decode step over a 32-bit cache with first positions: the blocks of a sequence join their sums by themselves."""
+    _cuda(q, "attention.q", torch.float32)
+    _cuda(k_pool, "attention.k_pool", torch.float32)
+    _cuda(v_pool, "attention.v_pool", torch.float32)
+    _cuda(block_table, "attention.block_table", torch.int32)
+    M = out.shape[0]
+    assert out.shape == (M, nh * vd) and q.shape == (M, nh * hd)
+    assert k_pool.shape[1:] == (nkv, page_size, hd) and v_pool.shape[1:] == (nkv, vd, page_size)
+    gate_stride, gate_elem = _gate_layout(gate, M, nh, vd, out.dtype)
+    _check(lib().leb_attention_stream_f32(
+        _ptr(out), _ptr(q), _ptr(k_pool), _ptr(v_pool), _ptr(block_table), block_table.shape[1], _ptr(batch.seq_slot), _ptr(batch.seq_pos0),
+        _ptr(batch.seq_qstart), _ptr(gate), gate_stride, gate_elem, batch.n_seqs, nh, nkv, hd, vd, page_size, window, chunk, first,
+        float(scale), _ptr(slopes), _ptr(sinks), batch.max_kvlen, _stream_splits, _stream()))
 
 
 def _attention_general(out, q, k_pool, v_pool, block_table, batch, nh, nkv, hd, vd, page_size, window, scale, gate,
