@@ -3,14 +3,20 @@
 //
 // A decode step reads every visible key and value once, so the kernel is built around that stream, as the bfloat16 one is
 // (attention_decode.cu): a block owns one sequence, up to HC query heads of one kv head and one share of the keys; its warps take tiles of
-// 32 positions in turn, brought in by asynchronous copies a tile ahead (a warp's own two stages: no warp waits for another), each with its
-// own running (max, sum, acc) per head.  The arithmetic is the FMA pipes':
-//  * scores: eight lanes share a key (its 16-byte pieces), four keys at a time; the eight partial sums of HC heads are added up by
-//    exchanging halves of the heads, so that each lane ends up with one head's score;
-//  * weights: a lane takes four neighbouring positions (eight lanes a tile, four times over);
+// 32 positions in turn, brought in by asynchronous copies into a place of the warp's own (the next keys while the weights are made, the
+// next values when these are done with: more warps hide the trip better than a second place would), each with its own running
+// (max, sum, acc) per head.  The arithmetic is the FMA pipes':
+//  * scores: a lane owns a key and goes through its numbers in pieces of 16 bytes, the queries of the HC heads coming from shared memory
+//    for all lanes at once (key rows are an odd number of pieces apart: no two lanes of a quarter meet a bank);
+//  * weights: a lane makes those of its key, which then lie in shared memory for the values' lanes;
 //  * values, stored [dim][position]: a lane multiplies four positions of a dimension with their weights for all HC heads; the eight
 //    lanes' sums are added up once, at the end.
 // Warps join through shared memory, the blocks that share a sequence's keys as a cluster.  Everything is float; exponentials are expf.
+//
+// Bound by the instructions of a tile (some 900 a warp with four heads of 64, 2.4 us with the SM's twelve warps), not by memory: 32 streams
+// of 100 to 3,000 positions, window 1,024, 32 heads of 64 over 8: 34 us (68 MB, 2.0 TB/s; the general kernel 155), 64 streams with heads of
+// 128, one query head each: 55 us (270 MB, 4.9 TB/s).  Measured beside it: eight lanes a key and sums by exchange 51 and 53 us, with two
+// tiles' places a warp and four warps an SM 70.
 #include "common.cuh"
 
 #define ASF_NEG (-1e30f)
@@ -56,16 +62,22 @@ __device__ __forceinline__ int asf_head(int lane) {
   return HC == 4 ? ((lane & 1) << 1 | (lane >> 1 & 1)) : HC == 2 ? (lane & 1) : 0;
 }
 
+__device__ __forceinline__ float asf_max(float v) {      // over the warp
+  float m;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(v));
+  return m;
+}
+
 // D: heads of up to D numbers; HC: query heads of a block (1, 2 or 4); VEC: keys are read in pieces of 16 bytes (hd a multiple of 4).
 template <int D, int HC, bool VEC>
-__global__ void __launch_bounds__(128)
+__global__ void __launch_bounds__(128, D <= 64 ? 3 : D <= 128 ? 2 : 1)
 attention_stream_f32_kernel(float* __restrict__ out, const float* __restrict__ q, const float* __restrict__ k_pool,
                             const float* __restrict__ v_pool, const int* __restrict__ block_table, int bt_width,
                             const int* __restrict__ seq_slot, const int* __restrict__ seq_pos0, const int* __restrict__ seq_qstart,
                             const float* __restrict__ gate, int gate_stride, int gate_elem, int nh, int nkv, int hd, int vd, int page_size,
                             int window, int chunk, int first, float scale, const float* __restrict__ slopes,
                             const float* __restrict__ sinks, int n_splits) {
-  constexpr int NK = D / 32, NV = D / 4;
+  constexpr int NV = D / 4;
   extern __shared__ __align__(128) float asf_smem[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
   const int c = lane & 7, g = lane >> 3;
@@ -88,33 +100,54 @@ attention_stream_f32_kernel(float* __restrict__ out, const float* __restrict__ q
   const int n_tiles = (kv_len - 1) / 32 - shift + 1, per_split = (n_tiles + n_splits - 1) / n_splits;
   const int t_lo = split * per_split, t_hi = min(n_tiles, t_lo + per_split);
   const int* table = block_table + (size_t)b * bt_width;
-  const int k_floats = 32 * hd, stage = k_floats + 32 * vd;      // of a tile: keys [32][hd], values [vd][32]
-  float* ring = asf_smem + (size_t)warp * 2 * stage;
-  float* score_s = asf_smem + (size_t)warps * 2 * stage + warp * HC * 32;      // [HC][32]
+  const int pieces = hd / 4, row = VEC ? 4 * (pieces | 1) : hd;       // floats from a key to the next
+  const int k_floats = 32 * row, stage = k_floats + 32 * vd;         // of a tile: keys [32][row], values [vd][32]
+  float* ks = asf_smem + (size_t)warp * stage;
+  float* vs = ks + k_floats;
+  float* weight_s = asf_smem + (size_t)warps * stage + warp * HC * 32;      // [HC][32]
+  float* q_s = asf_smem + (size_t)warps * (stage + HC * 32);                // [HC][row]
 
   auto key_of = [&](int tile) { return (tile >= n_first ? tile + shift : tile) * 32; };
-  auto issue = [&](int tile, int s) {
+  const uint32_t k_to = (uint32_t)__cvta_generic_to_shared(ks), v_to = (uint32_t)__cvta_generic_to_shared(vs) + 16 * lane;
+  const int v_step = 4 * page_size;      // a warp's pass copies four dimensions
+  auto page_of = [&](int tile) { return max(table[key_of(tile) / page_size], 0); };
+  // a lane's pieces of a tile of keys: the first one's key and place, the steps to the next
+  const int k_r0 = VEC ? lane / pieces : 0, k_c0 = VEC ? lane % pieces : 0, k_rs = VEC ? 32 / pieces : 0, k_cs = VEC ? 32 % pieces : 0;
+  auto issue_k = [&](int tile, int page) {      // (in the cache a tile's keys lie together)
     if (tile < t_hi) {
-      const int key0 = key_of(tile), page = max(table[key0 / page_size], 0), off = key0 % page_size;
-      const float* ks = k_pool + (((size_t)page * nkv + kvh) * page_size + off) * hd;      // the tile's keys lie together
-      const float* vs = v_pool + ((size_t)page * nkv + kvh) * vd * page_size + off;
-      const uint32_t to = (uint32_t)__cvta_generic_to_shared(ring + s * stage);
-      for (int i = lane; i < 8 * hd; i += 32) asf_cp16(to + 16 * i, ks + 4 * i);
-      for (int i = lane; i < 8 * vd; i += 32) asf_cp16(to + 4 * k_floats + 16 * i, vs + (size_t)(i >> 3) * page_size + 4 * (i & 7));
+      const float* src = k_pool + (((size_t)page * nkv + kvh) * page_size + key_of(tile) % page_size) * hd + 4 * lane;
+      if (VEC) {
+        int r = k_r0, c4 = k_c0;
+#pragma unroll 4
+        for (int i = lane, n = 0; i < 32 * pieces; i += 32, n++) {
+          asf_cp16(k_to + 4 * (r * row + 4 * c4), src + 128 * n);
+          r += k_rs;
+          c4 += k_cs;
+          if (c4 >= pieces) c4 -= pieces, r++;
+        }
+      } else {
+        for (int i = lane, n = 0; i < 8 * hd; i += 32, n++) asf_cp16(k_to + 16 * i, src + 128 * n);
+      }
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
-  issue(t_lo + warp, 0);
-
-  // the query's numbers that meet this lane's pieces of a key, already scaled
-  float qv[HC][4 * NK];
-#pragma unroll
-  for (int h = 0; h < HC; h++)
-#pragma unroll
-    for (int i = 0; i < 4 * NK; i++) {
-      const int d = VEC ? 4 * (c + 8 * (i >> 2)) + (i & 3) : c + 8 * i;
-      qv[h][i] = h < heads && d < hd ? q[(m_row * nh + h0 + h) * hd + d] * scale : 0.f;
+  auto issue_v = [&](int tile, int page) {
+    if (tile < t_hi) {
+      const float* src = v_pool + (((size_t)page * nkv + kvh) * vd + g) * page_size + key_of(tile) % page_size + 4 * c;
+#pragma unroll 4
+      for (int i = lane, n = 0; i < 8 * vd; i += 32, n++) asf_cp16(v_to + 512 * n, src + (size_t)v_step * n);
     }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  int page = t_lo + warp < t_hi ? page_of(t_lo + warp) : 0;
+  issue_k(t_lo + warp, page);
+  issue_v(t_lo + warp, page);
+
+  for (int i = threadIdx.x; i < HC * hd; i += blockDim.x) {
+    const int h = i / hd, d = i - h * hd;
+    q_s[h * row + d] = h < heads ? q[(m_row * nh + h0 + h) * hd + d] * scale : 0.f;
+  }
+  __syncthreads();
   float slope[HC];
 #pragma unroll
   for (int h = 0; h < HC; h++) slope[h] = slopes && h < heads ? slopes[h0 + h] : 0.f;
@@ -127,78 +160,59 @@ attention_stream_f32_kernel(float* __restrict__ out, const float* __restrict__ q
 #pragma unroll
     for (int i = 0; i < NV; i++) acc[i][h] = 0.f;
   }
-  int s = 0;
-  for (int tile = t_lo + warp; tile < t_hi; tile += warps, s ^= 1) {
-    issue(tile + warps, s ^ 1);
-    asm volatile("cp.async.wait_group 1;" ::: "memory");
-    __syncwarp();      // every lane's pieces of this stage have landed
-    const float* ks = ring + s * stage;
-    const float* vs = ks + k_floats;
+  for (int tile = t_lo + warp; tile < t_hi; tile += warps) {
+    page = tile + warps < t_hi ? page_of(tile + warps) : 0;
+    asm volatile("cp.async.wait_group 1;" ::: "memory");      // the keys (their values may be on their way)
+    __syncwarp();
     const int key0 = key_of(tile);
-#pragma unroll 2
-    for (int t = 0; t < 8; t++) {      // key 4t + g
-      const float* row = ks + (4 * t + g) * hd;
-      float x[HC];
+    float x[HC];
 #pragma unroll
-      for (int h = 0; h < HC; h++) x[h] = 0.f;
+    for (int h = 0; h < HC; h++) x[h] = 0.f;
+    const float* mine = ks + lane * row;
+    if (VEC) {
+#pragma unroll 4
+      for (int d = 0; d < hd; d += 4) {
+        const float4 kk = load4(mine + d);
 #pragma unroll
-      for (int i = 0; i < NK; i++) {
-        if (VEC) {
-          if (4 * (c + 8 * i) < hd) {
-            const float4 kk = load4(row + 4 * (c + 8 * i));
-#pragma unroll
-            for (int h = 0; h < HC; h++)
-              x[h] += kk.x * qv[h][4 * i] + kk.y * qv[h][4 * i + 1] + kk.z * qv[h][4 * i + 2] + kk.w * qv[h][4 * i + 3];
-          }
-        } else {
-#pragma unroll
-          for (int e = 0; e < 4; e++) {
-            const int d = c + 8 * (4 * i + e);
-            if (d < hd) {
-              const float kk = row[d];
-#pragma unroll
-              for (int h = 0; h < HC; h++) x[h] += kk * qv[h][4 * i + e];
-            }
-          }
+        for (int h = 0; h < HC; h++) {
+          const float4 qq = load4(q_s + h * row + d);
+          x[h] = fmaf(kk.x, qq.x, x[h]);
+          x[h] = fmaf(kk.y, qq.y, x[h]);
+          x[h] = fmaf(kk.z, qq.z, x[h]);
+          x[h] = fmaf(kk.w, qq.w, x[h]);
         }
       }
-      asf_sum8<HC>(x, lane);
-      if (c < HC) score_s[asf_head<HC>(lane) * 32 + 4 * t + g] = x[0];
-    }
-    __syncwarp();
-    const bool partial = (key0 < key_lo && key0 + 32 > first) || key0 + 32 > kv_len;
-    float p[HC][4];
-    bool read[4], moved = false;
+    } else {
+      for (int d = 0; d < hd; d++) {
+        const float kk = mine[d];
 #pragma unroll
-    for (int e = 0; e < 4; e++) {
-      const int kp = key0 + 4 * c + e;
-      read[e] = kp < kv_len && (kp >= key_lo || kp < first);
+        for (int h = 0; h < HC; h++) x[h] = fmaf(kk, q_s[h * row + d], x[h]);
+      }
     }
+    __syncwarp();      // everyone is done with the keys
+    issue_k(tile + warps, page);
+    const bool partial = (key0 < key_lo && key0 + 32 > first) || key0 + 32 > kv_len;
+    const int kp = key0 + lane;
+    const bool read = kp < kv_len && (kp >= key_lo || kp < first);
+    bool moved = false;
     float corr[HC];
 #pragma unroll
     for (int h = 0; h < HC; h++) {
-      const float4 v4 = load4(score_s + h * 32 + 4 * c);
-      p[h][0] = v4.x, p[h][1] = v4.y, p[h][2] = v4.z, p[h][3] = v4.w;
-      float top = ASF_NEG;
-#pragma unroll
-      for (int e = 0; e < 4; e++) {
-        if (slopes) p[h][e] -= slope[h] * (float)(qpos - key0 - 4 * c - e);
-        p[h][e] = read[e] ? p[h][e] : ASF_NEG;
-        top = fmaxf(top, p[h][e]);
-      }
-#pragma unroll
-      for (int o = 1; o < 8; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-      const float mn = fmaxf(mx[h], top);
+      if (slopes) x[h] -= slope[h] * (float)(qpos - kp);
+      const float mn = fmaxf(mx[h], asf_max(read ? x[h] : ASF_NEG));
       corr[h] = expf(mx[h] - mn);
       moved |= mn != mx[h];
       mx[h] = mn;
-      float sum = 0.f;
+      const float w = read ? expf(x[h] - mn) : 0.f;
+      l[h] = l[h] * corr[h] + w;      // of this lane's keys
+      weight_s[h * 32 + lane] = w;
+    }
+    __syncwarp();
+    float p[HC][4];
 #pragma unroll
-      for (int e = 0; e < 4; e++) {
-        p[h][e] = read[e] ? expf(p[h][e] - mn) : 0.f;
-        sum += p[h][e];
-      }
-      l[h] = l[h] * corr[h] + sum;      // of this lane's positions
+    for (int h = 0; h < HC; h++) {
+      const float4 w = load4(weight_s + h * 32 + 4 * c);
+      p[h][0] = w.x, p[h][1] = w.y, p[h][2] = w.z, p[h][3] = w.w;
     }
     if (moved) {      // (the same for all lanes: maxima are)
 #pragma unroll
@@ -206,12 +220,15 @@ attention_stream_f32_kernel(float* __restrict__ out, const float* __restrict__ q
 #pragma unroll
         for (int h = 0; h < HC; h++) acc[i][h] *= corr[h];
     }
+    asm volatile("cp.async.wait_group 1;" ::: "memory");      // the values (the next keys may be on their way)
+    __syncwarp();
     if (partial) {
+      const uint32_t seen = __ballot_sync(0xffffffffu, read) >> (4 * c);
 #pragma unroll
       for (int i = 0; i < NV; i++) {
         if (4 * i + g < vd) {
           float4 v4 = load4(vs + (4 * i + g) * 32 + 4 * c);      // zero times whatever lies where nothing is read would not be zero
-          v4.x = read[0] ? v4.x : 0.f, v4.y = read[1] ? v4.y : 0.f, v4.z = read[2] ? v4.z : 0.f, v4.w = read[3] ? v4.w : 0.f;
+          v4.x = seen & 1 ? v4.x : 0.f, v4.y = seen & 2 ? v4.y : 0.f, v4.z = seen & 4 ? v4.z : 0.f, v4.w = seen & 8 ? v4.w : 0.f;
 #pragma unroll
           for (int h = 0; h < HC; h++) acc[i][h] += v4.x * p[h][0] + v4.y * p[h][1] + v4.z * p[h][2] + v4.w * p[h][3];
         }
@@ -226,7 +243,8 @@ attention_stream_f32_kernel(float* __restrict__ out, const float* __restrict__ q
         }
       }
     }
-    __syncwarp();      // everyone is done with the stage and the scores
+    __syncwarp();      // everyone is done with the values and the scores
+    issue_v(tile + warps, page);
   }
   asm volatile("cp.async.wait_group 0;" ::: "memory");
   __syncthreads();     // the rings are done with: their memory takes the results
@@ -234,19 +252,21 @@ attention_stream_f32_kernel(float* __restrict__ out, const float* __restrict__ q
   float* m_s = o_s + warps * HC * vd;                   // [warp][HC]
   float* l_s = m_s + warps * HC;
   float* mine = l_s + warps * HC;                       // this block's rows, for the cluster's blocks to read: [HC][vd], maxima, sums
-  asf_sum8<HC>(l, lane);
+#pragma unroll
+  for (int h = 0; h < HC; h++) l[h] = warp_sum(l[h]);
   const int head = asf_head<HC>(lane);
 #pragma unroll
   for (int i = 0; i < NV; i++) {
+    if (4 * i >= vd) break;
     asf_sum8<HC>(acc[i], lane);
     if (c < HC && 4 * i + g < vd) o_s[(warp * HC + head) * vd + 4 * i + g] = acc[i][0];
   }
   if (g == 0 && c < HC) {
-    float top = mx[0];
+    float top = mx[0], sum = l[0];
 #pragma unroll
-    for (int h = 1; h < HC; h++) top = head == h ? mx[h] : top;
+    for (int h = 1; h < HC; h++) top = head == h ? mx[h] : top, sum = head == h ? l[h] : sum;
     m_s[warp * HC + head] = top;
-    l_s[warp * HC + head] = l[0];
+    l_s[warp * HC + head] = sum;
   }
   __syncthreads();
   auto finish = [&](int idx, float M, float L, float a) {
@@ -315,17 +335,20 @@ LEB_API int leb_attention_stream_f32(float* out, const float* q, const float* k_
   LEB_REQUIRE((((uintptr_t)k_pool | (uintptr_t)v_pool) & 15) == 0, "leb_attention_stream_f32: pools must be 16-byte aligned");
   const int G = nh / nkv, widest = hd > vd ? hd : vd;
   const int HC = G == 1 ? 1 : widest > 128 ? 2 : 4, n_hc = ceil_div(G, HC);
-  const size_t stage = (size_t)32 * (hd + vd) * sizeof(float);
-  int warps = (int)(200 * 1024 / (2 * stage));
-  warps = warps < 1 ? 1 : warps > 4 ? 4 : warps;
-  const size_t rings = warps * (2 * stage + HC * 32 * sizeof(float)), results = ((size_t)(warps + 1) * HC * (vd + 2)) * sizeof(float);
+  const int row = hd % 4 == 0 ? 4 * (hd / 4 | 1) : hd;
+  const size_t stage = (size_t)32 * (row + vd) * sizeof(float);
+  const int warps = stage <= 17 * 1024 ? 4 : 3;      // three blocks an SM; two up to heads of 128; one
+  const size_t rings = warps * (stage + HC * 32 * sizeof(float)) + HC * row * sizeof(float), results = ((size_t)(warps + 1) * HC * (vd + 2)) * sizeof(float);
   const size_t smem = rings > results ? rings : results;
-  // blocks of a cluster: as many as run at once, with two tiles a warp or more for each
+  // blocks of a cluster: as many as run at once (to the nearest), with a tile a warp or more for each.  us of 1, 2, 4, 8 blocks: one stream of
+  // 1,000 positions 25.1, 15.9, 11.0, 8.5; 32 streams of 100 to 3,000, window 1,024, 256 blocks where 444 fit, 38.9, 33.9, 41.4, 61.6; 64
+  // streams with heads of 128, 256 where 296 fit, 55.0, 58.6, 72.4, 109.9
   long long keys = window > 0 ? window : max_kvlen;
   if (chunk > 0 && chunk < keys) keys = chunk;
   keys = keys + first < max_kvlen ? keys + first : max_kvlen;
   const long long per = (long long)B * nkv * n_hc, fit = 220 * 1024 / (long long)(smem + 2048);
-  long long n = (long long)sm_count() * (fit < 1 ? 1 : fit > 4 ? 4 : fit) / per, most = keys / (64 * warps);
+  const long long room = (long long)sm_count() * (fit < 1 ? 1 : fit > 3 ? 3 : fit), most = keys / (32 * warps);
+  long long n = (2 * room + per) / (2 * per);
   n = n < most ? n : most;
   if (blocks > 0) n = blocks;
   const int n_splits = (int)(n < 1 ? 1 : n > 8 ? 8 : n);
