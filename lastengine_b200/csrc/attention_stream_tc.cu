@@ -1,8 +1,9 @@
-// Prompt attention of streams on the fifth-generation tensor cores: a window and a sequence's first positions, heads of 64 or 128.
+// Prompt attention of streams on the fifth-generation tensor cores: a window and a sequence's first positions, key and value heads of up
+// to 128 numbers (multiples of 8; tiles of 64 or 128, filled up with zeros by the copies), pages of 64 positions or a multiple.
 //
 // A row at position p reads positions j <= p with j >= first_key(p) or j < first.  A block owns a tile of 128 rows: the G query heads
 // of one kv head times TP = 128 / G consecutive positions (a multiple of 8; the rows that are left are idle).  It walks a list of
-// pages, those of first positions and then those from its first row's window to its last row, two pages (128 keys) at a time:
+// pages (or halves, .. of pages: always 64 positions), those of first positions and then those from its first row's window to its last row, two pages (128 keys) at a time:
 //
 //   S[128, 128] = Q[128, HD] . K[128, HD]^T       operands in shared memory, S in tensor memory
 //   P           = exp2(S * scale * log2 e - m)     two threads per row, one a page, P (bfloat16) to tensor memory
@@ -68,16 +69,17 @@ __device__ __forceinline__ float4 ast_remote4(const float* p, int rank) {
 // The lowest n bits (none for n <= 0, all from 32 on).
 __device__ __forceinline__ uint32_t ast_below(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; }
 
-// SHARED: a cluster of n_splits blocks shares a tile's keys (else n_splits is 1).
-template <int HD, bool SHARED>
+// SHARED: a cluster of n_splits blocks shares a tile's keys (else n_splits is 1).  EXACT: heads of HD numbers and pages of 64 positions (the
+// same with these as arguments takes some 5 us longer on the turns of 12 streams).
+template <int HD, bool SHARED, bool EXACT>
 __global__ void __launch_bounds__(AstShape<HD>::THREADS, 2)
 attention_stream_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                            const __grid_constant__ CUtensorMap map_v, bf16* __restrict__ out, const int* __restrict__ block_table,
                            int bt_width, const int* __restrict__ seq_slot, const int* __restrict__ seq_pos0,
                            const int* __restrict__ seq_qstart, const int* __restrict__ seq_qlen, const bf16* __restrict__ gate,
-                           int gate_stride, int gate_elem, int nh, int nkv, int G, int TP, int window, int chunk, int first,
+                           int gate_stride, int gate_elem, int nh, int nkv, int G, int TP, int hd_, int vd_, int per_page_, int window, int chunk, int first,
                            float scale, const float* __restrict__ slopes, const float* __restrict__ sinks, int n_blocks, int* __restrict__ status) {
-  const int n_splits = SHARED ? n_blocks : 1;
+  const int n_splits = SHARED ? n_blocks : 1, hd = EXACT ? HD : hd_, vd = EXACT ? HD : vd_, per_page = EXACT ? 1 : per_page_;
   using Shape = AstShape<HD>;
   constexpr int PAGE = 64, NS = Shape::STAGES, HALVES = HD / 64;
   constexpr int Q_BYTES = Shape::Q_BYTES, KV_BYTES = Shape::KV_BYTES;
@@ -90,7 +92,8 @@ attention_stream_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gr
   uint8_t* sv = sk + NS * KV_BYTES;           // [stage][page][dimension][64 positions]
   __shared__ uint64_t q_full, k_full[NS], v_full[NS], k_empty[NS], v_empty[NS], s_full, s_free, p_full, pv_done;
   __shared__ float row_s[2][2][128];          // what the two threads of a row tell each other: [iteration's parity][thread][row]
-  __shared__ float last_s[2][SHARED ? 128 : 1], join_s[AST_MOST_SPLITS][SHARED ? 64 : 1];      // maxima and sums of this block's rows; factors of the rows it joins
+  __shared__ float last_s[2][128], join_s[SHARED ? AST_MOST_SPLITS : 1][SHARED ? 64 : 128];      // maxima and sums of this block's rows; factors of the rows it stores
+  __shared__ int place_s[SHARED ? 64 : 128];      // and where those lie in out, from the tile's first row and head on (-1: nowhere)
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_s;
   volatile int* abort_flag = &abort_s;
@@ -115,9 +118,9 @@ attention_stream_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gr
   const int n_pages = nf + (key_hi - 1) / PAGE - jb0 + 1, n_all = (n_pages + 1) / 2;
   if (!live) {   // a padding sequence: its rows are zero
     pdl_wait();
-    for (int idx = split * blockDim.x + threadIdx.x; idx < rows * G * (HD / 8); idx += n_splits * blockDim.x) {
-      const int i = idx / (G * (HD / 8)), rest = idx % (G * (HD / 8));
-      reinterpret_cast<uint4*>(out + ((m_base + i) * nh + h0) * HD)[rest] = make_uint4(0, 0, 0, 0);
+    for (int idx = split * blockDim.x + threadIdx.x; idx < rows * G * (vd / 8); idx += n_splits * blockDim.x) {
+      const int i = idx / (G * (vd / 8)), rest = idx % (G * (vd / 8));
+      reinterpret_cast<uint4*>(out + ((m_base + i) * nh + h0) * vd)[rest] = make_uint4(0, 0, 0, 0);
     }
     return;
   }
@@ -161,23 +164,37 @@ attention_stream_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gr
         if (n_it > 0) mbar_expect_tx(&q_full, G * HALVES * TP * 128);
         for (int g = 0; g < G && n_it > 0; g++)
           for (int h = 0; h < HALVES; h++)
-            tma_load_2d(sq + h * (128 * 128) + g * (TP * 128), &map_q, &q_full, (h0 + g) * HD + h * 64, (int)m_base);
-        auto page_of = [&](int v) { v += 2 * it0; return v < n_pages ? max(table[v < nf ? v : jb0 + v - nf], 0) : -1; };   // (a page given back: every key of it is masked)
-        int p0 = page_of(0), p1 = page_of(1);
+            if (hd == HD) tma_load_2d(sq + h * (128 * 128) + g * (TP * 128), &map_q, &q_full, (h0 + g) * HD + h * 64, (int)m_base);
+            else tma_load_3d(sq + h * (128 * 128) + g * (TP * 128), &map_q, &q_full, h * 64, h0 + g, (int)m_base);
+        // where 64 positions lie: their head's page (-1: there are none; a page given back, of which every key is masked: 0) and which 64
+        struct At { int page, part; };
+        auto at_of = [&](int v) {
+          v += 2 * it0;
+          if (v >= n_pages) return At{-1, 0};
+          const int j = v < nf ? v : jb0 + v - nf;
+          return per_page == 1 ? At{max(table[j], 0) * nkv + kvh, 0} : At{max(table[j / per_page], 0) * nkv + kvh, j % per_page};
+        };
+        At p0 = at_of(0), p1 = at_of(1);
         for (int i = 0; i < n_it; i++) {
-          const int s = i % NS, a = p0, c = p1;
-          p0 = page_of(2 * i + 2), p1 = page_of(2 * i + 3);      // asked for before the waits below
-          const uint32_t bytes = c >= 0 ? KV_BYTES : KV_BYTES / 2;
+          const int s = i % NS;
+          const At a = p0, c = p1;
+          p0 = at_of(2 * i + 2), p1 = at_of(2 * i + 3);      // asked for before the waits below
+          const uint32_t bytes = c.page >= 0 ? KV_BYTES : KV_BYTES / 2;
           if (!mbar_wait(&k_empty[s], ((i / NS) & 1) ^ 1, abort_flag)) { atomicExch(status, 31); break; }
           mbar_expect_tx(&k_full[s], bytes);
           for (int h = 0; h < HALVES; h++) {
-            tma_load_2d(sk + s * KV_BYTES + h * (128 * 128), &map_k, &k_full[s], h * 64, (a * nkv + kvh) * PAGE);
-            if (c >= 0) tma_load_2d(sk + s * KV_BYTES + h * (128 * 128) + 64 * 128, &map_k, &k_full[s], h * 64, (c * nkv + kvh) * PAGE);
+            tma_load_2d(sk + s * KV_BYTES + h * (128 * 128), &map_k, &k_full[s], h * 64, (a.page * per_page + a.part) * PAGE);
+            if (c.page >= 0) tma_load_2d(sk + s * KV_BYTES + h * (128 * 128) + 64 * 128, &map_k, &k_full[s], h * 64, (c.page * per_page + c.part) * PAGE);
           }
           if (!mbar_wait(&v_empty[s], ((i / NS) & 1) ^ 1, abort_flag)) { atomicExch(status, 32); break; }
           mbar_expect_tx(&v_full[s], bytes);
-          tma_load_2d(sv + s * KV_BYTES, &map_v, &v_full[s], 0, (a * nkv + kvh) * HD);
-          if (c >= 0) tma_load_2d(sv + s * KV_BYTES + HD * 128, &map_v, &v_full[s], 0, (c * nkv + kvh) * HD);
+          if (vd == HD) {
+            tma_load_2d(sv + s * KV_BYTES, &map_v, &v_full[s], a.part * PAGE, a.page * HD);
+            if (c.page >= 0) tma_load_2d(sv + s * KV_BYTES + HD * 128, &map_v, &v_full[s], c.part * PAGE, c.page * HD);
+          } else {      // (a head's dimensions end inside the box: zeros behind them)
+            tma_load_3d(sv + s * KV_BYTES, &map_v, &v_full[s], a.part * PAGE, 0, a.page);
+            if (c.page >= 0) tma_load_3d(sv + s * KV_BYTES + HD * 128, &map_v, &v_full[s], c.part * PAGE, 0, c.page);
+          }
         }
       }
     } else if (warp == 9) {
@@ -230,7 +247,6 @@ attention_stream_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gr
     // ---- softmax: two threads own row r = (head r / TP, position r % TP), `half` 0 the first page of an iteration, 1 the second ----
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Shape::REGS_SOFTMAX));
     const int half = warp >> 2, r = threadIdx.x & 127, g = r / TP, pi = r % TP;
-    const bool row_valid = g < G && pi < rows;
     const int qpos = q_lo + pi;
     const int key_lo_row = first_key(qpos, window, chunk);
     const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
@@ -365,11 +381,12 @@ attention_stream_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gr
       l += row_s[n_it & 1][half ^ 1][r];
     }
     tc_fence_after();
-    if (!SHARED) {
+    if (!SHARED && vd == HD && !(gate && gate_elem)) {      // every thread stores its half of a row
       if (ok) {
+        const bool row_valid = g < G && pi < rows;
         float inv = l > 0.f ? 1.0f / l : 0.f;
         if (sinks && row_valid) inv = sink_quotient(m_used * 0.6931471805599453f, l, sinks[h0 + g]);
-        if (gate && !gate_elem && row_valid) inv *= head_gate(gate, m_base + pi, gate_stride, h0 + g, 0, HD, 0);
+        if (gate && row_valid) inv *= head_gate(gate, m_base + pi, gate_stride, h0 + g, 0, HD, 0);
 #pragma unroll
         for (int d0 = 0; d0 < HD / 2; d0 += 32) {
           __syncwarp();      // idle rows left the branch below early: the loads take the whole warp
@@ -377,20 +394,13 @@ attention_stream_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gr
           tmem_ld32(t_o + d0, o);
           tmem_ld_wait();
           if (row_valid) {
-            const int d = half * (HD / 2) + d0;
-            uint4* orow = reinterpret_cast<uint4*>(out + ((m_base + pi) * nh + h0 + g) * HD + d);
-#pragma unroll
-            for (int c = 0; c < 32; c++) {
-              float x = __uint_as_float(o[c]) * inv;
-              if (gate && gate_elem) x *= head_gate(gate, m_base + pi, gate_stride, h0 + g, d + c, HD, 1);
-              o[c] = __float_as_uint(x);
-            }
+            uint4* orow = reinterpret_cast<uint4*>(out + ((m_base + pi) * nh + h0 + g) * HD + half * (HD / 2) + d0);
 #pragma unroll
             for (int c = 0; c < 32; c += 8) {
               uint32_t w[4];
 #pragma unroll
               for (int e = 0; e < 4; e++) {
-                __nv_bfloat162 pp = __floats2bfloat162_rn(__uint_as_float(o[c + 2 * e]), __uint_as_float(o[c + 2 * e + 1]));
+                __nv_bfloat162 pp = __floats2bfloat162_rn(__uint_as_float(o[c + 2 * e]) * inv, __uint_as_float(o[c + 2 * e + 1]) * inv);
                 w[e] = *reinterpret_cast<uint32_t*>(&pp);
               }
               orow[c / 8] = make_uint4(w[0], w[1], w[2], w[3]);
@@ -399,8 +409,8 @@ attention_stream_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gr
         }
       }
     } else {
-      // The blocks of a tile (a cluster) lay their rows of O, their maxima and sums out in their shared memory (keys and values are done
-      // with); each then joins 128 / n_splits rows, reading from all of them, in the blocks' order.
+      // Rows of O, their maxima and sums go to shared memory (keys and values are done with), from where they are stored row by row.  The
+      // blocks that share a tile each join 128 / n_splits of its rows, reading from all of them, in the blocks' order.
       float* so = reinterpret_cast<float*>(sk);      // [row][16-byte pieces moved by row & 7]
       const bool any = ok && n_it > 0;
       if (half == 0) {
@@ -408,53 +418,58 @@ attention_stream_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gr
         last_s[1][r] = any ? l : 0.f;
       }
       if (any) {
-#pragma unroll
+  #pragma unroll
         for (int d0 = 0; d0 < HD / 2; d0 += 32) {
           uint32_t o[32];
           tmem_ld32(t_o + d0, o);
           tmem_ld_wait();
-#pragma unroll
+  #pragma unroll
           for (int c = 0; c < 32; c += 4) {
             const int piece = (half * (HD / 2) + d0 + c) / 4;
             *reinterpret_cast<uint4*>(so + r * HD + ((piece ^ (r & 7)) << 2)) = make_uint4(o[c], o[c + 1], o[c + 2], o[c + 3]);
           }
         }
       }
-      ast_cluster_sync();
+      if (SHARED) ast_cluster_sync();
+      else asm volatile("bar.sync 9, 256;" ::: "memory");
+      auto from = [&](const float* p, int rank) { return SHARED ? ast_remote(p, rank) : *p; };
       const int share = (128 + n_splits - 1) / n_splits, r0 = split * share, n_rows = min(share, 128 - r0);
       for (int i = threadIdx.x; i < n_rows; i += 256) {      // a row's factors, one per block
         const int row = r0 + i, gg = row / TP, ii = row % TP;
         float top = AST_NEG, sum = 0.f;
-        for (int j = 0; j < n_splits; j++) top = fmaxf(top, ast_remote(&last_s[0][row], j));
-        for (int j = 0; j < n_splits; j++) sum += ast_remote(&last_s[1][row], j) * ex2(ast_remote(&last_s[0][row], j) - top);
+        for (int j = 0; j < n_splits; j++) top = fmaxf(top, from(&last_s[0][row], j));
+        for (int j = 0; j < n_splits; j++) sum += from(&last_s[1][row], j) * ex2(from(&last_s[0][row], j) - top);
         float inv = sum > 0.f ? 1.0f / sum : 0.f;
         if (gg < G && ii < rows) {
           if (sinks) inv = sink_quotient(top * 0.6931471805599453f, sum, sinks[h0 + gg]);
-          if (gate && !gate_elem) inv *= head_gate(gate, m_base + ii, gate_stride, h0 + gg, 0, HD, 0);
+          if (gate && !gate_elem) inv *= head_gate(gate, m_base + ii, gate_stride, h0 + gg, 0, vd, 0);
         }
         for (int j = 0; j < n_splits; j++)
-          join_s[j][i] = ast_remote(&last_s[1][row], j) > 0.f ? inv * ex2(ast_remote(&last_s[0][row], j) - top) : 0.f;
+          join_s[j][i] = from(&last_s[1][row], j) > 0.f ? inv * ex2(from(&last_s[0][row], j) - top) : 0.f;
+        place_s[i] = gg < G && ii < rows ? ii * nh + gg : -1;
       }
       asm volatile("bar.sync 9, 256;" ::: "memory");
       for (int idx = threadIdx.x; idx < n_rows * (HD / 4); idx += 256) {
-        const int i = idx / (HD / 4), piece = idx % (HD / 4), row = r0 + i, gg = row / TP, ii = row % TP;
-        if (gg >= G || ii >= rows) continue;
+        const int i = idx / (HD / 4), piece = idx % (HD / 4), row = r0 + i, place = place_s[i];
+        if (place < 0 || 4 * piece >= vd) continue;
         float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
         for (int j = 0; j < n_splits; j++) {
           const float f = join_s[j][i];
           if (f == 0.f) continue;      // (that block read nothing for this row: its numbers may be anything)
-          const float4 y = ast_remote4(so + row * HD + ((piece ^ (row & 7)) << 2), j);
+          const float* at = so + row * HD + ((piece ^ (row & 7)) << 2);
+          const float4 y = SHARED ? ast_remote4(at, j) : load4(at);
           x.x += f * y.x, x.y += f * y.y, x.z += f * y.z, x.w += f * y.w;
         }
-        const size_t m = m_base + ii;
         if (gate && gate_elem) {
-          x.x *= head_gate(gate, m, gate_stride, h0 + gg, 4 * piece, HD, 1), x.y *= head_gate(gate, m, gate_stride, h0 + gg, 4 * piece + 1, HD, 1);
-          x.z *= head_gate(gate, m, gate_stride, h0 + gg, 4 * piece + 2, HD, 1), x.w *= head_gate(gate, m, gate_stride, h0 + gg, 4 * piece + 3, HD, 1);
+          const size_t m = m_base + row % TP;
+          const int h = h0 + row / TP;
+          x.x *= head_gate(gate, m, gate_stride, h, 4 * piece, vd, 1), x.y *= head_gate(gate, m, gate_stride, h, 4 * piece + 1, vd, 1);
+          x.z *= head_gate(gate, m, gate_stride, h, 4 * piece + 2, vd, 1), x.w *= head_gate(gate, m, gate_stride, h, 4 * piece + 3, vd, 1);
         }
-        store4(out + (m * nh + h0 + gg) * HD + 4 * piece, x);
+        store4(out + (m_base * nh + h0 + place) * vd + 4 * piece, x);
       }
-      ast_cluster_sync();      // no block ends while others read its memory
     }
+    if (SHARED) ast_cluster_sync();      // no block ends while others read its memory
   }
   tc_fence_before();
   __syncthreads();
@@ -480,25 +495,29 @@ static int ast_splits(int M, int B, int nh, int nkv, int window, int chunk, int 
 }
 
 // Returns 1 when the sizes are ones this kernel takes.
-LEB_API int leb_attention_stream_tc_supported(int nh, int nkv, int hd, int page_size) {
-  return (hd == 64 || hd == 128) && page_size == 64 && nkv > 0 && nh % nkv == 0 && nh / nkv <= 16;
+LEB_API int leb_attention_stream_tc_supported(int nh, int nkv, int hd, int vd, int page_size) {
+  return hd > 0 && vd > 0 && hd % 8 == 0 && vd % 8 == 0 && hd <= 128 && vd <= 128 && page_size > 0 && page_size % 64 == 0 && nkv > 0 &&
+         nh % nkv == 0 && nh / nkv <= 16;
 }
 
-template <int HD, bool SHARED>
+template <int HD, bool SHARED, bool EXACT>
 static int launch_attention_stream_tc(void* out, const void* q, int q_stride, int M, const void* k_pool, const void* v_pool, int n_pages,
                                       const int* block_table, int bt_width, const int* seq_slot, const int* seq_pos0,
                                       const int* seq_qstart, const int* seq_qlen, const void* gate, int gate_stride, int gate_elem,
-                                      int B, int nh, int nkv, int window, int chunk, int first, float scale, const float* slopes,
+                                      int B, int nh, int nkv, int hd, int vd, int page_size, int window, int chunk, int first, float scale, const float* slopes,
                                       const float* sinks, int max_qlen, int n_splits, int* status, cudaStream_t st) {
   using Shape = AstShape<HD>;
   const int G = nh / nkv, TP = ast_positions(G);
   CUtensorMap mq, mk, mv;
-  if (tensor_map(&mq, q, M, nh * HD, q_stride, TP)) return 1;
-  if (tensor_map(&mk, k_pool, n_pages * nkv * 64, HD, HD, 64)) return 1;
-  if (tensor_map(&mv, v_pool, n_pages * nkv * HD, 64, 64, HD)) return 1;
+  if (hd == HD ? tensor_map(&mq, q, M, nh * HD, q_stride, TP) : tensor_map3(&mq, "leb_attention_stream_tc", q, hd, nh, M, hd, q_stride, 1, TP)) return 1;
+  if (tensor_map(&mk, k_pool, n_pages * nkv * page_size, hd, hd, 64)) return 1;
+  if (vd == HD) {
+    // the same through a map of two dimensions
+    if (tensor_map(&mv, v_pool, n_pages * nkv * HD, page_size, page_size, HD)) return 1;
+  } else if (tensor_map3(&mv, "leb_attention_stream_tc", v_pool, page_size, vd, n_pages * nkv, page_size, (long long)vd * page_size, HD, 1)) return 1;
   dim3 grid(nkv, B, ceil_div(max_qlen, TP) * n_splits);
   LEB_REQUIRE(grid.y <= 65535 && grid.z <= 65535, "leb_attention_stream_tc: grid too large (%u, %u)", grid.y, grid.z);
-  constexpr auto kern = attention_stream_tc_kernel<HD, SHARED>;
+  constexpr auto kern = attention_stream_tc_kernel<HD, SHARED, EXACT>;
   // The warpgroups share out the registers of the launch: with fewer than REGS a thread they would wait for ever.
   static std::atomic<int> regs{0};
   if (regs.load(std::memory_order_relaxed) == 0) {
@@ -511,33 +530,37 @@ static int launch_attention_stream_tc(void* out, const void* q, int q_stride, in
   const cudaError_t e = leb_allow_smem<kern, Shape::SMEM>();
   if (e != cudaSuccess) return leb_fail("leb_attention_stream_tc: shared memory %d: %s", Shape::SMEM, cudaGetErrorString(e));
   leb_launch_cluster(SHARED ? n_splits : 1, kern, grid, dim3(Shape::THREADS), Shape::SMEM, st, mq, mk, mv, (bf16*)out, block_table, bt_width,
-                     seq_slot, seq_pos0, seq_qstart, seq_qlen, (const bf16*)gate, gate_stride, gate_elem, nh, nkv, G, TP, window, chunk, first,
+                     seq_slot, seq_pos0, seq_qstart, seq_qlen, (const bf16*)gate, gate_stride, gate_elem, nh, nkv, G, TP, hd, vd, page_size / 64, window, chunk, first,
                      scale, slopes, sinks, n_splits, status);
   LEB_CHECK_LAUNCH("leb_attention_stream_tc");
   return 0;
 }
 
 // Prompt attention of the step's rows over the paged cache (which already holds their keys and values).  q: [M, nh*hd] with row
-// stride q_stride; k_pool [n_pages][nkv][64][hd], v_pool [n_pages][nkv][hd][64]; out [M, nh*hd].  status: device int, set non-zero by a
+// stride q_stride; k_pool [n_pages][nkv][page_size][hd], v_pool [n_pages][nkv][vd][page_size]; out [M, nh*vd].  status: device int, set non-zero by a
 // block whose bounded wait gave up.  slopes, sinks [nh] or null as in leb_attention.  max_kvlen: the most positions a sequence of the step holds.
 // n_splits: blocks that share a tile's keys (0: as many as suit the step).
 LEB_API int leb_attention_stream_tc(void* out, const void* q, int q_stride, int M, const void* k_pool, const void* v_pool, int n_pages,
                                     const int* block_table, int bt_width, const int* seq_slot, const int* seq_pos0,
                                     const int* seq_qstart, const int* seq_qlen, const void* gate, int gate_stride, int gate_elem, int B,
-                                    int nh, int nkv, int hd, int page_size, int window, int chunk, int first, float scale,
+                                    int nh, int nkv, int hd, int vd, int page_size, int window, int chunk, int first, float scale,
                                     const float* slopes, const float* sinks, int max_qlen, int max_kvlen, int n_splits,
                                     int* status, cudaStream_t st) {
   if (B <= 0 || max_qlen <= 0 || M <= 0) return 0;
-  LEB_REQUIRE(leb_attention_stream_tc_supported(nh, nkv, hd, page_size),
-              "leb_attention_stream_tc: sizes not taken (heads %d, kv heads %d, head_dim %d, page %d)", nh, nkv, hd, page_size);
+  LEB_REQUIRE(leb_attention_stream_tc_supported(nh, nkv, hd, vd, page_size),
+              "leb_attention_stream_tc: sizes not taken (heads %d, kv heads %d, widths %d and %d, page %d)", nh, nkv, hd, vd, page_size);
   LEB_REQUIRE(status != nullptr, "leb_attention_stream_tc: a status word is required");
-  LEB_REQUIRE(((uintptr_t)q & 15) == 0 && q_stride % 8 == 0 && ((uintptr_t)out & 15) == 0,
-              "leb_attention_stream_tc: q and out must be 16-byte aligned, q's row stride a multiple of 8");
+  LEB_REQUIRE((((uintptr_t)q | (uintptr_t)out | (uintptr_t)k_pool | (uintptr_t)v_pool) & 15) == 0 && q_stride % 8 == 0,
+              "leb_attention_stream_tc: q, out and the pools must be 16-byte aligned, q's row stride a multiple of 8");
   LEB_REQUIRE(n_splits >= 0 && n_splits <= AST_MOST_SPLITS, "leb_attention_stream_tc: %d blocks for a tile's keys, %d at most", n_splits, AST_MOST_SPLITS);
   if (n_splits == 0) n_splits = ast_splits(M, B, nh, nkv, window, chunk, first, max_qlen, max_kvlen);
 #define LEB_AST_ARGS out, q, q_stride, M, k_pool, v_pool, n_pages, block_table, bt_width, seq_slot, seq_pos0, seq_qstart, seq_qlen, gate, \
-                     gate_stride, gate_elem, B, nh, nkv, window, chunk, first, scale, slopes, sinks, max_qlen, n_splits, status, st
-  if (n_splits > 1) return hd == 64 ? launch_attention_stream_tc<64, true>(LEB_AST_ARGS) : launch_attention_stream_tc<128, true>(LEB_AST_ARGS);
-  return hd == 64 ? launch_attention_stream_tc<64, false>(LEB_AST_ARGS) : launch_attention_stream_tc<128, false>(LEB_AST_ARGS);
+                     gate_stride, gate_elem, B, nh, nkv, hd, vd, page_size, window, chunk, first, scale, slopes, sinks, max_qlen, n_splits, status, st
+  const bool exact = page_size == 64 && hd == vd && (hd == 64 || hd == 128), narrow = hd <= 64 && vd <= 64;
+#define LEB_AST(HD_, SHARED_) \
+  (exact ? launch_attention_stream_tc<HD_, SHARED_, true>(LEB_AST_ARGS) : launch_attention_stream_tc<HD_, SHARED_, false>(LEB_AST_ARGS))
+  if (n_splits > 1) return narrow ? LEB_AST(64, true) : LEB_AST(128, true);
+  return narrow ? LEB_AST(64, false) : LEB_AST(128, false);
+#undef LEB_AST
 #undef LEB_AST_ARGS
 }

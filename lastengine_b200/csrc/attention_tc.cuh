@@ -76,3 +76,54 @@ __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 __device__ __forceinline__ void fence_proxy_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+__device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, uint64_t* bar, int x, int y, int z) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+      ::"r"(smem_u32(dst)), "l"((uint64_t)map), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z)
+      : "memory");
+}
+
+struct MapKey3 {
+  const void* ptr;
+  int n[3];
+  long long ld[2];
+  int box[2];
+  bool operator==(const MapKey3& o) const {
+    return ptr == o.ptr && n[0] == o.n[0] && n[1] == o.n[1] && n[2] == o.n[2] && ld[0] == o.ld[0] && ld[1] == o.ld[1] && box[0] == o.box[0] &&
+           box[1] == o.box[1];
+  }
+};
+struct MapKey3Hash {
+  size_t operator()(const MapKey3& k) const {
+    size_t h = std::hash<const void*>()(k.ptr);
+    for (long long v : {(long long)k.n[0], (long long)k.n[1], (long long)k.n[2], k.ld[0], k.ld[1], (long long)k.box[0], (long long)k.box[1]})
+      h = h * 1000003u ^ std::hash<long long>()(v);
+    return h;
+  }
+};
+
+// A [n2][n1][n0] bfloat16 array with strides ld1, ld0 (elements) of its two outer indexes, read in boxes of 64 numbers x box1 x box2 under the
+// 128-byte swizzle; out-of-range elements read as zero.
+static int tensor_map3(CUtensorMap* out, const char* who, const void* ptr, int n0, int n1, int n2, long long ld0, long long ld1, int box1, int box2) {
+  static std::unordered_map<MapKey3, CUtensorMap, MapKey3Hash> cache;
+  static std::mutex mu;
+  const MapKey3 key{ptr, {n0, n1, n2}, {ld0, ld1}, {box1, box2}};
+  std::lock_guard<std::mutex> g(mu);
+  auto it = cache.find(key);
+  if (it != cache.end()) {
+    *out = it->second;
+    return 0;
+  }
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return leb_fail("%s: the driver has no cuTensorMapEncodeTiled", who);
+  cuuint64_t dims[3] = {(cuuint64_t)n0, (cuuint64_t)n1, (cuuint64_t)n2};
+  cuuint64_t strides[2] = {(cuuint64_t)ld0 * 2, (cuuint64_t)ld1 * 2};
+  cuuint32_t box[3] = {64, (cuuint32_t)box1, (cuuint32_t)box2}, estr[3] = {1, 1, 1};
+  const CUresult r = fn(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return leb_fail("%s: cuTensorMapEncodeTiled failed (%d) for [%d,%d,%d]", who, (int)r, n2, n1, n0);
+  if (cache.size() > 4096) cache.clear();
+  cache[key] = *out;
+  return 0;
+}

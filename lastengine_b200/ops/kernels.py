@@ -311,8 +311,8 @@ def _declare(L) -> None:
         "leb_attention_pooled_tc": [P, P, I, I, P, P, I, P, I, P, P, I, P, I, P, P, P, P, P, P, I, I, I, I, I, I, I, I, I, P, P],
         "leb_attention_pooled_tc_value_dim": [I],
         "leb_attention_prefill": [P, P, P, P, P, I, P, P, P, P, P, I, I, I, I, I, I, I, I, I, I, I, F, P, P, I, P],
-        "leb_attention_stream_tc_supported": [I, I, I, I],
-        "leb_attention_stream_tc": [P, P, I, I, P, P, I, P, I, P, P, P, P, P, I, I, I, I, I, I, I, I, I, I, F, P, P, I, I, I, P, P],
+        "leb_attention_stream_tc_supported": [I, I, I, I, I],
+        "leb_attention_stream_tc": [P, P, I, I, P, P, I, P, I, P, P, P, P, P, I, I, I, I, I, I, I, I, I, I, I, F, P, P, I, I, I, P, P],
         "leb_attention_stream_f32_supported": [I, I, I, I, I],
         "leb_attention_stream_f32": [P, P, P, P, P, I, P, P, P, P, I, I, I, I, I, I, I, I, I, I, I, F, P, P, I, I, P],
         "leb_stream_tables": [P, I, P, P, P, P, P, P, P, P, P, P, I, P, I, P, I, P, I, I, I, P],
@@ -1703,6 +1703,10 @@ def attention(out: torch.Tensor, q: torch.Tensor | None, k_pool: torch.Tensor, v
             and (k_pool.data_ptr() | v_pool.data_ptr()) & 15 == 0 and lib().leb_attention_stream_f32_supported(nh, nkv, hd, vd or hd, page_size)):
         return _attention_stream_f32(out, q, k_pool, v_pool, block_table, batch, nh, nkv, hd, int(vd or hd), page_size, window, scale, gate,
                                      chunk, slopes, sinks, first)
+    if (first > 0 and raw is None and not wide and out.dtype == torch.bfloat16 and batch.max_qlen > 1 and q.stride(0) % 8 == 0
+            and lib().leb_attention_stream_tc_supported(nh, nkv, hd, vd or hd, page_size)):
+        return _attention_stream_tc(out, q, k_pool, v_pool, block_table, batch, nh, nkv, hd, int(vd or hd), page_size, window, scale, gate,
+                                    chunk, slopes, sinks, first)
     if vd is not None and vd != hd:
         return _attention_general(out, q, k_pool, v_pool, block_table, batch, nh, nkv, hd, int(vd), page_size, window,
                                   scale, gate, n_splits, scratch, chunk, slopes, sinks, first)
@@ -1734,14 +1738,6 @@ def attention(out: torch.Tensor, q: torch.Tensor | None, k_pool: torch.Tensor, v
         if n_splits > 1:
             _check(L.leb_attention_merge(_ptr(out), _ptr(scratch), BF16, _ptr(gate), gate_stride, gate_elem, _ptr(sinks), M,
                                          nh, hd, n_splits, _stream()))
-        return
-    if (first > 0 and not wide and out.dtype == torch.bfloat16 and batch.max_qlen > 1
-            and q.stride(0) % 8 == 0 and L.leb_attention_stream_tc_supported(nh, nkv, hd, page_size)):
-        _check(L.leb_attention_stream_tc(
-            _ptr(out), _ptr(q), q.stride(0), M, _ptr(k_pool), _ptr(v_pool), k_pool.shape[0], _ptr(block_table),
-            block_table.shape[1], _ptr(batch.seq_slot), _ptr(batch.seq_pos0), _ptr(batch.seq_qstart),
-            _ptr(batch.seq_qlen), _ptr(gate), gate_stride, gate_elem, batch.n_seqs, nh, nkv, hd, page_size, window, chunk,
-            first, float(scale), _ptr(slopes), _ptr(sinks), batch.max_qlen, batch.max_kvlen, _stream_splits, _ptr(_status_word(out.device)), _stream()))
         return
     if (out.dtype == torch.bfloat16 and n_splits == 1 and batch.max_qlen >= TC_ATTENTION_MIN_ROWS
             and q.stride(0) % 8 == 0 and L.leb_attention_prefill_tc_supported(nh, nkv, hd, page_size)):
@@ -1783,6 +1779,24 @@ def _attention_stream_f32(out, q, k_pool, v_pool, block_table, batch, nh, nkv, h
         _ptr(out), _ptr(q), _ptr(k_pool), _ptr(v_pool), _ptr(block_table), block_table.shape[1], _ptr(batch.seq_slot), _ptr(batch.seq_pos0),
         _ptr(batch.seq_qstart), _ptr(gate), gate_stride, gate_elem, batch.n_seqs, nh, nkv, hd, vd, page_size, window, chunk, first,
         float(scale), _ptr(slopes), _ptr(sinks), batch.max_kvlen, _stream_splits, _stream()))
+
+
+def _attention_stream_tc(out, q, k_pool, v_pool, block_table, batch, nh, nkv, hd, vd, page_size, window, scale, gate, chunk, slopes, sinks,
+                         first) -> None:
+    """Prompts with first positions over a bfloat16 cache: tcgen05 tiles, a cluster's blocks per tile where there are few."""
+    _cuda(q, "attention.q", torch.bfloat16)
+    _cuda(k_pool, "attention.k_pool", torch.bfloat16)
+    _cuda(v_pool, "attention.v_pool", torch.bfloat16)
+    _cuda(block_table, "attention.block_table", torch.int32)
+    M = out.shape[0]
+    assert out.shape == (M, nh * vd) and q.shape == (M, nh * hd)
+    assert k_pool.shape[1:] == (nkv, page_size, hd) and v_pool.shape[1:] == (nkv, vd, page_size)
+    gate_stride, gate_elem = _gate_layout(gate, M, nh, vd, out.dtype)
+    _check(lib().leb_attention_stream_tc(
+        _ptr(out), _ptr(q), q.stride(0), M, _ptr(k_pool), _ptr(v_pool), k_pool.shape[0], _ptr(block_table), block_table.shape[1],
+        _ptr(batch.seq_slot), _ptr(batch.seq_pos0), _ptr(batch.seq_qstart), _ptr(batch.seq_qlen), _ptr(gate), gate_stride, gate_elem,
+        batch.n_seqs, nh, nkv, hd, vd, page_size, window, chunk, first, float(scale), _ptr(slopes), _ptr(sinks), batch.max_qlen,
+        batch.max_kvlen, _stream_splits, _ptr(_status_word(out.device)), _stream()))
 
 
 def _attention_general(out, q, k_pool, v_pool, block_table, batch, nh, nkv, hd, vd, page_size, window, scale, gate,

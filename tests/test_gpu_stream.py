@@ -141,7 +141,9 @@ def test_single_tokens(dtype, nh, nkv, hd, vd, page, window, first):
     (BF16, 8, 2, 64, 64, 64), (BF16, 3, 3, 64, 64, 64), (BF16, 8, 1, 64, 64, 64), (BF16, 4, 2, 64, 64, 64), (BF16, 3, 1, 64, 64, 64),
     (BF16, 4, 2, 32, 32, 32), (BF16, 8, 2, 128, 128, 64), (BF16, 3, 3, 128, 128, 64), (BF16, 8, 1, 128, 128, 64), (BF16, 5, 1, 128, 128, 64),
     (BF16, 2, 2, 96, 96, 64), (BF16, 16, 1, 64, 64, 64), (BF16, 2, 1, 64, 64, 128), (BF16, 4, 2, 80, 80, 64), (BF16, 2, 1, 64, 32, 64),
-    (F32, 4, 2, 64, 64, 64), (F32, 6, 2, 80, 48, 32)])
+    (BF16, 4, 2, 128, 128, 128),
+    (BF16, 2, 1, 8, 128, 192), (BF16, 3, 1, 72, 40, 64), (BF16, 4, 4, 32, 96, 64), (BF16, 2, 1, 64, 20, 64), (BF16, 34, 2, 64, 64, 64),
+    (BF16, 2, 1, 192, 192, 64), (F32, 4, 2, 64, 64, 64), (F32, 6, 2, 80, 48, 32)])
 @pytest.mark.parametrize("window,first", WINDOWS)
 def test_chunks_of_tokens(dtype, nh, nkv, hd, vd, page, window, first):
     c = Case(CHUNKS, nh, nkv, hd, vd, page, window, first, dtype, seed=window + first, padding=[5])
@@ -150,14 +152,14 @@ def test_chunks_of_tokens(dtype, nh, nkv, hd, vd, page, window, first):
     assert torch.equal(a, c.run())
 
 
-@pytest.mark.parametrize("nh,nkv,hd", [(8, 2, 64), (3, 3, 64), (8, 2, 128), (5, 1, 128)])
+@pytest.mark.parametrize("nh,nkv,hd,vd", [(8, 2, 64, 64), (3, 3, 64, 64), (8, 2, 128, 128), (5, 1, 128, 128), (4, 2, 72, 40)])
 @pytest.mark.parametrize("window,first", [(1, 1), (64, 64), (300, 33), (33, 1000), (900, 4)])
-def test_blocks_that_share_a_tile_s_keys(nh, nkv, hd, window, first):
+def test_blocks_that_share_a_tile_s_keys(nh, nkv, hd, vd, window, first):
     """1 to 8 blocks for the keys of a tile, also where some of them get none; with sinks and gates, which the join takes."""
-    c = Case(CHUNKS + [(1500, 20), (0, 3)], nh, nkv, hd, hd, 64, window, first, BF16, seed=window, padding=[5])
+    c = Case(CHUNKS + [(1500, 20), (0, 3)], nh, nkv, hd, vd, 64, window, first, BF16, seed=window, padding=[5])
     g = torch.Generator().manual_seed(1)
     sinks, gate = torch.randn(nh, generator=g), torch.randn(c.rows, nh, generator=g).to(BF16)
-    numbers = torch.randn(c.rows, nh * hd, generator=g).to(BF16)
+    numbers = torch.randn(c.rows, nh * vd, generator=g).to(BF16)
     try:
         for n in (1, 2, 3, 5, 8):
             K().set_stream_attention_splits(n)
@@ -165,7 +167,7 @@ def test_blocks_that_share_a_tile_s_keys(nh, nkv, hd, window, first):
             c.check(a)
             assert torch.equal(a, c.run())
             c.check(c.run(sinks=sinks.to(DEV), gate=gate.to(DEV)), sinks=sinks.double(), factor=torch.sigmoid(gate.double())[:, :, None])
-            c.check(c.run(gate=numbers.to(DEV)), factor=torch.sigmoid(numbers.double()).view(c.rows, nh, hd))
+            c.check(c.run(gate=numbers.to(DEV)), factor=torch.sigmoid(numbers.double()).view(c.rows, nh, vd))
     finally:
         K().set_stream_attention_splits(0)
 
