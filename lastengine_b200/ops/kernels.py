@@ -1699,14 +1699,11 @@ def attention(out: torch.Tensor, q: torch.Tensor | None, k_pool: torch.Tensor, v
         if t is not None:
             _cuda(t, f"attention.{name}", torch.float32)
             assert t.numel() == nh
-    if (first > 0 and raw is None and out.dtype == torch.float32 and batch.max_qlen == 1 and out.shape[0] == batch.n_seqs
-            and (k_pool.data_ptr() | v_pool.data_ptr()) & 15 == 0 and lib().leb_attention_stream_f32_supported(nh, nkv, hd, vd or hd, page_size)):
-        return _attention_stream_f32(out, q, k_pool, v_pool, block_table, batch, nh, nkv, hd, int(vd or hd), page_size, window, scale, gate,
-                                     chunk, slopes, sinks, first)
-    if (first > 0 and raw is None and not wide and out.dtype == torch.bfloat16 and batch.max_qlen > 1 and q.stride(0) % 8 == 0
-            and lib().leb_attention_stream_tc_supported(nh, nkv, hd, vd or hd, page_size)):
-        return _attention_stream_tc(out, q, k_pool, v_pool, block_table, batch, nh, nkv, hd, int(vd or hd), page_size, window, scale, gate,
-                                    chunk, slopes, sinks, first)
+    if first > 0 and raw is None:
+        form = _stream_form(out, batch, nh, nkv, hd, vd or hd, page_size, wide, q, k_pool, v_pool)
+        if form is not None:
+            return form(out, q, k_pool, v_pool, block_table, batch, nh, nkv, hd, vd or hd, page_size, window, float(scale), gate, chunk, slopes, sinks,
+                        first, wide, n_splits, scratch)
     if vd is not None and vd != hd:
         return _attention_general(out, q, k_pool, v_pool, block_table, batch, nh, nkv, hd, int(vd), page_size, window,
                                   scale, gate, n_splits, scratch, chunk, slopes, sinks, first)
@@ -1764,39 +1761,78 @@ def attention(out: torch.Tensor, q: torch.Tensor | None, k_pool: torch.Tensor, v
         hd, page_size, window, chunk, first, float(scale), _ptr(slopes), _ptr(sinks), batch.max_qlen, n_splits, hd, _stream()))
 
 
-def _attention_stream_f32(out, q, k_pool, v_pool, block_table, batch, nh, nkv, hd, vd, page_size, window, scale, gate, chunk, slopes, sinks,
-                          first) -> None:
-    """A decode step over a 32-bit cache with first positions: the blocks of a sequence join their sums by themselves."""
-    _cuda(q, "attention.q", torch.float32)
-    _cuda(k_pool, "attention.k_pool", torch.float32)
-    _cuda(v_pool, "attention.v_pool", torch.float32)
-    _cuda(block_table, "attention.block_table", torch.int32)
+@functools.lru_cache(maxsize=256)
+def _stream_takes(entry: str, *sizes: int) -> bool:
+    return bool(getattr(lib(), entry)(*sizes))
+
+
+def _stream_form(out, batch, nh, nkv, hd, vd, page_size, wide, q, k_pool, v_pool):
+    """The kernel made for rows with first positions that takes a step, None where the ones for all rows do."""
+    if batch.max_qlen == 1:
+        if out.shape[0] != batch.n_seqs:
+            return None
+        if out.dtype is torch.bfloat16:
+            return _attention_stream_decode if vd == hd and _stream_takes("leb_attention_decode_supported", nh, nkv, hd, page_size) else None
+        return _attention_stream_f32 if (k_pool.data_ptr() | v_pool.data_ptr()) & 15 == 0 \
+            and _stream_takes("leb_attention_stream_f32_supported", nh, nkv, hd, vd, page_size) else None
+    if out.dtype is torch.bfloat16 and not wide and q.stride(0) % 8 == 0 \
+            and _stream_takes("leb_attention_stream_tc_supported", nh, nkv, hd, vd, page_size):
+        return _attention_stream_tc
+    return None
+
+
+def _stream_operands(out, q, k_pool, v_pool, block_table, nh, nkv, hd, vd, page_size) -> int:
+    """Checks what every one of these kernels takes; the step's rows."""
+    dtype, ks, vs = out.dtype, k_pool.shape, v_pool.shape
+    for t in (q, k_pool, v_pool):
+        if t.dtype is not dtype or not t.is_cuda or not t.is_contiguous():
+            raise KernelError(f"attention: contiguous {dtype} tensors on a CUDA device, got {t.dtype} {tuple(t.shape)} on {t.device}")
+    _words("attention.block_table", block_table)
     M = out.shape[0]
-    assert out.shape == (M, nh * vd) and q.shape == (M, nh * hd)
-    assert k_pool.shape[1:] == (nkv, page_size, hd) and v_pool.shape[1:] == (nkv, vd, page_size)
+    assert out.shape[1] == nh * vd and q.shape[0] == M and q.shape[1] == nh * hd
+    assert ks[1] == vs[1] == nkv and ks[2] == vs[3] == page_size and ks[3] == hd and vs[2] == vd
+    return M
+
+
+def _attention_stream_decode(out, q, k_pool, v_pool, block_table, batch, nh, nkv, hd, vd, page_size, window, scale, gate, chunk, slopes, sinks,
+                             first, wide, n_splits, scratch) -> None:
+    """A decode step over a bfloat16 cache with first positions: the tensor-core decode kernel; without splits of the caller's the blocks of a
+    sequence join their sums by themselves."""
+    M = _stream_operands(out, q, k_pool, v_pool, block_table, nh, nkv, hd, vd, page_size)
+    gate_stride, gate_elem = _gate_layout(gate, M, nh, hd, out.dtype)
+    if n_splits > 1 and (scratch is None or scratch.numel() < M * nh * n_splits * (hd + 2) or scratch.dtype is not torch.float32):
+        raise KernelError(f"attention: {n_splits} splits need {M * nh * n_splits * (hd + 2)} floats of scratch")
+    L = lib()
+    _check(L.leb_attention_decode(
+        out.data_ptr(), _ptr(scratch), q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), block_table.data_ptr(), block_table.shape[1],
+        batch.seq_slot.data_ptr(), batch.seq_pos0.data_ptr(), batch.seq_qstart.data_ptr(), _ptr(gate), gate_stride, gate_elem, M, nh, nkv, hd,
+        page_size, window, chunk, first, int(wide), scale, _ptr(slopes), _ptr(sinks), n_splits, batch.max_kvlen, _stream_splits, _stream()))
+    if n_splits > 1:
+        _check(L.leb_attention_merge(out.data_ptr(), scratch.data_ptr(), BF16, _ptr(gate), gate_stride, gate_elem, _ptr(sinks), M, nh, hd, n_splits,
+                                     _stream()))
+
+
+def _attention_stream_f32(out, q, k_pool, v_pool, block_table, batch, nh, nkv, hd, vd, page_size, window, scale, gate, chunk, slopes, sinks,
+                          first, wide, n_splits, scratch) -> None:
+    """A decode step over a 32-bit cache with first positions: the blocks of a sequence join their sums by themselves."""
+    M = _stream_operands(out, q, k_pool, v_pool, block_table, nh, nkv, hd, vd, page_size)
     gate_stride, gate_elem = _gate_layout(gate, M, nh, vd, out.dtype)
     _check(lib().leb_attention_stream_f32(
-        _ptr(out), _ptr(q), _ptr(k_pool), _ptr(v_pool), _ptr(block_table), block_table.shape[1], _ptr(batch.seq_slot), _ptr(batch.seq_pos0),
-        _ptr(batch.seq_qstart), _ptr(gate), gate_stride, gate_elem, batch.n_seqs, nh, nkv, hd, vd, page_size, window, chunk, first,
-        float(scale), _ptr(slopes), _ptr(sinks), batch.max_kvlen, _stream_splits, _stream()))
+        out.data_ptr(), q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), block_table.data_ptr(), block_table.shape[1],
+        batch.seq_slot.data_ptr(), batch.seq_pos0.data_ptr(), batch.seq_qstart.data_ptr(), _ptr(gate), gate_stride, gate_elem, M, nh, nkv, hd, vd,
+        page_size, window, chunk, first, scale, _ptr(slopes), _ptr(sinks), batch.max_kvlen, _stream_splits, _stream()))
 
 
 def _attention_stream_tc(out, q, k_pool, v_pool, block_table, batch, nh, nkv, hd, vd, page_size, window, scale, gate, chunk, slopes, sinks,
-                         first) -> None:
+                         first, wide, n_splits, scratch) -> None:
     """Prompts with first positions over a bfloat16 cache: tcgen05 tiles, a cluster's blocks per tile where there are few."""
-    _cuda(q, "attention.q", torch.bfloat16)
-    _cuda(k_pool, "attention.k_pool", torch.bfloat16)
-    _cuda(v_pool, "attention.v_pool", torch.bfloat16)
-    _cuda(block_table, "attention.block_table", torch.int32)
-    M = out.shape[0]
-    assert out.shape == (M, nh * vd) and q.shape == (M, nh * hd)
-    assert k_pool.shape[1:] == (nkv, page_size, hd) and v_pool.shape[1:] == (nkv, vd, page_size)
+    M = _stream_operands(out, q, k_pool, v_pool, block_table, nh, nkv, hd, vd, page_size)
     gate_stride, gate_elem = _gate_layout(gate, M, nh, vd, out.dtype)
     _check(lib().leb_attention_stream_tc(
-        _ptr(out), _ptr(q), q.stride(0), M, _ptr(k_pool), _ptr(v_pool), k_pool.shape[0], _ptr(block_table), block_table.shape[1],
-        _ptr(batch.seq_slot), _ptr(batch.seq_pos0), _ptr(batch.seq_qstart), _ptr(batch.seq_qlen), _ptr(gate), gate_stride, gate_elem,
-        batch.n_seqs, nh, nkv, hd, vd, page_size, window, chunk, first, float(scale), _ptr(slopes), _ptr(sinks), batch.max_qlen,
-        batch.max_kvlen, _stream_splits, _ptr(_status_word(out.device)), _stream()))
+        out.data_ptr(), q.data_ptr(), q.stride(0), M, k_pool.data_ptr(), v_pool.data_ptr(), k_pool.shape[0], block_table.data_ptr(),
+        block_table.shape[1], batch.seq_slot.data_ptr(), batch.seq_pos0.data_ptr(), batch.seq_qstart.data_ptr(), batch.seq_qlen.data_ptr(),
+        _ptr(gate), gate_stride, gate_elem, batch.n_seqs, nh, nkv, hd, vd, page_size, window, chunk, first, scale, _ptr(slopes), _ptr(sinks),
+        batch.max_qlen, batch.max_kvlen, _stream_splits, _ptr(_status_word(out.device)), _stream()))
 
 
 def _attention_general(out, q, k_pool, v_pool, block_table, batch, nh, nkv, hd, vd, page_size, window, scale, gate,
@@ -1937,20 +1973,20 @@ def store_rows(k_pool: torch.Tensor, v_pool: torch.Tensor, k: torch.Tensor, v: t
     """Keys `k` [M, kv heads * width] and values `v` [M, kv heads * value width] into the paged cache: row m at place
     slot_map[m] % page size of page slot_map[m] / page size, -1 nowhere (int32 [M]; no place is named twice).  k and v may be
     column slices of one fused projection; k_pool [page, kv head, place, width], v_pool [page, kv head, value width, place]."""
-    _cuda(k_pool, "store_rows.k_pool")
     dt = _dt(k_pool, "store_rows")
-    _cuda(v_pool, "store_rows.v_pool", k_pool.dtype)
-    _cuda(k, "store_rows.k", k_pool.dtype, contiguous=False)
-    _cuda(v, "store_rows.v", k_pool.dtype, contiguous=False)
-    _cuda(slot_map, "store_rows.slot_map", torch.int32)
+    for x, dense in ((k_pool, True), (v_pool, True), (k, False), (v, False)):
+        if x.dtype is not k_pool.dtype or not x.is_cuda or (dense and not x.is_contiguous()):
+            raise KernelError(f"store_rows: {k_pool.dtype} tensors on a CUDA device (pools contiguous), got {x.dtype} {tuple(x.shape)} on {x.device}")
+    _words("store_rows.slot_map", slot_map)
     n_pages, nkv, P, hd = k_pool.shape
-    vd, M = v_pool.shape[2], slot_map.numel()
-    if v_pool.shape != (n_pages, nkv, vd, P) or k.shape != (M, nkv * hd) or v.shape != (M, nkv * vd):
+    M, vs, ks = slot_map.numel(), v_pool.shape, k.shape
+    vd = vs[2]
+    if vs[0] != n_pages or vs[1] != nkv or vs[3] != P or ks[0] != M or ks[1] != nkv * hd or v.shape[0] != M or v.shape[1] != nkv * vd:
         raise KernelError(f"store_rows: {M} rows of {tuple(k.shape)} and {tuple(v.shape)} into pools {tuple(k_pool.shape)} and {tuple(v_pool.shape)}")
     if M > 0 and (k.stride(1) != 1 or v.stride(1) != 1):
         raise KernelError("store_rows: the numbers of a row must lie one behind the other")
-    _check(lib().leb_store_rows(_ptr(k_pool), _ptr(v_pool), _ptr(k), k.stride(0), _ptr(v), v.stride(0), dt, _ptr(slot_map), n_pages, M,
-                                nkv, hd, vd, P, _stream()))
+    _check(lib().leb_store_rows(k_pool.data_ptr(), v_pool.data_ptr(), k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0), dt,
+                                slot_map.data_ptr(), n_pages, M, nkv, hd, vd, P, _stream()))
 
 
 # ----------------------------------------------------------------------------------------------

@@ -582,3 +582,15 @@ def test_a_model_whose_windowed_layers_see_first_positions(name, cfg, dtype, bf1
     params = SamplingParams(temperature=0.0)
     with_graphs = eng.generate(requests, params, max_new_tokens=40, use_graphs=True).tokens
     assert with_graphs == eng.generate(requests, params, max_new_tokens=40, use_graphs=False).tokens
+
+
+def test_the_example_runs():
+    import os
+    import subprocess
+    import sys
+    env = dict(os.environ, PYTHONPATH=H.ROOT)
+    r = subprocess.run([sys.executable, os.path.join(H.ROOT, "examples", "endless_stream.py"), "--streams", "3", "--steps", "500", "--window", "130",
+                        "--prompt", "70", "--layers", "2"], env=env, cwd=H.ROOT, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]
+    held = [int(x) for x in r.stdout.split("[")[1].split("]")[0].split(",")]
+    assert max(held[2:]) <= 3 * 5 and "571 positions" in r.stdout
