@@ -1,5 +1,6 @@
-// Decode attention of 32-bit caches with first positions: one new token per sequence against its window and its sequence's first
-// positions (first_tiles in common.cuh), any width of key and value heads up to 256.
+// Decode attention with first positions for 32-bit caches, and for bfloat16 caches of heads that the tensor-core kernel does not take: one
+// new token per sequence against its window and its sequence's first positions (first_tiles in common.cuh), any width of key and value
+// heads up to 256.
 //
 // A decode step reads every visible key and value once, so the kernel is built around that stream, as the bfloat16 one is
 // (attention_decode.cu): a block owns one sequence, up to HC query heads of one kv head and one share of the keys; its warps take tiles of
@@ -68,16 +69,16 @@ __device__ __forceinline__ float asf_max(float v) {      // over the warp
   return m;
 }
 
-// D: heads of up to D numbers; HC: query heads of a block (1, 2 or 4); VEC: keys are read in pieces of 16 bytes (hd a multiple of 4).
-template <int D, int HC, bool VEC>
+// T: the cache's numbers; D: heads of up to D numbers; HC: query heads of a block (1, 2 or 4); VEC: a key is a number of 16-byte pieces.
+template <typename T, int D, int HC, bool VEC>
 __global__ void __launch_bounds__(128, D <= 64 ? 3 : D <= 128 ? 2 : 1)
-attention_stream_f32_kernel(float* __restrict__ out, const float* __restrict__ q, const float* __restrict__ k_pool,
-                            const float* __restrict__ v_pool, const int* __restrict__ block_table, int bt_width,
+attention_stream_any_kernel(T* __restrict__ out, const T* __restrict__ q, const T* __restrict__ k_pool,
+                            const T* __restrict__ v_pool, const int* __restrict__ block_table, int bt_width,
                             const int* __restrict__ seq_slot, const int* __restrict__ seq_pos0, const int* __restrict__ seq_qstart,
-                            const float* __restrict__ gate, int gate_stride, int gate_elem, int nh, int nkv, int hd, int vd, int page_size,
+                            const T* __restrict__ gate, int gate_stride, int gate_elem, int nh, int nkv, int hd, int vd, int page_size,
                             int window, int chunk, int first, float scale, const float* __restrict__ slopes,
                             const float* __restrict__ sinks, int n_splits) {
-  constexpr int NV = D / 4;
+  constexpr int NV = D / 4, E = 16 / sizeof(T), VP = 32 / E;      // numbers of a 16-byte piece, pieces of a dimension's 32 values
   extern __shared__ __align__(128) float asf_smem[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
   const int c = lane & 7, g = lane >> 3;
@@ -91,7 +92,7 @@ attention_stream_f32_kernel(float* __restrict__ out, const float* __restrict__ q
   if (m_row >= gridDim.y) return;
   if (slot < 0) {  // padding sequence
     for (int idx = split * blockDim.x + threadIdx.x; idx < heads * vd; idx += n_splits * blockDim.x)
-      out[(m_row * nh + h0 + idx / vd) * vd + idx % vd] = 0.f;
+      out[(m_row * nh + h0 + idx / vd) * vd + idx % vd] = from_f32<T>(0.f);
     return;
   }
   const int qpos = seq_pos0[b], kv_len = qpos + 1;
@@ -100,42 +101,43 @@ attention_stream_f32_kernel(float* __restrict__ out, const float* __restrict__ q
   const int n_tiles = (kv_len - 1) / 32 - shift + 1, per_split = (n_tiles + n_splits - 1) / n_splits;
   const int t_lo = split * per_split, t_hi = min(n_tiles, t_lo + per_split);
   const int* table = block_table + (size_t)b * bt_width;
-  const int pieces = hd / 4, row = VEC ? 4 * (pieces | 1) : hd;       // floats from a key to the next
-  const int k_floats = 32 * row, stage = k_floats + 32 * vd;         // of a tile: keys [32][row], values [vd][32]
-  float* ks = asf_smem + (size_t)warp * stage;
-  float* vs = ks + k_floats;
-  float* weight_s = asf_smem + (size_t)warps * stage + warp * HC * 32;      // [HC][32]
-  float* q_s = asf_smem + (size_t)warps * (stage + HC * 32);                // [HC][row]
+  const int pieces = hd / E, row = VEC ? E * (pieces | 1) : hd;         // numbers from a key to the next
+  const int k_numbers = 32 * row, stage = k_numbers + 32 * vd;         // of a tile: keys [32][row], values [vd][32]
+  T* ks = reinterpret_cast<T*>(asf_smem) + (size_t)warp * stage;
+  T* vs = ks + k_numbers;
+  float* weight_s = reinterpret_cast<float*>(reinterpret_cast<T*>(asf_smem) + (size_t)warps * stage) + warp * HC * 32;      // [HC][32]
+  float* q_s = weight_s + (warps - warp) * HC * 32;                      // [HC][q_row]
+  const int q_row = (hd + 3) & ~3;
 
   auto key_of = [&](int tile) { return (tile >= n_first ? tile + shift : tile) * 32; };
   const uint32_t k_to = (uint32_t)__cvta_generic_to_shared(ks), v_to = (uint32_t)__cvta_generic_to_shared(vs) + 16 * lane;
-  const int v_step = 4 * page_size;      // a warp's pass copies four dimensions
+  const int v_step = 32 / VP * page_size;      // a warp's pass copies 32 / VP dimensions
   auto page_of = [&](int tile) { return max(table[key_of(tile) / page_size], 0); };
   // a lane's pieces of a tile of keys: the first one's key and place, the steps to the next
   const int k_r0 = VEC ? lane / pieces : 0, k_c0 = VEC ? lane % pieces : 0, k_rs = VEC ? 32 / pieces : 0, k_cs = VEC ? 32 % pieces : 0;
   auto issue_k = [&](int tile, int page) {      // (in the cache a tile's keys lie together)
     if (tile < t_hi) {
-      const float* src = k_pool + (((size_t)page * nkv + kvh) * page_size + key_of(tile) % page_size) * hd + 4 * lane;
+      const T* src = k_pool + (((size_t)page * nkv + kvh) * page_size + key_of(tile) % page_size) * hd + E * lane;
       if (VEC) {
         int r = k_r0, c4 = k_c0;
 #pragma unroll 4
         for (int i = lane, n = 0; i < 32 * pieces; i += 32, n++) {
-          asf_cp16(k_to + 4 * (r * row + 4 * c4), src + 128 * n);
+          asf_cp16(k_to + sizeof(T) * (r * row + E * c4), src + 32 * E * n);
           r += k_rs;
           c4 += k_cs;
           if (c4 >= pieces) c4 -= pieces, r++;
         }
       } else {
-        for (int i = lane, n = 0; i < 8 * hd; i += 32, n++) asf_cp16(k_to + 16 * i, src + 128 * n);
+        for (int i = lane, n = 0; i < 2 * hd * (int)sizeof(T); i += 32, n++) asf_cp16(k_to + 16 * i, src + 32 * E * n);
       }
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
   auto issue_v = [&](int tile, int page) {
     if (tile < t_hi) {
-      const float* src = v_pool + (((size_t)page * nkv + kvh) * vd + g) * page_size + key_of(tile) % page_size + 4 * c;
+      const T* src = v_pool + (((size_t)page * nkv + kvh) * vd + lane / VP) * page_size + key_of(tile) % page_size + E * (lane % VP);
 #pragma unroll 4
-      for (int i = lane, n = 0; i < 8 * vd; i += 32, n++) asf_cp16(v_to + 512 * n, src + (size_t)v_step * n);
+      for (int i = lane, n = 0; i < VP * vd; i += 32, n++) asf_cp16(v_to + 512 * n, src + (size_t)v_step * n);
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
@@ -145,7 +147,7 @@ attention_stream_f32_kernel(float* __restrict__ out, const float* __restrict__ q
 
   for (int i = threadIdx.x; i < HC * hd; i += blockDim.x) {
     const int h = i / hd, d = i - h * hd;
-    q_s[h * row + d] = h < heads ? q[(m_row * nh + h0 + h) * hd + d] * scale : 0.f;
+    q_s[h * q_row + d] = h < heads ? to_f32(q[(m_row * nh + h0 + h) * hd + d]) * scale : 0.f;
   }
   __syncthreads();
   float slope[HC];
@@ -168,14 +170,14 @@ attention_stream_f32_kernel(float* __restrict__ out, const float* __restrict__ q
     float x[HC];
 #pragma unroll
     for (int h = 0; h < HC; h++) x[h] = 0.f;
-    const float* mine = ks + lane * row;
+    const T* mine = ks + lane * row;
     if (VEC) {
 #pragma unroll 4
       for (int d = 0; d < hd; d += 4) {
         const float4 kk = load4(mine + d);
 #pragma unroll
         for (int h = 0; h < HC; h++) {
-          const float4 qq = load4(q_s + h * row + d);
+          const float4 qq = load4(q_s + h * q_row + d);
           x[h] = fmaf(kk.x, qq.x, x[h]);
           x[h] = fmaf(kk.y, qq.y, x[h]);
           x[h] = fmaf(kk.z, qq.z, x[h]);
@@ -184,9 +186,9 @@ attention_stream_f32_kernel(float* __restrict__ out, const float* __restrict__ q
       }
     } else {
       for (int d = 0; d < hd; d++) {
-        const float kk = mine[d];
+        const float kk = to_f32(mine[d]);
 #pragma unroll
-        for (int h = 0; h < HC; h++) x[h] = fmaf(kk, q_s[h * row + d], x[h]);
+        for (int h = 0; h < HC; h++) x[h] = fmaf(kk, q_s[h * q_row + d], x[h]);
       }
     }
     __syncwarp();      // everyone is done with the keys
@@ -272,7 +274,7 @@ attention_stream_f32_kernel(float* __restrict__ out, const float* __restrict__ q
   auto finish = [&](int idx, float M, float L, float a) {
     const int h = h0 + idx / vd, d = idx % vd;
     const float inv = sinks ? sink_quotient(M, L, sinks[h]) : (L > 0.f ? 1.0f / L : 0.f);
-    out[(m_row * nh + h) * vd + d] = a * inv * (gate ? head_gate(gate, m_row, gate_stride, h, d, vd, gate_elem) : 1.f);
+    out[(m_row * nh + h) * vd + d] = from_f32<T>(a * inv * (gate ? head_gate(gate, m_row, gate_stride, h, d, vd, gate_elem) : 1.f));
   };
   for (int idx = threadIdx.x; idx < heads * vd; idx += blockDim.x) {
     const int h = idx / vd;
@@ -318,28 +320,24 @@ attention_stream_f32_kernel(float* __restrict__ out, const float* __restrict__ q
 }
 
 // Returns 1 when the sizes are ones this kernel takes.
-LEB_API int leb_attention_stream_f32_supported(int nh, int nkv, int hd, int vd, int page_size) {
+LEB_API int leb_attention_stream_any_supported(int nh, int nkv, int hd, int vd, int page_size) {
   return nkv > 0 && nh % nkv == 0 && hd >= 1 && hd <= 256 && vd >= 1 && vd <= 256 && page_size > 0 && page_size % 32 == 0;
 }
 
-// A decode step over a 32-bit cache: every sequence brings one row.  q [B][nh*hd], out [B][nh*vd], pools [page][nkv][page_size][hd] and
-// [page][nkv][vd][page_size] on 16-byte boundaries.  max_kvlen: the most positions a sequence holds; blocks: of a cluster that shares a
-// sequence's keys (0: as many as suit the step).
-LEB_API int leb_attention_stream_f32(float* out, const float* q, const float* k_pool, const float* v_pool, const int* block_table, int bt_width,
-                                     const int* seq_slot, const int* seq_pos0, const int* seq_qstart, const float* gate, int gate_stride,
-                                     int gate_elem, int B, int nh, int nkv, int hd, int vd, int page_size, int window, int chunk, int first,
-                                     float scale, const float* slopes, const float* sinks, int max_kvlen, int blocks, cudaStream_t st) {
-  if (B <= 0) return 0;
-  LEB_REQUIRE(leb_attention_stream_f32_supported(nh, nkv, hd, vd, page_size),
-              "leb_attention_stream_f32: sizes not taken (heads %d, kv heads %d, widths %d and %d, page %d)", nh, nkv, hd, vd, page_size);
-  LEB_REQUIRE((((uintptr_t)k_pool | (uintptr_t)v_pool) & 15) == 0, "leb_attention_stream_f32: pools must be 16-byte aligned");
+template <typename T>
+static int launch_attention_stream_any(T* out, const T* q, const T* k_pool, const T* v_pool, const int* block_table, int bt_width,
+                                       const int* seq_slot, const int* seq_pos0, const int* seq_qstart, const T* gate, int gate_stride,
+                                       int gate_elem, int B, int nh, int nkv, int hd, int vd, int page_size, int window, int chunk, int first,
+                                       float scale, const float* slopes, const float* sinks, int max_kvlen, int blocks, cudaStream_t st) {
+  constexpr int E = 16 / sizeof(T);
   const int G = nh / nkv, widest = hd > vd ? hd : vd;
   const int HC = G == 1 ? 1 : widest > 128 ? 2 : 4, n_hc = ceil_div(G, HC);
-  const int row = hd % 4 == 0 ? 4 * (hd / 4 | 1) : hd;
-  const size_t stage = (size_t)32 * (row + vd) * sizeof(float);
-  const int warps = stage <= 17 * 1024 ? 4 : 3;      // three blocks an SM; two up to heads of 128; one
-  const size_t rings = warps * (stage + HC * 32 * sizeof(float)) + HC * row * sizeof(float), results = ((size_t)(warps + 1) * HC * (vd + 2)) * sizeof(float);
-  const size_t smem = rings > results ? rings : results;
+  const bool vec = hd % E == 0;
+  const int row = vec ? E * (hd / E | 1) : hd;
+  const size_t stage = (size_t)32 * (row + vd) * sizeof(T);
+  const int warps = stage <= 17 * 1024 ? 4 : 3;      // three blocks an SM; with wider 32-bit heads two or one
+  const size_t rings = warps * (stage + HC * 32 * sizeof(float)) + HC * ((hd + 3) & ~3) * sizeof(float);
+  const size_t results = ((size_t)(warps + 1) * HC * (vd + 2)) * sizeof(float), smem = rings > results ? rings : results;
   // blocks of a cluster: as many as run at once (to the nearest), with a tile a warp or more for each.  us of 1, 2, 4, 8 blocks: one stream of
   // 1,000 positions 25.1, 15.9, 11.0, 8.5; 32 streams of 100 to 3,000, window 1,024, 256 blocks where 444 fit, 38.9, 33.9, 41.4, 61.6; 64
   // streams with heads of 128, 256 where 296 fit, 55.0, 58.6, 72.4, 109.9
@@ -353,18 +351,18 @@ LEB_API int leb_attention_stream_f32(float* out, const float* q, const float* k_
   if (blocks > 0) n = blocks;
   const int n_splits = (int)(n < 1 ? 1 : n > 8 ? 8 : n);
   dim3 grid(nkv * n_hc, B, n_splits);
-  LEB_REQUIRE(grid.y <= 65535, "leb_attention_stream_f32: grid too large");
+  LEB_REQUIRE(grid.y <= 65535, "leb_attention_stream_any: grid too large");
 #define LEB_ASF_K(D_, HC_, VEC_)                                                                                                      \
   {                                                                                                                                   \
-    constexpr auto kern = attention_stream_f32_kernel<D_, HC_, VEC_>;                                                                 \
+    constexpr auto kern = attention_stream_any_kernel<T, D_, HC_, VEC_>;                                                              \
     const cudaError_t e = leb_allow_smem<kern>();                                                                                     \
-    if (e != cudaSuccess) return leb_fail("leb_attention_stream_f32: shared memory %zu: %s", smem, cudaGetErrorString(e));            \
+    if (e != cudaSuccess) return leb_fail("leb_attention_stream_any: shared memory %zu: %s", smem, cudaGetErrorString(e));            \
     leb_launch_cluster(n_splits, kern, grid, dim3(32 * warps), smem, st, out, q, k_pool, v_pool, block_table, bt_width, seq_slot, seq_pos0, \
                        seq_qstart, gate, gate_stride, gate_elem, nh, nkv, hd, vd, page_size, window, chunk, first, scale, slopes, sinks, n_splits); \
   }
 #define LEB_ASF(D_, HC_)               \
   {                                    \
-    if (hd % 4 == 0) LEB_ASF_K(D_, HC_, true) else LEB_ASF_K(D_, HC_, false) \
+    if (vec) LEB_ASF_K(D_, HC_, true) else LEB_ASF_K(D_, HC_, false) \
   }
   if (widest <= 64) {
     if (HC == 1) LEB_ASF(64, 1) else LEB_ASF(64, 4)
@@ -375,6 +373,27 @@ LEB_API int leb_attention_stream_f32(float* out, const float* q, const float* k_
   }
 #undef LEB_ASF
 #undef LEB_ASF_K
-  LEB_CHECK_LAUNCH("leb_attention_stream_f32");
+  LEB_CHECK_LAUNCH("leb_attention_stream_any");
   return 0;
+}
+
+// A decode step: every sequence brings one row.  q [B][nh*hd], out [B][nh*vd], pools [page][nkv][page_size][hd] and
+// [page][nkv][vd][page_size] on 16-byte boundaries, all of `dtype`.  max_kvlen: the most positions a sequence holds; blocks: of a cluster
+// that shares a sequence's keys (0: as many as suit the step).
+LEB_API int leb_attention_stream_any(void* out, const void* q, const void* k_pool, const void* v_pool, int dtype, const int* block_table,
+                                     int bt_width, const int* seq_slot, const int* seq_pos0, const int* seq_qstart, const void* gate,
+                                     int gate_stride, int gate_elem, int B, int nh, int nkv, int hd, int vd, int page_size, int window, int chunk,
+                                     int first, float scale, const float* slopes, const float* sinks, int max_kvlen, int blocks, cudaStream_t st) {
+  if (B <= 0) return 0;
+  LEB_REQUIRE(leb_attention_stream_any_supported(nh, nkv, hd, vd, page_size),
+              "leb_attention_stream_any: sizes not taken (heads %d, kv heads %d, widths %d and %d, page %d)", nh, nkv, hd, vd, page_size);
+  LEB_REQUIRE((((uintptr_t)k_pool | (uintptr_t)v_pool) & 15) == 0, "leb_attention_stream_any: pools must be 16-byte aligned");
+#define LEB_ASF_T(T)                                                                                                                    \
+  launch_attention_stream_any((T*)out, (const T*)q, (const T*)k_pool, (const T*)v_pool, block_table, bt_width, seq_slot, seq_pos0, seq_qstart, \
+                              (const T*)gate, gate_stride, gate_elem, B, nh, nkv, hd, vd, page_size, window, chunk, first, scale, slopes, \
+                              sinks, max_kvlen, blocks, st)
+  if (dtype == LEB_F32) return LEB_ASF_T(float);
+  if (dtype == LEB_BF16) return LEB_ASF_T(bf16);
+#undef LEB_ASF_T
+  return leb_fail("leb_attention_stream_any: unknown dtype %d", dtype);
 }

@@ -18,7 +18,8 @@
 //
 // Kernels of a step read its tables ahead of their own wait for the kernel before them (common.cuh): they count on everything the
 // tables were made by being complete when the step's first such kernel starts.  `advance` behind `tables` gives a step that: it waits for
-// the tables, and lets nothing behind it start before it has ended.
+// the tables, and lets nothing behind it start before it has ended.  Decode attention reads what earlier steps stored ahead of its wait in
+// the same way; the stores therefore let nothing start before they have ended either.
 #include "common.cuh"
 
 #define STB_THREADS 256
@@ -319,7 +320,7 @@ template <typename T>
 __global__ void __launch_bounds__(256)
 store_rows_kernel(T* __restrict__ k_pool, T* __restrict__ v_pool, const T* __restrict__ k, int k_stride, const T* __restrict__ v,
                   int v_stride, const int* __restrict__ slots, int n_pages, int M, int nkv, int hd, int vd, int page) {
-  pdl_wait();
+  stb_wait();
   const int m = blockIdx.x;
   const int slot = slots[m];
   const int pg = slot / page, off = slot % page;
@@ -345,7 +346,7 @@ store_tile_kernel(T* __restrict__ k_pool, T* __restrict__ v_pool, const T* __res
   constexpr int W = 16 / sizeof(T), STRIDE = DC + 4 / sizeof(T);      // a row of v_s is an odd number of words
   __shared__ int slot_s[STR_ROWS];
   __shared__ __align__(16) T v_s[STR_ROWS * STRIDE];
-  pdl_wait();
+  stb_wait();
   const int m0 = blockIdx.x * STR_ROWS, head = blockIdx.y, rows = min(STR_ROWS, M - m0);
   if (threadIdx.x < STR_ROWS) {
     int s = (int)threadIdx.x < rows ? slots[m0 + threadIdx.x] : -1;

@@ -313,8 +313,8 @@ def _declare(L) -> None:
         "leb_attention_prefill": [P, P, P, P, P, I, P, P, P, P, P, I, I, I, I, I, I, I, I, I, I, I, F, P, P, I, P],
         "leb_attention_stream_tc_supported": [I, I, I, I, I],
         "leb_attention_stream_tc": [P, P, I, I, P, P, I, P, I, P, P, P, P, P, I, I, I, I, I, I, I, I, I, I, I, F, P, P, I, I, I, P, P],
-        "leb_attention_stream_f32_supported": [I, I, I, I, I],
-        "leb_attention_stream_f32": [P, P, P, P, P, I, P, P, P, P, I, I, I, I, I, I, I, I, I, I, I, F, P, P, I, I, P],
+        "leb_attention_stream_any_supported": [I, I, I, I, I],
+        "leb_attention_stream_any": [P, P, P, P, I, P, I, P, P, P, P, I, I, I, I, I, I, I, I, I, I, I, F, P, P, I, I, P],
         "leb_stream_tables": [P, I, P, P, P, P, P, P, P, P, P, P, I, P, I, P, I, P, I, I, I, P],
         "leb_stream_advance": [P, P, P, I, P, P, I, P, I, P, I, I, I, I, P],
         "leb_stream_release": [P, P, I, P, P, I, P, I, P, I, I, I, P],
@@ -1771,10 +1771,10 @@ def _stream_form(out, batch, nh, nkv, hd, vd, page_size, wide, q, k_pool, v_pool
     if batch.max_qlen == 1:
         if out.shape[0] != batch.n_seqs:
             return None
-        if out.dtype is torch.bfloat16:
-            return _attention_stream_decode if vd == hd and _stream_takes("leb_attention_decode_supported", nh, nkv, hd, page_size) else None
-        return _attention_stream_f32 if (k_pool.data_ptr() | v_pool.data_ptr()) & 15 == 0 \
-            and _stream_takes("leb_attention_stream_f32_supported", nh, nkv, hd, vd, page_size) else None
+        if out.dtype is torch.bfloat16 and vd == hd and _stream_takes("leb_attention_decode_supported", nh, nkv, hd, page_size):
+            return _attention_stream_decode
+        return _attention_stream_any if (k_pool.data_ptr() | v_pool.data_ptr()) & 15 == 0 \
+            and _stream_takes("leb_attention_stream_any_supported", nh, nkv, hd, vd, page_size) else None
     if out.dtype is torch.bfloat16 and not wide and q.stride(0) % 8 == 0 \
             and _stream_takes("leb_attention_stream_tc_supported", nh, nkv, hd, vd, page_size):
         return _attention_stream_tc
@@ -1812,13 +1812,14 @@ def _attention_stream_decode(out, q, k_pool, v_pool, block_table, batch, nh, nkv
                                      _stream()))
 
 
-def _attention_stream_f32(out, q, k_pool, v_pool, block_table, batch, nh, nkv, hd, vd, page_size, window, scale, gate, chunk, slopes, sinks,
+def _attention_stream_any(out, q, k_pool, v_pool, block_table, batch, nh, nkv, hd, vd, page_size, window, scale, gate, chunk, slopes, sinks,
                           first, wide, n_splits, scratch) -> None:
-    """A decode step over a 32-bit cache with first positions: the blocks of a sequence join their sums by themselves."""
+    """A decode step with first positions over a 32-bit cache, or with heads the tensor-core kernel does not take: the blocks of a sequence
+    join their sums by themselves."""
     M = _stream_operands(out, q, k_pool, v_pool, block_table, nh, nkv, hd, vd, page_size)
     gate_stride, gate_elem = _gate_layout(gate, M, nh, vd, out.dtype)
-    _check(lib().leb_attention_stream_f32(
-        out.data_ptr(), q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), block_table.data_ptr(), block_table.shape[1],
+    _check(lib().leb_attention_stream_any(
+        out.data_ptr(), q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), _dt(out, "attention"), block_table.data_ptr(), block_table.shape[1],
         batch.seq_slot.data_ptr(), batch.seq_pos0.data_ptr(), batch.seq_qstart.data_ptr(), _ptr(gate), gate_stride, gate_elem, M, nh, nkv, hd, vd,
         page_size, window, chunk, first, scale, _ptr(slopes), _ptr(sinks), batch.max_kvlen, _stream_splits, _stream()))
 

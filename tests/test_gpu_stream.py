@@ -119,7 +119,8 @@ CHUNKS = [(0, 1), (0, 70), (63, 2), (200, 130), (517, 33), (64, 64), (3, 300)]
 
 @pytest.mark.parametrize("dtype,nh,nkv,hd,vd,page", [
     (BF16, 8, 2, 64, 64, 64), (BF16, 32, 8, 64, 64, 64), (BF16, 3, 1, 32, 32, 32), (BF16, 16, 1, 128, 128, 64), (BF16, 6, 6, 96, 96, 128),
-    (BF16, 4, 2, 80, 80, 64), (BF16, 4, 2, 64, 48, 64), (F32, 4, 2, 64, 64, 64), (F32, 6, 2, 80, 48, 32), (F32, 20, 1, 33, 33, 64),
+    (BF16, 4, 2, 80, 80, 64), (BF16, 4, 2, 64, 48, 64), (BF16, 5, 5, 20, 12, 32), (BF16, 6, 2, 33, 65, 64), (BF16, 3, 1, 192, 192, 64),
+    (BF16, 34, 2, 64, 64, 64), (BF16, 4, 1, 256, 256, 128), (F32, 4, 2, 64, 64, 64), (F32, 6, 2, 80, 48, 32), (F32, 20, 1, 33, 33, 64),
     (F32, 3, 3, 128, 128, 64), (F32, 8, 1, 128, 40, 32), (F32, 5, 1, 256, 200, 64), (F32, 2, 2, 200, 256, 64), (F32, 7, 1, 3, 1, 32)])
 @pytest.mark.parametrize("window,first", WINDOWS)
 def test_single_tokens(dtype, nh, nkv, hd, vd, page, window, first):
