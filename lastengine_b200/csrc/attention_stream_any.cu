@@ -75,7 +75,7 @@ __global__ void __launch_bounds__(128, D <= 64 ? 3 : D <= 128 ? 2 : 1)
 attention_stream_any_kernel(T* __restrict__ out, const T* __restrict__ q, const T* __restrict__ k_pool,
                             const T* __restrict__ v_pool, const int* __restrict__ block_table, int bt_width,
                             const int* __restrict__ seq_slot, const int* __restrict__ seq_pos0, const int* __restrict__ seq_qstart,
-                            const T* __restrict__ gate, int gate_stride, int gate_elem, int nh, int nkv, int hd, int vd, int page_size,
+                            const int* __restrict__ row_seq, const int* __restrict__ row_pos, const T* __restrict__ gate, int gate_stride, int gate_elem, int nh, int nkv, int hd, int vd, int page_size,
                             int window, int chunk, int first, float scale, const float* __restrict__ slopes,
                             const float* __restrict__ sinks, int n_splits) {
   constexpr int NV = D / 4, E = 16 / sizeof(T), VP = 32 / E;      // numbers of a 16-byte piece, pieces of a dimension's 32 values
@@ -86,8 +86,9 @@ attention_stream_any_kernel(T* __restrict__ out, const T* __restrict__ q, const 
   const int kvh = blockIdx.x / n_hc, hc = blockIdx.x % n_hc, b = blockIdx.y, split = blockIdx.z;
   const int h0 = kvh * G + hc * HC, heads = min(HC, G - hc * HC);
   pdl_wait();
-  const int slot = seq_slot[b];
-  const size_t m_row = seq_qstart[b];
+  // a block's row: that of sequence b, or (row_seq) row b, of any sequence
+  const int seq = row_seq ? row_seq[b] : b, slot = seq_slot[seq];
+  const size_t m_row = row_seq ? b : seq_qstart[b];
   // (as in the bfloat16 kernel: out has one row per sequence of the launch; the same for all blocks of a cluster)
   if (m_row >= gridDim.y) return;
   if (slot < 0) {  // padding sequence
@@ -95,12 +96,12 @@ attention_stream_any_kernel(T* __restrict__ out, const T* __restrict__ q, const 
       out[(m_row * nh + h0 + idx / vd) * vd + idx % vd] = from_f32<T>(0.f);
     return;
   }
-  const int qpos = seq_pos0[b], kv_len = qpos + 1;
+  const int qpos = row_seq ? row_pos[b] : seq_pos0[b], kv_len = qpos + 1;
   const int key_lo = first_key(qpos, window, chunk);
   const int n_first = first_tiles(first, key_lo, 32), shift = key_lo / 32 - n_first;
   const int n_tiles = (kv_len - 1) / 32 - shift + 1, per_split = (n_tiles + n_splits - 1) / n_splits;
   const int t_lo = split * per_split, t_hi = min(n_tiles, t_lo + per_split);
-  const int* table = block_table + (size_t)b * bt_width;
+  const int* table = block_table + (size_t)seq * bt_width;
   const int pieces = hd / E, row = VEC ? E * (pieces | 1) : hd;         // numbers from a key to the next
   const int k_numbers = 32 * row, stage = k_numbers + 32 * vd;         // of a tile: keys [32][row], values [vd][32]
   T* ks = reinterpret_cast<T*>(asf_smem) + (size_t)warp * stage;
@@ -326,7 +327,8 @@ LEB_API int leb_attention_stream_any_supported(int nh, int nkv, int hd, int vd, 
 
 template <typename T>
 static int launch_attention_stream_any(T* out, const T* q, const T* k_pool, const T* v_pool, const int* block_table, int bt_width,
-                                       const int* seq_slot, const int* seq_pos0, const int* seq_qstart, const T* gate, int gate_stride,
+                                       const int* seq_slot, const int* seq_pos0, const int* seq_qstart, const int* row_seq, const int* row_pos,
+                                       const T* gate, int gate_stride,
                                        int gate_elem, int B, int nh, int nkv, int hd, int vd, int page_size, int window, int chunk, int first,
                                        float scale, const float* slopes, const float* sinks, int max_kvlen, int blocks, cudaStream_t st) {
   constexpr int E = 16 / sizeof(T);
@@ -358,7 +360,7 @@ static int launch_attention_stream_any(T* out, const T* q, const T* k_pool, cons
     const cudaError_t e = leb_allow_smem<kern>();                                                                                     \
     if (e != cudaSuccess) return leb_fail("leb_attention_stream_any: shared memory %zu: %s", smem, cudaGetErrorString(e));            \
     leb_launch_cluster(n_splits, kern, grid, dim3(32 * warps), smem, st, out, q, k_pool, v_pool, block_table, bt_width, seq_slot, seq_pos0, \
-                       seq_qstart, gate, gate_stride, gate_elem, nh, nkv, hd, vd, page_size, window, chunk, first, scale, slopes, sinks, n_splits); \
+                       seq_qstart, row_seq, row_pos, gate, gate_stride, gate_elem, nh, nkv, hd, vd, page_size, window, chunk, first, scale, slopes, sinks, n_splits); \
   }
 #define LEB_ASF(D_, HC_)               \
   {                                    \
@@ -377,20 +379,22 @@ static int launch_attention_stream_any(T* out, const T* q, const T* k_pool, cons
   return 0;
 }
 
-// A decode step: every sequence brings one row.  q [B][nh*hd], out [B][nh*vd], pools [page][nkv][page_size][hd] and
+// A decode step: every sequence brings one row; or, with row_seq and row_pos [B], B rows of any sequences (each then reads its keys by
+// itself: for chunks of few rows).  q [B][nh*hd], out [B][nh*vd], pools [page][nkv][page_size][hd] and
 // [page][nkv][vd][page_size] on 16-byte boundaries, all of `dtype`.  max_kvlen: the most positions a sequence holds; blocks: of a cluster
 // that shares a sequence's keys (0: as many as suit the step).
 LEB_API int leb_attention_stream_any(void* out, const void* q, const void* k_pool, const void* v_pool, int dtype, const int* block_table,
-                                     int bt_width, const int* seq_slot, const int* seq_pos0, const int* seq_qstart, const void* gate,
-                                     int gate_stride, int gate_elem, int B, int nh, int nkv, int hd, int vd, int page_size, int window, int chunk,
+                                     int bt_width, const int* seq_slot, const int* seq_pos0, const int* seq_qstart, const int* row_seq,
+                                     const int* row_pos, const void* gate, int gate_stride, int gate_elem, int B, int nh, int nkv, int hd, int vd, int page_size, int window, int chunk,
                                      int first, float scale, const float* slopes, const float* sinks, int max_kvlen, int blocks, cudaStream_t st) {
   if (B <= 0) return 0;
   LEB_REQUIRE(leb_attention_stream_any_supported(nh, nkv, hd, vd, page_size),
               "leb_attention_stream_any: sizes not taken (heads %d, kv heads %d, widths %d and %d, page %d)", nh, nkv, hd, vd, page_size);
+  LEB_REQUIRE((row_seq == nullptr) == (row_pos == nullptr), "leb_attention_stream_any: rows come with their sequences and positions");
   LEB_REQUIRE((((uintptr_t)k_pool | (uintptr_t)v_pool) & 15) == 0, "leb_attention_stream_any: pools must be 16-byte aligned");
 #define LEB_ASF_T(T)                                                                                                                    \
   launch_attention_stream_any((T*)out, (const T*)q, (const T*)k_pool, (const T*)v_pool, block_table, bt_width, seq_slot, seq_pos0, seq_qstart, \
-                              (const T*)gate, gate_stride, gate_elem, B, nh, nkv, hd, vd, page_size, window, chunk, first, scale, slopes, \
+                              row_seq, row_pos, (const T*)gate, gate_stride, gate_elem, B, nh, nkv, hd, vd, page_size, window, chunk, first, scale, slopes, \
                               sinks, max_kvlen, blocks, st)
   if (dtype == LEB_F32) return LEB_ASF_T(float);
   if (dtype == LEB_BF16) return LEB_ASF_T(bf16);

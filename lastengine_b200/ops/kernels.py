@@ -314,7 +314,7 @@ def _declare(L) -> None:
         "leb_attention_stream_tc_supported": [I, I, I, I, I],
         "leb_attention_stream_tc": [P, P, I, I, P, P, I, P, I, P, P, P, P, P, I, I, I, I, I, I, I, I, I, I, I, F, P, P, I, I, I, P, P],
         "leb_attention_stream_any_supported": [I, I, I, I, I],
-        "leb_attention_stream_any": [P, P, P, P, I, P, I, P, P, P, P, I, I, I, I, I, I, I, I, I, I, I, F, P, P, I, I, P],
+        "leb_attention_stream_any": [P, P, P, P, I, P, I, P, P, P, P, P, P, I, I, I, I, I, I, I, I, I, I, I, F, P, P, I, I, P],
         "leb_stream_tables": [P, I, P, P, P, P, P, P, P, P, P, P, I, P, I, P, I, P, I, I, I, P],
         "leb_stream_advance": [P, P, P, I, P, P, I, P, I, P, I, I, I, I, P],
         "leb_stream_release": [P, P, I, P, P, I, P, I, P, I, I, I, P],
@@ -1766,18 +1766,29 @@ def _stream_takes(entry: str, *sizes: int) -> bool:
     return bool(getattr(lib(), entry)(*sizes))
 
 
+# Rows of a bfloat16 step up to which each reads its keys by itself where only the mma.sync kernel takes the prompt.  us of a chunk with 32
+# heads of 64 over 8, pages of 32, window 1,024, that kernel and this: 2 rows 33.8 and 11.5, 16 34.5 and 18.4, 32 34.5 and 46.3.
+# (The general kernel is behind at every size: 32-bit, 16 rows 400 and 20, 256 422 and 183, 2,048 2,937 and 1,336.)
+STREAM_ROWS = 16
+
+
 def _stream_form(out, batch, nh, nkv, hd, vd, page_size, wide, q, k_pool, v_pool):
     """The kernel made for rows with first positions that takes a step, None where the ones for all rows do."""
-    if batch.max_qlen == 1:
-        if out.shape[0] != batch.n_seqs:
-            return None
-        if out.dtype is torch.bfloat16 and vd == hd and _stream_takes("leb_attention_decode_supported", nh, nkv, hd, page_size):
+    M, single = out.shape[0], batch.max_qlen == 1
+    aligned = (k_pool.data_ptr() | v_pool.data_ptr()) & 15 == 0
+    if out.dtype is torch.bfloat16:
+        mma = vd == hd and _stream_takes("leb_attention_prefill_supported", nh, nkv, hd, page_size)
+        if mma and not aligned:
+            raise KernelError("attention: the pools of these heads must lie on 16-byte boundaries")
+        if single and mma and M == batch.n_seqs and _stream_takes("leb_attention_decode_supported", nh, nkv, hd, page_size):
             return _attention_stream_decode
-        return _attention_stream_any if (k_pool.data_ptr() | v_pool.data_ptr()) & 15 == 0 \
-            and _stream_takes("leb_attention_stream_any_supported", nh, nkv, hd, vd, page_size) else None
-    if out.dtype is torch.bfloat16 and not wide and q.stride(0) % 8 == 0 \
-            and _stream_takes("leb_attention_stream_tc_supported", nh, nkv, hd, vd, page_size):
-        return _attention_stream_tc
+        if (not single and not wide and aligned and (q.data_ptr() | out.data_ptr()) & 15 == 0 and q.stride(0) % 8 == 0
+                and _stream_takes("leb_attention_stream_tc_supported", nh, nkv, hd, vd, page_size)):
+            return _attention_stream_tc
+        if mma and not single and M > STREAM_ROWS:
+            return None
+    if aligned and M <= 65535 and _stream_takes("leb_attention_stream_any_supported", nh, nkv, hd, vd, page_size):
+        return _attention_stream_any
     return None
 
 
@@ -1820,8 +1831,9 @@ def _attention_stream_any(out, q, k_pool, v_pool, block_table, batch, nh, nkv, h
     gate_stride, gate_elem = _gate_layout(gate, M, nh, vd, out.dtype)
     _check(lib().leb_attention_stream_any(
         out.data_ptr(), q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), _dt(out, "attention"), block_table.data_ptr(), block_table.shape[1],
-        batch.seq_slot.data_ptr(), batch.seq_pos0.data_ptr(), batch.seq_qstart.data_ptr(), _ptr(gate), gate_stride, gate_elem, M, nh, nkv, hd, vd,
-        page_size, window, chunk, first, scale, _ptr(slopes), _ptr(sinks), batch.max_kvlen, _stream_splits, _stream()))
+        batch.seq_slot.data_ptr(), batch.seq_pos0.data_ptr(), batch.seq_qstart.data_ptr(),
+        *((None, None) if batch.max_qlen == 1 and M == batch.n_seqs else (batch.row_seq.data_ptr(), batch.row_pos.data_ptr())),
+        _ptr(gate), gate_stride, gate_elem, M, nh, nkv, hd, vd, page_size, window, chunk, first, scale, _ptr(slopes), _ptr(sinks), batch.max_kvlen, _stream_splits, _stream()))
 
 
 def _attention_stream_tc(out, q, k_pool, v_pool, block_table, batch, nh, nkv, hd, vd, page_size, window, scale, gate, chunk, slopes, sinks,

@@ -214,6 +214,25 @@ def test_slopes_sinks_and_gates_beside_first_positions(seqs, dtype, hd):
     c.check(c.run(gate=gate.to(DEV)), factor=torch.sigmoid(gate.double())[:, :, None])
 
 
+def test_steps_that_only_the_general_kernel_takes():
+    """Pools off a 16-byte boundary."""
+    for seqs in (DECODE, CHUNKS):
+        for dtype, hd, vd in ((F32, 48, 48), (BF16, 72, 24)):
+            c = Case(seqs, 4, 2, hd, vd, 64, 90, 6, dtype, seed=8, padding=[3])
+            want = c.run()
+            for name in ("k_pool", "v_pool"):
+                pool = getattr(c, name)
+                moved = torch.empty(pool.numel() + 2, dtype=dtype, device=DEV)[2:].view(pool.shape)
+                setattr(c, name, moved.copy_(pool))
+            got = c.run()
+            c.check(got)
+            assert float((got.float() - want.float()).abs().max()) < 0.05
+        c = Case(seqs, 4, 2, 64, 64, 64, 90, 6, BF16, seed=8)
+        c.k_pool = torch.empty(c.k_pool.numel() + 2, dtype=BF16, device=DEV)[2:].view(c.k_pool.shape)
+        with pytest.raises(K().KernelError):
+            c.run()
+
+
 def test_large_scores_and_a_first_key_that_takes_all_the_weight():
     """Scores of a few hundred: the running maximum moves by far more than an exponential's range, up and down the walk."""
     for spread in (30.0, 200.0):
