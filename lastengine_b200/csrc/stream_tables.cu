@@ -336,61 +336,74 @@ store_rows_kernel(T* __restrict__ k_pool, T* __restrict__ v_pool, const T* __res
 // Where there are few blocks, gridDim.z of them share the keys and the dimensions of a tile.
 // VK / VV: keys / values can be loaded (and keys stored) in pieces of 16 bytes.
 #define STR_ROWS 64
-#ifndef STR_FEW
+// From which rows on, us by rows and by tiles (8 kv heads of 64): a prompt of 64, 128, 256, 512 rows 2.59, 2.78, 3.68, 5.26 and 2.29, 2.30,
+// 2.30, 2.46; single tokens of as many streams 2.60, 2.59, 3.03, 4.48 and 3.41, 3.40, 3.58, 4.75.  Bound by memory: 16,439 rows (67 MB) 12.8 us,
+// 5.2 TB/s (a block per row 77; with the places worked out by divisions for every piece 15.8, 69% of the issue slots).
 #define STR_FEW 192
-#endif
+// The pieces (0 .. per - 1) of `rows` rows, shared out over the eight warps of `parts` blocks: calls f(row, piece).  A lane's place in a row is
+// worked out once: a warp takes as many rows at a time as it has lanes for, or one.
+template <typename F>
+__device__ __forceinline__ void str_pieces(int rows, int per, int part, int parts, F f) {
+  const int lane = threadIdx.x & 31, warp = part * 8 + (threadIdx.x >> 5), warps = parts * 8;
+  if (per <= 32) {
+    const int at_once = 32 / per, row = lane / per, c = lane - row * per;
+    if (row < at_once) {
+#pragma unroll 2
+      for (int r = warp * at_once + row; r < rows; r += warps * at_once) f(r, c);
+    }
+  } else {
+    for (int r = warp; r < rows; r += warps)
+#pragma unroll 2
+      for (int c = lane; c < per; c += 32) f(r, c);
+  }
+}
 template <typename T, bool VK, bool VV, int DC>
 __global__ void __launch_bounds__(256)
 store_tile_kernel(T* __restrict__ k_pool, T* __restrict__ v_pool, const T* __restrict__ k, int k_stride, const T* __restrict__ v,
                   int v_stride, const int* __restrict__ slots, int n_pages, int M, int nkv, int hd, int vd, int page) {
   constexpr int W = 16 / sizeof(T), STRIDE = DC + 4 / sizeof(T);      // a row of v_s is an odd number of words
   __shared__ int slot_s[STR_ROWS];
+  __shared__ long long place_s[STR_ROWS];      // of a row's page and head: the first position's place in a pool of one number a position
   __shared__ __align__(16) T v_s[STR_ROWS * STRIDE];
   stb_wait();
   const int m0 = blockIdx.x * STR_ROWS, head = blockIdx.y, rows = min(STR_ROWS, M - m0);
   if (threadIdx.x < STR_ROWS) {
     int s = (int)threadIdx.x < rows ? slots[m0 + threadIdx.x] : -1;
-    slot_s[threadIdx.x] = s >= 0 && s / page < n_pages ? s : -1;
+    const int pg = s / page;
+    if (pg >= n_pages) s = -1;
+    slot_s[threadIdx.x] = s < 0 ? -1 : s - pg * page;      // from here on a row's place in its page
+    place_s[threadIdx.x] = s < 0 ? 0 : ((long long)pg * nkv + head) * page;
   }
   __syncthreads();
   const T* ks = k + (size_t)m0 * k_stride + (size_t)head * hd;
   const T* vs = v + (size_t)m0 * v_stride + (size_t)head * vd;
-  const int per = VK ? hd / W : hd;
-#pragma unroll 2
-  for (int i = blockIdx.z * 256 + threadIdx.x; i < rows * per; i += 256 * gridDim.z) {
-    const int row = i / per, c = i - row * per, slot = slot_s[row];
-    if (slot < 0) continue;
-    T* dst = k_pool + (((size_t)(slot / page) * nkv + head) * page + slot % page) * hd;
+  str_pieces(rows, VK ? hd / W : hd, blockIdx.z, gridDim.z, [&](int row, int c) {
+    const int off = slot_s[row];
+    if (off < 0) return;
+    T* dst = k_pool + (place_s[row] + off) * hd;
     if (VK) reinterpret_cast<uint4*>(dst)[c] = *reinterpret_cast<const uint4*>(ks + (size_t)row * k_stride + c * W);
     else dst[c] = ks[(size_t)row * k_stride + c];
-  }
+  });
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   for (int d0 = blockIdx.z * DC; d0 < vd; d0 += DC * gridDim.z) {
     const int n = min(DC, vd - d0);
     if (d0 >= DC * (int)gridDim.z) __syncthreads();
-    if (VV) {
-      const int vper = n / W;
-#pragma unroll 2
-      for (int i = threadIdx.x; i < rows * vper; i += 256) {
-        const int row = i / vper, c = i - row * vper;
+    str_pieces(rows, VV ? n / W : n, 0, 1, [&](int row, int c) {
+      if (VV) {
         const uint4 x = *reinterpret_cast<const uint4*>(vs + (size_t)row * v_stride + d0 + c * W);
         uint32_t* to = reinterpret_cast<uint32_t*>(v_s + row * STRIDE + c * W);
         to[0] = x.x, to[1] = x.y, to[2] = x.z, to[3] = x.w;
-      }
-    } else {
-      for (int i = threadIdx.x; i < rows * n; i += 256) {
-        const int row = i / n, c = i - row * n;
+      } else {
         v_s[row * STRIDE + c] = vs[(size_t)row * v_stride + d0 + c];
       }
-    }
+    });
     __syncthreads();
     if (sizeof(T) == 2) {
       // two rows a lane, two dimensions a warp's turn
       const int ra = 2 * lane, sa = slot_s[ra], sb = slot_s[ra + 1];
-      const bool joined = sa >= 0 && sb == sa + 1 && ((sa | page) & 1) == 0;      // both places in one aligned word
-      T* const base = v_pool + (size_t)head * vd * page;
-      T* const pa = base + (size_t)(sa < 0 ? 0 : sa / page) * nkv * vd * page + (sa < 0 ? 0 : sa % page);
-      T* const pb = base + (size_t)(sb < 0 ? 0 : sb / page) * nkv * vd * page + (sb < 0 ? 0 : sb % page);
+      const bool joined = sa >= 0 && sb == sa + 1 && place_s[ra] == place_s[ra + 1] && ((sa | page) & 1) == 0;      // both places in one aligned word
+      T* const pa = v_pool + place_s[ra] * vd + max(sa, 0);
+      T* const pb = v_pool + place_s[ra + 1] * vd + max(sb, 0);
       for (int d = 2 * warp; d < n; d += 16) {
         const uint32_t a = *reinterpret_cast<const uint32_t*>(v_s + ra * STRIDE + d), c = *reinterpret_cast<const uint32_t*>(v_s + (ra + 1) * STRIDE + d);
         const size_t at = (size_t)(d0 + d) * page;
@@ -416,7 +429,7 @@ store_tile_kernel(T* __restrict__ k_pool, T* __restrict__ v_pool, const T* __res
       for (int h = 0; h < STR_ROWS; h += 32) {
         const int slot = slot_s[h + lane];
         if (slot < 0) continue;
-        T* to = v_pool + (((size_t)(slot / page) * nkv + head) * vd + d0) * page + slot % page;
+        T* to = v_pool + place_s[h + lane] * vd + (size_t)d0 * page + slot;
         for (int d = warp; d < n; d += 8) to[(size_t)d * page] = v_s[(h + lane) * STRIDE + d];
       }
     }
