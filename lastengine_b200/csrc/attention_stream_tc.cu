@@ -3,14 +3,15 @@
 //
 // A row at position p reads positions j <= p with j >= first_key(p) or j < first.  A block owns a tile of 128 rows: the G query heads
 // of one kv head times TP = 128 / G consecutive positions (a multiple of 8; the rows that are left are idle).  It walks a list of
-// pages (or halves, .. of pages: always 64 positions), those of first positions and then those from its first row's window to its last row, two pages (128 keys) at a time:
+// pages (of larger pages: their parts of 64 positions), those of first positions and then those from its first row's window to its last
+// row, two pages (128 keys) at a time:
 //
 //   S[128, 128] = Q[128, HD] . K[128, HD]^T       operands in shared memory, S in tensor memory
 //   P           = exp2(S * scale * log2 e - m)     two threads per row, one a page, P (bfloat16) to tensor memory
 //   O[128, HD] += P[128, 128] . V[128, HD]         P from tensor memory, V from shared memory
 //
-// Warps: eight for the softmax, one that brings Q and pages by TMA, one that issues the products, two that fill their warpgroup
-// (registers move between warpgroups).  Two blocks share an SM, so that one's products run under the other's exponentials, and a
+// Warps: eight for the softmax, one that brings Q and pages by TMA, one that issues the products, two that put zeros where a page holds
+// values no row of the tile reads (registers move between warpgroups).  Two blocks share an SM, so that one's products run under the other's exponentials, and a
 // scheduler has four softmax warps: what bounds the loop is the chain from a row's scores to its weights, not a pipe.
 // Where there are few tiles, a cluster of n_splits blocks shares the pages of one and joins its sums through shared memory.
 // With heads of 64, P has columns beside S and the next scores are issued as soon as a row of S is in registers; with heads of 128, O
@@ -18,11 +19,12 @@
 //
 // Bounds: 128 keys of a tile are 1,024 cycles of the SM's special function unit (16 exponentials a cycle) and 512 (heads of 64) or 1,024
 // of its tensor cores, 512 or 1,280 of shared memory's 128 bytes a cycle; a tile alone takes some 2,400, two blocks on an SM 1,250 each.
-// 8,191 rows, window 4,096, 128 first positions, 32 heads over 8: heads of 64 308 us (683 TFLOP/s; the form with pages of 64 keys and
-// three blocks an SM, attention_prefill_tc.cu, 390), heads of 128 408 us (1,031); turns of 100 to 2,047 rows, 16 heads of 128 over 4,
-// window 2,048: 67 us (mma.sync 190).  Measured beside it: one thread a row 311 to 317 and 77 us on 12 streams' turns (71 now), two tiles
-// a block (one block an SM) 329, 64 keys at a time with two buffers of S 323 (heads of 128: 442), an eighth to a half of the
-// exponentials as polynomials on the multiply-add pipes 304 to 365 (heads of 128: 428 to 515).
+// 8,191 rows, window 4,096, 128 first positions, 32 heads over 8: heads of 64 299 us (704 TFLOP/s; the form with pages of 64 keys and
+// three blocks an SM, attention_prefill_tc.cu, 390), heads of 128 403 us (1,045); turns of 3 to 1,500 rows of 12 streams, window 1,024, 53 us
+// (83), of 100 to 2,047 rows, 16 heads of 128 over 4, window 2,048, 45 us (mma.sync 190).  A block's fixed part is some 6,000 cycles; zeros
+// by the softmax warps, rows stored by their own threads and blocks without a tile cost another 8,000 on the turns (69 and 66 us).
+// Measured beside it: one thread a row 311 to 317, two tiles a block (one block an SM) 329, 64 keys at a time with two buffers of S 323 (heads
+// of 128: 442), an eighth to a half of the exponentials as polynomials on the multiply-add pipes 304 to 365 (heads of 128: 428 to 515).
 //
 // Every wait on an mbarrier is bounded; a wait that gives up sets the status word, all roles leave their loops, tensor memory is freed
 // and the block returns.
@@ -30,6 +32,7 @@
 
 #define AST_NEG (-1e30f)
 #define AST_MOST_SPLITS 8      // blocks that share a tile's keys: a portable cluster
+#define AST_LISTED 128         // sequences whose tiles a grid may list
 
 template <int HD>
 struct AstShape {
@@ -77,7 +80,7 @@ attention_stream_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gr
                            const __grid_constant__ CUtensorMap map_v, bf16* __restrict__ out, const int* __restrict__ block_table,
                            int bt_width, const int* __restrict__ seq_slot, const int* __restrict__ seq_pos0,
                            const int* __restrict__ seq_qstart, const int* __restrict__ seq_qlen, const bf16* __restrict__ gate,
-                           int gate_stride, int gate_elem, int nh, int nkv, int G, int TP, int hd_, int vd_, int per_page_, int window, int chunk, int first,
+                           int gate_stride, int gate_elem, int nh, int nkv, int n_seqs, int G, int TP, int hd_, int vd_, int per_page_, int window, int chunk, int first,
                            float scale, const float* __restrict__ slopes, const float* __restrict__ sinks, int n_blocks, int* __restrict__ status) {
   const int n_splits = SHARED ? n_blocks : 1, hd = EXACT ? HD : hd_, vd = EXACT ? HD : vd_, per_page = EXACT ? 1 : per_page_;
   using Shape = AstShape<HD>;
@@ -90,7 +93,7 @@ attention_stream_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gr
   uint8_t* sq = smem;                         // [64 dimensions][128 rows][128 bytes]
   uint8_t* sk = sq + Q_BYTES;                 // [stage][64 dimensions][128 keys][128 bytes]
   uint8_t* sv = sk + NS * KV_BYTES;           // [stage][page][dimension][64 positions]
-  __shared__ uint64_t q_full, k_full[NS], v_full[NS], k_empty[NS], v_empty[NS], s_full, s_free, p_full, pv_done;
+  __shared__ uint64_t q_full, k_full[NS], v_full[NS], k_empty[NS], v_empty[NS], s_full, s_free, p_full, pv_done, zeroed[NS];
   __shared__ float row_s[2][2][128];          // what the two threads of a row tell each other: [iteration's parity][thread][row]
   __shared__ float last_s[2][128], join_s[SHARED ? AST_MOST_SPLITS : 1][SHARED ? 64 : 128];      // maxima and sums of this block's rows; factors of the rows it stores
   __shared__ int place_s[SHARED ? 64 : 128];      // and where those lie in out, from the tile's first row and head on (-1: nowhere)
@@ -99,10 +102,41 @@ attention_stream_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gr
   volatile int* abort_flag = &abort_s;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  // kv heads, then sequences vary fastest; the tiles with the longest key range come first
-  const int kvh = blockIdx.x, b = blockIdx.y;
-  const int split = blockIdx.z % n_splits, row0 = (int)(gridDim.z / n_splits - 1 - blockIdx.z / n_splits) * TP;
-  const int qlen = seq_qlen[b];      // step data: written long before the kernel before this one
+  // kv heads vary fastest; of a sequence's tiles the ones with the longest key range come first
+  const int kvh = blockIdx.x, split = blockIdx.z % n_splits;
+  int b = blockIdx.y, tile = (int)(gridDim.z / n_splits - 1 - blockIdx.z / n_splits), qlen;
+  if (n_seqs > 0) {      // the tiles of up to AST_LISTED sequences one after the other: which is this one (every warp looks for itself)
+    const int t = blockIdx.z / n_splits;
+    int q[AST_LISTED / 32], n[AST_LISTED / 32], sum = 0;
+#pragma unroll
+    for (int e = 0; e < AST_LISTED / 32; e++) {
+      const int j = lane * (AST_LISTED / 32) + e;
+      q[e] = j < n_seqs ? seq_qlen[j] : 0;
+      n[e] = (q[e] + TP - 1) / TP;
+      sum += n[e];
+    }
+    int end = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, end, o);
+      if (lane >= o) end += up;
+    }
+    const unsigned past = __ballot_sync(0xffffffffu, end > t);
+    const int owner = past ? __ffs(past) - 1 : 31;
+    int at = end - sum, found = 0;
+    tile = qlen = 0;
+#pragma unroll
+    for (int e = 0; e < AST_LISTED / 32; e++) {
+      if (t >= at && t < at + n[e]) found = lane * (AST_LISTED / 32) + e, tile = at + n[e] - 1 - t, qlen = q[e];
+      at += n[e];
+    }
+    b = __shfl_sync(0xffffffffu, found, owner);
+    tile = __shfl_sync(0xffffffffu, tile, owner);
+    qlen = __shfl_sync(0xffffffffu, past ? qlen : 0, owner);      // (behind the last tile: nothing to do)
+  } else {
+    qlen = seq_qlen[b];      // step data: written long before the kernel before this one
+  }
+  const int row0 = tile * TP;
   if (row0 >= qlen) {
     pdl_wait();   // a kernel counts as complete when its blocks are: none may finish before its predecessor has
     return;
@@ -128,6 +162,28 @@ attention_stream_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gr
   const int per_split = (n_all + n_splits - 1) / n_splits, it0 = split * per_split, n_it = max(0, min(n_all - it0, per_split));
   const int* table = block_table + (size_t)b * bt_width;
 
+  // where 64 positions lie: their head's page (-1: there are none; a page given back, of which every key is masked: 0) and which 64
+  struct At { int page, part; };
+  auto at_of = [&](int v) {
+    v += 2 * it0;
+    if (v >= n_pages) return At{-1, 0};
+    const int j = v < nf ? v : jb0 + v - nf;
+    return per_page == 1 ? At{max(table[j], 0) * nkv + kvh, 0} : At{max(table[j / per_page], 0) * nkv + kvh, j % per_page};
+  };
+  At p0{-1, 0}, p1{-1, 0};
+  if (threadIdx.x == 32 * 8) {      // the TMA producer: asked for before the wait for the kernel before, as the step's other tables are
+    p0 = at_of(0), p1 = at_of(1);
+    asm volatile("prefetch.tensormap [%0];" ::"l"((uint64_t)&map_q) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"((uint64_t)&map_k) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"((uint64_t)&map_v) : "memory");
+  }
+  // Whether iteration i brings value columns that no row of the tile reads (between the first positions and the tile's window, or beyond
+  // the last row): they become zero before the product reads them, whatever they hold.
+  auto key_of = [&](int v) { return (v < nf ? v : jb0 + v - nf) * PAGE; };
+  auto unread = [&](int v) {
+    const int key0 = key_of(v);
+    return v < n_pages && ((key_lo > key0 && first - key0 < min(key_lo - key0, PAGE)) || key_hi < key0 + PAGE);
+  };
   if (threadIdx.x == 0) {
     abort_s = 0;
     mbar_init(&q_full, 1);
@@ -136,6 +192,7 @@ attention_stream_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gr
       mbar_init(&v_full[s], 1);
       mbar_init(&k_empty[s], 1);
       mbar_init(&v_empty[s], 1);
+      mbar_init(&zeroed[s], 2);
     }
     mbar_init(&s_full, 1);
     mbar_init(&s_free, 8);
@@ -166,15 +223,6 @@ attention_stream_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gr
           for (int h = 0; h < HALVES; h++)
             if (hd == HD) tma_load_2d(sq + h * (128 * 128) + g * (TP * 128), &map_q, &q_full, (h0 + g) * HD + h * 64, (int)m_base);
             else tma_load_3d(sq + h * (128 * 128) + g * (TP * 128), &map_q, &q_full, h * 64, h0 + g, (int)m_base);
-        // where 64 positions lie: their head's page (-1: there are none; a page given back, of which every key is masked: 0) and which 64
-        struct At { int page, part; };
-        auto at_of = [&](int v) {
-          v += 2 * it0;
-          if (v >= n_pages) return At{-1, 0};
-          const int j = v < nf ? v : jb0 + v - nf;
-          return per_page == 1 ? At{max(table[j], 0) * nkv + kvh, 0} : At{max(table[j / per_page], 0) * nkv + kvh, j % per_page};
-        };
-        At p0 = at_of(0), p1 = at_of(1);
         for (int i = 0; i < n_it; i++) {
           const int s = i % NS;
           const At a = p0, c = p1;
@@ -226,7 +274,8 @@ attention_stream_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gr
         const int s = i % NS, steps = i == n - 1 && odd ? 4 : 8;
         // P beside S: the next scores wait until every softmax warp holds its rows of these
         if (OWN_P && i + 1 < n && !(arrived(&s_free, i & 1, 35) && scores(i + 1))) break;
-        if (!arrived(&v_full[s], (i / NS) & 1, 36) || !arrived(&p_full, i & 1, 37)) break;
+        if (!arrived(&v_full[s], (i / NS) & 1, 36)) break;
+        if (!arrived(&zeroed[s], (i / NS) & 1, 42) || !arrived(&p_full, i & 1, 37)) break;
         tc_fence_after();
         if (elect_lane()) {
           for (int kk = 0; kk < steps; kk++)
@@ -237,6 +286,37 @@ attention_stream_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gr
         __syncwarp();
         // P over S: the tensor pipe runs the product that reads it before the one that overwrites it
         if (!OWN_P && i + 1 < n && !scores(i + 1)) break;
+      }
+    } else {
+      // ---- the other two warps: unread value columns, a page each ----
+      const int p = warp - 10;
+      for (int i = 0; i < n_it; i++) {
+        const int s = i % NS, v = 2 * (it0 + i) + p;
+        // (every iteration, so that no phase of a stage's barriers passes these warps by: the product waits for them)
+        if (!mbar_wait_warp(&v_full[s], (i / NS) & 1, abort_flag)) { atomicExch(status, 39); break; }
+        if (unread(v)) {
+          const int key0 = key_of(v);
+          for (int r = lane; r < HD; r += 32) {
+            uint8_t* vrow = sv + s * KV_BYTES + p * (HD * 128) + r * 128;   // dimension r: 64 positions, 16-byte pieces swizzled by r & 7
+#pragma unroll 2
+            for (int e = 0; e < 8; e++) {
+              const int at = key0 + 8 * e;
+              const uint32_t keep = (ast_below(first - at) | ~ast_below(key_lo - at)) & ast_below(key_hi - at) & 255u;
+              if (keep == 255u) continue;
+              uint4* piece = reinterpret_cast<uint4*>(vrow + ((e ^ (r & 7)) << 4));
+              uint4 x = make_uint4(0, 0, 0, 0);
+              if (keep) {
+                auto pair = [&](uint32_t w, int j) { return w & ((keep >> j & 1 ? 0xffffu : 0u) | (keep >> (j + 1) & 1 ? 0xffff0000u : 0u)); };
+                x = *piece;
+                x = make_uint4(pair(x.x, 0), pair(x.y, 2), pair(x.z, 4), pair(x.w, 6));
+              }
+              *piece = x;
+            }
+          }
+          fence_proxy_async_smem();
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&zeroed[s]);
       }
     }
     if (SHARED) {
@@ -264,7 +344,7 @@ attention_stream_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gr
     // row and begin at or behind the last row's window, or hold first positions only.  (Idle rows read what comes: they are never written.)
     const int lo_last = first_key(key_hi - 1, window, chunk);
     for (int i = 0; i < n_it; i++) {
-      const int s = i % NS, vp = 2 * (it0 + i) + half, key0 = (vp < nf ? vp : jb0 + vp - nf) * PAGE;
+      const int vp = 2 * (it0 + i) + half, key0 = key_of(vp);
       const bool there = vp < n_pages;
       const bool whole = there && key0 + PAGE - 1 <= q_lo && (key0 >= lo_last || key0 + PAGE <= first);
       if (!mbar_wait_warp(&s_full, i & 1, abort_flag)) { atomicExch(status, 38); ok = false; break; }
@@ -292,29 +372,6 @@ attention_stream_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gr
 #pragma unroll
           for (int c = 0; c < 32; c++)
             if (!(seen & (1u << c))) v[h + c] = __float_as_uint(AST_NEG);
-        }
-        // value columns that no row of the tile reads become zero before the product reads them, whatever they hold: those between
-        // the first positions and the tile's window, and those beyond the last row
-        if (there && ((key_lo > key0 && c_first < min(key_lo - key0, PAGE)) || key_hi < key0 + PAGE)) {
-          if (!mbar_wait_warp(&v_full[s], (i / NS) & 1, abort_flag)) { atomicExch(status, 39); ok = false; break; }
-          if (r < HD) {
-            uint8_t* vrow = sv + s * KV_BYTES + half * (HD * 128) + r * 128;   // dimension r: 64 positions, 16-byte pieces swizzled by r & 7
-#pragma unroll 1
-            for (int e = 0; e < 8; e++) {
-              const int at = 8 * e;
-              const uint32_t keep = (ast_below(c_first - at) | ~ast_below(key_lo - key0 - at)) & ast_below(key_hi - key0 - at) & 255u;
-              uint4* piece = reinterpret_cast<uint4*>(vrow + ((e ^ (r & 7)) << 4));
-              if (keep == 255u) continue;
-              uint4 x = make_uint4(0, 0, 0, 0);
-              if (keep) {
-                auto pair = [&](uint32_t w, int j) { return w & ((keep >> j & 1 ? 0xffffu : 0u) | (keep >> (j + 1) & 1 ? 0xffff0000u : 0u)); };
-                x = *piece;
-                x = make_uint4(pair(x.x, 0), pair(x.y, 2), pair(x.z, 4), pair(x.w, 6));
-              }
-              *piece = x;
-            }
-          }
-          fence_proxy_async_smem();
         }
       }
       float rm[2] = {AST_NEG, AST_NEG};
@@ -381,32 +438,39 @@ attention_stream_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gr
       l += row_s[n_it & 1][half ^ 1][r];
     }
     tc_fence_after();
-    if (!SHARED && vd == HD && !(gate && gate_elem)) {      // every thread stores its half of a row
+    if (!SHARED && vd == HD && !(gate && gate_elem)) {
+      // Finished rows go to shared memory as bfloat16 (keys are done with) and out from there, whole rows at a time: stored by their own
+      // threads every store would touch 32 lines.
+      const bool row_valid = ok && g < G && pi < rows;
+      float inv = l > 0.f ? 1.0f / l : 0.f;
+      if (sinks && row_valid) inv = sink_quotient(m_used * 0.6931471805599453f, l, sinks[h0 + g]);
+      if (gate && row_valid) inv *= head_gate(gate, m_base + pi, gate_stride, h0 + g, 0, HD, 0);
+      if (half == 0) place_s[r] = row_valid ? pi * nh + g : -1;
       if (ok) {
-        const bool row_valid = g < G && pi < rows;
-        float inv = l > 0.f ? 1.0f / l : 0.f;
-        if (sinks && row_valid) inv = sink_quotient(m_used * 0.6931471805599453f, l, sinks[h0 + g]);
-        if (gate && row_valid) inv *= head_gate(gate, m_base + pi, gate_stride, h0 + g, 0, HD, 0);
 #pragma unroll
         for (int d0 = 0; d0 < HD / 2; d0 += 32) {
-          __syncwarp();      // idle rows left the branch below early: the loads take the whole warp
           uint32_t o[32];
           tmem_ld32(t_o + d0, o);
           tmem_ld_wait();
-          if (row_valid) {
-            uint4* orow = reinterpret_cast<uint4*>(out + ((m_base + pi) * nh + h0 + g) * HD + half * (HD / 2) + d0);
 #pragma unroll
-            for (int c = 0; c < 32; c += 8) {
-              uint32_t w[4];
+          for (int c = 0; c < 32; c += 8) {
+            uint32_t w[4];
 #pragma unroll
-              for (int e = 0; e < 4; e++) {
-                __nv_bfloat162 pp = __floats2bfloat162_rn(__uint_as_float(o[c + 2 * e]) * inv, __uint_as_float(o[c + 2 * e + 1]) * inv);
-                w[e] = *reinterpret_cast<uint32_t*>(&pp);
-              }
-              orow[c / 8] = make_uint4(w[0], w[1], w[2], w[3]);
+            for (int e = 0; e < 4; e++) {
+              __nv_bfloat162 pp = __floats2bfloat162_rn(__uint_as_float(o[c + 2 * e]) * inv, __uint_as_float(o[c + 2 * e + 1]) * inv);
+              w[e] = *reinterpret_cast<uint32_t*>(&pp);
             }
+            const int piece = (half * (HD / 2) + d0 + c) / 8;
+            *reinterpret_cast<uint4*>(sk + r * (HD * 2) + ((piece ^ (r & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
           }
         }
+      }
+      asm volatile("bar.sync 9, 256;" ::: "memory");
+#pragma unroll
+      for (int n = 0; n < 128 * (HD / 8) / 256; n++) {
+        const int row = (n * 256 + (int)threadIdx.x) / (HD / 8), piece = threadIdx.x % (HD / 8), place = place_s[row];
+        if (place >= 0)
+          reinterpret_cast<uint4*>(out + (m_base * nh + h0 + place) * HD)[piece] = *reinterpret_cast<const uint4*>(sk + row * (HD * 2) + ((piece ^ (row & 7)) << 4));
       }
     } else {
       // Rows of O, their maxima and sums go to shared memory (keys and values are done with), from where they are stored row by row.  The
@@ -515,7 +579,11 @@ static int launch_attention_stream_tc(void* out, const void* q, int q_stride, in
     // the same through a map of two dimensions
     if (tensor_map(&mv, v_pool, n_pages * nkv * HD, page_size, page_size, HD)) return 1;
   } else if (tensor_map3(&mv, "leb_attention_stream_tc", v_pool, page_size, vd, n_pages * nkv, page_size, (long long)vd * page_size, HD, 1)) return 1;
+  // Sequences of very different lengths: a list of tiles, so that none of the blocks of a full grid has to come and go for nothing (952 tiles of
+  // 12 sequences, 4,512 blocks otherwise).
   dim3 grid(nkv, B, ceil_div(max_qlen, TP) * n_splits);
+  const bool listed = B > 1 && B <= AST_LISTED && M / TP + B < ceil_div(max_qlen, TP) * B;
+  if (listed) grid = dim3(nkv, 1, (M / TP + B) * n_splits);
   LEB_REQUIRE(grid.y <= 65535 && grid.z <= 65535, "leb_attention_stream_tc: grid too large (%u, %u)", grid.y, grid.z);
   constexpr auto kern = attention_stream_tc_kernel<HD, SHARED, EXACT>;
   // The warpgroups share out the registers of the launch: with fewer than REGS a thread they would wait for ever.
@@ -530,7 +598,7 @@ static int launch_attention_stream_tc(void* out, const void* q, int q_stride, in
   const cudaError_t e = leb_allow_smem<kern, Shape::SMEM>();
   if (e != cudaSuccess) return leb_fail("leb_attention_stream_tc: shared memory %d: %s", Shape::SMEM, cudaGetErrorString(e));
   leb_launch_cluster(SHARED ? n_splits : 1, kern, grid, dim3(Shape::THREADS), Shape::SMEM, st, mq, mk, mv, (bf16*)out, block_table, bt_width,
-                     seq_slot, seq_pos0, seq_qstart, seq_qlen, (const bf16*)gate, gate_stride, gate_elem, nh, nkv, G, TP, hd, vd, page_size / 64, window, chunk, first,
+                     seq_slot, seq_pos0, seq_qstart, seq_qlen, (const bf16*)gate, gate_stride, gate_elem, nh, nkv, listed ? B : 0, G, TP, hd, vd, page_size / 64, window, chunk, first,
                      scale, slopes, sinks, n_splits, status);
   LEB_CHECK_LAUNCH("leb_attention_stream_tc");
   return 0;

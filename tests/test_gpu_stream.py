@@ -195,6 +195,16 @@ def test_chunks_of_a_few_rows_and_of_none(nh, nkv, hd):
         c.check(c.run())
 
 
+@pytest.mark.parametrize("n_seqs", [2, 31, 33, 128, 129, 200])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_many_sequences_of_unequal_lengths(n_seqs, hd):
+    """Tiles are listed for up to 128 sequences of unequal lengths, some of which bring nothing, padding at both ends."""
+    rng = np.random.default_rng(n_seqs)
+    seqs = [(int(rng.integers(0, 150)), int(rng.integers(0, 7)) if i % 9 else int(rng.integers(40, 120))) for i in range(n_seqs)]
+    c = Case(seqs, 4, 2, hd, hd, 64, 60, 5, BF16, seed=n_seqs, padding=[0, n_seqs - 1] if n_seqs > 2 else [])
+    c.check(c.run())
+
+
 @pytest.mark.parametrize("nh,nkv,hd,window,first", [(8, 2, 64, 200, 70), (4, 4, 128, 333, 4), (2, 1, 128, 64, 65), (8, 1, 64, 1, 1)])
 def test_many_tiles(nh, nkv, hd, window, first):
     """More tiles than the SMs take at once, and long sequences."""
