@@ -223,6 +223,7 @@ attention_stream_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gr
           for (int h = 0; h < HALVES; h++)
             if (hd == HD) tma_load_2d(sq + h * (128 * 128) + g * (TP * 128), &map_q, &q_full, (h0 + g) * HD + h * 64, (int)m_base);
             else tma_load_3d(sq + h * (128 * 128) + g * (TP * 128), &map_q, &q_full, h * 64, h0 + g, (int)m_base);
+        int keys = 0, values = 0;      // iterations whose copies are under way
         for (int i = 0; i < n_it; i++) {
           const int s = i % NS;
           const At a = p0, c = p1;
@@ -234,6 +235,7 @@ attention_stream_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gr
             tma_load_2d(sk + s * KV_BYTES + h * (128 * 128), &map_k, &k_full[s], h * 64, (a.page * per_page + a.part) * PAGE);
             if (c.page >= 0) tma_load_2d(sk + s * KV_BYTES + h * (128 * 128) + 64 * 128, &map_k, &k_full[s], h * 64, (c.page * per_page + c.part) * PAGE);
           }
+          keys = i + 1;
           if (!mbar_wait(&v_empty[s], ((i / NS) & 1) ^ 1, abort_flag)) { atomicExch(status, 32); break; }
           mbar_expect_tx(&v_full[s], bytes);
           if (vd == HD) {
@@ -243,7 +245,15 @@ attention_stream_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gr
             tma_load_3d(sv + s * KV_BYTES, &map_v, &v_full[s], a.part * PAGE, 0, a.page);
             if (c.page >= 0) tma_load_3d(sv + s * KV_BYTES + HD * 128, &map_v, &v_full[s], c.part * PAGE, 0, c.page);
           }
+          values = i + 1;
         }
+        // the block stays until its copies have landed, also where a role gave up
+        auto landed = [](uint64_t* bar, uint32_t parity) {
+          for (int n = 0; n < 1 << 16 && !mbar_try_wait(bar, parity); n++) {}
+        };
+        if (n_it > 0) landed(&q_full, 0);
+        for (int i = max(keys - NS, 0); i < keys; i++) landed(&k_full[i % NS], (i / NS) & 1);
+        for (int i = max(values - NS, 0); i < values; i++) landed(&v_full[i % NS], (i / NS) & 1);
       }
     } else if (warp == 9) {
       // ---- MMA issuer: the whole warp walks the loop, one lane issues ----
