@@ -9,10 +9,13 @@ only launches.  At the end the memory held is what it was after the first window
 """
 import argparse
 import math
+import os
+import sys
 import time
 
 import torch
 
+sys.path.insert(0, os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
 from lastengine_b200.cache import StreamCache
 from lastengine_b200.ops import kernels
 
