@@ -401,7 +401,8 @@ store_tile_kernel(T* __restrict__ k_pool, T* __restrict__ v_pool, const T* __res
     if (sizeof(T) == 2) {
       // two rows a lane, two dimensions a warp's turn
       const int ra = 2 * lane, sa = slot_s[ra], sb = slot_s[ra + 1];
-      const bool joined = sa >= 0 && sb == sa + 1 && place_s[ra] == place_s[ra + 1] && ((sa | page) & 1) == 0;      // both places in one aligned word
+      const bool joined = sa >= 0 && sb == sa + 1 && place_s[ra] == place_s[ra + 1] && ((sa | page) & 1) == 0 &&      // both places in one aligned word
+                          ((uintptr_t)v_pool & 3) == 0;
       T* const pa = v_pool + place_s[ra] * vd + max(sa, 0);
       T* const pb = v_pool + place_s[ra + 1] * vd + max(sb, 0);
       for (int d = 2 * warp; d < n; d += 16) {

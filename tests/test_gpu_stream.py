@@ -1,5 +1,6 @@
 """Streams with a window and first positions that stay visible: attention, the tables built on the device, stores by slot map, and
 what runs them together, against plain arithmetic in double precision and plain bookkeeping."""
+import math
 import types
 
 import numpy as np
@@ -479,6 +480,22 @@ def test_stores_beyond_32_bits_and_outside_the_pool():
     assert torch.equal(kd[-1, :, -1].reshape(-1), k[0]) and torch.equal(vdev.view(n_pages, nkv, hd, page)[-1, :, :, -1].reshape(-1), k[0])
     assert torch.equal(kd[0, :, 3].reshape(-1), k[2])
     assert int((kd != 0).sum()) == int((k[[0, 2]] != 0).sum())
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("M", [5, 500])
+def test_stores_into_pools_that_begin_anywhere(dtype, M):
+    """Pools one number behind a 16-byte boundary, rows whose places follow one another."""
+    nkv, hd, page, n_pages = 2, 64, 64, 9
+    at = lambda *shape: torch.zeros(1 + math.prod(shape), dtype=dtype, device=DEV)[1:].view(shape)
+    kd, vdev = at(n_pages, nkv, page, hd), at(n_pages, nkv, hd, page)
+    k, v = torch.randn(M, nkv * hd).to(dtype), torch.randn(M, nkv * hd).to(dtype)
+    K().store_rows(kd, vdev, k.to(DEV), v.to(DEV), words(np.arange(2, 2 + M)))
+    want_k, want_v = torch.zeros(kd.shape, dtype=dtype), torch.zeros(vdev.shape, dtype=dtype)
+    s = torch.arange(2, 2 + M)
+    want_k[s // page, :, s % page] = k.view(M, nkv, hd)
+    want_v[s // page, :, :, s % page] = v.view(M, nkv, hd)
+    assert torch.equal(kd.cpu(), want_k) and torch.equal(vdev.cpu(), want_v)
 
 
 def test_stores_refuse():
