@@ -630,6 +630,8 @@ LEB_API int leb_attention_stream_tc(void* out, const void* q, int q_stride, int 
   LEB_REQUIRE(status != nullptr, "leb_attention_stream_tc: a status word is required");
   LEB_REQUIRE((((uintptr_t)q | (uintptr_t)out | (uintptr_t)k_pool | (uintptr_t)v_pool) & 15) == 0 && q_stride % 8 == 0,
               "leb_attention_stream_tc: q, out and the pools must be 16-byte aligned, q's row stride a multiple of 8");
+  LEB_REQUIRE((long long)n_pages * nkv * (page_size > vd ? page_size : vd) < 1ll << 31, "leb_attention_stream_tc: pools of %d pages of %d positions and %d kv heads",
+              n_pages, page_size, nkv);
   LEB_REQUIRE(n_splits >= 0 && n_splits <= AST_MOST_SPLITS, "leb_attention_stream_tc: %d blocks for a tile's keys, %d at most", n_splits, AST_MOST_SPLITS);
   if (n_splits == 0) n_splits = ast_splits(M, B, nh, nkv, window, chunk, first, max_qlen, max_kvlen);
 #define LEB_AST_ARGS out, q, q_stride, M, k_pool, v_pool, n_pages, block_table, bt_width, seq_slot, seq_pos0, seq_qstart, seq_qlen, gate, \

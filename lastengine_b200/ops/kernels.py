@@ -1775,15 +1775,16 @@ STREAM_ROWS = 16
 def _stream_form(out, batch, nh, nkv, hd, vd, page_size, wide, q, k_pool, v_pool):
     """The kernel made for rows with first positions that takes a step, None where the ones for all rows do."""
     M, single = out.shape[0], batch.max_qlen == 1
-    aligned = (k_pool.data_ptr() | v_pool.data_ptr()) & 15 == 0
+    aligned, rows_aligned = (k_pool.data_ptr() | v_pool.data_ptr()) & 15 == 0, (q.data_ptr() | out.data_ptr()) & 15 == 0
     if out.dtype is torch.bfloat16:
         mma = vd == hd and _stream_takes("leb_attention_prefill_supported", nh, nkv, hd, page_size)
         if mma and not aligned:
             raise KernelError("attention: the pools of these heads must lie on 16-byte boundaries")
+        mma = mma and rows_aligned      # (rows that begin anywhere: the kernel for any widths)
         if single and mma and M == batch.n_seqs and _stream_takes("leb_attention_decode_supported", nh, nkv, hd, page_size):
             return _attention_stream_decode
-        if (not single and not wide and aligned and (q.data_ptr() | out.data_ptr()) & 15 == 0 and q.stride(0) % 8 == 0
-                and _stream_takes("leb_attention_stream_tc_supported", nh, nkv, hd, vd, page_size)):
+        if (not single and not wide and aligned and rows_aligned and q.stride(0) % 8 == 0
+                and k_pool.numel() < (hd << 31) and _stream_takes("leb_attention_stream_tc_supported", nh, nkv, hd, vd, page_size)):
             return _attention_stream_tc
         if mma and not single and M > STREAM_ROWS:
             return None

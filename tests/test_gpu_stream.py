@@ -281,6 +281,19 @@ def test_offsets_beyond_32_bits():
         torch.cuda.empty_cache()
 
 
+@pytest.mark.parametrize("seqs", [DECODE, CHUNKS])
+@pytest.mark.parametrize("dtype,hd", [(BF16, 64), (BF16, 128), (F32, 48)])
+def test_rows_that_begin_anywhere(seqs, dtype, hd):
+    """q and out one number behind a 16-byte boundary."""
+    c = Case(seqs, 8, 2, hd, hd, 64, 100, 70, dtype, seed=21)
+    q = torch.empty(1 + c.qd.numel(), dtype=dtype, device=DEV)[1:].view(c.qd.shape)
+    q.copy_(c.qd)
+    c.qd = q
+    out = torch.full((1 + c.rows * 8 * hd,), float("nan"), dtype=dtype, device=DEV)[1:].view(c.rows, 8 * hd)
+    K().attention(out, c.qd, c.k_pool, c.v_pool, c.table, c.batch, 8, 2, hd, 64, 100, c.scale, vd=hd, first=70)
+    c.check(out)
+
+
 def test_on_another_stream():
     st = torch.cuda.Stream()
     with torch.cuda.stream(st):
