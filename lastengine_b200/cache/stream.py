@@ -68,6 +68,9 @@ class StreamCache:
             raise ValueError("page size must be a multiple of 32")
         if min(n_layers, n_kv_heads, head_dim, max_seqs, max_tokens, max_len) < 1 or window < 0 or first < 0:
             raise ValueError("sizes of a stream cache must be positive, window and first positions not negative")
+        if max_len > 2 ** 31 - 2 ** 16:
+            raise ValueError(f"a sequence of {max_len} positions: they are counted in 32 bits")
+        window, first = (min(int(n), int(max_len)) for n in (window, first))      # (more are as many)
         self.page_size, self.window, self.first = int(page_size), int(window), int(first)
         self.nkv, self.hd, self.vd = int(n_kv_heads), int(head_dim), int(v_head_dim or head_dim)
         self.max_len = int(max_len)

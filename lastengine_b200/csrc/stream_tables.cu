@@ -83,7 +83,8 @@ stream_tables_kernel(int* __restrict__ table, int width, int* __restrict__ slot_
   __shared__ int2 warps[STB_THREADS / 32];
   stb_wait();
   const int n_free = min(counts[0], n_pages);
-  int rows = 0, need = 0, bad = 0, longer = 0;
+  int rows = 0, need = 0, bad = 0, longer = 0, more = 0;
+  const long long longest = min((long long)min(width, pages_width) * page, 0x80000000ll - page);      // positions are counted in 32 bits
   for (int b0 = 0; b0 < B; b0 += STB_THREADS * STB_ITEMS) {
     const int first = b0 + threadIdx.x * STB_ITEMS;
     StbSeq s[STB_ITEMS];
@@ -99,7 +100,7 @@ stream_tables_kernel(int* __restrict__ table, int width, int* __restrict__ slot_
       nn[e] = 0;
       if (s[e].slot >= 0) {
         const long long end = (long long)s[e].pos0 + s[e].qlen;
-        if (end > (long long)min(width, pages_width) * page) longer = 1;
+        if (end > longest) longer = 1;
         else nn[e] = (int)((end + page - 1) / page) - (s[e].pos0 + page - 1) / page;
       }
       q += nq[e];
@@ -114,6 +115,7 @@ stream_tables_kernel(int* __restrict__ table, int width, int* __restrict__ slot_
         pos0_s[first + e] = s[e].pos0;
         slot_s[first + e] = s[e].slot;
       }
+      more |= nq[e] > M || (unsigned)q + (unsigned)nq[e] > (unsigned)M;      // (the first sum above M is exact, later ones may have gone round)
       q += nq[e];
       n += nn[e];
     }
@@ -121,7 +123,8 @@ stream_tables_kernel(int* __restrict__ table, int width, int* __restrict__ slot_
   if (threadIdx.x == 0) qstart[B] = rows;
   bad = __syncthreads_or(bad);
   longer = __syncthreads_or(longer);
-  const int status = bad ? -3 : longer ? -1 : rows != M ? -2 : need > n_free ? need - n_free : 0;
+  more = __syncthreads_or(more);
+  const int status = bad ? -3 : longer ? -1 : more || rows != M ? -2 : need > n_free ? need - n_free : 0;
   const bool ok = status == 0;
   const int at = blockIdx.x * STB_THREADS + threadIdx.x, step = gridDim.x * STB_THREADS;
   if (at == 0) counts[1] = status;

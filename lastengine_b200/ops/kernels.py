@@ -1674,6 +1674,9 @@ def _gate_layout(gate: torch.Tensor | None, M: int, nh: int, width: int, dtype: 
     return gate.stride(0), int(gate.shape[1] != nh)
 
 
+_MOST_FIRST = 2 ** 31 - 2 ** 16      # first positions: more are as many (the kernels round them up to tiles and pages in 32 bits)
+
+
 def attention(out: torch.Tensor, q: torch.Tensor | None, k_pool: torch.Tensor, v_pool: torch.Tensor,
               block_table: torch.Tensor, batch, nh: int, nkv: int, hd: int, page_size: int,
               window: int, scale: float, gate: torch.Tensor | None = None,
@@ -1693,7 +1696,7 @@ def attention(out: torch.Tensor, q: torch.Tensor | None, k_pool: torch.Tensor, v
     row of a sequence reaches no result, whatever it is."""
     if first < 0:
         raise KernelError(f"attention: {first} first positions")
-    first = int(first) if window > 0 or chunk > 0 else 0
+    first = min(int(first), _MOST_FIRST) if window > 0 or chunk > 0 else 0
     _cuda(out, "attention.out")
     for name, t in (("slopes", slopes), ("sinks", sinks)):
         if t is not None:
@@ -1923,8 +1926,8 @@ def _stream_state(name: str, lens: torch.Tensor, pages: torch.Tensor, free: torc
     n_slots, n_pages, shape = lens.numel(), free.numel(), pages.shape
     if len(shape) != 2 or shape[0] != n_slots or counts.numel() != 2 or n_slots < 1 or shape[1] < 1:
         raise KernelError(f"{name}: page lists {tuple(shape)} of {n_slots} slots, {counts.numel()} counts (2)")
-    if page_size < 1 or n_pages * page_size > 2 ** 31:
-        raise KernelError(f"{name}: {n_pages} pages of {page_size} positions (2^31 positions at most)")
+    if not 1 <= page_size <= 2 ** 16 or n_pages * page_size > 2 ** 31:
+        raise KernelError(f"{name}: {n_pages} pages of {page_size} positions (of 1 to 65,536; 2^31 together at most)")
     return n_slots, shape[1], n_pages
 
 
@@ -1965,11 +1968,11 @@ def stream_advance(seq_slot: torch.Tensor, seq_qlen: torch.Tensor, lens: torch.T
     May be called before the step's kernels are: what goes back is given out by the next step's tables at the earliest."""
     _words("stream_advance", seq_slot, seq_qlen, lens, kept, pages, free, counts)
     n_slots, width, n_pages = _stream_state("stream_advance", lens, pages, free, counts, page_size)
-    if seq_slot.numel() != seq_qlen.numel() or kept.numel() != lens.numel() or window < 0 or first < 0:
+    if seq_slot.numel() != seq_qlen.numel() or kept.numel() != lens.numel() or not 0 <= window < 2 ** 31 or first < 0:
         raise KernelError(f"stream_advance: {seq_slot.numel()} slots and {seq_qlen.numel()} row counts, window {window}, first {first}")
     _check(lib().leb_stream_advance(
         seq_slot.data_ptr(), seq_qlen.data_ptr(), lens.data_ptr(), n_slots, kept.data_ptr(), pages.data_ptr(), width, free.data_ptr(), n_pages,
-        counts.data_ptr(), seq_slot.numel(), page_size, window, first, _stream()))
+        counts.data_ptr(), seq_slot.numel(), page_size, window, min(first, _MOST_FIRST), _stream()))
 
 
 def stream_release(seq_slot: torch.Tensor, lens: torch.Tensor, kept: torch.Tensor, pages: torch.Tensor, free: torch.Tensor,
@@ -1980,7 +1983,7 @@ def stream_release(seq_slot: torch.Tensor, lens: torch.Tensor, kept: torch.Tenso
     if kept.numel() != lens.numel() or first < 0:
         raise KernelError(f"stream_release: {kept.numel()} of {lens.numel()} slots, first {first}")
     _check(lib().leb_stream_release(seq_slot.data_ptr(), lens.data_ptr(), n_slots, kept.data_ptr(), pages.data_ptr(), width,
-                                    free.data_ptr(), n_pages, counts.data_ptr(), seq_slot.numel(), page_size, first, _stream()))
+                                    free.data_ptr(), n_pages, counts.data_ptr(), seq_slot.numel(), page_size, min(first, _MOST_FIRST), _stream()))
 
 
 def store_rows(k_pool: torch.Tensor, v_pool: torch.Tensor, k: torch.Tensor, v: torch.Tensor, slot_map: torch.Tensor) -> None:

@@ -270,6 +270,15 @@ def test_first_positions_without_a_window_or_beyond_the_sequence_are_the_whole_o
             assert float((c.run().float() - whole.float()).abs().max()) < 0.05
 
 
+@pytest.mark.parametrize("seqs", [DECODE, CHUNKS])
+@pytest.mark.parametrize("dtype,hd", [(BF16, 64), (BF16, 128), (BF16, 32), (F32, 48)])
+def test_more_first_positions_than_32_bits_count(seqs, dtype, hd):
+    c = Case(seqs, 4, 2, hd, hd, 64, 0, 0, dtype, seed=3)
+    c.window = 10
+    for c.first in (2 ** 31 - 1, 2 ** 31, 2 ** 33 + 5):
+        c.check(c.run())
+
+
 def test_offsets_beyond_32_bits():
     """Pools of more than 2^31 numbers, the sequences' pages at their end."""
     for hd, vd, seqs in ((64, 64, DECODE[:6]), (64, 64, CHUNKS[:4]), (128, 128, CHUNKS[:4]), (64, 32, CHUNKS[:4])):
@@ -412,6 +421,18 @@ def test_a_step_that_cannot_be_laid_out_changes_nothing():
     d.same_as(plain)
     o, t = d.tables([0, 1], [1, 2], 3, width=3), plain.tables([0, 1], [1, 2], 3)
     same_tables(o, t, [0, 1], [1, 2])
+
+
+def test_row_counts_whose_sum_goes_round():
+    """Padding with row counts that add up to 2^32 more than the step's rows, and a sequence among them."""
+    top = 2 ** 31 - 1
+    for slots, qlens, rows in (([-1, -1, -1, 1], [top, top, 2, 7], 7), ([-1, 0, -1, -1], [top, 3, top, 2], 3), ([-1] * 600 + [2], [2 ** 23] * 512 + [0] * 88 + [4], 4)):
+        d = Tables(6, 3, 4, 32, 0, 0)
+        o = d.tables(slots, qlens, rows)
+        assert int(d.counts[1]) == -2
+        assert o["slot"].tolist() == [-1] * len(slots) and o["qlen"].tolist() == [0] * len(slots) and bool((o["slot_map"] == -1).all())
+        d.advance(o)
+        d.same_as(S.PlainTables(6, 3, 4, 32, 0, 0))
 
 
 def test_tables_without_rows_and_without_sequences():

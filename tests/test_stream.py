@@ -95,3 +95,11 @@ def test_calls_off_the_gpu_are_refused():
         K.stream_advance(i, i, i, i, i.view(4, 1), i, i[:2], 64)
     with pytest.raises(K.KernelError):
         K.store_rows(torch.zeros(1, 1, 32, 8), torch.zeros(1, 1, 8, 32), torch.zeros(4, 8), torch.zeros(4, 8), i)
+
+
+def test_a_stream_cache_refuses_lengths_that_32_bits_do_not_count():
+    from lastengine_b200.cache import StreamCache
+    with pytest.raises(ValueError):
+        StreamCache(1, 1, 8, max_seqs=1, max_tokens=64, max_len=2 ** 31, window=64, first=4, device="cpu")
+    cache = StreamCache(1, 1, 8, max_seqs=1, max_tokens=64, max_len=128, window=2 ** 40, first=2 ** 40, device="cpu")
+    assert cache.kept.tolist() == [2] and (cache.window, cache.first) == (128, 128)
