@@ -19,7 +19,7 @@
 //
 // Bounds: 128 keys of a tile are 1,024 cycles of the SM's special function unit (16 exponentials a cycle) and 512 (heads of 64) or 1,024
 // of its tensor cores, 512 or 1,280 of shared memory's 128 bytes a cycle; a tile alone takes some 2,400, two blocks on an SM 1,250 each.
-// 8,191 rows, window 4,096, 128 first positions, 32 heads over 8: heads of 64 299 us (704 TFLOP/s; the form with pages of 64 keys and
+// 8,191 rows, window 4,096, 128 first positions, 32 heads over 8: heads of 64 300 us (701 TFLOP/s; the form with pages of 64 keys and
 // three blocks an SM, attention_prefill_tc.cu, 390), heads of 128 403 us (1,045); turns of 3 to 1,500 rows of 12 streams, window 1,024, 53 us
 // (83), of 100 to 2,047 rows, 16 heads of 128 over 4, window 2,048, 45 us (mma.sync 190).  A block's fixed part is some 6,000 cycles; zeros
 // by the softmax warps, rows stored by their own threads and blocks without a tile cost another 8,000 on the turns (69 and 66 us).
@@ -98,7 +98,7 @@ attention_stream_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gr
   __shared__ float last_s[2][128], join_s[SHARED ? AST_MOST_SPLITS : 1][SHARED ? 64 : 128];      // maxima and sums of this block's rows; factors of the rows it stores
   __shared__ int place_s[SHARED ? 64 : 128];      // and where those lie in out, from the tile's first row and head on (-1: nowhere)
   __shared__ uint32_t tmem_slot;
-  __shared__ int abort_s;
+  __shared__ int abort_s, sent_s[2];      // sent_s: iterations whose keys and values were asked for
   volatile int* abort_flag = &abort_s;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -186,6 +186,7 @@ attention_stream_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gr
   };
   if (threadIdx.x == 0) {
     abort_s = 0;
+    sent_s[0] = sent_s[1] = n_it;
     mbar_init(&q_full, 1);
     for (int s = 0; s < NS; s++) {
       mbar_init(&k_full[s], 1);
@@ -223,20 +224,18 @@ attention_stream_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gr
           for (int h = 0; h < HALVES; h++)
             if (hd == HD) tma_load_2d(sq + h * (128 * 128) + g * (TP * 128), &map_q, &q_full, (h0 + g) * HD + h * 64, (int)m_base);
             else tma_load_3d(sq + h * (128 * 128) + g * (TP * 128), &map_q, &q_full, h * 64, h0 + g, (int)m_base);
-        int keys = 0, values = 0;      // iterations whose copies are under way
         for (int i = 0; i < n_it; i++) {
           const int s = i % NS;
           const At a = p0, c = p1;
           p0 = at_of(2 * i + 2), p1 = at_of(2 * i + 3);      // asked for before the waits below
           const uint32_t bytes = c.page >= 0 ? KV_BYTES : KV_BYTES / 2;
-          if (!mbar_wait(&k_empty[s], ((i / NS) & 1) ^ 1, abort_flag)) { atomicExch(status, 31); break; }
+          if (!mbar_wait(&k_empty[s], ((i / NS) & 1) ^ 1, abort_flag)) { atomicExch(status, 31); sent_s[0] = sent_s[1] = i; break; }
           mbar_expect_tx(&k_full[s], bytes);
           for (int h = 0; h < HALVES; h++) {
             tma_load_2d(sk + s * KV_BYTES + h * (128 * 128), &map_k, &k_full[s], h * 64, (a.page * per_page + a.part) * PAGE);
             if (c.page >= 0) tma_load_2d(sk + s * KV_BYTES + h * (128 * 128) + 64 * 128, &map_k, &k_full[s], h * 64, (c.page * per_page + c.part) * PAGE);
           }
-          keys = i + 1;
-          if (!mbar_wait(&v_empty[s], ((i / NS) & 1) ^ 1, abort_flag)) { atomicExch(status, 32); break; }
+          if (!mbar_wait(&v_empty[s], ((i / NS) & 1) ^ 1, abort_flag)) { atomicExch(status, 32); sent_s[0] = i + 1; sent_s[1] = i; break; }
           mbar_expect_tx(&v_full[s], bytes);
           if (vd == HD) {
             tma_load_2d(sv + s * KV_BYTES, &map_v, &v_full[s], a.part * PAGE, a.page * HD);
@@ -245,15 +244,7 @@ attention_stream_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gr
             tma_load_3d(sv + s * KV_BYTES, &map_v, &v_full[s], a.part * PAGE, 0, a.page);
             if (c.page >= 0) tma_load_3d(sv + s * KV_BYTES + HD * 128, &map_v, &v_full[s], c.part * PAGE, 0, c.page);
           }
-          values = i + 1;
         }
-        // the block stays until its copies have landed, also where a role gave up
-        auto landed = [](uint64_t* bar, uint32_t parity) {
-          for (int n = 0; n < 1 << 16 && !mbar_try_wait(bar, parity); n++) {}
-        };
-        if (n_it > 0) landed(&q_full, 0);
-        for (int i = max(keys - NS, 0); i < keys; i++) landed(&k_full[i % NS], (i / NS) & 1);
-        for (int i = max(values - NS, 0); i < values; i++) landed(&v_full[i % NS], (i / NS) & 1);
       }
     } else if (warp == 9) {
       // ---- MMA issuer: the whole warp walks the loop, one lane issues ----
@@ -547,6 +538,15 @@ attention_stream_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gr
   }
   tc_fence_before();
   __syncthreads();
+  if (abort_s && threadIdx.x == 32 * 8) {      // a role gave up: the block stays until its copies have landed (else every one has been read)
+    auto landed = [](uint64_t* bar, int phase) {
+      for (int n = 0; n < 1 << 16 && !mbar_try_wait(bar, phase & 1); n++) {}
+    };
+    if (n_it > 0) landed(&q_full, 0);
+    for (int i = max(sent_s[0] - NS, 0); i < sent_s[0]; i++) landed(&k_full[i % NS], i / NS);
+    for (int i = max(sent_s[1] - NS, 0); i < sent_s[1]; i++) landed(&v_full[i % NS], i / NS);
+  }
+  __syncwarp();
   if (warp == 8) tmem_dealloc(tmem, Shape::COLUMNS);
 }
 
