@@ -315,6 +315,8 @@ def _declare(L) -> None:
         "leb_attention_stream_tc": [P, P, I, I, P, P, I, P, I, P, P, P, P, P, I, I, I, I, I, I, I, I, I, I, I, F, P, P, I, I, I, P, P],
         "leb_attention_stream_any_supported": [I, I, I, I, I],
         "leb_attention_stream_any": [P, P, P, P, I, P, I, P, P, P, P, P, P, I, I, I, I, I, I, I, I, I, I, I, F, P, P, I, I, P],
+        "leb_attention_stream_rows_supported": [I, I, I, I, I],
+        "leb_attention_stream_rows": [P, P, P, P, I, P, I, P, P, P, P, P, I, I, I, I, I, I, I, I, I, I, I, I, F, P, P, I, I, I, P],
         "leb_stream_tables": [P, I, P, P, P, P, P, P, P, P, P, P, I, P, I, P, I, P, I, I, I, P],
         "leb_stream_advance": [P, P, P, I, P, P, I, P, I, P, I, I, I, I, P],
         "leb_stream_release": [P, P, I, P, P, I, P, I, P, I, I, I, P],
@@ -1703,7 +1705,8 @@ def attention(out: torch.Tensor, q: torch.Tensor | None, k_pool: torch.Tensor, v
             _cuda(t, f"attention.{name}", torch.float32)
             assert t.numel() == nh
     if first > 0 and raw is None:
-        form = _stream_form(out, batch, nh, nkv, hd, vd or hd, page_size, wide, q, k_pool, v_pool)
+        form = _stream_form(out, batch, nh, nkv, hd, vd or hd, page_size, wide, q, k_pool, v_pool,
+                            _read_length(batch.max_kvlen, window, chunk, first))
         if form is not None:
             return form(out, q, k_pool, v_pool, block_table, batch, nh, nkv, hd, vd or hd, page_size, window, float(scale), gate, chunk, slopes, sinks,
                         first, wide, n_splits, scratch)
@@ -1774,8 +1777,14 @@ def _stream_takes(entry: str, *sizes: int) -> bool:
 # (The general kernel is behind at every size: 32-bit, 16 rows 400 and 20, 256 422 and 183, 2,048 2,937 and 1,336.)
 STREAM_ROWS = 16
 
+# A chunk's rows x heads x keys x (width + value width) from which its rows go in tiles instead of one by one.  us one by one and in tiles, window
+# 1,024: 32 heads of 64 over 8, 32 rows (134 million) 47 and 51, 64 rows 69 and 66, 700 rows 473 and 280; 16 of 128 over 2, 64 rows (268 million) 70 and
+# 76, 128 rows 133 and 83; 8 of 256 over 2, 32 rows 88 and 109, 64 rows 174 and 110; window 64, 9 heads of 64, 4 chunks of 30 to 70 rows (16
+# million) 19 and 47.
+STREAM_TILE_WORK = 200_000_000
 
-def _stream_form(out, batch, nh, nkv, hd, vd, page_size, wide, q, k_pool, v_pool):
+
+def _stream_form(out, batch, nh, nkv, hd, vd, page_size, wide, q, k_pool, v_pool, keys):
     """The kernel made for rows with first positions that takes a step, None where the ones for all rows do."""
     M, single = out.shape[0], batch.max_qlen == 1
     aligned, rows_aligned = (k_pool.data_ptr() | v_pool.data_ptr()) & 15 == 0, (q.data_ptr() | out.data_ptr()) & 15 == 0
@@ -1791,6 +1800,8 @@ def _stream_form(out, batch, nh, nkv, hd, vd, page_size, wide, q, k_pool, v_pool
             return _attention_stream_tc
         if mma and not single and M > STREAM_ROWS:
             return None
+    if not single and aligned and M * nh * keys * (hd + vd) >= STREAM_TILE_WORK and _stream_takes("leb_attention_stream_rows_supported", nh, nkv, hd, vd, page_size):
+        return _attention_stream_rows
     if aligned and M <= 65535 and _stream_takes("leb_attention_stream_any_supported", nh, nkv, hd, vd, page_size):
         return _attention_stream_any
     return None
@@ -1838,6 +1849,18 @@ def _attention_stream_any(out, q, k_pool, v_pool, block_table, batch, nh, nkv, h
         batch.seq_slot.data_ptr(), batch.seq_pos0.data_ptr(), batch.seq_qstart.data_ptr(),
         *((None, None) if batch.max_qlen == 1 and M == batch.n_seqs else (batch.row_seq.data_ptr(), batch.row_pos.data_ptr())),
         _ptr(gate), gate_stride, gate_elem, M, nh, nkv, hd, vd, page_size, window, chunk, first, scale, _ptr(slopes), _ptr(sinks), batch.max_kvlen, _stream_splits, _stream()))
+
+
+def _attention_stream_rows(out, q, k_pool, v_pool, block_table, batch, nh, nkv, hd, vd, page_size, window, scale, gate, chunk, slopes, sinks,
+                           first, wide, n_splits, scratch) -> None:
+    """Chunks with first positions over a 32-bit cache, or with heads and pages that no tensor-core kernel takes: tiles of rows on the FMA pipes."""
+    M = _stream_operands(out, q, k_pool, v_pool, block_table, nh, nkv, hd, vd, page_size)
+    gate_stride, gate_elem = _gate_layout(gate, M, nh, vd, out.dtype)
+    _check(lib().leb_attention_stream_rows(
+        out.data_ptr(), q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), _dt(out, "attention"), block_table.data_ptr(), block_table.shape[1],
+        batch.seq_slot.data_ptr(), batch.seq_pos0.data_ptr(), batch.seq_qstart.data_ptr(), batch.seq_qlen.data_ptr(), _ptr(gate), gate_stride,
+        gate_elem, M, batch.n_seqs, nh, nkv, hd, vd, page_size, window, chunk, first, scale, _ptr(slopes), _ptr(sinks), batch.max_qlen,
+        batch.max_kvlen, _stream_splits, _stream()))
 
 
 def _attention_stream_tc(out, q, k_pool, v_pool, block_table, batch, nh, nkv, hd, vd, page_size, window, scale, gate, chunk, slopes, sinks,

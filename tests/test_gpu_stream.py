@@ -290,6 +290,43 @@ def test_offsets_beyond_32_bits():
         torch.cuda.empty_cache()
 
 
+@pytest.mark.parametrize("blocks", [0, 1, 2, 3, 8])
+@pytest.mark.parametrize("dtype,nh,nkv,hd,vd,page", [(F32, 8, 2, 64, 64, 64), (F32, 3, 3, 128, 128, 32), (F32, 10, 2, 80, 48, 128), (F32, 4, 2, 33, 7, 64),
+                                                     (F32, 2, 1, 256, 256, 64), (F32, 34, 1, 16, 40, 64), (BF16, 4, 2, 80, 80, 32), (BF16, 6, 2, 33, 50, 64)])
+@pytest.mark.parametrize("window,first", [(1, 1), (64, 64), (300, 33), (33, 1000), (900, 4)])
+def test_chunks_whose_rows_go_in_tiles(blocks, dtype, nh, nkv, hd, vd, page, window, first, monkeypatch):
+    monkeypatch.setattr(K(), "STREAM_TILE_WORK", 0)
+    c = Case(CHUNKS + [(5, 0), (700, 9)], nh, nkv, hd, vd, page, window, first, dtype, seed=5, padding=(2,))
+    try:
+        K().set_stream_attention_splits(blocks)
+        c.check(c.run())
+    finally:
+        K().set_stream_attention_splits(0)
+
+
+@pytest.mark.parametrize("dtype,hd,vd", [(F32, 64, 64), (F32, 48, 24), (BF16, 80, 72)])
+def test_rows_in_tiles_with_slopes_sinks_and_gates(dtype, hd, vd, monkeypatch):
+    """The same as rows one by one, up to roundings; an infinity that one row sees stays out of the rows that do not see it."""
+    c = Case(CHUNKS, 6, 2, hd, vd, 32, 60, 9, dtype, seed=8)
+    g = torch.Generator().manual_seed(3)
+    slopes, sinks = torch.rand(6, generator=g).to(DEV), torch.randn(6, generator=g).to(DEV)
+    for width in (6, 6 * vd):
+        gate = torch.randn(c.rows, width, generator=g).to(dtype).to(DEV)
+        one = c.run(slopes=slopes, sinks=sinks, gate=gate).float()
+        with monkeypatch.context() as m:
+            m.setattr(K(), "STREAM_TILE_WORK", 0)
+            tiles = c.run(slopes=slopes, sinks=sinks, gate=gate).float()
+        assert float((one - tiles).abs().max()) <= (2 ** -7 if dtype == BF16 else 2 ** -16) * float(one.abs().max())
+    at = int(c.table[4, 530 // 32])      # a value that the rows up to 59 positions behind 530 see
+    c.v_pool[at, :, :, 530 % 32] = float("inf")
+    monkeypatch.setattr(K(), "STREAM_TILE_WORK", 0)
+    out = c.run()
+    row = sum(n for _, n in CHUNKS[:4])
+    seen = torch.zeros(c.rows, dtype=torch.bool)
+    seen[row + 530 - 517:row + 33] = True
+    assert torch.isfinite(out.cpu().float()).all(1).eq(~seen).all()
+
+
 @pytest.mark.parametrize("seqs", [DECODE, CHUNKS])
 @pytest.mark.parametrize("dtype,hd", [(BF16, 64), (BF16, 128), (F32, 48)])
 def test_rows_that_begin_anywhere(seqs, dtype, hd):
