@@ -114,9 +114,11 @@ class StreamCache:
         return StreamStep(int(n_seqs), int(n_rows), int(max_qlen), most, -(-most // self.page_size), self.device)
 
     def begin(self, step: StreamStep) -> None:
-        """Lays the step out and lets its sequences grow by its rows; a step that does not fit becomes padding (see `check`)."""
+        """Lays the step out and lets its sequences grow by its rows; a step that does not fit becomes padding (see `check`): nothing is
+        stored for it, and `attend` gives zeros."""
         kernels.stream_tables(step.table, step.slot_map, step.row_seq, step.row_pos, step.seq_slot, step.seq_qlen, step.seq_pos0,
-                              step.seq_qstart, step.slots, step.row_counts, self.lens, self.pages, self.free, self.counts, self.page_size)
+                              step.seq_qstart, step.slots, step.row_counts, self.lens, self.pages, self.free, self.counts, self.page_size,
+                              keep_rows=True)
         kernels.stream_advance(step.seq_slot, step.seq_qlen, self.lens, self.kept, self.pages, self.free, self.counts, self.page_size,
                                self.window, self.first)
 

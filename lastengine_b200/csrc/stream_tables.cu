@@ -13,8 +13,8 @@
 //
 // A step is laid out whole or not at all: a step that asks for more pages than there are (status: how many are short), that is
 // longer than its tables (-1), whose rows are not as many as its lengths say (-2) or that names a slot or a
-// length that cannot be (-3) leaves everything as it was, and all its sequences become padding (slot -1, no rows), which no
-// kernel reads or writes a cache for.
+// length that cannot be (-3) leaves everything as it was, and all its sequences become padding (slot -1), which no kernel reads or writes
+// a cache for.  They have no rows, or (`keep_rows`) share the step's rows out among themselves, for which attention then stores zeros.
 //
 // Kernels of a step read its tables ahead of their own wait for the kernel before them (common.cuh): they count on everything the
 // tables were made by being complete when the step's first such kernel starts.  `advance` behind `tables` gives a step that: it waits for
@@ -74,7 +74,7 @@ stream_tables_kernel(int* __restrict__ table, int width, int* __restrict__ slot_
                      int* __restrict__ row_pos, int* __restrict__ step_slot, int* __restrict__ step_qlen,
                      int* __restrict__ pos0_out, int* __restrict__ qstart_out, const int* __restrict__ seq_slot,
                      const int* __restrict__ seq_qlen, const int* lens, int n_slots, int* pages, int pages_width,
-                     const int* free_pages, int n_pages, int* counts, int M, int B, int page) {
+                     const int* free_pages, int n_pages, int* counts, int M, int B, int page, int keep_rows) {
   extern __shared__ int stb_smem[];
   int* qstart = stb_smem;          // [B + 1] first row
   int* taken = qstart + B + 1;     // [B] of the step's new pages, those of the sequences before
@@ -128,12 +128,15 @@ stream_tables_kernel(int* __restrict__ table, int width, int* __restrict__ slot_
   const bool ok = status == 0;
   const int at = blockIdx.x * STB_THREADS + threadIdx.x, step = gridDim.x * STB_THREADS;
   if (at == 0) counts[1] = status;
+  // of a refused step's rows, where they are kept: the first one of sequence b (as many for each as for the others, to one row: no more than
+  // any share of the rows among the sequences gives the longest)
+  auto share = [&](int b) { return (int)((long long)b * M / B); };
   for (int b = at; b < B; b += step) {
     const int slot = ok ? slot_s[b] : -1;
     step_slot[b] = slot;
-    step_qlen[b] = ok ? qstart[b + 1] - qstart[b] : 0;
+    step_qlen[b] = ok ? qstart[b + 1] - qstart[b] : keep_rows ? share(b + 1) - share(b) : 0;
     pos0_out[b] = slot >= 0 ? pos0_s[b] : 0;
-    qstart_out[b] = ok ? qstart[b] : min(b, max(M - 1, 0));
+    qstart_out[b] = ok ? qstart[b] : keep_rows ? share(b) : min(b, max(M - 1, 0));
   }
   // Rows, then table lines (a warp takes 128 places of one), shared out over all threads.  The sequence of a row is the last one that starts
   // at or before it (of those that start there, the one with rows).
@@ -157,6 +160,9 @@ stream_tables_kernel(int* __restrict__ table, int width, int* __restrict__ slot_
         const int pg = j < had ? pages[(size_t)slot * pages_width + j] : free_pages[n_free - 1 - (taken[b] + j - had)];
         to = pg * page + pos % page;
       }
+    } else if (keep_rows) {      // the last sequence whose share begins at or before the row
+      b = (int)(((long long)(r + 1) * B - 1) / M);
+      pos = r - share(b);
     }
     row_seq[r] = b;
     row_pos[r] = pos;
@@ -270,7 +276,7 @@ static const int STB_MOST_SEQS = 8192;      // sequences a step may have: four w
 LEB_API int leb_stream_tables(int* table, int width, int* slot_map, int* row_seq, int* row_pos, int* step_slot, int* step_qlen,
                               int* pos0, int* qstart, const int* seq_slot, const int* seq_qlen, const int* lens, int n_slots,
                               int* pages, int pages_width, const int* free_pages, int n_pages, int* counts, int M, int B, int page,
-                              cudaStream_t st) {
+                              int keep_rows, cudaStream_t st) {
   if (B <= 0) return 0;
   LEB_REQUIRE(B <= STB_MOST_SEQS, "leb_stream_tables: %d sequences in a step, %d at most", B, STB_MOST_SEQS);
   LEB_REQUIRE(page > 0 && width > 0 && pages_width > 0 && n_slots > 0 && M >= 0, "leb_stream_tables: sizes (page %d, width %d, slots %d, rows %d)",
@@ -286,7 +292,7 @@ LEB_API int leb_stream_tables(int* table, int width, int* slot_map, int* row_seq
   const long long most = 4ll * sm_count(), want = (lines + (M + 31) / 32 * 32 + STB_THREADS - 1) / STB_THREADS;
   const int blocks = (int)(want < 1 ? 1 : want < most ? want : most);
   leb_launch(kern, dim3(blocks), dim3(STB_THREADS), smem, st, table, width, slot_map, row_seq, row_pos, step_slot, step_qlen, pos0, qstart,
-             seq_slot, seq_qlen, lens, n_slots, pages, pages_width, free_pages, n_pages, counts, M, B, page);
+             seq_slot, seq_qlen, lens, n_slots, pages, pages_width, free_pages, n_pages, counts, M, B, page, keep_rows);
   LEB_CHECK_LAUNCH("leb_stream_tables");
   return 0;
 }

@@ -317,7 +317,7 @@ def _declare(L) -> None:
         "leb_attention_stream_any": [P, P, P, P, I, P, I, P, P, P, P, P, P, I, I, I, I, I, I, I, I, I, I, I, F, P, P, I, I, P],
         "leb_attention_stream_rows_supported": [I, I, I, I, I],
         "leb_attention_stream_rows": [P, P, P, P, I, P, I, P, P, P, P, P, I, I, I, I, I, I, I, I, I, I, I, I, F, P, P, I, I, I, P],
-        "leb_stream_tables": [P, I, P, P, P, P, P, P, P, P, P, P, I, P, I, P, I, P, I, I, I, P],
+        "leb_stream_tables": [P, I, P, P, P, P, P, P, P, P, P, P, I, P, I, P, I, P, I, I, I, I, P],
         "leb_stream_advance": [P, P, P, I, P, P, I, P, I, P, I, I, I, I, P],
         "leb_stream_release": [P, P, I, P, P, I, P, I, P, I, I, I, P],
         "leb_store_rows": [P, P, P, I, P, I, I, P, I, I, I, I, I, I, P],
@@ -1956,7 +1956,8 @@ def _stream_state(name: str, lens: torch.Tensor, pages: torch.Tensor, free: torc
 
 def stream_tables(table: torch.Tensor, slot_map: torch.Tensor, row_seq: torch.Tensor, row_pos: torch.Tensor, step_slot: torch.Tensor,
                   step_qlen: torch.Tensor, pos0: torch.Tensor, qstart: torch.Tensor, seq_slot: torch.Tensor, seq_qlen: torch.Tensor,
-                  lens: torch.Tensor, pages: torch.Tensor, free: torch.Tensor, counts: torch.Tensor, page_size: int) -> None:
+                  lens: torch.Tensor, pages: torch.Tensor, free: torch.Tensor, counts: torch.Tensor, page_size: int,
+                  keep_rows: bool = False) -> None:
     """A step's tables from its sequences' slots and row counts (`seq_slot`, `seq_qlen` [B]; slot -1 is padding), all int32 on the device.
 
     State: `lens` [slots] positions held, `pages` [slots, width] page lists (-1: nothing held), `free` [pages] a stack of
@@ -1967,7 +1968,8 @@ def stream_tables(table: torch.Tensor, slot_map: torch.Tensor, row_seq: torch.Te
 
     counts[1] is 0, or why the step is refused: how many pages it is short of, -1 a sequence longer than its tables, -2 rows
     that are not as many as seq_qlen says, -3 a slot or row count that cannot be.  A refused step changes no state, and all of its
-    sequences are padding without rows.  Every slot may be named once.
+    sequences are padding without rows: attention over it writes nothing.  With `keep_rows` they share its rows out evenly, and attention's
+    results are zeros.  Every slot may be named once.
     (Kernels may read a step's tables ahead of the wait for the kernel launched before: `stream_advance`, a copy or a
     graph's launch lies between this call and them.)"""
     _words("stream_tables", table, slot_map, row_seq, row_pos, step_slot, step_qlen, pos0, qstart, seq_slot, seq_qlen, lens, pages, free, counts)
@@ -1979,7 +1981,7 @@ def stream_tables(table: torch.Tensor, slot_map: torch.Tensor, row_seq: torch.Te
     _check(lib().leb_stream_tables(
         table.data_ptr(), shape[1], slot_map.data_ptr(), row_seq.data_ptr(), row_pos.data_ptr(), step_slot.data_ptr(), step_qlen.data_ptr(),
         pos0.data_ptr(), qstart.data_ptr(), seq_slot.data_ptr(), seq_qlen.data_ptr(), lens.data_ptr(), n_slots, pages.data_ptr(), width,
-        free.data_ptr(), n_pages, counts.data_ptr(), M, B, page_size, _stream()))
+        free.data_ptr(), n_pages, counts.data_ptr(), M, B, page_size, int(keep_rows), _stream()))
 
 
 def stream_advance(seq_slot: torch.Tensor, seq_qlen: torch.Tensor, lens: torch.Tensor, kept: torch.Tensor, pages: torch.Tensor,
