@@ -16,7 +16,7 @@ be as long as its page list (`max_len`).
     cache.begin(step)                                   # tables; the sequences are longer
     cache.store(layer, step, k, v)                      # per layer
     cache.attend(layer, step, out, q, heads)
-    cache.check()                                       # raises if a step was refused (reads one word: not in every step)
+    cache.check()                                       # raises if a step since the last check was refused (waits: not in every step)
     cache.close(slots)
 """
 from __future__ import annotations
@@ -79,12 +79,12 @@ class StreamCache:
         self.k = torch.zeros((n_layers, n_pages, self.nkv, page_size, self.hd), dtype=dtype, device=device)
         self.v = torch.zeros((n_layers, n_pages, self.nkv, self.vd, page_size), dtype=dtype, device=device)
         # all bookkeeping in one buffer: saved and put back by one copy
-        sizes = (max_seqs, max_seqs, max_seqs * width, n_pages, 2)
+        sizes = (max_seqs, max_seqs, max_seqs * width, n_pages, 2, 2)
         at = [0]
         for n in sizes:
             at.append(at[-1] + -(-n // 4) * 4)
         self.state = torch.zeros(at[-1], dtype=torch.int32, device=device)
-        self.lens, self.kept, pages, self.free, self.counts = (self.state[o:o + n] for o, n in zip(at, sizes))
+        self.lens, self.kept, pages, self.free, self.counts, self.refused = (self.state[o:o + n] for o, n in zip(at, sizes))
         self.pages = pages.view(max_seqs, width)
         self.pages.fill_(-1)
         self.kept.fill_(-(-self.first // page_size))
@@ -118,7 +118,7 @@ class StreamCache:
         stored for it, and `attend` gives zeros."""
         kernels.stream_tables(step.table, step.slot_map, step.row_seq, step.row_pos, step.seq_slot, step.seq_qlen, step.seq_pos0,
                               step.seq_qstart, step.slots, step.row_counts, self.lens, self.pages, self.free, self.counts, self.page_size,
-                              keep_rows=True)
+                              keep_rows=True, refused=self.refused)
         kernels.stream_advance(step.seq_slot, step.seq_qlen, self.lens, self.kept, self.pages, self.free, self.counts, self.page_size,
                                self.window, self.first)
 
@@ -144,14 +144,18 @@ class StreamCache:
         return step.n_rows * n_heads * self._splits(step, n_heads) * (max(self.hd, self.vd) + 2)
 
     def check(self) -> None:
-        """Raises what became of the last step where it was refused.  Waits for the stream."""
-        status = int(self.counts[1])
+        """Raises why the first step since the last call was refused, where one was.  Waits for the stream."""
+        n, status = self.refused.tolist()
+        if n == 0:
+            return
+        self.refused.zero_()
+        more = f" ({n} steps were refused)" if n > 1 else ""
         if status > 0:
-            raise CacheFull(f"the step needs {status} more cache pages of {self.page_size} positions than are free")
+            raise CacheFull(f"the step needs {status} more cache pages of {self.page_size} positions than are free{more}")
         if status == -1:
-            raise CacheError(f"a sequence grew longer than the step's tables (the cache takes {self.max_len} positions a sequence)")
-        if status < 0:
-            raise CacheError("the step's rows are not those of its sequences" if status == -2 else "the step names a slot or a row count that cannot be")
+            raise CacheError(f"a sequence grew longer than the step's tables (the cache takes {self.max_len} positions a sequence){more}")
+        raise CacheError(("the step's rows are not those of its sequences" if status == -2 else "the step names a slot or a row count that cannot be")
+                         + more)
 
     def lengths(self, slots: Sequence[int]) -> list[int]:
         held = self.lens.tolist()

@@ -3,7 +3,8 @@
 //
 // State, per cache: lens [slots], kept [slots] (the first page of a sequence's list, behind those of its first positions, that
 // has not been given back), pages [slots][width] (page list, -1 where nothing is held), free (a stack of page numbers),
-// counts {pages on the stack, status of the last step's tables}.
+// counts {pages on the stack, status of the last step's tables}, and (or null) refused {steps refused, status of the first of them},
+// which the tables only add to: it is for the program to read and clear, however many steps ran in between.
 //
 //   tables   pos0 = lens[slot]; sequence b, in order, takes ceil((pos0 + qlen) / P) - ceil(pos0 / P) pages off the top of the
 //            stack: of all pages a step takes, number t is free[n_free - 1 - t].  Only page lists are written, beyond
@@ -74,7 +75,7 @@ stream_tables_kernel(int* __restrict__ table, int width, int* __restrict__ slot_
                      int* __restrict__ row_pos, int* __restrict__ step_slot, int* __restrict__ step_qlen,
                      int* __restrict__ pos0_out, int* __restrict__ qstart_out, const int* __restrict__ seq_slot,
                      const int* __restrict__ seq_qlen, const int* lens, int n_slots, int* pages, int pages_width,
-                     const int* free_pages, int n_pages, int* counts, int M, int B, int page, int keep_rows) {
+                     const int* free_pages, int n_pages, int* counts, int* refused, int M, int B, int page, int keep_rows) {
   extern __shared__ int stb_smem[];
   int* qstart = stb_smem;          // [B + 1] first row
   int* taken = qstart + B + 1;     // [B] of the step's new pages, those of the sequences before
@@ -127,7 +128,14 @@ stream_tables_kernel(int* __restrict__ table, int width, int* __restrict__ slot_
   const int status = bad ? -3 : longer ? -1 : more || rows != M ? -2 : need > n_free ? need - n_free : 0;
   const bool ok = status == 0;
   const int at = blockIdx.x * STB_THREADS + threadIdx.x, step = gridDim.x * STB_THREADS;
-  if (at == 0) counts[1] = status;
+  if (at == 0) {
+    counts[1] = status;
+    if (refused && !ok) {
+      const int before = refused[0];
+      if (before == 0) refused[1] = status;
+      if (before < 0x7fffffff) refused[0] = before + 1;
+    }
+  }
   // of a refused step's rows, where they are kept: the first one of sequence b (as many for each as for the others, to one row: no more than
   // any share of the rows among the sequences gives the longest)
   auto share = [&](int b) { return (int)((long long)b * M / B); };
@@ -275,8 +283,8 @@ static const int STB_MOST_SEQS = 8192;      // sequences a step may have: four w
 
 LEB_API int leb_stream_tables(int* table, int width, int* slot_map, int* row_seq, int* row_pos, int* step_slot, int* step_qlen,
                               int* pos0, int* qstart, const int* seq_slot, const int* seq_qlen, const int* lens, int n_slots,
-                              int* pages, int pages_width, const int* free_pages, int n_pages, int* counts, int M, int B, int page,
-                              int keep_rows, cudaStream_t st) {
+                              int* pages, int pages_width, const int* free_pages, int n_pages, int* counts, int* refused, int M, int B,
+                              int page, int keep_rows, cudaStream_t st) {
   if (B <= 0) return 0;
   LEB_REQUIRE(B <= STB_MOST_SEQS, "leb_stream_tables: %d sequences in a step, %d at most", B, STB_MOST_SEQS);
   LEB_REQUIRE(page > 0 && width > 0 && pages_width > 0 && n_slots > 0 && M >= 0, "leb_stream_tables: sizes (page %d, width %d, slots %d, rows %d)",
@@ -292,7 +300,7 @@ LEB_API int leb_stream_tables(int* table, int width, int* slot_map, int* row_seq
   const long long most = 4ll * sm_count(), want = (lines + (M + 31) / 32 * 32 + STB_THREADS - 1) / STB_THREADS;
   const int blocks = (int)(want < 1 ? 1 : want < most ? want : most);
   leb_launch(kern, dim3(blocks), dim3(STB_THREADS), smem, st, table, width, slot_map, row_seq, row_pos, step_slot, step_qlen, pos0, qstart,
-             seq_slot, seq_qlen, lens, n_slots, pages, pages_width, free_pages, n_pages, counts, M, B, page, keep_rows);
+             seq_slot, seq_qlen, lens, n_slots, pages, pages_width, free_pages, n_pages, counts, refused, M, B, page, keep_rows);
   LEB_CHECK_LAUNCH("leb_stream_tables");
   return 0;
 }

@@ -317,7 +317,7 @@ def _declare(L) -> None:
         "leb_attention_stream_any": [P, P, P, P, I, P, I, P, P, P, P, P, P, I, I, I, I, I, I, I, I, I, I, I, F, P, P, I, I, P],
         "leb_attention_stream_rows_supported": [I, I, I, I, I],
         "leb_attention_stream_rows": [P, P, P, P, I, P, I, P, P, P, P, P, I, I, I, I, I, I, I, I, I, I, I, I, F, P, P, I, I, I, P],
-        "leb_stream_tables": [P, I, P, P, P, P, P, P, P, P, P, P, I, P, I, P, I, P, I, I, I, I, P],
+        "leb_stream_tables": [P, I, P, P, P, P, P, P, P, P, P, P, I, P, I, P, I, P, P, I, I, I, I, P],
         "leb_stream_advance": [P, P, P, I, P, P, I, P, I, P, I, I, I, I, P],
         "leb_stream_release": [P, P, I, P, P, I, P, I, P, I, I, I, P],
         "leb_store_rows": [P, P, P, I, P, I, I, P, I, I, I, I, I, I, P],
@@ -1957,7 +1957,7 @@ def _stream_state(name: str, lens: torch.Tensor, pages: torch.Tensor, free: torc
 def stream_tables(table: torch.Tensor, slot_map: torch.Tensor, row_seq: torch.Tensor, row_pos: torch.Tensor, step_slot: torch.Tensor,
                   step_qlen: torch.Tensor, pos0: torch.Tensor, qstart: torch.Tensor, seq_slot: torch.Tensor, seq_qlen: torch.Tensor,
                   lens: torch.Tensor, pages: torch.Tensor, free: torch.Tensor, counts: torch.Tensor, page_size: int,
-                  keep_rows: bool = False) -> None:
+                  keep_rows: bool = False, refused: torch.Tensor | None = None) -> None:
     """A step's tables from its sequences' slots and row counts (`seq_slot`, `seq_qlen` [B]; slot -1 is padding), all int32 on the device.
 
     State: `lens` [slots] positions held, `pages` [slots, width] page lists (-1: nothing held), `free` [pages] a stack of
@@ -1969,10 +1969,15 @@ def stream_tables(table: torch.Tensor, slot_map: torch.Tensor, row_seq: torch.Te
     counts[1] is 0, or why the step is refused: how many pages it is short of, -1 a sequence longer than its tables, -2 rows
     that are not as many as seq_qlen says, -3 a slot or row count that cannot be.  A refused step changes no state, and all of its
     sequences are padding without rows: attention over it writes nothing.  With `keep_rows` they share its rows out evenly, and attention's
-    results are zeros.  Every slot may be named once.
+    results are zeros.  `refused` (two words): how many steps were refused and why the first of them was, added to here and cleared by the
+    caller, so that a refusal does not go unnoticed behind a later step.  Every slot may be named once.
     (Kernels may read a step's tables ahead of the wait for the kernel launched before: `stream_advance`, a copy or a
     graph's launch lies between this call and them.)"""
     _words("stream_tables", table, slot_map, row_seq, row_pos, step_slot, step_qlen, pos0, qstart, seq_slot, seq_qlen, lens, pages, free, counts)
+    if refused is not None:
+        _words("stream_tables.refused", refused)
+        if refused.numel() != 2:
+            raise KernelError(f"stream_tables: {refused.numel()} words of refusals (2)")
     n_slots, width, n_pages = _stream_state("stream_tables", lens, pages, free, counts, page_size)
     B, M, shape = seq_slot.numel(), slot_map.numel(), table.shape
     if (len(shape) != 2 or shape[0] != B or shape[1] < 1 or row_seq.numel() != M or row_pos.numel() != M or seq_qlen.numel() != B
@@ -1981,7 +1986,7 @@ def stream_tables(table: torch.Tensor, slot_map: torch.Tensor, row_seq: torch.Te
     _check(lib().leb_stream_tables(
         table.data_ptr(), shape[1], slot_map.data_ptr(), row_seq.data_ptr(), row_pos.data_ptr(), step_slot.data_ptr(), step_qlen.data_ptr(),
         pos0.data_ptr(), qstart.data_ptr(), seq_slot.data_ptr(), seq_qlen.data_ptr(), lens.data_ptr(), n_slots, pages.data_ptr(), width,
-        free.data_ptr(), n_pages, counts.data_ptr(), M, B, page_size, int(keep_rows), _stream()))
+        free.data_ptr(), n_pages, counts.data_ptr(), _ptr(refused), M, B, page_size, int(keep_rows), _stream()))
 
 
 def stream_advance(seq_slot: torch.Tensor, seq_qlen: torch.Tensor, lens: torch.Tensor, kept: torch.Tensor, pages: torch.Tensor,

@@ -84,3 +84,65 @@ def test_rows_of_a_refused_step_are_shared_out_or_dropped():
                 assert qlen.tolist() == [0] * B
             K().stream_advance(slot, qlen, lens, kept, pages, free, counts2, 32)
             assert lens.tolist() == [0] * 3 and counts2.tolist() == [4, status] and free.tolist() == [3, 2, 1, 0] and bool((pages == -1).all())
+
+
+def test_a_refusal_is_reported_however_many_steps_follow():
+    from lastengine_b200.cache import CacheError, CacheFull
+    cache = cache_of()
+    a, b = cache.open(), cache.open()
+    run(cache, [a, b], [64, 128])
+    cache.check()
+    run(cache, [a, b], [200, 1])                # short of pages
+    run(cache, [a, b], [1, 600])                # longer than the tables
+    run(cache, [a], [1])
+    run(cache, [a], [2])
+    with pytest.raises(CacheFull, match="2 steps were refused"):
+        cache.check()
+    cache.check()                               # reported once
+    run(cache, [a], [500])
+    run(cache, [a], [1])
+    with pytest.raises(CacheError):
+        cache.check()
+    assert cache.lengths([a, b]) == [68, 128]
+
+
+def test_replayed_steps_that_were_refused_until_a_sequence_ended_are_reported():
+    """A captured decode step is refused while the pages are short, and runs again once another sequence has ended."""
+    from lastengine_b200.cache import CacheFull
+    cache = cache_of(window=0, first=0)
+    a, b = cache.open(), cache.open()
+    run(cache, [a, b], [63, 192])
+    step = cache.plan(1, 1, 1)
+    step.set([a], [1])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        cache.begin(step)
+    graph.replay()                              # the 64th position
+    cache.check()
+    for _ in range(5):
+        graph.replay()
+    cache.close([b])
+    for _ in range(3):
+        graph.replay()
+    assert cache.lengths([a]) == [67]
+    with pytest.raises(CacheFull, match="5 steps were refused"):
+        cache.check()
+    cache.check()
+
+
+def test_refusals_are_added_up_until_the_program_clears_them():
+    lens, pages, free, counts, refused = words([0] * 2), torch.full((2, 2), -1, dtype=torch.int32, device=DEV), words([1, 0]), words([2, 0]), words([0, 0])
+    step = lambda slots, n, word=refused: K().stream_tables(torch.zeros(len(n), 2, dtype=torch.int32, device=DEV), *(words([0] * sum(n)) for _ in range(3)),
+                                                            *(words([0] * len(n)) for _ in range(4)), words(slots), words(n), lens, pages, free, counts, 32, refused=word)
+    step([0], [3])
+    assert refused.tolist() == [0, 0] and counts[1] == 0
+    step([0, 1], [64, 33])
+    step([5], [1])
+    step([0], [3])
+    assert refused.tolist() == [2, 2] and counts[1] == 0
+    refused.copy_(words([2 ** 31 - 1, 7]))
+    step([5], [1])
+    assert refused.tolist() == [2 ** 31 - 1, 7] and counts[1] == -3
+    for bad in (words([0]), refused.long(), refused.cpu()):
+        with pytest.raises(K().KernelError):
+            step([0], [1], bad)
