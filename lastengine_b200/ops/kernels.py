@@ -1742,7 +1742,7 @@ def attention(out: torch.Tensor, q: torch.Tensor | None, k_pool: torch.Tensor, v
             _check(L.leb_attention_merge(_ptr(out), _ptr(scratch), BF16, _ptr(gate), gate_stride, gate_elem, _ptr(sinks), M,
                                          nh, hd, n_splits, _stream()))
         return
-    if (out.dtype == torch.bfloat16 and n_splits == 1 and batch.max_qlen >= TC_ATTENTION_MIN_ROWS
+    if (out.dtype == torch.bfloat16 and n_splits == 1 and batch.max_qlen >= TC_ATTENTION_MIN_ROWS and (first == 0 or wide)
             and q.stride(0) % 8 == 0 and L.leb_attention_prefill_tc_supported(nh, nkv, hd, page_size)):
         # prompts: tcgen05 tiles of 128 (position, head) rows, pages brought in by TMA
         _check(L.leb_attention_prefill_tc(
@@ -1784,27 +1784,35 @@ STREAM_ROWS = 16
 STREAM_TILE_WORK = 200_000_000
 
 
+_MOST_BLOCKS = 65535      # of a grid's second and third dimension: sequences, rows, a sequence's tiles
+
+
 def _stream_form(out, batch, nh, nkv, hd, vd, page_size, wide, q, k_pool, v_pool, keys):
-    """The kernel made for rows with first positions that takes a step, None where the ones for all rows do."""
-    M, single = out.shape[0], batch.max_qlen == 1
+    """The kernel made for rows with first positions that takes a step, None where the ones for all rows do (which want q, out and pools on 16-byte
+    boundaries)."""
+    M, B, longest, single = out.shape[0], batch.n_seqs, batch.max_qlen, batch.max_qlen == 1
     aligned, rows_aligned = (k_pool.data_ptr() | v_pool.data_ptr()) & 15 == 0, (q.data_ptr() | out.data_ptr()) & 15 == 0
+    mma = False
     if out.dtype is torch.bfloat16:
         mma = vd == hd and _stream_takes("leb_attention_prefill_supported", nh, nkv, hd, page_size)
         if mma and not aligned:
             raise KernelError("attention: the pools of these heads must lie on 16-byte boundaries")
-        mma = mma and rows_aligned      # (rows that begin anywhere: the kernel for any widths)
-        if single and mma and M == batch.n_seqs and _stream_takes("leb_attention_decode_supported", nh, nkv, hd, page_size):
+        mma = mma and rows_aligned      # (rows that begin anywhere: the kernels for any widths)
+        if single and mma and M == B and _stream_takes("leb_attention_decode_supported", nh, nkv, hd, page_size):
             return _attention_stream_decode
         if (not single and not wide and aligned and rows_aligned and q.stride(0) % 8 == 0
-                and k_pool.numel() < (hd << 31) and _stream_takes("leb_attention_stream_tc_supported", nh, nkv, hd, vd, page_size)):
+                and k_pool.numel() < (hd << 31) and _stream_takes("leb_attention_stream_tc_supported", nh, nkv, hd, vd, page_size)
+                and B <= _MOST_BLOCKS and longest <= _MOST_BLOCKS * (128 * nkv // nh // 8 * 8)):
             return _attention_stream_tc
         if mma and not single and M > STREAM_ROWS:
             return None
-    if not single and aligned and M * nh * keys * (hd + vd) >= STREAM_TILE_WORK and _stream_takes("leb_attention_stream_rows_supported", nh, nkv, hd, vd, page_size):
+    tiles = (aligned and _stream_takes("leb_attention_stream_rows_supported", nh, nkv, hd, vd, page_size)
+             and B <= _MOST_BLOCKS and longest <= _MOST_BLOCKS * (64 * nkv // nh))
+    if not single and tiles and M * nh * keys * (hd + vd) >= STREAM_TILE_WORK:
         return _attention_stream_rows
-    if aligned and M <= 65535 and _stream_takes("leb_attention_stream_any_supported", nh, nkv, hd, vd, page_size):
+    if aligned and M <= _MOST_BLOCKS and _stream_takes("leb_attention_stream_any_supported", nh, nkv, hd, vd, page_size):
         return _attention_stream_any
-    return None
+    return _attention_stream_rows if tiles else _attention_stream_general
 
 
 def _stream_operands(out, q, k_pool, v_pool, block_table, nh, nkv, hd, vd, page_size) -> int:
@@ -1861,6 +1869,13 @@ def _attention_stream_rows(out, q, k_pool, v_pool, block_table, batch, nh, nkv, 
         batch.seq_slot.data_ptr(), batch.seq_pos0.data_ptr(), batch.seq_qstart.data_ptr(), batch.seq_qlen.data_ptr(), _ptr(gate), gate_stride,
         gate_elem, M, batch.n_seqs, nh, nkv, hd, vd, page_size, window, chunk, first, scale, _ptr(slopes), _ptr(sinks), batch.max_qlen,
         batch.max_kvlen, _stream_splits, _stream()))
+
+
+def _attention_stream_general(out, q, k_pool, v_pool, block_table, batch, nh, nkv, hd, vd, page_size, window, scale, gate, chunk, slopes, sinks,
+                              first, wide, n_splits, scratch) -> None:
+    """Steps with first positions that no kernel made for them takes: pools off a 16-byte boundary, more rows than the others' grids."""
+    _attention_general(out, q, k_pool, v_pool, block_table, batch, nh, nkv, hd, vd, page_size, window, scale, gate, n_splits, scratch, chunk, slopes,
+                       sinks, first)
 
 
 def _attention_stream_tc(out, q, k_pool, v_pool, block_table, batch, nh, nkv, hd, vd, page_size, window, scale, gate, chunk, slopes, sinks,
