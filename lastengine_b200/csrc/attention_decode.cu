@@ -587,6 +587,8 @@ static int attention_decode_launch(void* out, float* part, const void* q, const 
   if (B <= 0) return 0;
   LEB_REQUIRE(leb_attention_decode_supported(nh, nkv, hd, page_size),
               "leb_attention_decode: sizes not taken (heads %d, kv heads %d, head_dim %d, page %d)", nh, nkv, hd, page_size);
+  LEB_REQUIRE((((uintptr_t)(prep.q_raw ? nullptr : q) | (uintptr_t)k_pool | (uintptr_t)v_pool) & 15) == 0,
+              "leb_attention_decode: q and the pools must be 16-byte aligned");
   // with first positions and without splits of the caller's: a cluster of as many blocks as suit the step, or of `blocks`
   const bool joined = first > 0 && n_splits == 1;
   if (joined) {

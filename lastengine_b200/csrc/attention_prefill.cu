@@ -352,6 +352,8 @@ LEB_API int leb_attention_prefill(void* out, const void* q, const void* k_pool, 
   if (B <= 0 || max_qlen <= 0) return 0;
   LEB_REQUIRE(leb_attention_prefill_supported(nh, nkv, hd, page_size),
               "leb_attention_prefill: sizes not taken (heads %d, kv heads %d, head_dim %d, page %d)", nh, nkv, hd, page_size);
+  LEB_REQUIRE((((uintptr_t)q | (uintptr_t)k_pool | (uintptr_t)v_pool) & 15) == 0 && ((uintptr_t)out & 3) == 0,
+              "leb_attention_prefill: q and the pools must be 16-byte aligned, out 4-byte aligned");
   const int G = nh / nkv;
   const int MT = hd <= 32 ? 2 : 1;
   const int rows_per_block = ATP_WARPS * MT * 16;

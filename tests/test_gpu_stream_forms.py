@@ -60,3 +60,22 @@ def test_more_rows_than_a_grid_s_second_dimension(dtype, nh, hd, vd, page, rows_
         else:
             bound = want.abs() * 2 ** -22 + 2 * mass * ((hd + 8) * 2 ** -24 * size + 35 * 2 ** -24 + 2 ** -20)
         assert bool(((out[:, h * vd:(h + 1) * vd].double() - want).abs() <= bound + 1e-30).all()), h
+
+
+@pytest.mark.parametrize("M,B", [(4, 4), (6, 2), (40, 2), (300, 1)])
+@pytest.mark.parametrize("hd", [32, 64, 128])
+def test_addresses_that_the_kernels_for_all_rows_do_not_take_are_refused(M, B, hd):
+    """Without first positions: nothing is launched on rows or pools off the boundaries that 16-byte loads want."""
+    word = lambda v: torch.tensor(v, dtype=torch.int32, device=DEV)
+    n = M // B
+    batch = types.SimpleNamespace(n_rows=M, n_seqs=B, max_qlen=n, max_kvlen=n, row_seq=word([i // n for i in range(M)]), row_pos=word([i % n for i in range(M)]),
+                                  seq_slot=word(list(range(B))), seq_pos0=word([0] * B), seq_qstart=word([b * n for b in range(B)]), seq_qlen=word([n] * B))
+    pages = -(-n // 64)
+    table = torch.arange(B * pages, dtype=torch.int32, device=DEV).view(B, pages)
+    q, k, v = (torch.randn(s, device=DEV).to(BF16) for s in ((M, 2 * hd), (B * pages, 1, 64, hd), (B * pages, 1, hd, 64)))
+    run = lambda q, k, v: K().attention(torch.empty(M, 2 * hd, dtype=BF16, device=DEV), q, k, v, table, batch, 2, 1, hd, 64, 0, hd ** -0.5)
+    run(q, k, v)
+    for args in ((at(q, 1), k, v), (q, at(k, 4), v), (q, k, at(v, 1))):
+        with pytest.raises(K().KernelError):
+            run(*args)
+    torch.cuda.synchronize()
