@@ -601,13 +601,10 @@ static int attention_decode_launch(void* out, float* part, const void* q, const 
 #define LEB_ATD_F(HD_, S_, W_, F_)                                                                \
   {                                                                                               \
     constexpr int smem = ATD_WARPS * S_ * 2 * 32 * HD_ * 2;                                        \
-    static bool set = false;                                                                      \
-    if (!set) {                                                                                   \
-      if (cudaFuncSetAttribute(attention_decode_kernel<HD_, S_, W_, F_>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) \
-        return leb_fail("leb_attention_decode: %d bytes of shared memory per block refused", smem); \
-      set = true;                                                                                 \
-    }                                                                                             \
-    leb_launch_cluster(F_ && joined ? n_splits : 1, attention_decode_kernel<HD_, S_, W_, F_>, grid, dim3(32 * ATD_WARPS), smem, st, \
+    constexpr auto kern = attention_decode_kernel<HD_, S_, W_, F_>;                               \
+    if (leb_allow_smem<kern, smem>() != cudaSuccess)                                              \
+      return leb_fail("leb_attention_decode: %d bytes of shared memory per block refused", smem); \
+    leb_launch_cluster(F_ && joined ? n_splits : 1, kern, grid, dim3(32 * ATD_WARPS), smem, st, \
         (bf16*)out, part, (const bf16*)q, (const bf16*)k_pool, (const bf16*)v_pool, block_table,  \
         bt_width, seq_slot, seq_pos0, seq_qstart, (const bf16*)gate, gate_stride, gate_elem, nh, nkv, \
         page_size, window, chunk, first, scale, slopes, sinks, n_splits, prep);                   \

@@ -490,16 +490,13 @@ static int launch_attention_prefill_tc(const char* who, void* out, const void* q
   }
   dim3 grid(nkv, ceil_div(max_qlen, TP), B);
   LEB_REQUIRE(grid.y <= 65535 && grid.z <= 65535, "%s: grid too large", who);
-  const size_t smem = 1024 + 128 * 64 * 2 + AtcShape<DEEP>::STAGES * (64 + VD) * 64 * 2 + (DEEP ? 0 : 128 * 64 * 2);
+  constexpr size_t smem = 1024 + 128 * 64 * 2 + AtcShape<DEEP>::STAGES * (64 + VD) * 64 * 2 + (DEEP ? 0 : 128 * 64 * 2);
 #define LEB_ATC(GS_)                                                                                              \
   {                                                                                                               \
-    static bool set = false;                                                                                      \
-    if (!set) {                                                                                                   \
-      if (cudaFuncSetAttribute(attention_prefill_tc_kernel<GS_, POOLED, WIDE, DEEP, VD, FIRST>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) \
-        return leb_fail("%s: %zu bytes of shared memory per block refused", who, smem);                         \
-      set = true;                                                                                                 \
-    }                                                                                                             \
-    leb_launch(attention_prefill_tc_kernel<GS_, POOLED, WIDE, DEEP, VD, FIRST>, grid, dim3(ATC_THREADS), smem, st,                       \
+    constexpr auto kern = attention_prefill_tc_kernel<GS_, POOLED, WIDE, DEEP, VD, FIRST>;                        \
+    if (leb_allow_smem<kern, (int)smem>() != cudaSuccess)                                                         \
+      return leb_fail("%s: %zu bytes of shared memory per block refused", who, smem);                             \
+    leb_launch(kern, grid, dim3(ATC_THREADS), smem, st,                       \
         mq, mk, mv, mpk, mpv, (bf16*)out, block_table, bt_width, pool_table, pt_width, seq_slot, seq_pos0, seq_qstart, \
         seq_qlen, (const bf16*)gate, gate_stride, gate_elem, nh, nkv, window, chunk, first, pooled ? pool : 0, scale, head_scale, freq_v, slopes, \
         sinks, status); \

@@ -79,3 +79,16 @@ def test_many_rows_that_begin_anywhere_do_not_go_to_the_kernels_of_16_byte_loads
     assert form_of(BF16, 1, 1, 64, 64, 64, 70000, 1, 70000, rows_at=8, keys=20) is K._attention_stream_rows
     assert form_of(F32, 1, 1, 32, 32, 32, 70000, 1, 70000, pools_at=4) is K._attention_stream_general
     assert form_of(F32, 64, 1, 32, 32, 32, 70000, 1, 70000) is K._attention_stream_general
+
+
+@pytest.mark.parametrize("source", ["attention.cu", "attention_decode.cu", "attention_prefill.cu", "attention_prefill_tc.cu", "attention_stream_any.cu",
+                                    "attention_stream_rows.cu", "attention_stream_tc.cu", "stream_tables.cu"])
+def test_shared_memory_is_allowed_on_every_device_that_launches_a_kernel(source):
+    """The limit belongs to a device's copy of a kernel: it is raised by leb_allow_smem, which keeps count of devices, and behind no flag of the
+    whole process."""
+    import os
+    from lastengine_b200.ops import build
+    with open(os.path.join(build.CSRC, source)) as f:
+        text = f.read()
+    assert "cudaFuncSetAttribute" not in text
+    assert "leb_allow_smem" in text or "extern __shared__" not in text
