@@ -258,7 +258,7 @@ attention_decode_kernel(bf16* __restrict__ out, float* __restrict__ part, const 
   auto issue = [&]() {
     if (p_blk < blk_hi) {
       const int key0 = (FIRST && p_blk >= n_first ? p_blk + shift : p_blk) * 32;
-      const int page = table[key0 / page_size];
+      const int page = max(table[key0 / page_size], 0);      // (a page given back is read by no row: no address is formed from its -1)
       const int off = key0 % page_size;
       const bf16* kbase = k_pool + (((size_t)page * nkv + kvh) * page_size + off) * HD;   // 32 rows of HD, contiguous
       const bf16* vbase = v_pool + ((size_t)page * nkv + kvh) * HD * page_size + off;     // HD rows, 32 positions of each

@@ -164,7 +164,8 @@ attention_prefill_kernel(bf16* __restrict__ out, const bf16* __restrict__ q,
   uint4 kn[4][KB], vn[NT];      // the next block, in flight meanwhile
   auto load_block = [&](int blk, uint4 (&kd)[4][KB], uint4 (&vd)[NT]) {
     const int key0 = (FIRST && blk >= n_first ? blk + shift : blk) * 32;
-    const int page = table[key0 / page_size];
+    int page = table[key0 / page_size];
+    if (FIRST) page = max(page, 0);      // (a page given back is read by no row: no address is formed from its -1)
     const int off = key0 % page_size;
     const bf16* kbase = k_pool + (((size_t)page * nkv + kvh) * page_size + off) * HD;
     const bf16* vbase = v_pool + ((size_t)page * nkv + kvh) * HD * page_size + off;
