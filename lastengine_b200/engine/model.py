@@ -9,7 +9,7 @@ from __future__ import annotations
 import torch
 
 from .. import parts as _parts  # noqa: F401  (registers the built-in parts)
-from ..parts.base import BuildEnv, ModelPlan, TensorSpec
+from ..parts.base import BuildEnv, KVSpec, LatentSpec, ModelPlan, TensorSpec, keeps_for
 from ..ops import kernels
 from ..parts.base import MATRIX, VECTOR
 from ..registry import BLOCKS, EMBEDDINGS, FEED_FORWARDS, GATES, HEADS, MIXERS, NORMS
@@ -34,6 +34,7 @@ class Model:
             self.blocks.append(BLOCKS.get(ls.block)(
                 mixer=mixer, ffn=ffn, mixer_norm=norm(ls.mixer_norm), ffn_norm=norm(ls.ffn_norm),
                 post_mixer_norm=norm(ls.post_mixer_norm), post_ffn_norm=norm(ls.post_ffn_norm), **gates, **ls.block_params))
+        self._check_shared_entries()
         self.hidden_size, self.vocab_size = plan.hidden_size, plan.vocab_size
         # additions to the residual stream between schedule entries, and the tables they take rows from
         self.stream_adds: dict[int, list] = {}
@@ -64,6 +65,22 @@ class Model:
             held = getattr(p, "__dict__", {}).values()
         for q in held:
             yield from cls._objects_in(q, seen)
+
+    def _check_shared_entries(self) -> None:
+        """A layer that reads another's cache entry reads positions that the entry still holds."""
+        paged = lambda layer: [s for s in self._several(self.blocks[layer].mixer.cache_spec()) if isinstance(s, (KVSpec, LatentSpec))]
+        for i, e in enumerate(self.plan.schedule):
+            if e.cache is None or e.cache == i:
+                continue
+            for owner in paged(self.plan.schedule[e.cache].layer):
+                for reader in paged(e.layer):
+                    if not keeps_for(owner, reader):
+                        raise ValueError(f"schedule[{i}] reads cache entry {e.cache}, which gives back positions that it reads: kept as {owner}, "
+                                         f"read as {reader}")
+
+    @staticmethod
+    def _several(spec):
+        return list(spec) if isinstance(spec, (tuple, list)) else [spec]
 
     # ---- tensors ------------------------------------------------------------------------
     def named_parts(self) -> list[tuple[str, object]]:

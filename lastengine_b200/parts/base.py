@@ -118,6 +118,17 @@ class StateSpec:
     dtype: torch.dtype = torch.float32
 
 
+def keeps_for(owner, reader) -> bool:
+    """Whether a cache entry kept as `owner` says (a KVSpec or LatentSpec) holds, at every position, all that a layer reads whose own entry
+    would be kept as `reader` says."""
+    w, c = reader.window, reader.chunk
+    if owner.window <= 0 and owner.chunk <= 0:
+        return True
+    in_window = owner.window <= 0 or 0 < w <= owner.window or 0 < c <= owner.window
+    in_chunk = owner.chunk <= 0 or w == 1 or (c > 0 and owner.chunk % c == 0)
+    return in_window and in_chunk and getattr(reader, "first", 0) <= getattr(owner, "first", 0)
+
+
 @dataclass(frozen=True)
 class PartSpec:
     kind: str                      # name in the registry of its family
