@@ -1610,10 +1610,14 @@ def attention_splits(batch, nkv: int, G: int, sm_count: int | None = None, hd: i
     unsplit, 89 us in 4 splits).  The general kernel (`general`: 32-bit caches) takes several times as long over a
     position as the tensor-core kernel: beyond 128 positions half as many of them make a split worth its start (two sequences
     of 190 and 333: 87 -> 25 us a layer with the wider loads of its tiles; 1 to 64 sequences of 100 to 8,000 positions, seven
-    layouts of heads: 0.18 to 0.83 of the time before both).
+    layouts of heads: 0.18 to 0.83 of the time before both).  With first positions (`first`) `general` says as well that the step does not go to
+    the tensor-core decode kernel for its values' width.
     """
     if batch.max_qlen != 1:
         return 1
+    beside = first > 0 and (window > 0 or chunk > 0)
+    if beside and (general or not _stream_decode_takes(nkv * G, nkv, hd)):
+        return 1      # the kernels for any widths join their blocks' sums by themselves: they take no splits and no scratch
     if sm_count is None:
         sm_count = globals()["sm_count"]()
     kv = max(_read_length(int(batch.max_kvlen), window, chunk, first), 1)
@@ -1622,8 +1626,8 @@ def attention_splits(batch, nkv: int, G: int, sm_count: int | None = None, hd: i
     slots = sm_count * max(1, min(3, (227 * 1024) // stage_bytes))      # blocks that run at once
     if per >= 2 * sm_count:
         return 1 if kv < 2048 else min(4, kv // 1024)
-    if first > 0 and (window > 0 or chunk > 0) and not general and hd in (32, 64, 96, 128) and G <= 16:
-        return 1      # the blocks of a sequence join their sums by themselves, without a second kernel
+    if beside:
+        return 1      # the same
     least = 128 if per * 8 <= sm_count else 256       # one or two sequences: latency counts, shorter blocks pay
     if general and kv > 128:
         least //= 2
@@ -1772,6 +1776,11 @@ def _stream_takes(entry: str, *sizes: int) -> bool:
     return bool(getattr(lib(), entry)(*sizes))
 
 
+def _stream_decode_takes(nh: int, nkv: int, hd: int) -> bool:
+    """Whether single tokens of these bfloat16 heads (values as wide, pages of any multiple of 32) go to the tensor-core decode kernel."""
+    return _stream_takes("leb_attention_decode_supported", nh, nkv, hd, 32)
+
+
 # Rows of a bfloat16 step up to which each reads its keys by itself where only the mma.sync kernel takes the prompt.  us of a chunk with 32
 # heads of 64 over 8, pages of 32, window 1,024, that kernel and this: 2 rows 33.8 and 11.5, 16 34.5 and 18.4, 32 34.5 and 46.3.
 # (The general kernel is behind at every size: 32-bit, 16 rows 400 and 20, 256 422 and 183, 2,048 2,937 and 1,336.)
@@ -1798,7 +1807,7 @@ def _stream_form(out, batch, nh, nkv, hd, vd, page_size, wide, q, k_pool, v_pool
         if mma and not aligned:
             raise KernelError("attention: the pools of these heads must lie on 16-byte boundaries")
         mma = mma and rows_aligned      # (rows that begin anywhere: the kernels for any widths)
-        if single and mma and M == B and _stream_takes("leb_attention_decode_supported", nh, nkv, hd, page_size):
+        if single and mma and M == B and _stream_decode_takes(nh, nkv, hd):
             return _attention_stream_decode
         if (not single and not wide and aligned and rows_aligned and q.stride(0) % 8 == 0
                 and k_pool.numel() < (hd << 31) and _stream_takes("leb_attention_stream_tc_supported", nh, nkv, hd, vd, page_size)

@@ -277,7 +277,7 @@ class AttentionMixer(Mixer):
                                   None, 0, True, nh, nkv, hd, cache.page_size)
         o = ws.get("attn.o", (M, nh * kvd), env.dtype)
         n_splits = kernels.attention_splits(batch, nkv, nh // nkv, hd=khd, chunk=self.chunk, window=self.window,
-                                            general=env.is_float32, first=self.first)
+                                            general=env.is_float32 or (self.first > 0 and kvd != khd), first=self.first)
         scratch = None
         if n_splits > 1:
             scratch = ws.get("attn.part", (M * nh * n_splits * (max(khd, kvd) + 2),), torch.float32)

@@ -92,3 +92,16 @@ def test_shared_memory_is_allowed_on_every_device_that_launches_a_kernel(source)
         text = f.read()
     assert "cudaFuncSetAttribute" not in text
     assert "leb_allow_smem" in text or "extern __shared__" not in text
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("nh,nkv,hd,vd", [(8, 2, 64, 64), (32, 8, 64, 64), (32, 8, 64, 48), (16, 1, 128, 128), (34, 2, 64, 64), (4, 2, 80, 80), (4, 4, 192, 192), (6, 6, 96, 32)])
+@pytest.mark.parametrize("B", [1, 8, 64, 300])
+@pytest.mark.parametrize("window,chunk", [(4096, 0), (0, 2048)])
+def test_splits_through_scratch_are_asked_for_only_where_they_are_read(dtype, nh, nkv, hd, vd, B, window, chunk):
+    batch = types.SimpleNamespace(n_rows=B, n_seqs=B, max_qlen=1, max_kvlen=9000)
+    n = K.attention_splits(batch, nkv, nh // nkv, sm_count=148, hd=hd, window=window, chunk=chunk, general=dtype is F32 or vd != hd, first=4)
+    form = form_of(dtype, nh, nkv, hd, vd, 64, B, B, 1, keys=4100)
+    assert n == 1 or form is K._attention_stream_decode
+    if form is K._attention_stream_decode and B * nkv >= 2 * 148:
+        assert n == (4 if window else 2)
