@@ -1683,6 +1683,10 @@ def _gate_layout(gate: torch.Tensor | None, M: int, nh: int, width: int, dtype: 
 _MOST_FIRST = 2 ** 31 - 2 ** 16      # first positions: more are as many (the kernels round them up to tiles and pages in 32 bits)
 
 
+# The tcgen05 kernels scale scores after masked ones have become -1e30: below this that would not leave them out.
+_LEAST_TC_SCALE = 1e-20
+
+
 def attention(out: torch.Tensor, q: torch.Tensor | None, k_pool: torch.Tensor, v_pool: torch.Tensor,
               block_table: torch.Tensor, batch, nh: int, nkv: int, hd: int, page_size: int,
               window: int, scale: float, gate: torch.Tensor | None = None,
@@ -1710,7 +1714,7 @@ def attention(out: torch.Tensor, q: torch.Tensor | None, k_pool: torch.Tensor, v
             assert t.numel() == nh
     if first > 0 and raw is None:
         form = _stream_form(out, batch, nh, nkv, hd, vd or hd, page_size, wide, q, k_pool, v_pool,
-                            _read_length(batch.max_kvlen, window, chunk, first))
+                            _read_length(batch.max_kvlen, window, chunk, first), scale)
         if form is not None:
             return form(out, q, k_pool, v_pool, block_table, batch, nh, nkv, hd, vd or hd, page_size, window, float(scale), gate, chunk, slopes, sinks,
                         first, wide, n_splits, scratch)
@@ -1747,7 +1751,7 @@ def attention(out: torch.Tensor, q: torch.Tensor | None, k_pool: torch.Tensor, v
                                          nh, hd, n_splits, _stream()))
         return
     if (out.dtype == torch.bfloat16 and n_splits == 1 and batch.max_qlen >= TC_ATTENTION_MIN_ROWS and (first == 0 or wide)
-            and q.stride(0) % 8 == 0 and L.leb_attention_prefill_tc_supported(nh, nkv, hd, page_size)):
+            and scale >= _LEAST_TC_SCALE and q.stride(0) % 8 == 0 and L.leb_attention_prefill_tc_supported(nh, nkv, hd, page_size)):
         # prompts: tcgen05 tiles of 128 (position, head) rows, pages brought in by TMA
         _check(L.leb_attention_prefill_tc(
             _ptr(out), _ptr(q), q.stride(0), M, _ptr(k_pool), _ptr(v_pool), k_pool.shape[0], _ptr(block_table),
@@ -1796,7 +1800,7 @@ STREAM_TILE_WORK = 200_000_000
 _MOST_BLOCKS = 65535      # of a grid's second and third dimension: sequences, rows, a sequence's tiles
 
 
-def _stream_form(out, batch, nh, nkv, hd, vd, page_size, wide, q, k_pool, v_pool, keys):
+def _stream_form(out, batch, nh, nkv, hd, vd, page_size, wide, q, k_pool, v_pool, keys, scale=1.0):
     """The kernel made for rows with first positions that takes a step, None where the ones for all rows do (which want q, out and pools on 16-byte
     boundaries)."""
     M, B, longest, single = out.shape[0], batch.n_seqs, batch.max_qlen, batch.max_qlen == 1
@@ -1809,7 +1813,7 @@ def _stream_form(out, batch, nh, nkv, hd, vd, page_size, wide, q, k_pool, v_pool
         mma = mma and rows_aligned      # (rows that begin anywhere: the kernels for any widths)
         if single and mma and M == B and _stream_decode_takes(nh, nkv, hd):
             return _attention_stream_decode
-        if (not single and not wide and aligned and rows_aligned and q.stride(0) % 8 == 0
+        if (not single and not wide and aligned and rows_aligned and q.stride(0) % 8 == 0 and scale >= _LEAST_TC_SCALE
                 and k_pool.numel() < (hd << 31) and _stream_takes("leb_attention_stream_tc_supported", nh, nkv, hd, vd, page_size)
                 and B <= _MOST_BLOCKS and longest <= _MOST_BLOCKS * (128 * nkv // nh // 8 * 8)):
             return _attention_stream_tc

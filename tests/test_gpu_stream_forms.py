@@ -79,3 +79,37 @@ def test_addresses_that_the_kernels_for_all_rows_do_not_take_are_refused(M, B, h
         with pytest.raises(K().KernelError):
             run(*args)
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("new", [1, 5, 150])
+@pytest.mark.parametrize("dtype,nh,nkv,hd,page", [(BF16, 8, 2, 64, 64), (BF16, 3, 3, 128, 64), (BF16, 4, 2, 32, 32), (BF16, 2, 1, 72, 64), (F32, 4, 2, 48, 32)])
+@pytest.mark.parametrize("first", [0, 70])
+@pytest.mark.parametrize("scale", [-0.125, 0.0, 1e-30, 1e-22])
+def test_scales_that_are_not_positive_or_next_to_nothing(new, dtype, nh, nkv, hd, page, first, scale):
+    """What a row does not see has no weight, whatever the scores that it sees are multiplied by."""
+    held, window, G = 250, 90, nh // nkv
+    T = held + new
+    word = lambda v: torch.tensor(v, dtype=torch.int32, device=DEV)
+    g = torch.Generator(device=DEV).manual_seed(2)
+    rand = lambda *s: torch.randn(s, generator=g, device=DEV).to(dtype)
+    n = -(-T // page)
+    q, k, v = rand(new, nh * hd), rand(n, nkv, page, hd), rand(n, nkv, hd, page)
+    batch = types.SimpleNamespace(n_rows=new, n_seqs=1, max_qlen=new, max_kvlen=T, row_seq=word([0] * new), row_pos=word(list(range(held, T))),
+                                  seq_slot=word([0]), seq_pos0=word([held]), seq_qstart=word([0]), seq_qlen=word([new]))
+    out = torch.full((new, nh * hd), float("nan"), dtype=dtype, device=DEV)
+    K().attention(out, q, k, v, torch.arange(n, dtype=torch.int32, device=DEV)[None], batch, nh, nkv, hd, page, window, scale, first=first)
+    K().check_device_status()
+    p, t = torch.arange(held, T, device=DEV)[:, None], torch.arange(T, device=DEV)[None]
+    ok = (t <= p) & ((t > p - window) | (t < first))
+    for h in range(nh):
+        qq = q[:, h * hd:(h + 1) * hd].double()
+        kk, vv = k[:, h // G].reshape(-1, hd)[:T].double(), v[:, h // G].transpose(1, 2).reshape(-1, hd)[:T].double()
+        w = torch.softmax((qq @ kk.T * scale).masked_fill(~ok, float("-inf")), -1)
+        size = (qq.abs() @ kk.abs().T * abs(scale)).amax(1, keepdim=True)
+        want, mass = w @ vv, w @ vv.abs()
+        # the roundings of tests/test_gpu_stream.py
+        if dtype == BF16:
+            bound = 2 ** -8 * (1 + 2 ** -6) * (want.abs() + mass) + 2 * mass * (hd * 2 ** -22 * size + T * 2 ** -24 + 2 ** -18)
+        else:
+            bound = want.abs() * 2 ** -22 + 2 * mass * ((hd + 8) * 2 ** -24 * size + T * 2 ** -24 + 2 ** -20)
+        assert bool(((out[:, h * hd:(h + 1) * hd].double() - want).abs() <= bound + 1e-30).all()), h
