@@ -93,7 +93,7 @@ attention_stream_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gr
   uint8_t* sq = smem;                         // [64 dimensions][128 rows][128 bytes]
   uint8_t* sk = sq + Q_BYTES;                 // [stage][64 dimensions][128 keys][128 bytes]
   uint8_t* sv = sk + NS * KV_BYTES;           // [stage][page][dimension][64 positions]
-  __shared__ uint64_t q_full, k_full[NS], v_full[NS], k_empty[NS], v_empty[NS], s_full, s_free, p_full, pv_done, zeroed[NS];
+  __shared__ uint64_t q_full, k_full[NS], v_full[NS], k_empty[NS], v_empty[NS], s_full, s_free, p_full, pv_done, zeroed[NS], drained;
   __shared__ float row_s[2][2][128];          // what the two threads of a row tell each other: [iteration's parity][thread][row]
   __shared__ float last_s[2][128], join_s[SHARED ? AST_MOST_SPLITS : 1][SHARED ? 64 : 128];      // maxima and sums of this block's rows; factors of the rows it stores
   __shared__ int place_s[SHARED ? 64 : 128];      // and where those lie in out, from the tile's first row and head on (-1: nowhere)
@@ -199,6 +199,7 @@ attention_stream_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gr
     mbar_init(&s_free, 8);
     mbar_init(&p_full, 8);
     mbar_init(&pv_done, 1);
+    mbar_init(&drained, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 8) {
@@ -538,13 +539,22 @@ attention_stream_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gr
   }
   tc_fence_before();
   __syncthreads();
-  if (abort_s && threadIdx.x == 32 * 8) {      // a role gave up: the block stays until its copies have landed (else every one has been read)
-    auto landed = [](uint64_t* bar, int phase) {
+  if (abort_s) {      // a role gave up: the block stays until its copies have landed and its products are done (else every one has been waited for)
+    auto passed = [](uint64_t* bar, int phase) {
       for (int n = 0; n < 1 << 16 && !mbar_try_wait(bar, phase & 1); n++) {}
     };
-    if (n_it > 0) landed(&q_full, 0);
-    for (int i = max(sent_s[0] - NS, 0); i < sent_s[0]; i++) landed(&k_full[i % NS], i / NS);
-    for (int i = max(sent_s[1] - NS, 0); i < sent_s[1]; i++) landed(&v_full[i % NS], i / NS);
+    if (threadIdx.x == 32 * 8) {
+      if (n_it > 0) passed(&q_full, 0);
+      for (int i = max(sent_s[0] - NS, 0); i < sent_s[0]; i++) passed(&k_full[i % NS], i / NS);
+      for (int i = max(sent_s[1] - NS, 0); i < sent_s[1]; i++) passed(&v_full[i % NS], i / NS);
+    } else if (warp == 9) {
+      if (elect_lane()) {
+        umma_commit(&drained);
+        passed(&drained, 0);
+      }
+      __syncwarp();
+    }
+    __syncthreads();
   }
   __syncwarp();
   if (warp == 8) tmem_dealloc(tmem, Shape::COLUMNS);
