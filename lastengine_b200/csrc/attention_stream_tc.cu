@@ -13,6 +13,8 @@
 // Warps: eight for the softmax, one that brings Q and pages by TMA, one that issues the products, two that put zeros where a page holds
 // values no row of the tile reads (registers move between warpgroups).  Two blocks share an SM, so that one's products run under the other's exponentials, and a
 // scheduler has four softmax warps: what bounds the loop is the chain from a row's scores to its weights, not a pipe.
+// P is rounded to bfloat16 (l is the sum of the floats): results are 1.26 to 1.28 times as far from 64 bits as results rounded once.  Callers that want
+// more ask for weights of two terms or 32 bits (`wide`), and get another kernel.
 // Where there are few tiles, a cluster of n_splits blocks shares the pages of one and joins its sums through shared memory.
 // With heads of 64, P has columns beside S and the next scores are issued as soon as a row of S is in registers; with heads of 128, O
 // takes those columns, P lies over S and the next scores follow the product that reads P.
@@ -26,8 +28,8 @@
 // Measured beside it: one thread a row 311 to 317, two tiles a block (one block an SM) 329, 64 keys at a time with two buffers of S 323 (heads
 // of 128: 442), an eighth to a half of the exponentials as polynomials on the multiply-add pipes 304 to 365 (heads of 128: 428 to 515).
 //
-// Every wait on an mbarrier is bounded; a wait that gives up sets the status word, all roles leave their loops, tensor memory is freed
-// and the block returns.
+// Every wait on an mbarrier is bounded; a wait that gives up sets the status word, all roles leave their loops, and the block returns once its copies
+// have landed, its products are done and tensor memory is freed.
 #include "attention_tc.cuh"
 
 #define AST_NEG (-1e30f)
@@ -626,7 +628,8 @@ static int launch_attention_stream_tc(void* out, const void* q, int q_stride, in
 
 // Prompt attention of the step's rows over the paged cache (which already holds their keys and values).  q: [M, nh*hd] with row
 // stride q_stride; k_pool [n_pages][nkv][page_size][hd], v_pool [n_pages][nkv][vd][page_size]; out [M, nh*vd].  status: device int, set non-zero by a
-// block whose bounded wait gave up.  slopes, sinks [nh] or null as in leb_attention.  max_kvlen: the most positions a sequence of the step holds.
+// block whose bounded wait gave up.  slopes, sinks [nh] or null as in leb_attention.  scale: 1e-20 or more (masked
+// scores are -1e30 before they are scaled).  max_kvlen: the most positions a sequence of the step holds.
 // n_splits: blocks that share a tile's keys (0: as many as suit the step).
 LEB_API int leb_attention_stream_tc(void* out, const void* q, int q_stride, int M, const void* k_pool, const void* v_pool, int n_pages,
                                     const int* block_table, int bt_width, const int* seq_slot, const int* seq_pos0,
