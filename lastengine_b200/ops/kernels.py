@@ -1703,8 +1703,8 @@ def attention(out: torch.Tensor, q: torch.Tensor | None, k_pool: torch.Tensor, v
     per head in the softmax's denominator, without a key and without a value, not scaled.
     `first` > 0: beside its window (or chunk) a row reads the sequence's first `first` positions, whose pages the cache then
     keeps; without either it reads every position anyway.  What lies in the cache between those positions and the window of the step's first
-    row of a sequence reaches no result, whatever it is.  (An infinity or NaN among the values that one row of a chunk sees may, on the tensor cores,
-    reach rows that do not see it.)"""
+    row of a sequence reaches no result, whatever it is.  (An infinity or NaN among the values that one row of a chunk sees may reach rows
+    of its sequence that do not see it.)"""
     if first < 0:
         raise KernelError(f"attention: {first} first positions")
     first = min(int(first), _MOST_FIRST) if window > 0 or chunk > 0 else 0
