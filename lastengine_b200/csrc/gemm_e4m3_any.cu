@@ -1,0 +1,100 @@
+// 8-bit matrix product for operands of any sizes and strides: C[m, n] (+)= (sum_k A[m, k] W[n, k]) sa[m] sw[n].
+// 64 x 64 results per block, four by four a thread, k in chunks of 32 through shared memory as floats, summed in order: a row's
+// result does not depend on the other rows.  It is the way for rows that are not 16 bytes apart to run at all; the tensor-core
+// kernels take the others.
+#include "e4m3_common.cuh"
+
+namespace {
+
+template <typename TC>
+__global__ void __launch_bounds__(256) gemm_e4m3_any_kernel(TC* __restrict__ C, const uint8_t* __restrict__ A, const float* __restrict__ sa,
+                                                            const uint8_t* __restrict__ W, const float* __restrict__ sw, int M, int N, int K,
+                                                            long long lda, long long ldw, long long ldc, int epilogue, const int* __restrict__ offsets,
+                                                            int m_tiles, long long w_group_stride) {
+  __shared__ float as[64][33], ws[64][33];
+  const int act = epilogue >> 8;
+  epilogue &= 255;
+  pdl_wait();
+  int lo = 0, hi = M;
+  if (offsets) {      // rows [offsets[e], offsets[e + 1]) go with expert e's weights (whatever the offsets hold, no row beyond the M is touched)
+    const int e = blockIdx.x / m_tiles;
+    lo = max(offsets[e], 0);
+    hi = min(offsets[e + 1], M);
+    W += e * w_group_stride;
+    sw += (size_t)e * N;
+  }
+  const int m0 = lo + (int)(blockIdx.x % m_tiles) * 64, n0 = blockIdx.y * 64;
+  if (m0 >= hi) return;
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4, kk = threadIdx.x & 31, row8 = threadIdx.x >> 5;
+  float acc[4][4] = {};
+  for (int k0 = 0; k0 < K; k0 += 32) {
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+      const int r = row8 + 8 * j, m = m0 + r, n = n0 + r, k = k0 + kk;
+      as[r][kk] = m < hi && k < K ? e4m3_to_f32(A[m * lda + k]) : 0.f;
+      ws[r][kk] = n < N && k < K ? e4m3_to_f32(W[n * ldw + k]) : 0.f;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < 32; k++)
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) acc[i][j] += as[ty * 4 + i][k] * ws[tx + 16 * j][k];
+    __syncthreads();
+  }
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    const int m = m0 + ty * 4 + i;
+    if (m >= hi) continue;
+    float z[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      const int n = n0 + tx + 16 * j;
+      z[j] = n < N ? acc[i][j] * sa[m] * sw[n] : 0.f;
+    }
+    TC* c = C + m * ldc;
+    if (epilogue == 2) {
+#pragma unroll
+      for (int j = 0; j < 4; j += 2)
+        if (n0 + 16 * j < N) c[n0 / 2 + 8 * j + tx] = from_f32<TC>(gate_mul<float>(z[j], z[j + 1], act));
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        const int n = n0 + tx + 16 * j;
+        if (n >= N) continue;
+        float v = z[j];
+        if (epilogue == 1) v += to_f32(c[n]);
+        else if (LEB_PLAIN_ACT_OK(act, epilogue)) v = plain_act(v, act);
+        c[n] = from_f32<TC>(v);
+      }
+    }
+  }
+}
+
+}  // namespace
+
+int leb_gemm_e4m3_any(void* C, int c_dtype, const void* A, const float* sa, const void* W, const float* sw, int M, int N, int K, long long lda,
+                              long long ldw, long long ldc, int epilogue, const int* offsets, int n_groups, long long w_group_stride, cudaStream_t st) {
+  if (M <= 0 || N <= 0) return 0;
+  if (const char* fault = e4m3_epilogue_fault(epilogue >> 8, epilogue & 255, c_dtype, N)) return leb_fail("leb_gemm_e4m3_any: %s (epilogue %d, N %d)", fault, epilogue, N);
+  const int m_tiles = ceil_div(M, 64);
+  const long long xs = (long long)m_tiles * (offsets ? n_groups : 1);
+  LEB_REQUIRE(K > 0 && xs < (1LL << 31) && ceil_div(N, 64) <= 65535, "leb_gemm_e4m3_any: %d rows in %d groups, %d columns, an inner size of %d in one launch", M, n_groups, N, K);
+  const dim3 grid((unsigned)xs, ceil_div(N, 64));
+  if (c_dtype == LEB_F32)
+    leb_launch(gemm_e4m3_any_kernel<float>, grid, dim3(256), 0, st, (float*)C, (const uint8_t*)A, sa, (const uint8_t*)W, sw, M, N, K, lda, ldw, ldc, epilogue, offsets, m_tiles, w_group_stride);
+  else
+    leb_launch(gemm_e4m3_any_kernel<bf16>, grid, dim3(256), 0, st, (bf16*)C, (const uint8_t*)A, sa, (const uint8_t*)W, sw, M, N, K, lda, ldw, ldc, epilogue, offsets, m_tiles, w_group_stride);
+  LEB_CHECK_LAUNCH("leb_gemm_e4m3_any");
+  return 0;
+}
+
+// C [M, N] (or [M, N / 2] gated; rows ldc apart) (+)= the product of A [M, K] with scales sa [M] and W [N, K] with scales sw [N]; with offsets
+// [n_groups + 1] (on the device) rows [offsets[e], offsets[e + 1]) with W[e], sw[e], experts w_group_stride apart, and rows beyond the last
+// offset left as they are.  epilogue: 0 store, 1 add into float C, 2 gated, an activation above it as in the bfloat16 products.
+LEB_API int leb_linear_e4m3(void* C, int c_dtype, const void* A, const float* sa, const void* W, const float* sw, int M, int N, int K, long long lda,
+                            long long ldw, long long ldc, int epilogue, const int* offsets, int n_groups, long long w_group_stride, int* status,
+                            cudaStream_t st) {
+  return leb_gemm_e4m3_any(C, c_dtype, A, sa, W, sw, M, N, K, lda, ldw, ldc, epilogue, offsets, n_groups, w_group_stride, st);
+}

@@ -289,6 +289,9 @@ def _declare(L) -> None:
         "leb_gemm_bf16_stream_conv": [P, P, P, I, I, I, I, I, P, P, P, P, P, I, P, I, I, F, P],
         "leb_gemm_bf16_tc_grouped": [P, I, P, P, I, I, I, I, I, I, P, I, P, P],
         "leb_gemm_bf16_tc2": [P, I, P, P, I, I, I, I, I, I, P, P],
+        "leb_quantize_e4m3": [P, P, P, I, P, P, I, I, I, I, LL, LL, P],
+        "leb_rmsnorm_e4m3": [P, P, P, P, P, I, P, I, I, I, F, LL, P],
+        "leb_linear_e4m3": [P, I, P, P, P, P, I, I, I, LL, LL, LL, I, P, I, LL, P, P],
         "leb_moe_router": [P, P, P, I, P, P, I, I, I, I, I, F, I, P],
         "leb_moe_align": [P, P, P, P, I, I, P],
         "leb_moe_align_gather": [P, P, P, P, I, P, P, P, I, I, I, I, P],
@@ -2250,6 +2253,150 @@ def linear(out: torch.Tensor, x: torch.Tensor, w: torch.Tensor, epilogue: int = 
         return
     _check(L.leb_gemm_bf16_small(_ptr(out), _dt(out, "linear.out"), _ptr(x), _ptr(w), M, N, K, lda, ldc,
                                  epilogue, _ptr(group_offsets), E, stride, hint, _stream()))
+
+
+# ---- products in 8 bits ------------------------------------------------------------------------
+# A row of 8-bit numbers q (torch.float8_e4m3fn) comes with a float scale s and stands for s q.  `quantize_e4m3` and `rmsnorm_e4m3`
+# make such rows, `linear_e4m3` multiplies them.  Weights are rows too (one scale per output): a program brings them to 8 bits
+# once with `quantize_e4m3`.  Rows 16 bytes apart (or a multiple of that, `e4m3_rows`) go to the tensor cores.
+E4M3 = torch.float8_e4m3fn
+
+
+def e4m3_rows(*shape: int, device=None) -> torch.Tensor:
+    """Room for 8-bit rows [..., K], each 16 bytes (or a multiple of that) behind the one before whatever K is."""
+    *rows, k = shape
+    return torch.empty((*rows, -(-k // 16) * 16), dtype=E4M3, device=device)[..., :k]
+
+
+def _on_device(name: str, **tensors: torch.Tensor | None) -> None:
+    """The tensors of a call lie on the current device, which it launches on."""
+    here = -1
+    for what, t in tensors.items():
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise KernelError(f"{name}.{what}: tensor is on {t.device}, the kernels run on CUDA only")
+        if here < 0:
+            here = torch.cuda.current_device()
+        if t.get_device() != here:
+            raise KernelError(f"{name}.{what}: tensor is on {t.device}, the current device is cuda:{here}")
+
+
+def _vector(name: str, t: torch.Tensor, dtype: torch.dtype, *shape: int) -> None:
+    if t.dtype != dtype or t.shape != shape or not t.is_contiguous():
+        raise KernelError(f"{name}: expected contiguous {dtype} {shape}, got {t.dtype} {tuple(t.shape)}")
+
+
+def _pitch(name: str, t: torch.Tensor, M: int, K: int, written: bool = False) -> int:
+    """How far the rows of a matrix [M, K] (or of each of a stack) of neighbouring numbers lie apart; rows that are written do not overlap."""
+    if t.shape[-2:] != (M, K):
+        raise KernelError(f"{name}: expected {(M, K)}, got {tuple(t.shape)}")
+    step, inner = t.stride()[-2:]
+    if inner != 1 and K > 1:
+        raise KernelError(f"{name}: the numbers of a row must be neighbours, they are {inner} apart")
+    if M <= 1:      # (where a row behind the only one would lie)
+        return -(-K // 16) * 16
+    if written and step < K:
+        raise KernelError(f"{name}: rows of {K} numbers that are {step} apart overlap")
+    return step
+
+
+def quantize_e4m3(out: torch.Tensor, scale: torch.Tensor, x: torch.Tensor, rows: torch.Tensor | None = None, div: int = 1,
+                  weights: torch.Tensor | None = None) -> None:
+    """Rows of x [M, K] (float or bfloat16) in 8 bits: out [P, K] = round(448 x / a) and scale [P] = a / 448 (float) with
+    a = max(max |x|, 2^-100), the row's largest magnitude.  `rows` (int32 [P]): row p is x[rows[p] // div] (P = M without), and with
+    `weights` (float) its scale is multiplied by weights[rows[p]].  A row of x with a number that is not finite, and one that
+    `rows` does not find in x, gets numbers and a scale that are NaN.  Numbers are rounded to the nearest, ties to even."""
+    _on_device("quantize_e4m3", out=out, scale=scale, x=x, rows=rows, weights=weights)
+    if x.dim() != 2 or out.dim() != 2 or out.dtype != E4M3:
+        raise KernelError(f"quantize_e4m3: expected rows of {E4M3} out of a matrix, got {out.dtype} {tuple(out.shape)} out of {tuple(x.shape)}")
+    M, K = x.shape
+    P_ = out.shape[0]
+    ldx, ldq = _pitch("quantize_e4m3.x", x, M, K), _pitch("quantize_e4m3.out", out, P_, K, True)
+    _vector("quantize_e4m3.scale", scale, torch.float32, P_)
+    if rows is not None:
+        _vector("quantize_e4m3.rows", rows, torch.int32, P_)
+        if div < 1:
+            raise KernelError(f"quantize_e4m3: div is {div}, at least 1 is wanted")
+        if weights is not None and (weights.dtype != torch.float32 or not weights.is_contiguous() or weights.numel() < M * div):
+            raise KernelError(f"quantize_e4m3.weights: expected {M * div} contiguous floats, got {weights.dtype} {tuple(weights.shape)}")
+    elif P_ != M or weights is not None or div != 1:
+        raise KernelError(f"quantize_e4m3: {P_} rows out of {M}, div and weights need a list of rows")
+    if P_ == 0 or K == 0:
+        if K == 0 and P_:
+            raise KernelError("quantize_e4m3: rows without numbers have no scale")
+        return
+    _check(lib().leb_quantize_e4m3(out.data_ptr(), scale.data_ptr(), x.data_ptr(), _dt(x, "quantize_e4m3.x"), _ptr(rows), _ptr(weights), int(div),
+                                   P_, M, K, ldx, ldq, _stream()))
+
+
+def rmsnorm_e4m3(out: torch.Tensor, scale: torch.Tensor, x: torch.Tensor, w: torch.Tensor, eps: float, y: torch.Tensor | None = None,
+                 h: torch.Tensor | None = None) -> None:
+    """`rmsnorm` with its result in 8 bits: with y [M, D] (float or bfloat16) first x += y; then with g = x w, r = 1 / sqrt(mean(x^2) + eps)
+    and a = max(max |g|, 2^-100): out = round(448 g / a), scale = r a / 448.  x (float) and y are contiguous.  With `h` [M, D] (float
+    or bfloat16, contiguous) the launch also leaves there the normed rows r g, for readers that want more than 8 bits (a router).
+    A row with a number that is not finite gets numbers and a scale that are NaN."""
+    _on_device("rmsnorm_e4m3", out=out, scale=scale, x=x, w=w, y=y, h=h)
+    if x.dim() != 2 or x.dtype != torch.float32 or not x.is_contiguous():
+        raise KernelError(f"rmsnorm_e4m3.x: expected a contiguous float matrix, got {x.dtype} {tuple(x.shape)}")
+    if out.dtype != E4M3:
+        raise KernelError(f"rmsnorm_e4m3.out: expected {E4M3}, got {out.dtype}")
+    M, D = x.shape
+    ldq = _pitch("rmsnorm_e4m3.out", out, M, D, True)
+    _vector("rmsnorm_e4m3.scale", scale, torch.float32, M)
+    _vector("rmsnorm_e4m3.w", w, torch.float32, D)
+    for what, t in (("y", y), ("h", h)):
+        if t is not None and (t.dtype not in _DT or t.shape != x.shape or not t.is_contiguous()):
+            raise KernelError(f"rmsnorm_e4m3.{what}: expected contiguous float or bfloat16 {(M, D)}, got {t.dtype} {tuple(t.shape)}")
+    if M == 0:
+        return
+    if D == 0:
+        raise KernelError("rmsnorm_e4m3: rows without numbers have no norm")
+    _check(lib().leb_rmsnorm_e4m3(out.data_ptr(), scale.data_ptr(), x.data_ptr(), w.data_ptr(), _ptr(y), _DT[y.dtype] if y is not None else F32,
+                                  _ptr(h), _DT[h.dtype] if h is not None else F32, M, D, float(eps), ldq, _stream()))
+
+
+def linear_e4m3(out: torch.Tensor, x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, epilogue: int = STORE,
+                group_offsets: torch.Tensor | None = None) -> None:
+    """`linear` in 8 bits: out (+)= (x . w^T) x_scale[:, None] w_scale with x [M, K], x_scale [M], w [N, K], w_scale [N] (rows and scales as
+    `quantize_e4m3` leaves them) and sums in float.  With group_offsets (int32 [E + 1]) w is [E, N, K], w_scale [E, N], rows
+    [group_offsets[e], group_offsets[e + 1]) of x and out go with expert e, and rows of out behind the last offset stay as they are.
+    `out` is bfloat16 or float.  `epilogue`: STORE, ACCUMULATE (out is the float residual), a gated epilogue (`gated_epilogue`: rows of w
+    interleaved in blocks of 16 gate and 16 up rows, out has N/2 columns) or, for a bfloat16 out, a plain activation's
+    (`plain_act_epilogue`); activations see the scaled sums.  Every size from one on and rows any number of bytes apart are taken;
+    operands whose rows begin on 16 bytes (`e4m3_rows`) go to the tensor cores.  A row's numbers depend on no other row's; they do
+    depend, in their last bits, on how many rows the call has.  `w` is fetched no earlier than the kernels launched before have ended."""
+    _on_device("linear_e4m3", out=out, x=x, x_scale=x_scale, w=w, w_scale=w_scale, group_offsets=group_offsets)
+    if x.dtype != E4M3 or w.dtype != E4M3 or x.dim() != 2 or out.dim() != 2:
+        raise KernelError(f"linear_e4m3: expected two operands of {E4M3}, got x {x.dtype} {tuple(x.shape)}, w {w.dtype}")
+    M, K = x.shape
+    if w.dim() != (2 if group_offsets is None else 3) or w.shape[-1] != K:
+        raise KernelError(f"linear_e4m3: w is {tuple(w.shape)}, x has {K} columns and {'no' if group_offsets is None else 'its'} groups of rows")
+    N = w.shape[-2]
+    E, stride = 1, 0
+    if group_offsets is None:
+        ldw = _pitch("linear_e4m3.w", w, N, K)
+        _vector("linear_e4m3.w_scale", w_scale, torch.float32, N)
+    else:
+        E = w.shape[0]
+        _vector("linear_e4m3.group_offsets", group_offsets, torch.int32, E + 1)
+        ldw = _pitch("linear_e4m3.w", w, N, K)
+        stride = w.stride(0) if E > 1 else N * ldw
+        _vector("linear_e4m3.w_scale", w_scale, torch.float32, E, N)
+    _vector("linear_e4m3.x_scale", x_scale, torch.float32, M)
+    gated = (epilogue & 255) == SWIGLU
+    n_out = N // 2 if gated else N
+    if gated and N % 32:
+        raise KernelError(f"linear_e4m3: gate and up rows come in blocks of 16 each, w has {N} rows")
+    ldx, ldc = _pitch("linear_e4m3.x", x, M, K), _pitch("linear_e4m3.out", out, M, n_out, True)
+    if epilogue == ACCUMULATE and out.dtype != torch.float32:
+        raise KernelError("linear_e4m3: adding needs a float out")
+    if M == 0 or N == 0 or E == 0:
+        return
+    if K == 0:
+        raise KernelError("linear_e4m3: an inner size of 0")
+    _check(lib().leb_linear_e4m3(out.data_ptr(), _dt(out, "linear_e4m3.out"), x.data_ptr(), x_scale.data_ptr(), w.data_ptr(), w_scale.data_ptr(),
+                                 M, N, K, ldx, ldw, ldc, int(epilogue), _ptr(group_offsets), E, stride, _status_word(x.device).data_ptr(), _stream()))
 
 
 # set by ops.tc_gemm when the tensor-core (tcgen05) kernel is present
