@@ -1,0 +1,130 @@
+// What the tcgen05 kernels of 8-bit numbers share beside tc_common.cuh: the products themselves, tensor maps of byte matrices, and the
+// walk over tiles of rows grouped by expert.  A block of 128 numbers of k is a row of 128 bytes, as 64 of bfloat16 are, so tiles,
+// swizzle and descriptors are the same; an instruction multiplies 32 of them.
+#pragma once
+#include "e4m3_common.cuh"
+#include "tc_common.cuh"
+
+#define E8_BK 128            // numbers of k in a stage
+#define E8_MAX_GROUPS 256
+
+// float accumulator, e4m3 A and B, both K-major
+__host__ __device__ constexpr uint32_t e8_idesc(int rows, int cols) { return (1u << 4) | ((uint32_t)(cols >> 3) << 17) | ((uint32_t)(rows >> 4) << 24); }
+
+__device__ __forceinline__ void umma_e4m3(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
+      ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// A tile's way to L2 only.  What L2 holds is current whoever writes it, so weights may be asked for so ahead of the wait for the
+// kernel before, even where that kernel makes them.
+__device__ __forceinline__ void tma_prefetch_2d(const CUtensorMap* map, int x, int y) {
+  asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"((uint64_t)map), "r"(x), "r"(y) : "memory");
+}
+__device__ __forceinline__ uint32_t e8_cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t e8_map_to_rank(uint32_t smem_addr, uint32_t rank) {   // the same place in another block of the cluster
+  uint32_t a;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_addr), "r"(rank));
+  return a;
+}
+__device__ __forceinline__ float e8_remote(uint32_t cluster_addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(cluster_addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ void e8_cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+
+// Rows grouped by expert: the offsets, held to the rows that there are, and the running count of tiles of `tile_rows` rows.
+struct E8Groups {
+  int off[E8_MAX_GROUPS + 1];      // first row of every expert
+  int end[E8_MAX_GROUPS];          // behind its last
+  int cum[E8_MAX_GROUPS + 1];      // tiles of the experts before
+};
+// All threads of the block; the offsets have been written by now.  Two barriers.
+__device__ __forceinline__ void e8_count_groups(E8Groups& g, const int* __restrict__ offsets, int n_groups, int M, int tile_rows, int n_tiles) {
+  for (int e = threadIdx.x; e < n_groups; e += blockDim.x) {
+    const int lo = min(max(offsets[e], 0), M), hi = min(max(offsets[e + 1], lo), M);
+    g.off[e] = lo;
+    g.end[e] = hi;
+  }
+  __syncthreads();
+  if (threadIdx.x < 32) {      // eight experts a lane
+    int n[E8_MAX_GROUPS / 32], sum = 0;
+#pragma unroll
+    for (int i = 0; i < E8_MAX_GROUPS / 32; i++) {
+      const int e = threadIdx.x * (E8_MAX_GROUPS / 32) + i;
+      n[i] = e < n_groups ? (g.end[e] - g.off[e] + tile_rows - 1) / tile_rows * n_tiles : 0;
+      sum += n[i];
+    }
+    int before = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, before, o);
+      if ((int)threadIdx.x >= o) before += v;
+    }
+    before -= sum;
+#pragma unroll
+    for (int i = 0; i < E8_MAX_GROUPS / 32; i++) {
+      const int e = threadIdx.x * (E8_MAX_GROUPS / 32) + i;
+      if (e < n_groups) g.cum[e] = before;
+      before += n[i];
+      if (e == n_groups - 1) g.cum[n_groups] = before;
+    }
+  }
+  __syncthreads();
+}
+// The expert of a tile: the last one whose count of tiles before it is not beyond the tile.
+__device__ __forceinline__ int e8_group_of(const E8Groups& g, int n_groups, int tile) {
+  int lo = 0, hi = n_groups;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (g.cum[mid] <= tile) lo = mid; else hi = mid;
+  }
+  return lo;
+}
+
+// A [rows, cols] byte matrix with rows ld bytes apart, read in boxes of box_rows x 128 under the 128-byte swizzle; what lies outside reads
+// as zero.
+static inline int e8_tensor_map(CUtensorMap* out, const void* ptr, long long rows, int cols, long long ld, int box_rows) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return leb_fail("leb_linear_e4m3: the driver has no cuTensorMapEncodeTiled");
+  cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+  cuuint64_t strides[1] = {(cuuint64_t)ld};
+  cuuint32_t box[2] = {(cuuint32_t)E8_BK, (cuuint32_t)box_rows};
+  cuuint32_t estr[2] = {1, 1};
+  CUresult r = fn(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return leb_fail("leb_linear_e4m3: cuTensorMapEncodeTiled failed (%d) for [%lld,%d] rows %lld apart", (int)r, rows, cols, ld);
+  return 0;
+}
+
+// A product as its kernels take it.
+struct E8Product {
+  void* C;
+  int c_dtype;
+  const void* A;
+  const float* sa;
+  const void* W;
+  const float* sw;
+  int M, N, K;
+  long long lda, ldw, ldc;
+  int epilogue;            // with its activation above
+  const int* offsets;      // [n_groups + 1] on the device, or null
+  int n_groups;
+  long long w_group_stride;
+  int* status;
+};
+int leb_gemm_e4m3_any(const E8Product& p, cudaStream_t st);
+int leb_gemm_e4m3_few(const E8Product& p, cudaStream_t st);

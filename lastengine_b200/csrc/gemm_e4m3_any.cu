@@ -2,7 +2,7 @@
 // 64 x 64 results per block, four by four a thread, k in chunks of 32 through shared memory as floats, summed in order: a row's
 // result does not depend on the other rows.  It is the way for rows that are not 16 bytes apart to run at all; the tensor-core
 // kernels take the others.
-#include "e4m3_common.cuh"
+#include "e4m3_tc.cuh"
 
 namespace {
 
@@ -74,27 +74,15 @@ __global__ void __launch_bounds__(256) gemm_e4m3_any_kernel(TC* __restrict__ C, 
 
 }  // namespace
 
-int leb_gemm_e4m3_any(void* C, int c_dtype, const void* A, const float* sa, const void* W, const float* sw, int M, int N, int K, long long lda,
-                              long long ldw, long long ldc, int epilogue, const int* offsets, int n_groups, long long w_group_stride, cudaStream_t st) {
-  if (M <= 0 || N <= 0) return 0;
-  if (const char* fault = e4m3_epilogue_fault(epilogue >> 8, epilogue & 255, c_dtype, N)) return leb_fail("leb_gemm_e4m3_any: %s (epilogue %d, N %d)", fault, epilogue, N);
-  const int m_tiles = ceil_div(M, 64);
-  const long long xs = (long long)m_tiles * (offsets ? n_groups : 1);
-  LEB_REQUIRE(K > 0 && xs < (1LL << 31) && ceil_div(N, 64) <= 65535, "leb_gemm_e4m3_any: %d rows in %d groups, %d columns, an inner size of %d in one launch", M, n_groups, N, K);
-  const dim3 grid((unsigned)xs, ceil_div(N, 64));
-  if (c_dtype == LEB_F32)
-    leb_launch(gemm_e4m3_any_kernel<float>, grid, dim3(256), 0, st, (float*)C, (const uint8_t*)A, sa, (const uint8_t*)W, sw, M, N, K, lda, ldw, ldc, epilogue, offsets, m_tiles, w_group_stride);
+int leb_gemm_e4m3_any(const E8Product& p, cudaStream_t st) {
+  const int m_tiles = ceil_div(p.M, 64);
+  const long long xs = (long long)m_tiles * (p.offsets ? p.n_groups : 1);
+  LEB_REQUIRE(xs < (1LL << 31) && ceil_div(p.N, 64) <= 65535, "leb_linear_e4m3: %d rows in %d groups and %d columns in one launch", p.M, p.n_groups, p.N);
+  const dim3 grid((unsigned)xs, ceil_div(p.N, 64));
+  if (p.c_dtype == LEB_F32)
+    leb_launch(gemm_e4m3_any_kernel<float>, grid, dim3(256), 0, st, (float*)p.C, (const uint8_t*)p.A, p.sa, (const uint8_t*)p.W, p.sw, p.M, p.N, p.K, p.lda, p.ldw, p.ldc, p.epilogue, p.offsets, m_tiles, p.w_group_stride);
   else
-    leb_launch(gemm_e4m3_any_kernel<bf16>, grid, dim3(256), 0, st, (bf16*)C, (const uint8_t*)A, sa, (const uint8_t*)W, sw, M, N, K, lda, ldw, ldc, epilogue, offsets, m_tiles, w_group_stride);
-  LEB_CHECK_LAUNCH("leb_gemm_e4m3_any");
+    leb_launch(gemm_e4m3_any_kernel<bf16>, grid, dim3(256), 0, st, (bf16*)p.C, (const uint8_t*)p.A, p.sa, (const uint8_t*)p.W, p.sw, p.M, p.N, p.K, p.lda, p.ldw, p.ldc, p.epilogue, p.offsets, m_tiles, p.w_group_stride);
+  LEB_CHECK_LAUNCH("leb_linear_e4m3");
   return 0;
-}
-
-// C [M, N] (or [M, N / 2] gated; rows ldc apart) (+)= the product of A [M, K] with scales sa [M] and W [N, K] with scales sw [N]; with offsets
-// [n_groups + 1] (on the device) rows [offsets[e], offsets[e + 1]) with W[e], sw[e], experts w_group_stride apart, and rows beyond the last
-// offset left as they are.  epilogue: 0 store, 1 add into float C, 2 gated, an activation above it as in the bfloat16 products.
-LEB_API int leb_linear_e4m3(void* C, int c_dtype, const void* A, const float* sa, const void* W, const float* sw, int M, int N, int K, long long lda,
-                            long long ldw, long long ldc, int epilogue, const int* offsets, int n_groups, long long w_group_stride, int* status,
-                            cudaStream_t st) {
-  return leb_gemm_e4m3_any(C, c_dtype, A, sa, W, sw, M, N, K, lda, ldw, ldc, epilogue, offsets, n_groups, w_group_stride, st);
 }

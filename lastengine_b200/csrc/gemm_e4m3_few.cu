@@ -1,0 +1,322 @@
+// 8-bit matrix product on tcgen05 with the weights as the 128-row operand: C[m, n] (+)= (sum_k A[m, k] W[n, k]) sa[m] sw[n], dense or
+// with rows grouped by expert.
+//
+// With few rows the product is bound by reading W, so a tile is 128 rows of W by MP rows of A (16 to 256) and the accumulator in
+// tensor memory is the transposed tile.  Where there are fewer tiles than SMs a cluster of up to eight blocks shares a tile: each
+// takes a part of K, leaves its sums in its shared memory, and after a cluster barrier adds up its share of the tile's rows from all of
+// them, in the blocks' order.  Otherwise the blocks walk the tiles, with two accumulators, so that loads go on under the epilogue.
+//
+// Roles: warp 0 asks for the tiles of W and A (TMA, 128 numbers of k a stage), warp 1 issues the products, warps 2-5 take the sums out of
+// tensor memory and apply the epilogue.  A lane of theirs owns a row of W: for one row of A a warp stores 32 neighbouring columns.
+//
+// Every wait is bounded: a role that gives up sets the status word and all leave; the block stays until the copies asked for have
+// landed and its products are done.
+#include "e4m3_tc.cuh"
+
+#define FEW_THREADS 192
+
+template <typename TC, int MP, int STAGES, int PER_SM, bool GROUPED>
+__global__ void __launch_bounds__(FEW_THREADS, PER_SM)
+gemm_e4m3_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_a, TC* __restrict__ C,
+                     const float* __restrict__ sa, const float* __restrict__ sw, int M, int N, int K, long long ldc, int epilogue, int n_slices,
+                     const int* __restrict__ offsets, int n_groups, int* __restrict__ status) {
+  constexpr int W_BYTES = 128 * E8_BK, A_BYTES = MP * E8_BK, CHUNKS = (MP + 31) / 32;
+  constexpr uint32_t TMEM_COLS = 2 * MP < 32 ? 32 : 2 * MP;
+  const int act = epilogue >> 8;
+  epilogue &= 255;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  uint8_t *s_w = smem, *s_a = smem + STAGES * W_BYTES;
+  __shared__ uint64_t full[STAGES], empty[STAGES], acc_full[2], acc_empty[2], drained;
+  __shared__ uint32_t tmem_slot;
+  __shared__ int abort_s, sent_s;
+  __shared__ E8Groups groups;
+  volatile int* abort_flag = &abort_s;
+
+  const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  const int nk = (K + E8_BK - 1) / E8_BK, per = (nk + n_slices - 1) / n_slices;
+  const int slice = n_slices > 1 ? (int)e8_cluster_rank() : 0;
+  const int kb_lo = slice * per, my_nk = max(0, min(nk, kb_lo + per) - kb_lo);
+  const int first = blockIdx.x / n_slices, step = gridDim.x / n_slices;
+  const int m_tiles = (M + MP - 1) / MP, n_tiles = (N + 127) / 128;
+  int num_tiles = m_tiles * n_tiles;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; s++) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int i = 0; i < 2; i++) {
+      mbar_init(&acc_full[i], 1);
+      mbar_init(&acc_empty[i], 4);
+    }
+    mbar_init(&drained, 1);
+    abort_s = sent_s = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  if (warp == 1) {
+    tmem_alloc(&tmem_slot, TMEM_COLS);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_acc = tmem_slot;
+  pdl_trigger();      // (not before tensor memory is this block's: the next kernel's blocks may hold theirs while they wait for this one)
+  if (!GROUPED && warp == 0 && first < num_tiles && elect_lane())      // the first tile's weights, on their way to L2 while the kernel before ends
+    for (int i = 0; i < min(my_nk, STAGES); i++) tma_prefetch_2d(&map_w, (kb_lo + i) * E8_BK, first / m_tiles * 128);
+  __syncwarp();
+  pdl_wait();
+  if (GROUPED) {
+    e8_count_groups(groups, offsets, n_groups, M, MP, n_tiles);
+    num_tiles = groups.cum[n_groups];
+  }
+  if (n_slices > 1) num_tiles = min(num_tiles, step);      // (a cluster has one tile at most, whatever the offsets hold)
+  // first row of A and C, the row its rows end at, first column of C, the expert
+  auto place = [&](int tile, int& m0, int& m_end, int& n0, int& e) {
+    if (GROUPED) {
+      e = e8_group_of(groups, n_groups, tile);
+      const int local = tile - groups.cum[e], mt = (groups.end[e] - groups.off[e] + MP - 1) / MP;
+      n0 = local / mt * 128;
+      m0 = groups.off[e] + local % mt * MP;
+      m_end = groups.end[e];
+    } else {
+      e = 0;
+      n0 = tile / m_tiles * 128;
+      m0 = tile % m_tiles * MP;
+      m_end = M;
+    }
+  };
+  // z, scaled, of row m and this lane's column n; every lane of the warp calls
+  auto finish = [&](int m, int n, float z, float old) {
+    if (epilogue == 2) {      // lanes 0-15 hold gate columns, lanes 16-31 their up columns
+      const float up = __shfl_down_sync(0xffffffffu, z, 16);
+      if (lane < 16 && n < N) C[m * ldc + 16 * (n >> 5) + lane] = from_f32<TC>(gate_mul<TC>(z, up, act));
+    } else if (n < N) {
+      if (epilogue == 1) z += old;
+      else if (sizeof(TC) == 2 && LEB_PLAIN_ACT_OK(act, epilogue)) z = plain_act(z, act);
+      C[m * ldc + n] = from_f32<TC>(z);
+    }
+  };
+
+  if (warp == 0) {
+    uint32_t s = 0, ph = 1;
+    int sent = 0;
+    bool ok = true;
+    for (int tile = first; tile < num_tiles && ok; tile += step) {
+      int m0, m_end, n0, e;
+      place(tile, m0, m_end, n0, e);
+      for (int kb = 0; kb < my_nk; kb++) {
+        if (!mbar_wait_warp(&empty[s], ph, abort_flag)) { ok = false; break; }
+        if (elect_lane()) {
+          mbar_expect_tx(&full[s], W_BYTES + A_BYTES);
+          tma_load_2d(s_w + s * W_BYTES, &map_w, &full[s], (kb_lo + kb) * E8_BK, e * N + n0);
+          tma_load_2d(s_a + s * A_BYTES, &map_a, &full[s], (kb_lo + kb) * E8_BK, m0);
+        }
+        __syncwarp();
+        sent++;
+        if (++s == STAGES) s = 0, ph ^= 1;
+      }
+    }
+    if (lane == 0) {
+      sent_s = sent;
+      if (!ok) atomicExch(status, 51);
+    }
+  } else if (warp == 1) {
+    const uint64_t w_desc = make_desc(smem_u32(s_w)), a_desc = make_desc(smem_u32(s_a));
+    uint32_t s = 0, ph = 0, t = 0;
+    int gave_up = 0;
+    for (int tile = first; tile < num_tiles && !gave_up; tile += step, t++) {
+      const uint32_t buf = t & 1;
+      if (!mbar_wait_warp(&acc_empty[buf], ((t >> 1) & 1) ^ 1, abort_flag)) { gave_up = 54; break; }
+      tc_fence_after();
+      const uint32_t d_tmem = tmem_acc + buf * MP;
+      for (int kb = 0; kb < my_nk; kb++) {
+        if (!mbar_wait_warp(&full[s], ph, abort_flag)) { gave_up = 52; break; }
+        tc_fence_after();
+        if (elect_lane()) {
+          const uint64_t dw = w_desc + (uint64_t)(s * (W_BYTES / 16)), da = a_desc + (uint64_t)(s * (A_BYTES / 16));
+#pragma unroll
+          for (int k = 0; k < E8_BK / 32; k++) umma_e4m3(d_tmem, dw + (uint64_t)(k * 2), da + (uint64_t)(k * 2), e8_idesc(128, MP), (kb | k) != 0);
+          umma_commit(&empty[s]);
+          if (kb + 1 == my_nk) umma_commit(&acc_full[buf]);
+        }
+        __syncwarp();
+        if (++s == STAGES) s = 0, ph ^= 1;
+      }
+    }
+    if (gave_up && lane == 0) atomicExch(status, gave_up);
+  } else {
+    const int quad = warp & 3, n_loc = quad * 32 + lane;
+    uint32_t t = 0;
+    for (int tile = first; tile < num_tiles; tile += step, t++) {
+      int m0, m_end, n0, e;
+      place(tile, m0, m_end, n0, e);
+      const uint32_t buf = t & 1, tm = tmem_acc + ((uint32_t)(quad * 32) << 16) + buf * MP;
+      const int n = n0 + n_loc;
+      const float swn = n < N ? sw[(size_t)e * N + n] : 0.f;
+      float sam[CHUNKS];      // lane i: the scale of row 32 c + i
+#pragma unroll
+      for (int c = 0; c < CHUNKS; c++) sam[c] = m0 + c * 32 + lane < m_end ? sa[m0 + c * 32 + lane] : 0.f;
+      if (my_nk > 0) {
+        const bool ok = mbar_wait_warp(&acc_full[buf], (t >> 1) & 1, abort_flag);
+        if (!ok) {
+          if (lane == 0) atomicExch(status, 53);
+          break;
+        }
+        tc_fence_after();
+      }
+      if (n_slices > 1) {      // this block's sums, [m][n] (its stages are done with)
+        float* part = reinterpret_cast<float*>(smem);
+        if (my_nk > 0) {
+#pragma unroll
+          for (int c0 = 0; c0 < MP; c0 += 16) {
+            uint32_t v[16];
+            asm volatile(
+                "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+                "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+                : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
+                  "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+                : "r"(tm + (uint32_t)c0));
+            tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 16; i++) part[(c0 + i) * 128 + n_loc] = __uint_as_float(v[i]);
+          }
+        }
+        break;      // (a cluster has one tile; it is finished below, where all threads meet)
+      }
+#pragma unroll
+      for (int c = 0; c < CHUNKS; c++) {
+        constexpr int W = MP < 32 ? MP : 32;
+        if (m0 + c * 32 >= m_end) break;
+        uint32_t v[32];
+        if (W == 32) tmem_ld32(tm + (uint32_t)(c * 32), v);
+        else
+          asm volatile(
+              "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+              "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+              : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
+                "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+              : "r"(tm + (uint32_t)(c * 32)));
+        float old[W];
+#pragma unroll
+        for (int i = 0; i < W; i++) old[i] = epilogue == 1 && n < N && m0 + c * 32 + i < m_end ? to_f32(C[(m0 + c * 32 + i) * ldc + n]) : 0.f;
+        tmem_ld_wait();
+#pragma unroll
+        for (int i = 0; i < W; i++) {
+          const float z = __uint_as_float(v[i]) * __shfl_sync(0xffffffffu, sam[c], i) * swn;
+          if (m0 + c * 32 + i < m_end) finish(m0 + c * 32 + i, n, z, old[i]);
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&acc_empty[buf]);
+    }
+  }
+
+  if (n_slices > 1) {
+    __syncwarp();
+    e8_cluster_sync();      // every block's sums lie in its shared memory
+    if (warp >= 2 && first < num_tiles && !abort_s) {
+      int m0, m_end, n0, e;
+      place(first, m0, m_end, n0, e);
+      const int n_loc = (warp & 3) * 32 + lane, n = n0 + n_loc, share = MP / n_slices, used = (nk + per - 1) / per;
+      const float swn = n < N ? sw[(size_t)e * N + n] : 0.f;
+      const uint32_t mine = smem_u32(smem) + (uint32_t)n_loc * 4;
+#pragma unroll 2
+      for (int i = slice * share; i < (slice + 1) * share; i++) {
+        const int m = m0 + i;
+        if (m >= m_end) break;
+        float v[8];
+#pragma unroll
+        for (int r = 0; r < 8; r++) v[r] = r < used ? e8_remote(e8_map_to_rank(mine + (uint32_t)i * 512, (uint32_t)r)) : 0.f;
+        const float old = epilogue == 1 && n < N ? to_f32(C[m * ldc + n]) : 0.f;
+        float z = v[0];
+#pragma unroll
+        for (int r = 1; r < 8; r++) z += v[r];
+        finish(m, n, z * sa[m] * swn, old);
+      }
+    }
+    __syncwarp();
+    e8_cluster_sync();      // nobody leaves while others read its memory
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (abort_s) {      // a role gave up: the copies asked for land and the products end before the block does (else every one has been waited for)
+    auto passed = [](uint64_t* bar, int phase) {
+      for (int n = 0; n < 1 << 16 && !mbar_try_wait(bar, phase & 1); n++) {}
+    };
+    if (threadIdx.x == 0) {
+      for (int i = max(sent_s - STAGES, 0); i < sent_s; i++) passed(&full[i % STAGES], i / STAGES);
+    } else if (warp == 1) {
+      if (elect_lane()) {
+        umma_commit(&drained);
+        passed(&drained, 0);
+      }
+      __syncwarp();
+    }
+    __syncthreads();
+  }
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem_acc, TMEM_COLS);
+  }
+}
+
+namespace {
+
+template <typename TC, int MP, int STAGES, int PER_SM, bool GROUPED>
+int launch_few(const E8Product& p, int n_slices, cudaStream_t st) {
+  constexpr size_t smem = (size_t)STAGES * (128 + MP) * E8_BK + 1024;
+  auto kern = gemm_e4m3_few_kernel<TC, MP, STAGES, PER_SM, GROUPED>;
+  cudaError_t e = leb_allow_smem<gemm_e4m3_few_kernel<TC, MP, STAGES, PER_SM, GROUPED>, (int)smem>();
+  if (e != cudaSuccess) return leb_fail("leb_linear_e4m3: shared memory %zu: %s", smem, cudaGetErrorString(e));
+  CUtensorMap mw, ma;
+  if (e8_tensor_map(&mw, p.W, (long long)p.N * (p.offsets ? p.n_groups : 1), p.K, p.ldw, 128)) return 1;
+  if (e8_tensor_map(&ma, p.A, p.M, p.K, p.lda, MP)) return 1;
+  // grouped: the most tiles the offsets can give (every expert with rows may end with a part tile)
+  const long long m_tiles = p.M / MP + (GROUPED ? min(p.n_groups, p.M) : (p.M % MP != 0)), tiles = m_tiles * ceil_div(p.N, 128);
+  long long clusters = tiles;
+  if (n_slices == 1 && tiles > (long long)sm_count() * PER_SM) clusters = (long long)sm_count() * PER_SM;
+  if (clusters * n_slices >= 1LL << 31) return leb_fail("leb_linear_e4m3: %lld tiles", tiles);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(clusters * n_slices));
+  cfg.blockDim = dim3(FEW_THREADS);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)n_slices;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = g_leb_pdl ? 2 : 1;
+  e = cudaLaunchKernelEx(&cfg, kern, mw, ma, (TC*)p.C, p.sa, p.sw, p.M, p.N, p.K, p.ldc, p.epilogue, n_slices, p.offsets, p.n_groups, p.status);
+  if (e != cudaSuccess) return leb_fail("leb_linear_e4m3: %s", cudaGetErrorString(e));
+  LEB_CHECK_LAUNCH("leb_linear_e4m3");
+  return 0;
+}
+
+template <typename TC, bool GROUPED>
+int launch_few_rows(const E8Product& p, int mp, int n_slices, cudaStream_t st) {
+  if (mp == 16) return launch_few<TC, 16, 6, 2, GROUPED>(p, n_slices, st);
+  if (mp == 32) return launch_few<TC, 32, 5, 2, GROUPED>(p, n_slices, st);
+  if (mp == 64) return launch_few<TC, 64, 4, 2, GROUPED>(p, n_slices, st);
+  return launch_few<TC, 128, 3, 2, GROUPED>(p, n_slices, st);
+}
+
+}  // namespace
+
+int leb_gemm_e4m3_few(const E8Product& p, cudaStream_t st) {
+  const int groups = p.offsets ? min(p.n_groups, p.M) : 1;
+  const int rows = ceil_div(p.M, groups);      // of a group, about
+  const int mp = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
+  const long long tiles = (long long)ceil_div(p.N, 128) * (p.offsets ? max(groups, p.M / mp) : ceil_div(p.M, mp));
+  const int nk = ceil_div(p.K, E8_BK);
+  int n_slices = 1;
+  while (n_slices < 8 && tiles * n_slices * 2 <= 2LL * sm_count() && nk >= n_slices * 2 * 2) n_slices *= 2;
+  if (p.c_dtype == LEB_F32) return p.offsets ? launch_few_rows<float, true>(p, mp, n_slices, st) : launch_few_rows<float, false>(p, mp, n_slices, st);
+  return p.offsets ? launch_few_rows<bf16, true>(p, mp, n_slices, st) : launch_few_rows<bf16, false>(p, mp, n_slices, st);
+}
