@@ -127,4 +127,5 @@ struct E8Product {
   int* status;
 };
 int leb_gemm_e4m3_any(const E8Product& p, cudaStream_t st);
-int leb_gemm_e4m3_few(const E8Product& p, cudaStream_t st);
+int leb_gemm_e4m3_few(const E8Product& p, int mp, int n_slices, cudaStream_t st);
+int leb_gemm_e4m3_pairs(const E8Product& p, cudaStream_t st);

@@ -16,5 +16,13 @@ LEB_API int leb_linear_e4m3(void* C, int c_dtype, const void* A, const float* sa
   const long long rows_w = (long long)N * (offsets ? n_groups : 1);
   const bool tma = lda % 16 == 0 && lda >= K && ldw % 16 == 0 && ldw >= K && ((uintptr_t)A & 15) == 0 && ((uintptr_t)W & 15) == 0 &&
                    (!offsets || n_groups == 1 || w_group_stride == N * ldw) && n_groups <= E8_MAX_GROUPS && rows_w < (1LL << 31) - 256 && M < (1LL << 31) - 256;
-  return tma ? leb_gemm_e4m3_few(p, st) : leb_gemm_e4m3_any(p, st);
+  if (!tma) return leb_gemm_e4m3_any(p, st);
+  const int groups = offsets ? min(n_groups, M) : 1, rows = ceil_div(M, groups);      // of a group, about
+  if (rows >= 512) return leb_gemm_e4m3_pairs(p, st);
+  const int mp = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
+  const long long tiles = (long long)ceil_div(N, 128) * (offsets ? max(groups, M / mp) : ceil_div(M, mp));
+  const int nk = ceil_div(K, E8_BK);
+  int n_slices = 1;
+  while (n_slices < 8 && tiles * n_slices <= sm_count() && nk >= n_slices * 2 * 2) n_slices *= 2;
+  return leb_gemm_e4m3_few(p, mp, n_slices, st);
 }

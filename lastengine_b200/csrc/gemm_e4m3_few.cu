@@ -309,14 +309,8 @@ int launch_few_rows(const E8Product& p, int mp, int n_slices, cudaStream_t st) {
 
 }  // namespace
 
-int leb_gemm_e4m3_few(const E8Product& p, cudaStream_t st) {
-  const int groups = p.offsets ? min(p.n_groups, p.M) : 1;
-  const int rows = ceil_div(p.M, groups);      // of a group, about
-  const int mp = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
-  const long long tiles = (long long)ceil_div(p.N, 128) * (p.offsets ? max(groups, p.M / mp) : ceil_div(p.M, mp));
-  const int nk = ceil_div(p.K, E8_BK);
-  int n_slices = 1;
-  while (n_slices < 8 && tiles * n_slices * 2 <= 2LL * sm_count() && nk >= n_slices * 2 * 2) n_slices *= 2;
+// mp: 16, 32, 64 or 128 rows of A a tile; n_slices: 1, 2, 4 or 8 blocks that share a tile's K.
+int leb_gemm_e4m3_few(const E8Product& p, int mp, int n_slices, cudaStream_t st) {
   if (p.c_dtype == LEB_F32) return p.offsets ? launch_few_rows<float, true>(p, mp, n_slices, st) : launch_few_rows<float, false>(p, mp, n_slices, st);
   return p.offsets ? launch_few_rows<bf16, true>(p, mp, n_slices, st) : launch_few_rows<bf16, false>(p, mp, n_slices, st);
 }
