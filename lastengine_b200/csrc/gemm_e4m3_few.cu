@@ -7,29 +7,35 @@
 // them, in the blocks' order.  Otherwise the blocks walk the tiles, with two accumulators, so that loads go on under the epilogue.
 //
 // Roles: warp 0 asks for the tiles of W and A (TMA, 128 numbers of k a stage), warp 1 issues the products, warps 2-5 take the sums out of
-// tensor memory and apply the epilogue.  A lane of theirs owns a row of W: for one row of A a warp stores 32 neighbouring columns.
+// tensor memory, where a lane has a row of W, and turn them in shared memory: a warp then finishes a row of A at a time, a lane four
+// neighbouring columns, so that the results of a tile's row leave in one store.  (Finished as they come out of tensor memory, a lane a
+// column, the unrolled epilogues of all rows were more code than time: 100 rows x 2,048 x 2,048 in 16 tiles 52.9 us.)
 //
 // Every wait is bounded: a role that gives up sets the status word and all leave; the block stays until the copies asked for have
 // landed and its products are done.
 #include "e4m3_tc.cuh"
 
 #define FEW_THREADS 192
+#ifndef FEW_AHEAD
+#define FEW_AHEAD 5
+#endif
 
 template <typename TC, int MP, int STAGES, int PER_SM, bool GROUPED>
 __global__ void __launch_bounds__(FEW_THREADS, PER_SM)
 gemm_e4m3_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_a, TC* __restrict__ C,
                      const float* __restrict__ sa, const float* __restrict__ sw, int M, int N, int K, long long ldc, int epilogue, int n_slices,
-                     const int* __restrict__ offsets, int n_groups, int* __restrict__ status) {
-  constexpr int W_BYTES = 128 * E8_BK, A_BYTES = MP * E8_BK, CHUNKS = (MP + 31) / 32;
+                     const int* __restrict__ offsets, int n_groups, int ahead, int* __restrict__ status) {
+  constexpr int W_BYTES = 128 * E8_BK, A_BYTES = MP * E8_BK;
   constexpr uint32_t TMEM_COLS = 2 * MP < 32 ? 32 : 2 * MP;
   const int act = epilogue >> 8;
   epilogue &= 255;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-  uint8_t *s_w = smem, *s_a = smem + STAGES * W_BYTES;
+  uint8_t *s_w = smem, *s_a = smem + STAGES * W_BYTES, *s_part = s_a + STAGES * A_BYTES;      // part: the sums that are being finished
   __shared__ uint64_t full[STAGES], empty[STAGES], acc_full[2], acc_empty[2], drained;
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_s, sent_s;
+  __shared__ float sa_s[2][MP];
   __shared__ E8Groups groups;
   volatile int* abort_flag = &abort_s;
 
@@ -65,7 +71,7 @@ gemm_e4m3_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
   const uint32_t tmem_acc = tmem_slot;
   pdl_trigger();      // (not before tensor memory is this block's: the next kernel's blocks may hold theirs while they wait for this one)
   if (!GROUPED && warp == 0 && first < num_tiles && elect_lane())      // the first tile's weights, on their way to L2 while the kernel before ends
-    for (int i = 0; i < min(my_nk, STAGES); i++) tma_prefetch_2d(&map_w, (kb_lo + i) * E8_BK, first / m_tiles * 128);
+    for (int i = 0; i < min(my_nk, ahead); i++) tma_prefetch_2d(&map_w, (kb_lo + i) * E8_BK, first / m_tiles * 128);
   __syncwarp();
   pdl_wait();
   if (GROUPED) {
@@ -88,18 +94,80 @@ gemm_e4m3_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
       m_end = M;
     }
   };
-  // z, scaled, of row m and this lane's column n; every lane of the warp calls
-  auto finish = [&](int m, int n, float z, float old) {
-    if (epilogue == 2) {      // lanes 0-15 hold gate columns, lanes 16-31 their up columns
-      const float up = __shfl_down_sync(0xffffffffu, z, 16);
-      if (lane < 16 && n < N) C[m * ldc + 16 * (n >> 5) + lane] = from_f32<TC>(gate_mul<TC>(z, up, act));
-    } else if (n < N) {
-      if (epilogue == 1) z += old;
-      else if (sizeof(TC) == 2 && LEB_PLAIN_ACT_OK(act, epilogue)) z = plain_act(z, act);
-      C[m * ldc + n] = from_f32<TC>(z);
+  // Rows [i0, i1) of a tile, this lane's four columns: the sums of all `used` slices, scaled, through the epilogue.  All lanes call.
+  auto finish = [&](int i0, int i1, int row0, int n0, float4 swn, const float* sa_t, uint32_t sums, int used, int m0) {
+    const int n = n0 + lane * 4;
+    const bool vec = ldc % 4 == 0 && ((uintptr_t)C & (sizeof(TC) * 4 - 1)) == 0 && n + 3 < N;
+    constexpr int U = MP >= 64 ? 4 : 2;      // rows at a time
+#pragma unroll 1
+    for (int i = i0 + (warp & 3); i < i1; i += 4 * U) {
+      float4 z[U], old[U];
+#pragma unroll
+      for (int u = 0; u < U; u++) {
+        const int r = i + 4 * u;
+        old[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (epilogue == 1 && r < i1) {
+          const TC* c = C + (m0 + r) * ldc + n;
+          if (vec) old[u] = load4(c);
+          else {
+            if (n < N) old[u].x = to_f32(c[0]);
+            if (n + 1 < N) old[u].y = to_f32(c[1]);
+            if (n + 2 < N) old[u].z = to_f32(c[2]);
+            if (n + 3 < N) old[u].w = to_f32(c[3]);
+          }
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < U; u++) {
+        const int r = i + 4 * u;
+        const uint32_t at = sums + (uint32_t)((r - row0) * 512 + lane * 16);
+        z[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (r >= i1) continue;
+        if (n_slices == 1) z[u] = e8_remote4(at);
+        else {
+          float4 v[8];
+#pragma unroll
+          for (int k = 0; k < 8; k++) v[k] = k < used ? e8_remote4(e8_map_to_rank(at, (uint32_t)k)) : make_float4(0.f, 0.f, 0.f, 0.f);
+          z[u] = v[0];
+#pragma unroll
+          for (int k = 1; k < 8; k++) z[u].x += v[k].x, z[u].y += v[k].y, z[u].z += v[k].z, z[u].w += v[k].w;
+        }
+        const float f = sa_t[r];
+        z[u].x *= f * swn.x, z[u].y *= f * swn.y, z[u].z *= f * swn.z, z[u].w *= f * swn.w;
+      }
+      if (epilogue == 2) {      // of eight lanes four hold 16 gate columns, four their up columns
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+          const float4 g = z[u];
+          z[u].x = gate_mul<TC>(g.x, __shfl_down_sync(0xffffffffu, g.x, 4), act);
+          z[u].y = gate_mul<TC>(g.y, __shfl_down_sync(0xffffffffu, g.y, 4), act);
+          z[u].z = gate_mul<TC>(g.z, __shfl_down_sync(0xffffffffu, g.z, 4), act);
+          z[u].w = gate_mul<TC>(g.w, __shfl_down_sync(0xffffffffu, g.w, 4), act);
+        }
+      } else if (epilogue == 0 && sizeof(TC) == 2 && LEB_PLAIN_ACT_OK(act, epilogue)) {
+#pragma unroll
+        for (int u = 0; u < U; u++) z[u] = make_float4(plain_act(z[u].x, act), plain_act(z[u].y, act), plain_act(z[u].z, act), plain_act(z[u].w, act));
+      }
+#pragma unroll
+      for (int u = 0; u < U; u++) {
+        const int r = i + 4 * u;
+        if (r >= i1) break;
+        if (epilogue == 1) z[u].x += old[u].x, z[u].y += old[u].y, z[u].z += old[u].z, z[u].w += old[u].w;
+        const bool mine = epilogue != 2 || (lane & 4) == 0;
+        TC* c = C + (m0 + r) * ldc + (epilogue == 2 ? (n >> 5) * 16 + (n & 15) : n);
+        if (!mine) continue;
+        if (vec) store4(c, z[u]);
+        else {
+          if (n < N) c[0] = from_f32<TC>(z[u].x);
+          if (n + 1 < N) c[1] = from_f32<TC>(z[u].y);
+          if (n + 2 < N) c[2] = from_f32<TC>(z[u].z);
+          if (n + 3 < N) c[3] = from_f32<TC>(z[u].w);
+        }
+      }
     }
   };
 
+  bool gave_up = false, met = false;
   if (warp == 0) {
     uint32_t s = 0, ph = 1;
     int sent = 0;
@@ -126,14 +194,14 @@ gemm_e4m3_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
   } else if (warp == 1) {
     const uint64_t w_desc = make_desc(smem_u32(s_w)), a_desc = make_desc(smem_u32(s_a));
     uint32_t s = 0, ph = 0, t = 0;
-    int gave_up = 0;
-    for (int tile = first; tile < num_tiles && !gave_up; tile += step, t++) {
+    int role = 0;
+    for (int tile = first; tile < num_tiles && !role; tile += step, t++) {
       const uint32_t buf = t & 1;
-      if (!mbar_wait_warp(&acc_empty[buf], ((t >> 1) & 1) ^ 1, abort_flag)) { gave_up = 54; break; }
+      if (!mbar_wait_warp(&acc_empty[buf], ((t >> 1) & 1) ^ 1, abort_flag)) { role = 54; break; }
       tc_fence_after();
       const uint32_t d_tmem = tmem_acc + buf * MP;
       for (int kb = 0; kb < my_nk; kb++) {
-        if (!mbar_wait_warp(&full[s], ph, abort_flag)) { gave_up = 52; break; }
+        if (!mbar_wait_warp(&full[s], ph, abort_flag)) { role = 52; break; }
         tc_fence_after();
         if (elect_lane()) {
           const uint64_t dw = w_desc + (uint64_t)(s * (W_BYTES / 16)), da = a_desc + (uint64_t)(s * (A_BYTES / 16));
@@ -146,100 +214,66 @@ gemm_e4m3_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
         if (++s == STAGES) s = 0, ph ^= 1;
       }
     }
-    if (gave_up && lane == 0) atomicExch(status, gave_up);
+    if (role && lane == 0) atomicExch(status, role);
   } else {
-    const int quad = warp & 3, n_loc = quad * 32 + lane;
+    const int quad = warp & 3, n_loc = quad * 32 + lane, tid = threadIdx.x - 64;
+    float* const part = n_slices > 1 ? reinterpret_cast<float*>(smem) : reinterpret_cast<float*>(s_part);      // (a cluster's stages are done with)
     uint32_t t = 0;
     for (int tile = first; tile < num_tiles; tile += step, t++) {
       int m0, m_end, n0, e;
       place(tile, m0, m_end, n0, e);
       const uint32_t buf = t & 1, tm = tmem_acc + ((uint32_t)(quad * 32) << 16) + buf * MP;
-      const int n = n0 + n_loc;
-      const float swn = n < N ? sw[(size_t)e * N + n] : 0.f;
-      float sam[CHUNKS];      // lane i: the scale of row 32 c + i
-#pragma unroll
-      for (int c = 0; c < CHUNKS; c++) sam[c] = m0 + c * 32 + lane < m_end ? sa[m0 + c * 32 + lane] : 0.f;
+      const int n = n0 + lane * 4;
+      const float* sw_e = sw + (size_t)e * N;
+      const float4 swn = make_float4(n < N ? sw_e[n] : 0.f, n + 1 < N ? sw_e[n + 1] : 0.f, n + 2 < N ? sw_e[n + 2] : 0.f, n + 3 < N ? sw_e[n + 3] : 0.f);
+      const int rows = min(MP, m_end - m0);
+      if (tid < rows) sa_s[buf][tid] = sa[m0 + tid];
       if (my_nk > 0) {
         const bool ok = mbar_wait_warp(&acc_full[buf], (t >> 1) & 1, abort_flag);
         if (!ok) {
           if (lane == 0) atomicExch(status, 53);
-          break;
+          gave_up = true;
         }
         tc_fence_after();
       }
-      if (n_slices > 1) {      // this block's sums, [m][n] (its stages are done with)
-        float* part = reinterpret_cast<float*>(smem);
-        if (my_nk > 0) {
-#pragma unroll
-          for (int c0 = 0; c0 < MP; c0 += 16) {
-            uint32_t v[16];
-            asm volatile(
-                "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
-                "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
-                : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
-                  "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
-                : "r"(tm + (uint32_t)c0));
-            tmem_ld_wait();
-#pragma unroll
-            for (int i = 0; i < 16; i++) part[(c0 + i) * 128 + n_loc] = __uint_as_float(v[i]);
-          }
-        }
-        break;      // (a cluster has one tile; it is finished below, where all threads meet)
-      }
-#pragma unroll
-      for (int c = 0; c < CHUNKS; c++) {
-        constexpr int W = MP < 32 ? MP : 32;
-        if (m0 + c * 32 >= m_end) break;
-        uint32_t v[32];
-        if (W == 32) tmem_ld32(tm + (uint32_t)(c * 32), v);
-        else
-          asm volatile(
-              "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
-              "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
-              : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
-                "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
-              : "r"(tm + (uint32_t)(c * 32)));
-        float old[W];
-#pragma unroll
-        for (int i = 0; i < W; i++) old[i] = epilogue == 1 && n < N && m0 + c * 32 + i < m_end ? to_f32(C[(m0 + c * 32 + i) * ldc + n]) : 0.f;
+      // the sums of the next 16 rows, [row][column]
+      auto turn = [&](int c0, int at) {
+        uint32_t v[16];
+        tmem_ld16(tm + (uint32_t)c0, v);
         tmem_ld_wait();
 #pragma unroll
-        for (int i = 0; i < W; i++) {
-          const float z = __uint_as_float(v[i]) * __shfl_sync(0xffffffffu, sam[c], i) * swn;
-          if (m0 + c * 32 + i < m_end) finish(m0 + c * 32 + i, n, z, old[i]);
-        }
+        for (int i = 0; i < 16; i++) part[(at + i) * 128 + n_loc] = __uint_as_float(v[i]);
+      };
+      if (n_slices > 1) {      // a cluster has one tile; it is finished where all blocks have left their sums
+        if (my_nk > 0 && !gave_up)
+          for (int c0 = 0; c0 < rows; c0 += 16) turn(c0, c0);
+        __syncwarp();
+        e8_cluster_sync();
+        met = true;
+        const int share = MP / n_slices, used = (nk + per - 1) / per;
+        if (!gave_up) finish(slice * share, min((slice + 1) * share, rows), 0, n0, swn, sa_s[buf], smem_u32(part), used, m0);
+        break;
       }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&acc_empty[buf]);
+      if (!e8_all<128>(!gave_up)) break;      // (the four warps leave together: they meet again below)
+#pragma unroll 1
+      for (int c0 = 0; c0 < rows; c0 += 16) {
+        turn(c0, 0);
+        if (c0 + 16 >= rows) {      // all sums are out of tensor memory: the accumulator is free
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&acc_empty[buf]);
+        }
+        asm volatile("bar.sync 1, 128;" ::: "memory");
+        finish(c0, min(c0 + 16, rows), c0, n0, swn, sa_s[buf], smem_u32(part), 1, m0);
+        asm volatile("bar.sync 1, 128;" ::: "memory");
+      }
     }
   }
 
-  if (n_slices > 1) {
+  if (n_slices > 1) {      // every thread of the cluster meets the others twice: once its sums are left, and before it leaves itself
     __syncwarp();
-    e8_cluster_sync();      // every block's sums lie in its shared memory
-    if (warp >= 2 && first < num_tiles && !abort_s) {
-      int m0, m_end, n0, e;
-      place(first, m0, m_end, n0, e);
-      const int n_loc = (warp & 3) * 32 + lane, n = n0 + n_loc, share = MP / n_slices, used = (nk + per - 1) / per;
-      const float swn = n < N ? sw[(size_t)e * N + n] : 0.f;
-      const uint32_t mine = smem_u32(smem) + (uint32_t)n_loc * 4;
-#pragma unroll 2
-      for (int i = slice * share; i < (slice + 1) * share; i++) {
-        const int m = m0 + i;
-        if (m >= m_end) break;
-        float v[8];
-#pragma unroll
-        for (int r = 0; r < 8; r++) v[r] = r < used ? e8_remote(e8_map_to_rank(mine + (uint32_t)i * 512, (uint32_t)r)) : 0.f;
-        const float old = epilogue == 1 && n < N ? to_f32(C[m * ldc + n]) : 0.f;
-        float z = v[0];
-#pragma unroll
-        for (int r = 1; r < 8; r++) z += v[r];
-        finish(m, n, z * sa[m] * swn, old);
-      }
-    }
-    __syncwarp();
-    e8_cluster_sync();      // nobody leaves while others read its memory
+    if (!met) e8_cluster_sync();
+    e8_cluster_sync();
   }
   tc_fence_before();
   __syncthreads();
@@ -268,7 +302,7 @@ namespace {
 
 template <typename TC, int MP, int STAGES, int PER_SM, bool GROUPED>
 int launch_few(const E8Product& p, int n_slices, cudaStream_t st) {
-  constexpr size_t smem = (size_t)STAGES * (128 + MP) * E8_BK + 1024;
+  constexpr size_t smem = (size_t)STAGES * (128 + MP) * E8_BK + 16 * 512 + 1024;
   auto kern = gemm_e4m3_few_kernel<TC, MP, STAGES, PER_SM, GROUPED>;
   cudaError_t e = leb_allow_smem<gemm_e4m3_few_kernel<TC, MP, STAGES, PER_SM, GROUPED>, (int)smem>();
   if (e != cudaSuccess) return leb_fail("leb_linear_e4m3: shared memory %zu: %s", smem, cudaGetErrorString(e));
@@ -293,7 +327,7 @@ int launch_few(const E8Product& p, int n_slices, cudaStream_t st) {
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = g_leb_pdl ? 2 : 1;
-  e = cudaLaunchKernelEx(&cfg, kern, mw, ma, (TC*)p.C, p.sa, p.sw, p.M, p.N, p.K, p.ldc, p.epilogue, n_slices, p.offsets, p.n_groups, p.status);
+  e = cudaLaunchKernelEx(&cfg, kern, mw, ma, (TC*)p.C, p.sa, p.sw, p.M, p.N, p.K, p.ldc, p.epilogue, n_slices, p.offsets, p.n_groups, FEW_AHEAD, p.status);
   if (e != cudaSuccess) return leb_fail("leb_linear_e4m3: %s", cudaGetErrorString(e));
   LEB_CHECK_LAUNCH("leb_linear_e4m3");
   return 0;
@@ -301,7 +335,7 @@ int launch_few(const E8Product& p, int n_slices, cudaStream_t st) {
 
 template <typename TC, bool GROUPED>
 int launch_few_rows(const E8Product& p, int mp, int n_slices, cudaStream_t st) {
-  if (mp == 16) return launch_few<TC, 16, 6, 2, GROUPED>(p, n_slices, st);
+  if (mp == 16) return launch_few<TC, 16, 5, 2, GROUPED>(p, n_slices, st);
   if (mp == 32) return launch_few<TC, 32, 5, 2, GROUPED>(p, n_slices, st);
   if (mp == 64) return launch_few<TC, 64, 4, 2, GROUPED>(p, n_slices, st);
   return launch_few<TC, 128, 3, 2, GROUPED>(p, n_slices, st);

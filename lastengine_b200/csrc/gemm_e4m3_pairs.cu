@@ -190,6 +190,7 @@ gemm_e4m3_pairs_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
     const bool vec = ldc % PER == 0 && ((uintptr_t)C & 15) == 0;
     const int r4 = lane >> 2, u4 = lane & 3;      // in a line's stores: rows r4 + 8 j, 16 bytes u4
     uint32_t t = 0;
+    bool gave_up = false;
     for (int tile = pair; tile < num_tiles; tile += n_pairs, t++) {
       int m0, m_end, n0, e;
       place(tile, m0, m_end, n0, e);
@@ -200,7 +201,8 @@ gemm_e4m3_pairs_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
         sw_s[buf][i] = n0 + i < N ? sw[(size_t)e * N + n0 + i] : 0.f;
       }
       const float sam = row0 + lane < m_end ? sa[row0 + lane] : 0.f;
-      asm volatile("bar.sync 1, 256;" ::: "memory");      // (the other buffer may still be read: a tile has one barrier, so nobody is two tiles ahead)
+      // (the other buffer may still be read: a tile has one barrier, so nobody is two tiles ahead; the warps leave together)
+      if (!e8_all<256>(!gave_up)) break;
       // old values of the 32 columns from c on, as the stores of their two lines will want them; the first are asked for while the products run
       float4 nxt[8];
       auto load_old = [&](int c) {
@@ -215,7 +217,8 @@ gemm_e4m3_pairs_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
       const bool ok = mbar_wait_warp(&acc_full[buf], (t >> 1) & 1, abort_flag);
       if (!ok) {
         if (lane == 0) atomicExch(status, 63);
-        break;
+        gave_up = true;
+        continue;
       }
       tc_fence_after();
       // Four times 16 bytes of this lane's row (columns from `col` on) go out by lines; old: the values to add
@@ -315,8 +318,8 @@ gemm_e4m3_pairs_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
   tc_fence_before();
   __syncthreads();
   e8_cluster_sync();      // both blocks are through: nobody frees tensor memory or leaves while the other may still use it
-  const bool gave_up = abort_s | remote_int(e8_map_to_rank(smem_u32(&abort_s), rank ^ 1));
-  if (gave_up) {      // the copies asked for land and the products end first (else every one has been waited for)
+  const bool left = abort_s | remote_int(e8_map_to_rank(smem_u32(&abort_s), rank ^ 1));
+  if (left) {      // the copies asked for land and the products end first (else every one has been waited for)
     auto passed = [](uint64_t* bar, int phase) {
       for (int n = 0; n < 1 << 16 && !mbar_try_wait(bar, phase & 1); n++) {}
     };

@@ -10,6 +10,7 @@ import collections
 import contextlib
 import ctypes
 import functools
+import struct
 import threading
 import types
 from ctypes import c_float, c_int, c_size_t, c_void_p
@@ -289,9 +290,9 @@ def _declare(L) -> None:
         "leb_gemm_bf16_stream_conv": [P, P, P, I, I, I, I, I, P, P, P, P, P, I, P, I, I, F, P],
         "leb_gemm_bf16_tc_grouped": [P, I, P, P, I, I, I, I, I, I, P, I, P, P],
         "leb_gemm_bf16_tc2": [P, I, P, P, I, I, I, I, I, I, P, P],
-        "leb_quantize_e4m3": [P, P, P, I, P, P, I, I, I, I, LL, LL, P],
-        "leb_rmsnorm_e4m3": [P, P, P, P, P, I, P, I, I, I, F, LL, P],
-        "leb_linear_e4m3": [P, I, P, P, P, P, I, I, I, LL, LL, LL, I, P, I, LL, P, P],
+        "leb_quantize_e4m3": [ctypes.c_char_p, P],
+        "leb_rmsnorm_e4m3": [ctypes.c_char_p, P],
+        "leb_linear_e4m3": [ctypes.c_char_p, P],
         "leb_moe_router": [P, P, P, I, P, P, I, I, I, I, I, F, I, P],
         "leb_moe_align": [P, P, P, P, I, I, P],
         "leb_moe_align_gather": [P, P, P, P, I, P, P, P, I, I, I, I, P],
@@ -2268,30 +2269,32 @@ def e4m3_rows(*shape: int, device=None) -> torch.Tensor:
     return torch.empty((*rows, -(-k // 16) * 16), dtype=E4M3, device=device)[..., :k]
 
 
-def _on_device(name: str, **tensors: torch.Tensor | None) -> None:
-    """The tensors of a call lie on the current device, which it launches on."""
-    here = -1
+# The entry points take their arguments as one packed row of 64-bit numbers: seventeen converted one by one cost the host some 2 us.
+_PACK_QUANTIZE, _PACK_NORM, _PACK_LINEAR = (struct.Struct(f).pack for f in ("12q", "11qd", "17q"))
+
+
+def _not_here(name: str, **tensors: torch.Tensor | None) -> None:
+    """Raises if a tensor of a call is not on the current device, which the call launches on."""
     for what, t in tensors.items():
-        if t is None:
-            continue
-        if not t.is_cuda:
+        if t is not None and not t.is_cuda:
             raise KernelError(f"{name}.{what}: tensor is on {t.device}, the kernels run on CUDA only")
-        if here < 0:
-            here = torch.cuda.current_device()
-        if t.get_device() != here:
+    here = torch.cuda.current_device()
+    for what, t in tensors.items():
+        if t is not None and t.get_device() != here:
             raise KernelError(f"{name}.{what}: tensor is on {t.device}, the current device is cuda:{here}")
 
 
-def _vector(name: str, t: torch.Tensor, dtype: torch.dtype, *shape: int) -> None:
-    if t.dtype != dtype or t.shape != shape or not t.is_contiguous():
+def _vector(name: str, t: torch.Tensor, dtype: torch.dtype, shape: tuple) -> None:
+    if t.dtype is not dtype or t.shape != shape or not t.is_contiguous():
         raise KernelError(f"{name}: expected contiguous {dtype} {shape}, got {t.dtype} {tuple(t.shape)}")
 
 
 def _pitch(name: str, t: torch.Tensor, M: int, K: int, written: bool = False) -> int:
     """How far the rows of a matrix [M, K] (or of each of a stack) of neighbouring numbers lie apart; rows that are written do not overlap."""
-    if t.shape[-2:] != (M, K):
+    *_, m, k = t.shape
+    if m != M or k != K:
         raise KernelError(f"{name}: expected {(M, K)}, got {tuple(t.shape)}")
-    step, inner = t.stride()[-2:]
+    *_, step, inner = t.stride()
     if inner != 1 and K > 1:
         raise KernelError(f"{name}: the numbers of a row must be neighbours, they are {inner} apart")
     if M <= 1:      # (where a row behind the only one would lie)
@@ -2307,27 +2310,32 @@ def quantize_e4m3(out: torch.Tensor, scale: torch.Tensor, x: torch.Tensor, rows:
     a = max(max |x|, 2^-100), the row's largest magnitude.  `rows` (int32 [P]): row p is x[rows[p] // div] (P = M without), and with
     `weights` (float) its scale is multiplied by weights[rows[p]].  A row of x with a number that is not finite, and one that
     `rows` does not find in x, gets numbers and a scale that are NaN.  Numbers are rounded to the nearest, ties to even."""
-    _on_device("quantize_e4m3", out=out, scale=scale, x=x, rows=rows, weights=weights)
-    if x.dim() != 2 or out.dim() != 2 or out.dtype != E4M3:
+    here = x.get_device()
+    if (here < 0 or out.get_device() != here or scale.get_device() != here or here != torch.cuda.current_device()
+            or (rows is not None and (rows.get_device() != here or (weights is not None and weights.get_device() != here)))):
+        _not_here("quantize_e4m3", out=out, scale=scale, x=x, rows=rows, weights=weights)
+    if x.dim() != 2 or out.dim() != 2 or out.dtype is not E4M3:
         raise KernelError(f"quantize_e4m3: expected rows of {E4M3} out of a matrix, got {out.dtype} {tuple(out.shape)} out of {tuple(x.shape)}")
     M, K = x.shape
     P_ = out.shape[0]
     ldx, ldq = _pitch("quantize_e4m3.x", x, M, K), _pitch("quantize_e4m3.out", out, P_, K, True)
-    _vector("quantize_e4m3.scale", scale, torch.float32, P_)
+    _vector("quantize_e4m3.scale", scale, torch.float32, (P_,))
     if rows is not None:
-        _vector("quantize_e4m3.rows", rows, torch.int32, P_)
+        _vector("quantize_e4m3.rows", rows, torch.int32, (P_,))
         if div < 1:
             raise KernelError(f"quantize_e4m3: div is {div}, at least 1 is wanted")
         if weights is not None and (weights.dtype != torch.float32 or not weights.is_contiguous() or weights.numel() < M * div):
             raise KernelError(f"quantize_e4m3.weights: expected {M * div} contiguous floats, got {weights.dtype} {tuple(weights.shape)}")
     elif P_ != M or weights is not None or div != 1:
         raise KernelError(f"quantize_e4m3: {P_} rows out of {M}, div and weights need a list of rows")
-    if P_ == 0 or K == 0:
-        if K == 0 and P_:
-            raise KernelError("quantize_e4m3: rows without numbers have no scale")
+    dtype = _dt(x, "quantize_e4m3.x")
+    if P_ == 0:
         return
-    _check(lib().leb_quantize_e4m3(out.data_ptr(), scale.data_ptr(), x.data_ptr(), _dt(x, "quantize_e4m3.x"), _ptr(rows), _ptr(weights), int(div),
-                                   P_, M, K, ldx, ldq, _stream()))
+    if K == 0:
+        raise KernelError("quantize_e4m3: rows without numbers have no scale")
+    _check(lib().leb_quantize_e4m3(
+        _PACK_QUANTIZE(out.data_ptr(), scale.data_ptr(), x.data_ptr(), dtype, 0 if rows is None else rows.data_ptr(),
+                       0 if weights is None else weights.data_ptr(), div, P_, M, K, ldx, ldq), _stream()))
 
 
 def rmsnorm_e4m3(out: torch.Tensor, scale: torch.Tensor, x: torch.Tensor, w: torch.Tensor, eps: float, y: torch.Tensor | None = None,
@@ -2335,25 +2343,35 @@ def rmsnorm_e4m3(out: torch.Tensor, scale: torch.Tensor, x: torch.Tensor, w: tor
     """`rmsnorm` with its result in 8 bits: with y [M, D] (float or bfloat16) first x += y; then with g = x w, r = 1 / sqrt(mean(x^2) + eps)
     and a = max(max |g|, 2^-100): out = round(448 g / a), scale = r a / 448.  x (float) and y are contiguous.  With `h` [M, D] (float
     or bfloat16, contiguous) the launch also leaves there the normed rows r g, for readers that want more than 8 bits (a router).
-    A row with a number that is not finite gets numbers and a scale that are NaN."""
-    _on_device("rmsnorm_e4m3", out=out, scale=scale, x=x, w=w, y=y, h=h)
-    if x.dim() != 2 or x.dtype != torch.float32 or not x.is_contiguous():
+    A row with a number that is not finite (or squares whose sum is not) gets numbers and a scale that are NaN."""
+    here = x.get_device()
+    if (here < 0 or out.get_device() != here or scale.get_device() != here or w.get_device() != here or here != torch.cuda.current_device()
+            or (y is not None and y.get_device() != here) or (h is not None and h.get_device() != here)):
+        _not_here("rmsnorm_e4m3", out=out, scale=scale, x=x, w=w, y=y, h=h)
+    if x.dim() != 2 or x.dtype is not torch.float32 or not x.is_contiguous():
         raise KernelError(f"rmsnorm_e4m3.x: expected a contiguous float matrix, got {x.dtype} {tuple(x.shape)}")
-    if out.dtype != E4M3:
-        raise KernelError(f"rmsnorm_e4m3.out: expected {E4M3}, got {out.dtype}")
-    M, D = x.shape
+    if out.dtype is not E4M3 or out.dim() != 2:
+        raise KernelError(f"rmsnorm_e4m3.out: expected rows of {E4M3}, got {out.dtype} {tuple(out.shape)}")
+    M, D = shape = x.shape
     ldq = _pitch("rmsnorm_e4m3.out", out, M, D, True)
-    _vector("rmsnorm_e4m3.scale", scale, torch.float32, M)
-    _vector("rmsnorm_e4m3.w", w, torch.float32, D)
-    for what, t in (("y", y), ("h", h)):
-        if t is not None and (t.dtype not in _DT or t.shape != x.shape or not t.is_contiguous()):
-            raise KernelError(f"rmsnorm_e4m3.{what}: expected contiguous float or bfloat16 {(M, D)}, got {t.dtype} {tuple(t.shape)}")
+    _vector("rmsnorm_e4m3.scale", scale, torch.float32, (M,))
+    _vector("rmsnorm_e4m3.w", w, torch.float32, (D,))
+    yd = hd = F32
+    if y is not None:
+        yd = _DT.get(y.dtype, -1)
+        if yd < 0 or y.shape != shape or not y.is_contiguous():
+            raise KernelError(f"rmsnorm_e4m3.y: expected contiguous float or bfloat16 {(M, D)}, got {y.dtype} {tuple(y.shape)}")
+    if h is not None:
+        hd = _DT.get(h.dtype, -1)
+        if hd < 0 or h.shape != shape or not h.is_contiguous():
+            raise KernelError(f"rmsnorm_e4m3.h: expected contiguous float or bfloat16 {(M, D)}, got {h.dtype} {tuple(h.shape)}")
     if M == 0:
         return
     if D == 0:
         raise KernelError("rmsnorm_e4m3: rows without numbers have no norm")
-    _check(lib().leb_rmsnorm_e4m3(out.data_ptr(), scale.data_ptr(), x.data_ptr(), w.data_ptr(), _ptr(y), _DT[y.dtype] if y is not None else F32,
-                                  _ptr(h), _DT[h.dtype] if h is not None else F32, M, D, float(eps), ldq, _stream()))
+    _check(lib().leb_rmsnorm_e4m3(
+        _PACK_NORM(out.data_ptr(), scale.data_ptr(), x.data_ptr(), w.data_ptr(), 0 if y is None else y.data_ptr(), yd,
+                   0 if h is None else h.data_ptr(), hd, M, D, ldq, eps), _stream()))
 
 
 def linear_e4m3(out: torch.Tensor, x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, epilogue: int = STORE,
@@ -2365,38 +2383,42 @@ def linear_e4m3(out: torch.Tensor, x: torch.Tensor, x_scale: torch.Tensor, w: to
     interleaved in blocks of 16 gate and 16 up rows, out has N/2 columns) or, for a bfloat16 out, a plain activation's
     (`plain_act_epilogue`); activations see the scaled sums.  Every size from one on and rows any number of bytes apart are taken;
     operands whose rows begin on 16 bytes (`e4m3_rows`) go to the tensor cores.  A row's numbers depend on no other row's; they do
-    depend, in their last bits, on how many rows the call has.  `w` is fetched no earlier than the kernels launched before have ended."""
-    _on_device("linear_e4m3", out=out, x=x, x_scale=x_scale, w=w, w_scale=w_scale, group_offsets=group_offsets)
-    if x.dtype != E4M3 or w.dtype != E4M3 or x.dim() != 2 or out.dim() != 2:
-        raise KernelError(f"linear_e4m3: expected two operands of {E4M3}, got x {x.dtype} {tuple(x.shape)}, w {w.dtype}")
+    depend, in their last bits, on how many rows the call has."""
+    here = x.get_device()
+    if (here < 0 or out.get_device() != here or x_scale.get_device() != here or w.get_device() != here or w_scale.get_device() != here
+            or here != torch.cuda.current_device() or (group_offsets is not None and group_offsets.get_device() != here)):
+        _not_here("linear_e4m3", out=out, x=x, x_scale=x_scale, w=w, w_scale=w_scale, group_offsets=group_offsets)
+    if x.dtype is not E4M3 or w.dtype is not E4M3 or x.dim() != 2 or out.dim() != 2:
+        raise KernelError(f"linear_e4m3: expected matrices and operands of {E4M3}, got out {tuple(out.shape)}, x {x.dtype} {tuple(x.shape)}, w {w.dtype}")
     M, K = x.shape
-    if w.dim() != (2 if group_offsets is None else 3) or w.shape[-1] != K:
-        raise KernelError(f"linear_e4m3: w is {tuple(w.shape)}, x has {K} columns and {'no' if group_offsets is None else 'its'} groups of rows")
-    N = w.shape[-2]
-    E, stride = 1, 0
     if group_offsets is None:
-        ldw = _pitch("linear_e4m3.w", w, N, K)
-        _vector("linear_e4m3.w_scale", w_scale, torch.float32, N)
+        if w.dim() != 2:
+            raise KernelError(f"linear_e4m3: w is {tuple(w.shape)} without groups of rows")
+        N, E, stride, offsets = w.shape[0], 1, 0, 0
+        ldw, scales = _pitch("linear_e4m3.w", w, N, K), (N,)
     else:
-        E = w.shape[0]
-        _vector("linear_e4m3.group_offsets", group_offsets, torch.int32, E + 1)
-        ldw = _pitch("linear_e4m3.w", w, N, K)
+        if w.dim() != 3:
+            raise KernelError(f"linear_e4m3: w is {tuple(w.shape)} for groups of rows")
+        E, N = w.shape[:2]
+        _vector("linear_e4m3.group_offsets", group_offsets, torch.int32, (E + 1,))
+        ldw, scales, offsets = _pitch("linear_e4m3.w", w, N, K), (E, N), group_offsets.data_ptr()
         stride = w.stride(0) if E > 1 else N * ldw
-        _vector("linear_e4m3.w_scale", w_scale, torch.float32, E, N)
-    _vector("linear_e4m3.x_scale", x_scale, torch.float32, M)
+    _vector("linear_e4m3.w_scale", w_scale, torch.float32, scales)
+    _vector("linear_e4m3.x_scale", x_scale, torch.float32, (M,))
     gated = (epilogue & 255) == SWIGLU
-    n_out = N // 2 if gated else N
     if gated and N % 32:
         raise KernelError(f"linear_e4m3: gate and up rows come in blocks of 16 each, w has {N} rows")
-    ldx, ldc = _pitch("linear_e4m3.x", x, M, K), _pitch("linear_e4m3.out", out, M, n_out, True)
-    if epilogue == ACCUMULATE and out.dtype != torch.float32:
-        raise KernelError("linear_e4m3: adding needs a float out")
+    ldx, ldc = _pitch("linear_e4m3.x", x, M, K), _pitch("linear_e4m3.out", out, M, N // 2 if gated else N, True)
+    dtype = _DT.get(out.dtype, -1)
+    if dtype < 0 or (epilogue == ACCUMULATE and dtype != F32):
+        raise KernelError(f"linear_e4m3: out is {out.dtype}; float or bfloat16 is wanted, and float where sums are added")
     if M == 0 or N == 0 or E == 0:
         return
     if K == 0:
         raise KernelError("linear_e4m3: an inner size of 0")
-    _check(lib().leb_linear_e4m3(out.data_ptr(), _dt(out, "linear_e4m3.out"), x.data_ptr(), x_scale.data_ptr(), w.data_ptr(), w_scale.data_ptr(),
-                                 M, N, K, ldx, ldw, ldc, int(epilogue), _ptr(group_offsets), E, stride, _status_word(x.device).data_ptr(), _stream()))
+    _check(lib().leb_linear_e4m3(
+        _PACK_LINEAR(out.data_ptr(), dtype, x.data_ptr(), x_scale.data_ptr(), w.data_ptr(), w_scale.data_ptr(), M, N, K, ldx, ldw, ldc, epilogue,
+                     offsets, E, stride, _status_word(x.device).data_ptr()), _stream()))
 
 
 # set by ops.tc_gemm when the tensor-core (tcgen05) kernel is present

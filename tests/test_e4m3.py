@@ -1,4 +1,5 @@
 """Products in 8 bits, on the host: what the calls refuse before anything is launched, and what they hand on."""
+import struct
 import types
 
 import pytest
@@ -16,11 +17,12 @@ def calls(monkeypatch):
     """The entry points' arguments, in the place of the entry points."""
     got = []
 
-    def record(name):
-        return lambda *a: got.append((name, a)) or 0
+    def record(name, form):
+        return lambda packed, stream: got.append((name, struct.unpack(form, packed))) or 0
 
-    monkeypatch.setattr(K, "lib", lambda: types.SimpleNamespace(**{n: record(n) for n in ("leb_quantize_e4m3", "leb_rmsnorm_e4m3", "leb_linear_e4m3")}))
-    monkeypatch.setattr(K, "_on_device", lambda *a, **k: None)
+    forms = {"leb_quantize_e4m3": "12q", "leb_rmsnorm_e4m3": "11qd", "leb_linear_e4m3": "17q"}
+    monkeypatch.setattr(K, "lib", lambda: types.SimpleNamespace(**{n: record(n, f) for n, f in forms.items()}))
+    monkeypatch.setattr(K, "_not_here", lambda *a, **k: None)
     monkeypatch.setattr(K, "_status_word", lambda device: torch.zeros(1, dtype=torch.int32))
     monkeypatch.setattr(K, "_stream", lambda: 0)
     return got
@@ -58,7 +60,7 @@ def test_another_device_is_refused(monkeypatch):
     monkeypatch.setattr(torch.cuda, "current_device", lambda: 1)
     there = types.SimpleNamespace(get_device=lambda: 0, device="cuda:0", is_cuda=True)
     with pytest.raises(K.KernelError, match="current device is cuda:1"):
-        K._on_device("linear_e4m3", x=None, w=there)
+        K._not_here("linear_e4m3", x=None, w=there)
 
 
 def quantize(out=None, scale=None, x=None, **kw):
@@ -80,7 +82,7 @@ def test_quantize_refusals(calls):
     quantize(x=torch.zeros(1, 32).expand(4, 32))                       # one row four times: read, not written
     quantize(out=K.e4m3_rows(4, 30), x=torch.zeros(4, 30, dtype=BF16))
     K.quantize_e4m3(eight(0, 32), torch.zeros(0), torch.zeros(0, 32))
-    assert [a[6:12] for _, a in calls] == [(3, 4, 2, 32, 32, 32), (1, 4, 4, 32, 0, 32), (1, 4, 4, 30, 30, 32)]
+    assert [a[6:] for _, a in calls] == [(3, 4, 2, 32, 32, 32), (1, 4, 4, 32, 0, 32), (1, 4, 4, 30, 30, 32)]
 
 
 def norm(out=None, scale=None, x=None, w=None, eps=1e-5, **kw):
@@ -99,7 +101,7 @@ def test_rmsnorm_refusals(calls):
     assert not calls
     norm(y=torch.zeros(4, 32, dtype=BF16), h=torch.zeros(4, 32))
     norm(out=torch.as_strided(eight(200), (4, 32), (33, 1)))
-    assert [(a[5], a[7], *a[8:10], a[11]) for _, a in calls] == [(K.BF16, K.F32, 4, 32, 32), (K.F32, K.F32, 4, 32, 33)]
+    assert [(a[5], *a[7:]) for _, a in calls] == [(K.BF16, K.F32, 4, 32, 32, 1e-5), (K.F32, K.F32, 4, 32, 33, 1e-5)]
 
 
 def linear(out=None, x=None, x_scale=None, w=None, w_scale=None, *a, **kw):
@@ -137,7 +139,7 @@ def test_linear_refusals(calls):
 
 def test_a_refusal_of_the_library_is_raised(monkeypatch):
     """Epilogues that only the library knows to be wrong: its message becomes the error, nothing is launched."""
-    monkeypatch.setattr(K, "_on_device", lambda *a, **k: None)
+    monkeypatch.setattr(K, "_not_here", lambda *a, **k: None)
     monkeypatch.setattr(K, "_status_word", lambda device: torch.zeros(1, dtype=torch.int32))
     monkeypatch.setattr(K, "_stream", lambda: 0)
     for epilogue, out in ((3, torch.zeros(4, 64)), (K.ACCUMULATE | (1 << 8), torch.zeros(4, 64)), (K.plain_act_epilogue(0), torch.zeros(4, 64)), (K.SWIGLU | (9 << 8), torch.zeros(4, 32))):

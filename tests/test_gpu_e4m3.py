@@ -60,7 +60,8 @@ def test_the_format():
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
-@pytest.mark.parametrize("M,D", [(1, 1), (3, 7), (5, 64), (2, 100), (7, 1000), (300, 1001), (1, 2048), (33, 2048), (9, 4096), (4, 8192), (2, 12001), (3, 20000), (2, 50000)])
+@pytest.mark.parametrize("M,D", [(1, 1), (3, 7), (5, 64), (2, 100), (7, 1000), (300, 1001), (1, 2048), (33, 2048), (9, 4096), (4, 8192),
+                                 (13, 250), (21, 512), (9, 520), (6, 600), (3, 2500), (3, 3996), (2, 6001), (2, 8200), (2, 12001), (1, 16384), (3, 20000), (2, 50000)])
 def test_quantize(dtype, M, D):
     x = gen(M, D, seed=M + D, dtype=dtype) * torch.exp(gen(M, 1, seed=3, scale=3.0)).to(dtype)
     for pitch_x, pitch_q in ((D, D), (D + 8, -(-D // 16) * 16), (D + 3, D + 5)):
@@ -134,7 +135,8 @@ def test_quantize_gathered(D, dtype):
 
 
 @pytest.mark.parametrize("y_dtype", [None, F32, BF16])
-@pytest.mark.parametrize("M,D", [(1, 1), (2, 24), (5, 64), (7, 1000), (64, 1001), (1, 2048), (33, 2048), (3, 4096), (2, 8192), (2, 12001), (2, 20000), (2000, 512)])
+@pytest.mark.parametrize("M,D", [(1, 1), (2, 24), (5, 64), (7, 1000), (64, 1001), (1, 2048), (33, 2048), (3, 4096), (2, 8192),
+                                 (13, 250), (21, 256), (9, 520), (3, 2500), (3, 3996), (2, 6001), (2, 8200), (2, 12001), (1, 16384), (2, 20000), (2000, 512)])
 def test_rmsnorm(y_dtype, M, D):
     eps = 1e-5
     x, w = gen(M, D, seed=1, scale=2.0), 1 + 0.2 * gen(D, seed=2)
