@@ -136,14 +136,14 @@ gemm_e4m3_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
         z[u].x *= f * swn.x, z[u].y *= f * swn.y, z[u].z *= f * swn.z, z[u].w *= f * swn.w;
       }
       if (epilogue == 2) {      // of eight lanes four hold 16 gate columns, four their up columns
+        float g[4 * U], up[4 * U];
 #pragma unroll
-        for (int u = 0; u < U; u++) {
-          const float4 g = z[u];
-          z[u].x = gate_mul<TC>(g.x, __shfl_down_sync(0xffffffffu, g.x, 4), act);
-          z[u].y = gate_mul<TC>(g.y, __shfl_down_sync(0xffffffffu, g.y, 4), act);
-          z[u].z = gate_mul<TC>(g.z, __shfl_down_sync(0xffffffffu, g.z, 4), act);
-          z[u].w = gate_mul<TC>(g.w, __shfl_down_sync(0xffffffffu, g.w, 4), act);
-        }
+        for (int u = 0; u < U; u++) g[4 * u] = z[u].x, g[4 * u + 1] = z[u].y, g[4 * u + 2] = z[u].z, g[4 * u + 3] = z[u].w;
+#pragma unroll
+        for (int k = 0; k < 4 * U; k++) up[k] = __shfl_down_sync(0xffffffffu, g[k], 4);
+        gate_all<TC, 4 * U>(g, up, act);
+#pragma unroll
+        for (int u = 0; u < U; u++) z[u] = make_float4(g[4 * u], g[4 * u + 1], g[4 * u + 2], g[4 * u + 3]);
       } else if (epilogue == 0 && sizeof(TC) == 2 && LEB_PLAIN_ACT_OK(act, epilogue)) {
 #pragma unroll
         for (int u = 0; u < U; u++) z[u] = make_float4(plain_act(z[u].x, act), plain_act(z[u].y, act), plain_act(z[u].z, act), plain_act(z[u].w, act));

@@ -203,17 +203,18 @@ gemm_e4m3_pairs_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
       const float sam = row0 + lane < m_end ? sa[row0 + lane] : 0.f;
       // (the other buffer may still be read: a tile has one barrier, so nobody is two tiles ahead; the warps leave together)
       if (!e8_all<256>(!gave_up)) break;
-      // old values of the 32 columns from c on, as the stores of their two lines will want them; the first are asked for while the products run
-      float4 nxt[8];
-      auto load_old = [&](int c) {
+      // old values of a line of 16 columns from c on, as its stores will want them; a line's are asked for under the line before, the first
+      // while the products run
+      float4 olds[2][4];
+      auto load_old = [&](int c, float4* o) {
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-          const int row = row0 + r4 + 8 * (j & 3), col = n0 + c + 16 * (j >> 2) + u4 * 4;
-          nxt[j] = row < m_end && col + 3 < N ? __ldcs(reinterpret_cast<const float4*>(C + row * ldc + col)) : make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int j = 0; j < 4; j++) {
+          const int row = row0 + r4 + 8 * j, col = n0 + c + u4 * 4;
+          o[j] = row < m_end && col + 3 < N ? __ldcs(reinterpret_cast<const float4*>(C + row * ldc + col)) : make_float4(0.f, 0.f, 0.f, 0.f);
         }
       };
       const bool adds = sizeof(TC) == 4 && epilogue == 1;
-      if (adds && vec) load_old(c_base);
+      if (adds && vec) load_old(c_base, olds[0]);
       const bool ok = mbar_wait_warp(&acc_full[buf], (t >> 1) & 1, abort_flag);
       if (!ok) {
         if (lane == 0) atomicExch(status, 63);
@@ -249,17 +250,13 @@ gemm_e4m3_pairs_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
         __syncwarp();
       };
       uint4 kept[2];      // of a gated bfloat16 result: the first half of a line
-#pragma unroll 1
-      for (int c = 0; c < 128; c += 32) {
-        if (n0 + c_base + c >= N) break;
-        uint32_t v[32];
-        tmem_ld32(tmem_acc + ((uint32_t)(quad * 32) << 16) + buf * 256 + (uint32_t)(c_base + c), v);
-        float4 old[8];
-        if (adds && vec) {
+      const uint32_t tm = tmem_acc + ((uint32_t)(quad * 32) << 16) + buf * 256 + (uint32_t)c_base;
+      const int c_end = min(128, N - n0 - c_base);      // (may be negative: nothing of this half)
+      uint32_t vs[5][32];      // unrolled, so that no copy of a piece's registers is made while its load is on its way
+      tmem_ld32(tm, vs[0]);
 #pragma unroll
-          for (int j = 0; j < 8; j++) old[j] = nxt[j];
-          if (c + 32 < 128) load_old(c_base + c + 32);
-        }
+      for (int c = 0; c < 128; c += 32) {
+        uint32_t* const v = vs[c / 32];
         tmem_ld_wait();
         float z[32];
 #pragma unroll
@@ -270,10 +267,11 @@ gemm_e4m3_pairs_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
           z[i + 2] = __uint_as_float(v[i + 2]) * sam * f.z;
           z[i + 3] = __uint_as_float(v[i + 3]) * sam * f.w;
         }
+        if (c + 32 < 128) tmem_ld32(tm + (uint32_t)(c + 32), vs[c / 32 + 1]);      // on its way while these are finished
+        if (c >= c_end) continue;
         const int col = n0 + c_base + c;
         if (epilogue == 2) {
-#pragma unroll
-          for (int i = 0; i < 16; i++) z[i] = gate_mul<TC>(z[i], z[16 + i], act);
+          gate_all<TC, 16>(z, z + 16, act);
         } else if (sizeof(TC) == 2 && LEB_PLAIN_ACT_OK(act, epilogue)) {
 #pragma unroll
           for (int i = 0; i < 32; i++) z[i] = plain_act(z[i], act);
@@ -283,10 +281,11 @@ gemm_e4m3_pairs_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
 #pragma unroll
           for (int l = 0; l < 2; l++) {
             if (l == 1 && (epilogue == 2 || col + 16 >= N)) break;
+            if (adds && vec && c + 16 * l + 16 < 128) load_old(c_base + c + 16 * l + 16, olds[l ^ 1]);
 #pragma unroll
             for (int i = 0; i < 4; i++)
               u[i] = make_uint4(__float_as_uint(z[16 * l + 4 * i]), __float_as_uint(z[16 * l + 4 * i + 1]), __float_as_uint(z[16 * l + 4 * i + 2]), __float_as_uint(z[16 * l + 4 * i + 3]));
-            put(u, epilogue == 2 ? col / 2 : col + 16 * l, old + 4 * l);
+            put(u, epilogue == 2 ? col / 2 : col + 16 * l, olds[l]);
           }
         } else if (epilogue == 2) {
           uint4 h[2];
@@ -295,10 +294,10 @@ gemm_e4m3_pairs_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
             h[i] = make_uint4(pack2(z[8 * i], z[8 * i + 1]), pack2(z[8 * i + 2], z[8 * i + 3]), pack2(z[8 * i + 4], z[8 * i + 5]), pack2(z[8 * i + 6], z[8 * i + 7]));
           if (c & 32) {
             u[0] = kept[0], u[1] = kept[1], u[2] = h[0], u[3] = h[1];
-            put(u, (col - 32) / 2, old);
+            put(u, (col - 32) / 2, olds[0]);
           } else if (col + 32 >= N) {      // nothing follows
             u[0] = h[0], u[1] = h[1], u[2] = u[3] = make_uint4(0, 0, 0, 0);
-            put(u, col / 2, old);
+            put(u, col / 2, olds[0]);
           } else {
             kept[0] = h[0], kept[1] = h[1];
           }
@@ -306,7 +305,7 @@ gemm_e4m3_pairs_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
 #pragma unroll
           for (int i = 0; i < 4; i++)
             u[i] = make_uint4(pack2(z[8 * i], z[8 * i + 1]), pack2(z[8 * i + 2], z[8 * i + 3]), pack2(z[8 * i + 4], z[8 * i + 5]), pack2(z[8 * i + 6], z[8 * i + 7]));
-          put(u, col, old);
+          put(u, col, olds[0]);
         }
       }
       // this warp has read its sums: tell the block that issues the products
