@@ -55,7 +55,8 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
 
 template <typename TC, bool GROUPED>
 __global__ void __launch_bounds__(PAIRS_THREADS, 1)
-gemm_e4m3_pairs_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w, TC* __restrict__ C,
+gemm_e4m3_pairs_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w,
+                       const __grid_constant__ CUtensorMap map_c, int tma_c, TC* __restrict__ C,
                        const float* __restrict__ sa, const float* __restrict__ sw, int M, int N, int K, long long ldc, int epilogue,
                        const int* __restrict__ offsets, int n_groups, int* __restrict__ status) {
   constexpr int STAGES = PAIRS_STAGES, HALF = 128 * E8_BK;      // bytes of a block's half of a stage of either operand
@@ -190,7 +191,8 @@ gemm_e4m3_pairs_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
     const bool vec = ldc % PER == 0 && ((uintptr_t)C & 15) == 0;
     const int r4 = lane >> 2, u4 = lane & 3;      // in a line's stores: rows r4 + 8 j, 16 bytes u4
     uint32_t t = 0;
-    bool gave_up = false;
+    bool gave_up = false, pending = false;
+    const bool adds = sizeof(TC) == 4 && epilogue == 1;
     for (int tile = pair; tile < num_tiles; tile += n_pairs, t++) {
       int m0, m_end, n0, e;
       place(tile, m0, m_end, n0, e);
@@ -203,18 +205,6 @@ gemm_e4m3_pairs_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
       const float sam = row0 + lane < m_end ? sa[row0 + lane] : 0.f;
       // (the other buffer may still be read: a tile has one barrier, so nobody is two tiles ahead; the warps leave together)
       if (!e8_all<256>(!gave_up)) break;
-      // old values of a line of 16 columns from c on, as its stores will want them; a line's are asked for under the line before, the first
-      // while the products run
-      float4 olds[2][4];
-      auto load_old = [&](int c, float4* o) {
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-          const int row = row0 + r4 + 8 * j, col = n0 + c + u4 * 4;
-          o[j] = row < m_end && col + 3 < N ? __ldcs(reinterpret_cast<const float4*>(C + row * ldc + col)) : make_float4(0.f, 0.f, 0.f, 0.f);
-        }
-      };
-      const bool adds = sizeof(TC) == 4 && epilogue == 1;
-      if (adds && vec) load_old(c_base, olds[0]);
       const bool ok = mbar_wait_warp(&acc_full[buf], (t >> 1) & 1, abort_flag);
       if (!ok) {
         if (lane == 0) atomicExch(status, 63);
@@ -222,24 +212,40 @@ gemm_e4m3_pairs_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
         continue;
       }
       tc_fence_after();
-      // Four times 16 bytes of this lane's row (columns from `col` on) go out by lines; old: the values to add
-      auto put = [&](const uint4* u, int col, const float4* old) {
+      // Four times 16 bytes of this lane's row (columns from `col` on) go out by lines of 64 bytes.  Whole groups of 32 rows are stored, or
+      // added, by a TMA copy (what lies beyond C is left out), an expert's last ones and results that TMA does not take by the lanes.
+      const bool copies = tma_c && row0 < m_end && (!GROUPED || row0 + 32 <= m_end);
+      auto put = [&](const uint4* u, int col) {
+        if (pending) {      // the line before has left shared memory
+          if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+          __syncwarp();
+        }
 #pragma unroll
         for (int i = 0; i < 4; i++) *reinterpret_cast<uint4*>(lines + lane * 64 + ((i ^ ((lane >> 1) & 3)) << 4)) = u[i];
+        if (copies) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
+        if (copies) {
+          if (lane == 0) {
+            if (adds)
+              asm volatile("cp.reduce.async.bulk.tensor.2d.global.shared::cta.add.tile.bulk_group [%0, {%2, %3}], [%1];"
+                           ::"l"((uint64_t)&map_c), "r"(smem_u32(lines)), "r"(col), "r"(row0) : "memory");
+            else
+              asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%2, %3}], [%1];"
+                           ::"l"((uint64_t)&map_c), "r"(smem_u32(lines)), "r"(col), "r"(row0) : "memory");
+            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+          }
+          pending = true;
+          return;
+        }
+        pending = false;
 #pragma unroll
         for (int j = 0; j < 4; j++) {
           const int r = r4 + 8 * j, row = row0 + r, c = col + u4 * PER;
-          uint4 x = *reinterpret_cast<const uint4*>(lines + r * 64 + ((u4 ^ ((r >> 1) & 3)) << 4));
+          const uint4 x = *reinterpret_cast<const uint4*>(lines + r * 64 + ((u4 ^ ((r >> 1) & 3)) << 4));
           if (row < m_end && c < n_out) {
             TC* o = C + row * ldc + c;
-            if (vec && c + PER <= n_out) {
-              if (adds) {
-                float4* f = reinterpret_cast<float4*>(&x);
-                f->x += old[j].x; f->y += old[j].y; f->z += old[j].z; f->w += old[j].w;
-              }
-              *reinterpret_cast<uint4*>(o) = x;
-            } else {
+            if (vec && !adds && c + PER <= n_out) *reinterpret_cast<uint4*>(o) = x;
+            else {
               const TC* f = reinterpret_cast<const TC*>(&x);
 #pragma unroll
               for (int i = 0; i < PER; i++)
@@ -281,11 +287,10 @@ gemm_e4m3_pairs_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
 #pragma unroll
           for (int l = 0; l < 2; l++) {
             if (l == 1 && (epilogue == 2 || col + 16 >= N)) break;
-            if (adds && vec && c + 16 * l + 16 < 128) load_old(c_base + c + 16 * l + 16, olds[l ^ 1]);
 #pragma unroll
             for (int i = 0; i < 4; i++)
               u[i] = make_uint4(__float_as_uint(z[16 * l + 4 * i]), __float_as_uint(z[16 * l + 4 * i + 1]), __float_as_uint(z[16 * l + 4 * i + 2]), __float_as_uint(z[16 * l + 4 * i + 3]));
-            put(u, epilogue == 2 ? col / 2 : col + 16 * l, olds[l]);
+            put(u, epilogue == 2 ? col / 2 : col + 16 * l);
           }
         } else if (epilogue == 2) {
           uint4 h[2];
@@ -294,10 +299,10 @@ gemm_e4m3_pairs_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
             h[i] = make_uint4(pack2(z[8 * i], z[8 * i + 1]), pack2(z[8 * i + 2], z[8 * i + 3]), pack2(z[8 * i + 4], z[8 * i + 5]), pack2(z[8 * i + 6], z[8 * i + 7]));
           if (c & 32) {
             u[0] = kept[0], u[1] = kept[1], u[2] = h[0], u[3] = h[1];
-            put(u, (col - 32) / 2, olds[0]);
+            put(u, (col - 32) / 2);
           } else if (col + 32 >= N) {      // nothing follows
             u[0] = h[0], u[1] = h[1], u[2] = u[3] = make_uint4(0, 0, 0, 0);
-            put(u, col / 2, olds[0]);
+            put(u, col / 2);
           } else {
             kept[0] = h[0], kept[1] = h[1];
           }
@@ -305,7 +310,7 @@ gemm_e4m3_pairs_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
 #pragma unroll
           for (int i = 0; i < 4; i++)
             u[i] = make_uint4(pack2(z[8 * i], z[8 * i + 1]), pack2(z[8 * i + 2], z[8 * i + 3]), pack2(z[8 * i + 4], z[8 * i + 5]), pack2(z[8 * i + 6], z[8 * i + 7]));
-          put(u, col, olds[0]);
+          put(u, col);
         }
       }
       // this warp has read its sums: tell the block that issues the products
@@ -313,6 +318,8 @@ gemm_e4m3_pairs_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
       __syncwarp();
       if (lane == 0) arrive_cluster(acc_empty0 + buf * 8);
     }
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+    __syncwarp();
   }
   tc_fence_before();
   __syncthreads();
@@ -348,6 +355,17 @@ int launch_pairs(const E8Product& p, cudaStream_t st) {
   CUtensorMap ma, mw;
   if (e8_tensor_map(&ma, p.A, p.M, p.K, p.lda, 128)) return 1;
   if (e8_tensor_map(&mw, p.W, (long long)p.N * (p.offsets ? p.n_groups : 1), p.K, p.ldw, 128)) return 1;
+  // results as the copies of the epilogue see them: 32 rows by 64 bytes, turned as the lanes leave them
+  const int n_out = (p.epilogue & 255) == 2 ? p.N / 2 : p.N, size = sizeof(TC);
+  const int tma_c = p.ldc * size % 16 == 0 && ((uintptr_t)p.C & 15) == 0 && p.ldc >= n_out;
+  CUtensorMap mc = ma;
+  if (tma_c) {
+    cuuint64_t dims[2] = {(cuuint64_t)n_out, (cuuint64_t)p.M}, strides[1] = {(cuuint64_t)p.ldc * size};
+    cuuint32_t box[2] = {(cuuint32_t)(64 / size), 32}, estr[2] = {1, 1};
+    CUresult r = encode_fn()(&mc, size == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, p.C, dims, strides, box, estr,
+                             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return leb_fail("leb_linear_e4m3: cuTensorMapEncodeTiled failed (%d) for the results [%d,%d] rows %lld apart", (int)r, p.M, n_out, p.ldc);
+  }
   const long long m_tiles = p.M / 256 + (GROUPED ? min(p.n_groups, p.M) : (p.M % 256 != 0)), tiles = m_tiles * ceil_div(p.N, 256);
   const long long pairs = tiles < sm_count() / 2 ? tiles : sm_count() / 2;
   cudaLaunchConfig_t cfg = {};
@@ -363,7 +381,7 @@ int launch_pairs(const E8Product& p, cudaStream_t st) {
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = g_leb_pdl ? 2 : 1;
-  e = cudaLaunchKernelEx(&cfg, kern, ma, mw, (TC*)p.C, p.sa, p.sw, p.M, p.N, p.K, p.ldc, p.epilogue, p.offsets, p.n_groups, p.status);
+  e = cudaLaunchKernelEx(&cfg, kern, ma, mw, mc, tma_c, (TC*)p.C, p.sa, p.sw, p.M, p.N, p.K, p.ldc, p.epilogue, p.offsets, p.n_groups, p.status);
   if (e != cudaSuccess) return leb_fail("leb_linear_e4m3: %s", cudaGetErrorString(e));
   LEB_CHECK_LAUNCH("leb_linear_e4m3");
   return 0;

@@ -7,8 +7,8 @@
 // squares' sum is not) gets a scale and numbers that are NaN.
 //
 // Bound by memory: a float row is read and a quarter of its bytes written.  A thread keeps its numbers in registers between the sums and the
-// rounding, so a row is read once, with all loads out before the first is used: eight neighbours at a time where rows begin on 16 bytes
-// (a warp a row up to 512 numbers, a block above), single numbers otherwise; rows of more than 16,384 (8,192) are read twice.  The largest
+// rounding, so a row is read once, with all loads out before the first is used: eight neighbours at a time where rows begin on 16 bytes,
+// single numbers (four of a thread side by side, so that they are written as one word) otherwise; rows of more than 16,384 are read twice.  The largest
 // |g| is taken over the bits (for numbers without a sign they order as the numbers do, infinity and NaN on top).
 #include "e4m3_common.cuh"
 
@@ -20,20 +20,20 @@ struct RowSums {
 };
 
 // Over the threads of a row: a warp, or the block (up to 512 threads); every thread gets the result, added up in the same order.
-// turn: 0 and 1 in turn from row to row (a thread may be a row ahead of the others, never two).
 template <bool WARP>
-__device__ __forceinline__ RowSums row_sums(float squares, uint32_t top, int turn) {
+__device__ __forceinline__ RowSums row_sums(float squares, uint32_t top) {
   squares = warp_sum(squares);
   top = __reduce_max_sync(0xffffffffu, top);
   RowSums r{squares, top};
   if (!WARP) {
-    __shared__ float red_s[2][16];
-    __shared__ uint32_t red_t[2][16];
+    __shared__ float red_s[16];
+    __shared__ uint32_t red_t[16];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = (blockDim.x + 31) >> 5;
-    if (lane == 0) red_s[turn][warp] = squares, red_t[turn][warp] = top;
+    if (nw == 1) return r;
+    if (lane == 0) red_s[warp] = squares, red_t[warp] = top;
     __syncthreads();
     r = RowSums{0.f, 0u};
-    for (int w = 0; w < nw; w++) r.squares += red_s[turn][w], r.top = max(r.top, red_t[turn][w]);
+    for (int w = 0; w < nw; w++) r.squares += red_s[w], r.top = max(r.top, red_t[w]);
   }
   return r;
 }
@@ -129,6 +129,8 @@ template <int V>
 __device__ __forceinline__ void store_eight(uint8_t* p, int n, const float (&v)[V]) {
   if (V == 8 && n >= V) {
     *reinterpret_cast<uint2*>(p) = make_uint2(f32x4_to_e4m3(v[0], v[1 % V], v[2 % V], v[3 % V]), f32x4_to_e4m3(v[4 % V], v[5 % V], v[6 % V], v[7 % V]));
+  } else if (V == 4 && n >= V) {
+    *reinterpret_cast<uint32_t*>(p) = f32x4_to_e4m3(v[0], v[1 % V], v[2 % V], v[3 % V]);
   } else {
 #pragma unroll
     for (int i = 0; i < V; i++)
@@ -136,204 +138,161 @@ __device__ __forceinline__ void store_eight(uint8_t* p, int n, const float (&v)[
   }
 }
 
-// CH pieces of V numbers a thread; ROWS > 1: a warp a row, that many rows at a time.  CH = 0: any width, the row read twice.
-// The blocks walk the rows; a row's loads go out before the row before it is rounded, so that memory is read while threads meet.
+// CH pieces of V numbers a thread; ROWS > 1: a warp a row, that many rows a block.  CH = 0: any width, the row read twice.
 template <typename TX, int V, int CH, int ROWS>
 __global__ void __launch_bounds__(512) quantize_kernel(uint8_t* __restrict__ q, float* __restrict__ scale, const TX* __restrict__ x, const int* __restrict__ rows,
-                                const float* __restrict__ weights, int div, int P, int M, int D, long long ldx, long long ldq) {
+                                                       const float* __restrict__ weights, int div, int P, int M, int D, long long ldx, long long ldq) {
   constexpr bool WARP = ROWS > 1;
-  const int tid = WARP ? threadIdx.x & 31 : threadIdx.x, T = WARP ? 32 : blockDim.x;
-  const int step = gridDim.x * ROWS;
-  int p = WARP ? blockIdx.x * ROWS + (threadIdx.x >> 5) : blockIdx.x;
-  pdl_wait();
-  if (CH == 0) {
-    for (int turn = 0; p < P; p += step, turn ^= 1) {
-      const long long m = source_row(rows, p, div, M);
-      const TX* xi = x + (m < 0 ? 0 : m) * ldx;
-      uint32_t top = m < 0 ? 0x7fffffffu : 0u;
-      for (int i = tid; i < (m < 0 ? 0 : D); i += T) top = max(top, magnitude(to_f32(xi[i])));
-      float inv, s;
-      row_factor(row_sums<WARP>(0.f, top, turn), inv, s);
-      if (tid == 0) scale[p] = weights && m >= 0 ? s * weights[rows[p]] : s;
-      uint8_t* o = q + p * ldq;
-      for (int i = tid; i < D; i += T) o[i] = f32_to_e4m3(m < 0 ? inv : to_f32(xi[i]) * inv);
-    }
-    return;
-  }
   constexpr int C = CH > 0 ? CH : 1;
-  Some<TX, V> next[C];
-  long long m_next = -1;
-  auto fetch = [&](int row) {
-    m_next = source_row(rows, row, div, M);
-    const TX* xi = x + (m_next < 0 ? 0 : m_next) * ldx;
-    const int width = m_next < 0 ? 0 : D;      // (a row that is not there: nothing is read)
+  const int tid = WARP ? threadIdx.x & 31 : threadIdx.x, T = WARP ? 32 : blockDim.x;
+  const int p = WARP ? blockIdx.x * ROWS + (threadIdx.x >> 5) : blockIdx.x;
+  pdl_wait();
+  if (p >= P) return;
+  const long long m = source_row(rows, p, div, M);
+  const TX* xi = x + (m < 0 ? 0 : m) * ldx;
+  const int width = m < 0 ? 0 : D;      // (a row that is not there: nothing is read)
+  uint32_t top = m < 0 ? 0x7fffffffu : 0u;
+  Some<TX, V> v[C];
+  if (CH > 0) {
 #pragma unroll
-    for (int c = 0; c < C; c++) next[c].load(xi + (tid + c * T) * V, width - (tid + c * T) * V);
-  };
-  if (p < P) fetch(p);
-  for (int turn = 0; p < P; p += step, turn ^= 1) {
-    Some<TX, V> now[C];
-    const long long m = m_next;
+    for (int c = 0; c < C; c++) v[c].load(xi + (tid + c * T) * V, width - (tid + c * T) * V);
 #pragma unroll
-    for (int c = 0; c < C; c++) now[c] = next[c];
-    if (p + step < P) fetch(p + step);
-    uint32_t top = m < 0 ? 0x7fffffffu : 0u;
-#pragma unroll
-    for (int c = 0; c < C; c++) top = max(top, now[c].top());
-    float inv, s;
-    row_factor(row_sums<WARP>(0.f, top, turn), inv, s);
-    if (tid == 0) scale[p] = weights && m >= 0 ? s * weights[rows[p]] : s;
-    uint8_t* o = q + p * ldq;
+    for (int c = 0; c < C; c++) top = max(top, v[c].top());
+  } else {
+    for (int i = tid; i < width; i += T) top = max(top, magnitude(to_f32(xi[i])));
+  }
+  float inv, s;
+  row_factor(row_sums<WARP>(0.f, top), inv, s);
+  if (tid == 0) scale[p] = weights && m >= 0 ? s * weights[rows[p]] : s;
+  uint8_t* o = q + p * ldq;
+  if (CH > 0) {
 #pragma unroll
     for (int c = 0; c < C; c++) {
-      float v[V];
+      float z[V];
 #pragma unroll
-      for (int i = 0; i < V; i++) v[i] = now[c].at(i) * inv;
-      store_eight<V>(o + (tid + c * T) * V, D - (tid + c * T) * V, v);
+      for (int i = 0; i < V; i++) z[i] = v[c].at(i) * inv;
+      store_eight<V>(o + (tid + c * T) * V, D - (tid + c * T) * V, z);
     }
+  } else {
+    for (int i = tid; i < D; i += T) o[i] = f32_to_e4m3(m < 0 ? inv : to_f32(xi[i]) * inv);
   }
 }
 
 template <typename TY, int V, int CH, int ROWS>
 __global__ void __launch_bounds__(512) rmsnorm_e4m3_kernel(uint8_t* __restrict__ q, float* __restrict__ scale, float* __restrict__ x, const float* __restrict__ w,
-                                    const TY* __restrict__ y, void* __restrict__ h, int h_dtype, int M, int D, float eps, long long ldq) {
+                                                           const TY* __restrict__ y, void* __restrict__ h, int h_dtype, int M, int D, float eps, long long ldq) {
   constexpr bool WARP = ROWS > 1;
-  const int tid = WARP ? threadIdx.x & 31 : threadIdx.x, T = WARP ? 32 : blockDim.x;
-  const int step = gridDim.x * ROWS;
-  int m = WARP ? blockIdx.x * ROWS + (threadIdx.x >> 5) : blockIdx.x;
-  pdl_wait();
-  auto finish = [&](RowSums t, float& inv, float& r) {
-    float s;
-    r = 1.0f / sqrtf(t.squares / (float)D + eps);
-    row_factor(t, inv, s);
-    if (tid == 0) scale[m] = s * r;
-  };
-  if (CH == 0) {
-    for (int turn = 0; m < M; m += step, turn ^= 1) {
-      const size_t at = (size_t)m * D;
-      float squares = 0.f, inv, r;
-      uint32_t top = 0u;
-      for (int i = tid; i < D; i += T) {
-        float a = x[at + i];
-        if (y) x[at + i] = a = a + to_f32(y[at + i]);
-        squares += a * a;
-        top = max(top, magnitude(a * w[i]));
-      }
-      finish(row_sums<WARP>(squares, top, turn), inv, r);
-      uint8_t* o = q + m * ldq;
-      for (int i = tid; i < D; i += T) {
-        const float a = x[at + i] * w[i];
-        o[i] = f32_to_e4m3(a * inv);
-        if (h && h_dtype == LEB_F32) ((float*)h)[at + i] = a * r;
-        else if (h) ((bf16*)h)[at + i] = from_f32<bf16>(a * r);
-      }
-    }
-    return;
-  }
   constexpr int C = CH > 0 ? CH : 1;
-  Some<float, V> next[C];
-  Some<TY, V> next_y[C];
-  auto fetch = [&](int row) {
-    const size_t at = (size_t)row * D;
+  const int tid = WARP ? threadIdx.x & 31 : threadIdx.x, T = WARP ? 32 : blockDim.x;
+  const int m = WARP ? blockIdx.x * ROWS + (threadIdx.x >> 5) : blockIdx.x;
+  pdl_wait();
+  if (m >= M) return;
+  const size_t at = (size_t)m * D;
+  float squares = 0.f;
+  uint32_t top = 0u;
+  Some<float, V> v[C];
+  if (CH > 0) {
 #pragma unroll
-    for (int c = 0; c < C; c++) next[c].load(x + at + (tid + c * T) * V, D - (tid + c * T) * V);
-    if (y)
+    for (int c = 0; c < C; c++) v[c].load(x + at + (tid + c * T) * V, D - (tid + c * T) * V);
+    if (y) {
+      Some<TY, V> b[C];
 #pragma unroll
-      for (int c = 0; c < C; c++) next_y[c].load(y + at + (tid + c * T) * V, D - (tid + c * T) * V);
-  };
-  if (m < M) fetch(m);
-  for (int turn = 0; m < M; m += step, turn ^= 1) {
-    const size_t at = (size_t)m * D;
-    float v[C][V];
+      for (int c = 0; c < C; c++) b[c].load(y + at + (tid + c * T) * V, D - (tid + c * T) * V);
 #pragma unroll
-    for (int c = 0; c < C; c++) {
+      for (int c = 0; c < C; c++) {
 #pragma unroll
-      for (int i = 0; i < V; i++) v[c][i] = y ? next[c].at(i) + next_y[c].at(i) : next[c].at(i);
-      if (y) store_some<V>(x + at + (tid + c * T) * V, D - (tid + c * T) * V, v[c]);
+        for (int i = 0; i < V; i++) v[c].v[i] += b[c].at(i);
+        store_some<V>(x + at + (tid + c * T) * V, D - (tid + c * T) * V, v[c].v);
+      }
     }
-    if (m + step < M) fetch(m + step);
-    float squares = 0.f, inv, r;
-    uint32_t top = 0u;
 #pragma unroll
     for (int c = 0; c < C; c++) {
       Some<float, V> f;
       f.load(w + (tid + c * T) * V, D - (tid + c * T) * V);
 #pragma unroll
       for (int i = 0; i < V; i++) {
-        squares += v[c][i] * v[c][i];
-        v[c][i] *= f.at(i);
-        top = max(top, magnitude(v[c][i]));
+        squares += v[c].v[i] * v[c].v[i];
+        v[c].v[i] *= f.v[i];
       }
+      top = max(top, v[c].top());
     }
-    finish(row_sums<WARP>(squares, top, turn), inv, r);
-    uint8_t* o = q + m * ldq;
+  } else {
+    for (int i = tid; i < D; i += T) {
+      float a = x[at + i];
+      if (y) x[at + i] = a = a + to_f32(y[at + i]);
+      squares += a * a;
+      top = max(top, magnitude(a * w[i]));
+    }
+  }
+  const RowSums t = row_sums<WARP>(squares, top);
+  const float r = 1.0f / sqrtf(t.squares / (float)D + eps);
+  float inv, s;
+  row_factor(t, inv, s);
+  if (tid == 0) scale[m] = s * r;
+  uint8_t* o = q + m * ldq;
+  if (CH > 0) {
 #pragma unroll
     for (int c = 0; c < C; c++) {
       const int i = (tid + c * T) * V;
       float z[V];
 #pragma unroll
-      for (int k = 0; k < V; k++) z[k] = v[c][k] * inv;
+      for (int k = 0; k < V; k++) z[k] = v[c].v[k] * inv;
       store_eight<V>(o + i, D - i, z);
       if (h) {
 #pragma unroll
-        for (int k = 0; k < V; k++) z[k] = v[c][k] * r;
+        for (int k = 0; k < V; k++) z[k] = v[c].v[k] * r;
         if (h_dtype == LEB_F32) store_some<V>((float*)h + at + i, D - i, z);
         else store_some<V>((bf16*)h + at + i, D - i, z);
       }
     }
+  } else {
+    for (int i = tid; i < D; i += T) {
+      const float a = x[at + i] * w[i];
+      o[i] = f32_to_e4m3(a * inv);
+      if (h && h_dtype == LEB_F32) ((float*)h)[at + i] = a * r;
+      else if (h) ((bf16*)h)[at + i] = from_f32<bf16>(a * r);
+    }
   }
 }
 
-// How a row of D numbers is shared out: GO(V, CH, ROWS, threads).
-#define ROW_SHAPES(wide, D)                \
-  if (wide) {                              \
-    if (D <= 256) GO(8, 1, 8, 256);        \
-    else if (D <= 512) GO(8, 2, 8, 256);   \
-    else if (D <= 1024) GO(8, 1, 1, 128);  \
-    else if (D <= 2048) GO(8, 1, 1, 256);  \
-    else if (D <= 4096) GO(8, 2, 1, 256);  \
-    else if (D <= 8192) GO(8, 2, 1, 512);  \
-    else if (D <= 16384) GO(8, 4, 1, 512); \
-    else GO(1, 0, 1, 512);                 \
-  } else {                                 \
-    if (D <= 128) GO(1, 4, 8, 256);        \
-    else if (D <= 1024) GO(1, 8, 1, 128);  \
-    else if (D <= 2048) GO(1, 8, 1, 256);  \
-    else if (D <= 4096) GO(1, 8, 1, 512);  \
-    else if (D <= 8192) GO(1, 16, 1, 512); \
-    else GO(1, 0, 1, 512);                 \
-  }
-
-// As many blocks as fit the SMs at once, or as there are rows for.
-template <typename... KArgs, typename... Args>
-int launch_rows(void (*kern)(KArgs...), int& resident, int at_a_time, int threads, int rows, cudaStream_t st, Args... args) {
-  if (resident == 0) {      // (the same for every caller, whoever is first)
-    int n = 0;
-    resident = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, threads, 0) == cudaSuccess && n > 0 ? n : 1;
-  }
-  const int blocks = ceil_div(rows, at_a_time), most = resident * sm_count();
-  return leb_launch(kern, dim3(blocks < most ? blocks : most), dim3(threads), 0, st, args...) == cudaSuccess ? 0 : 1;
-}
+// How rows of D numbers are shared out: GO(V, CH, ROWS, blocks, threads).  Few rows: many threads a row, whose loads are one trip to memory.
+// Many rows: few threads a row with many loads each, so that threads seldom wait for one another (8,191 bfloat16 rows of 8,192:
+// 512 threads with two pieces 54 us, FEWER_US).  CH_MANY pieces a thread at most then; four numbers a piece where rows begin anywhere.
+#define MANY_ROWS 1024
+#define ROW_SHAPES(wide, fours, D, rows, CH_MANY)                                          \
+  if (wide && D <= 256) GO(8, 1, 8, ceil_div(rows, 8), 256);                               \
+  else if (wide && D <= 512) GO(8, 2, 8, ceil_div(rows, 8), 256);                          \
+  else if (wide && rows >= MANY_ROWS && D <= 1024) GO(8, 4, 8, ceil_div(rows, 8), 256);    \
+  else if (wide && rows >= MANY_ROWS && D <= 256 * CH_MANY) GO(8, CH_MANY, 8, ceil_div(rows, 8), 256); \
+  else if (wide && rows >= MANY_ROWS && D <= 512 * CH_MANY) GO(8, CH_MANY, 1, rows, 64);   \
+  else if (wide && rows >= MANY_ROWS && D <= 1024 * CH_MANY) GO(8, CH_MANY, 1, rows, 128); \
+  else if (wide && rows >= MANY_ROWS && D <= 2048 * CH_MANY) GO(8, CH_MANY, 1, rows, 256); \
+  else if (wide && D <= 1024) GO(8, 1, 1, rows, 128);                                      \
+  else if (wide && D <= 2048) GO(8, 1, 1, rows, 256);                                      \
+  else if (wide && D <= 4096) GO(8, 1, 1, rows, 512);                                      \
+  else if (wide && D <= 8192) GO(8, 2, 1, rows, 512);                                      \
+  else if (wide && D <= 16384) GO(8, 4, 1, rows, 512);                                     \
+  else if (fours && D <= 512) GO(4, 4, 8, ceil_div(rows, 8), 256);                         \
+  else if (fours && D <= 2048) GO(4, 4, 1, rows, 128);                                     \
+  else if (fours && D <= 4096) GO(4, 4, 1, rows, 256);                                     \
+  else if (fours && D <= 8192) GO(4, 4, 1, rows, 512);                                     \
+  else if (fours && D <= 16384) GO(4, 8, 1, rows, 512);                                    \
+  else if (D <= 4096) GO(1, 8, 1, rows, 512);                                              \
+  else GO(1, 0, 1, rows, 512);
 
 template <typename TX>
-void launch_quantize(bool wide, uint8_t* q, float* scale, const TX* x, const int* rows, const float* weights, int div, int P, int M, int D, long long ldx,
-                     long long ldq, cudaStream_t st) {
-#define GO(V, CH, ROWS, threads)                                                                                                                     \
-  do {                                                                                                                                               \
-    static int resident = 0;                                                                                                                         \
-    launch_rows(quantize_kernel<TX, V, CH, ROWS>, resident, ROWS, threads, P, st, q, scale, x, rows, weights, div, P, M, D, ldx, ldq);              \
-  } while (0)
-  ROW_SHAPES(wide, D)
+void launch_quantize(bool wide, bool fours, uint8_t* q, float* scale, const TX* x, const int* rows, const float* weights, int div, int P, int M, int D,
+                     long long ldx, long long ldq, cudaStream_t st) {
+#define GO(V, CH, ROWS, blocks, threads) \
+  leb_launch(quantize_kernel<TX, V, CH, ROWS>, dim3(blocks), dim3(threads), 0, st, q, scale, x, rows, weights, div, P, M, D, ldx, ldq)
+  ROW_SHAPES(wide, fours, D, P, 8)
 #undef GO
 }
 template <typename TY>
-void launch_norm(bool wide, uint8_t* q, float* scale, float* x, const float* w, const TY* y, void* h, int h_dtype, int M, int D, float eps, long long ldq, cudaStream_t st) {
-#define GO(V, CH, ROWS, threads)                                                                                                                     \
-  do {                                                                                                                                               \
-    static int resident = 0;                                                                                                                         \
-    launch_rows(rmsnorm_e4m3_kernel<TY, V, CH, ROWS>, resident, ROWS, threads, M, st, q, scale, x, w, y, h, h_dtype, M, D, eps, ldq);               \
-  } while (0)
-  ROW_SHAPES(wide, D)
+void launch_norm(bool wide, bool fours, uint8_t* q, float* scale, float* x, const float* w, const TY* y, void* h, int h_dtype, int M, int D, float eps, long long ldq, cudaStream_t st) {
+#define GO(V, CH, ROWS, blocks, threads) \
+  leb_launch(rmsnorm_e4m3_kernel<TY, V, CH, ROWS>, dim3(blocks), dim3(threads), 0, st, q, scale, x, w, y, h, h_dtype, M, D, eps, ldq)
+  ROW_SHAPES(wide, fours, D, M, 4)
 #undef GO
 }
 
@@ -358,11 +317,11 @@ LEB_API int leb_quantize_e4m3(const void* packed, cudaStream_t st) {
   LEB_REQUIRE(a.D > 0 && a.D < MOST && a.P < MOST && a.M < MOST && a.div > 0 && a.div < MOST, "leb_quantize_e4m3: %lld rows out of %lld of %lld numbers, %lld places to a row", a.P, a.M, a.D, a.div);
   LEB_REQUIRE(a.rows || (a.P == a.M && !a.weights), "leb_quantize_e4m3: %lld rows out of %lld need a list of them", a.P, a.M);
   LEB_REQUIRE(a.x_dtype == LEB_F32 || a.x_dtype == LEB_BF16, "leb_quantize_e4m3: unknown type of x %lld", a.x_dtype);
-  const bool wide = (a.x & 15) == 0 && a.ldx % (a.x_dtype == LEB_F32 ? 4 : 8) == 0 && (a.q & 7) == 0 && a.ldq % 8 == 0;
+  const bool wide = (a.x & 15) == 0 && a.ldx % (a.x_dtype == LEB_F32 ? 4 : 8) == 0 && (a.q & 7) == 0 && a.ldq % 8 == 0, fours = (a.q & 3) == 0 && a.ldq % 4 == 0;
   if (a.x_dtype == LEB_F32)
-    launch_quantize(wide, (uint8_t*)a.q, (float*)a.scale, (const float*)a.x, (const int*)a.rows, (const float*)a.weights, (int)a.div, (int)a.P, (int)a.M, (int)a.D, a.ldx, a.ldq, st);
+    launch_quantize(wide, fours, (uint8_t*)a.q, (float*)a.scale, (const float*)a.x, (const int*)a.rows, (const float*)a.weights, (int)a.div, (int)a.P, (int)a.M, (int)a.D, a.ldx, a.ldq, st);
   else
-    launch_quantize(wide, (uint8_t*)a.q, (float*)a.scale, (const bf16*)a.x, (const int*)a.rows, (const float*)a.weights, (int)a.div, (int)a.P, (int)a.M, (int)a.D, a.ldx, a.ldq, st);
+    launch_quantize(wide, fours, (uint8_t*)a.q, (float*)a.scale, (const bf16*)a.x, (const int*)a.rows, (const float*)a.weights, (int)a.div, (int)a.P, (int)a.M, (int)a.D, a.ldx, a.ldq, st);
   LEB_CHECK_LAUNCH("leb_quantize_e4m3");
   return 0;
 }
@@ -373,11 +332,11 @@ LEB_API int leb_rmsnorm_e4m3(const void* packed, cudaStream_t st) {
   if (a.M <= 0) return 0;
   LEB_REQUIRE(a.D > 0 && a.D < MOST && a.M < MOST, "leb_rmsnorm_e4m3: %lld rows of %lld numbers", a.M, a.D);
   LEB_REQUIRE((a.y_dtype == LEB_F32 || a.y_dtype == LEB_BF16) && (a.h_dtype == LEB_F32 || a.h_dtype == LEB_BF16), "leb_rmsnorm_e4m3: unknown type of y (%lld) or h (%lld)", a.y_dtype, a.h_dtype);
-  const bool wide = a.D % 8 == 0 && ((a.x | a.w | a.y | a.h) & 15) == 0 && (a.q & 7) == 0 && a.ldq % 8 == 0;
+  const bool wide = a.D % 8 == 0 && ((a.x | a.w | a.y | a.h) & 15) == 0 && (a.q & 7) == 0 && a.ldq % 8 == 0, fours = (a.q & 3) == 0 && a.ldq % 4 == 0;
   if (a.y_dtype == LEB_F32)
-    launch_norm(wide, (uint8_t*)a.q, (float*)a.scale, (float*)a.x, (const float*)a.w, (const float*)a.y, (void*)a.h, (int)a.h_dtype, (int)a.M, (int)a.D, (float)a.eps, a.ldq, st);
+    launch_norm(wide, fours, (uint8_t*)a.q, (float*)a.scale, (float*)a.x, (const float*)a.w, (const float*)a.y, (void*)a.h, (int)a.h_dtype, (int)a.M, (int)a.D, (float)a.eps, a.ldq, st);
   else
-    launch_norm(wide, (uint8_t*)a.q, (float*)a.scale, (float*)a.x, (const float*)a.w, (const bf16*)a.y, (void*)a.h, (int)a.h_dtype, (int)a.M, (int)a.D, (float)a.eps, a.ldq, st);
+    launch_norm(wide, fours, (uint8_t*)a.q, (float*)a.scale, (float*)a.x, (const float*)a.w, (const bf16*)a.y, (void*)a.h, (int)a.h_dtype, (int)a.M, (int)a.D, (float)a.eps, a.ldq, st);
   LEB_CHECK_LAUNCH("leb_rmsnorm_e4m3");
   return 0;
 }
