@@ -2289,19 +2289,24 @@ def _vector(name: str, t: torch.Tensor, dtype: torch.dtype, shape: tuple) -> Non
         raise KernelError(f"{name}: expected contiguous {dtype} {shape}, got {t.dtype} {tuple(t.shape)}")
 
 
-def _pitch(name: str, t: torch.Tensor, M: int, K: int, written: bool = False) -> int:
-    """How far the rows of a matrix [M, K] (or of each of a stack) of neighbouring numbers lie apart; rows that are written do not overlap."""
-    *_, m, k = t.shape
-    if m != M or k != K:
-        raise KernelError(f"{name}: expected {(M, K)}, got {tuple(t.shape)}")
+def _pitch(name: str, t: torch.Tensor, shape: tuple, written: bool = False) -> int:
+    """How far the rows of a matrix of neighbouring numbers (or of each of a stack of them) lie apart; rows that are written do not overlap."""
+    if t.shape != shape:
+        raise KernelError(f"{name}: expected {shape}, got {tuple(t.shape)}")
     *_, step, inner = t.stride()
+    K = shape[-1]
     if inner != 1 and K > 1:
         raise KernelError(f"{name}: the numbers of a row must be neighbours, they are {inner} apart")
-    if M <= 1:      # (where a row behind the only one would lie)
+    if shape[-2] <= 1:      # (where a row behind the only one would lie)
         return -(-K // 16) * 16
     if written and step < K:
         raise KernelError(f"{name}: rows of {K} numbers that are {step} apart overlap")
     return step
+
+
+def _stream_on(device: int) -> int:
+    """The current stream of the current device, whose number the caller has at hand."""
+    return _raw_stream(device) if _raw_stream is not None else _stream()
 
 
 def quantize_e4m3(out: torch.Tensor, scale: torch.Tensor, x: torch.Tensor, rows: torch.Tensor | None = None, div: int = 1,
@@ -2318,7 +2323,7 @@ def quantize_e4m3(out: torch.Tensor, scale: torch.Tensor, x: torch.Tensor, rows:
         raise KernelError(f"quantize_e4m3: expected rows of {E4M3} out of a matrix, got {out.dtype} {tuple(out.shape)} out of {tuple(x.shape)}")
     M, K = x.shape
     P_ = out.shape[0]
-    ldx, ldq = _pitch("quantize_e4m3.x", x, M, K), _pitch("quantize_e4m3.out", out, P_, K, True)
+    ldx, ldq = _pitch("quantize_e4m3.x", x, (M, K)), _pitch("quantize_e4m3.out", out, (P_, K), True)
     _vector("quantize_e4m3.scale", scale, torch.float32, (P_,))
     if rows is not None:
         _vector("quantize_e4m3.rows", rows, torch.int32, (P_,))
@@ -2335,7 +2340,7 @@ def quantize_e4m3(out: torch.Tensor, scale: torch.Tensor, x: torch.Tensor, rows:
         raise KernelError("quantize_e4m3: rows without numbers have no scale")
     _check(lib().leb_quantize_e4m3(
         _PACK_QUANTIZE(out.data_ptr(), scale.data_ptr(), x.data_ptr(), dtype, 0 if rows is None else rows.data_ptr(),
-                       0 if weights is None else weights.data_ptr(), div, P_, M, K, ldx, ldq), _stream()))
+                       0 if weights is None else weights.data_ptr(), div, P_, M, K, ldx, ldq), _stream_on(here)))
 
 
 def rmsnorm_e4m3(out: torch.Tensor, scale: torch.Tensor, x: torch.Tensor, w: torch.Tensor, eps: float, y: torch.Tensor | None = None,
@@ -2353,7 +2358,7 @@ def rmsnorm_e4m3(out: torch.Tensor, scale: torch.Tensor, x: torch.Tensor, w: tor
     if out.dtype is not E4M3 or out.dim() != 2:
         raise KernelError(f"rmsnorm_e4m3.out: expected rows of {E4M3}, got {out.dtype} {tuple(out.shape)}")
     M, D = shape = x.shape
-    ldq = _pitch("rmsnorm_e4m3.out", out, M, D, True)
+    ldq = _pitch("rmsnorm_e4m3.out", out, shape, True)
     _vector("rmsnorm_e4m3.scale", scale, torch.float32, (M,))
     _vector("rmsnorm_e4m3.w", w, torch.float32, (D,))
     yd = hd = F32
@@ -2371,7 +2376,7 @@ def rmsnorm_e4m3(out: torch.Tensor, scale: torch.Tensor, x: torch.Tensor, w: tor
         raise KernelError("rmsnorm_e4m3: rows without numbers have no norm")
     _check(lib().leb_rmsnorm_e4m3(
         _PACK_NORM(out.data_ptr(), scale.data_ptr(), x.data_ptr(), w.data_ptr(), 0 if y is None else y.data_ptr(), yd,
-                   0 if h is None else h.data_ptr(), hd, M, D, ldq, eps), _stream()))
+                   0 if h is None else h.data_ptr(), hd, M, D, ldq, eps), _stream_on(here)))
 
 
 def linear_e4m3(out: torch.Tensor, x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, epilogue: int = STORE,
@@ -2395,20 +2400,20 @@ def linear_e4m3(out: torch.Tensor, x: torch.Tensor, x_scale: torch.Tensor, w: to
         if w.dim() != 2:
             raise KernelError(f"linear_e4m3: w is {tuple(w.shape)} without groups of rows")
         N, E, stride, offsets = w.shape[0], 1, 0, 0
-        ldw, scales = _pitch("linear_e4m3.w", w, N, K), (N,)
+        ldw, scales = _pitch("linear_e4m3.w", w, (N, K)), (N,)
     else:
         if w.dim() != 3:
             raise KernelError(f"linear_e4m3: w is {tuple(w.shape)} for groups of rows")
         E, N = w.shape[:2]
         _vector("linear_e4m3.group_offsets", group_offsets, torch.int32, (E + 1,))
-        ldw, scales, offsets = _pitch("linear_e4m3.w", w, N, K), (E, N), group_offsets.data_ptr()
+        ldw, scales, offsets = _pitch("linear_e4m3.w", w, (E, N, K)), (E, N), group_offsets.data_ptr()
         stride = w.stride(0) if E > 1 else N * ldw
     _vector("linear_e4m3.w_scale", w_scale, torch.float32, scales)
     _vector("linear_e4m3.x_scale", x_scale, torch.float32, (M,))
     gated = (epilogue & 255) == SWIGLU
     if gated and N % 32:
         raise KernelError(f"linear_e4m3: gate and up rows come in blocks of 16 each, w has {N} rows")
-    ldx, ldc = _pitch("linear_e4m3.x", x, M, K), _pitch("linear_e4m3.out", out, M, N // 2 if gated else N, True)
+    ldx, ldc = _pitch("linear_e4m3.x", x, (M, K)), _pitch("linear_e4m3.out", out, (M, N // 2 if gated else N), True)
     dtype = _DT.get(out.dtype, -1)
     if dtype < 0 or (epilogue == ACCUMULATE and dtype != F32):
         raise KernelError(f"linear_e4m3: out is {out.dtype}; float or bfloat16 is wanted, and float where sums are added")
@@ -2416,9 +2421,12 @@ def linear_e4m3(out: torch.Tensor, x: torch.Tensor, x_scale: torch.Tensor, w: to
         return
     if K == 0:
         raise KernelError("linear_e4m3: an inner size of 0")
+    status = _tc_status.get(here)
+    if status is None:
+        status = _status_word(x.device)
     _check(lib().leb_linear_e4m3(
         _PACK_LINEAR(out.data_ptr(), dtype, x.data_ptr(), x_scale.data_ptr(), w.data_ptr(), w_scale.data_ptr(), M, N, K, ldx, ldw, ldc, epilogue,
-                     offsets, E, stride, _status_word(x.device).data_ptr()), _stream()))
+                     offsets, E, stride, status.data_ptr()), _stream_on(here)))
 
 
 # set by ops.tc_gemm when the tensor-core (tcgen05) kernel is present

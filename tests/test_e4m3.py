@@ -24,7 +24,7 @@ def calls(monkeypatch):
     monkeypatch.setattr(K, "lib", lambda: types.SimpleNamespace(**{n: record(n, f) for n, f in forms.items()}))
     monkeypatch.setattr(K, "_not_here", lambda *a, **k: None)
     monkeypatch.setattr(K, "_status_word", lambda device: torch.zeros(1, dtype=torch.int32))
-    monkeypatch.setattr(K, "_stream", lambda: 0)
+    monkeypatch.setattr(K, "_stream_on", lambda device: 0)
     return got
 
 
@@ -141,7 +141,7 @@ def test_a_refusal_of_the_library_is_raised(monkeypatch):
     """Epilogues that only the library knows to be wrong: its message becomes the error, nothing is launched."""
     monkeypatch.setattr(K, "_not_here", lambda *a, **k: None)
     monkeypatch.setattr(K, "_status_word", lambda device: torch.zeros(1, dtype=torch.int32))
-    monkeypatch.setattr(K, "_stream", lambda: 0)
+    monkeypatch.setattr(K, "_stream_on", lambda device: 0)
     for epilogue, out in ((3, torch.zeros(4, 64)), (K.ACCUMULATE | (1 << 8), torch.zeros(4, 64)), (K.plain_act_epilogue(0), torch.zeros(4, 64)), (K.SWIGLU | (9 << 8), torch.zeros(4, 32))):
         with pytest.raises(K.KernelError, match="epilogue"):
             linear(out, epilogue=epilogue)
