@@ -50,6 +50,14 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t* v) {
 __device__ __forceinline__ void e8_cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
+#ifndef E8_PATIENT      // (the tests build kernels whose waits give up now and then, also before their first try)
+#define E8_PATIENT 1
+#endif
+// mbar_wait_warp: a bounded wait of all lanes of a warp together
+__device__ __forceinline__ bool e8_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+  if (E8_PATIENT) return mbar_wait_warp(bar, parity, abort_flag);
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag)) != 0;
+}
 // Whether all of the THREADS that share barrier 1 say so: they meet, and go on or leave together.
 template <int THREADS>
 __device__ __forceinline__ bool e8_all(bool ok) {
@@ -63,6 +71,22 @@ __device__ __forceinline__ bool e8_all(bool ok) {
       : "r"(ok ? 1u : 0u), "n"(THREADS)
       : "memory");
   return all != 0;
+}
+// A block that gave up stays until copies that it asked for have landed: a phase's end, or some milliseconds (copies land within microseconds;
+// a phase that a partner's copies belong to may never end).
+__device__ __forceinline__ void e8_passed(uint64_t* bar, int phase) {
+  for (int n = 0; n < 1 << 14; n++) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(phase & 1)
+        : "memory");
+    if (ok) return;
+    __nanosleep(64);
+  }
 }
 __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");

@@ -176,7 +176,7 @@ gemm_e4m3_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
       int m0, m_end, n0, e;
       place(tile, m0, m_end, n0, e);
       for (int kb = 0; kb < my_nk; kb++) {
-        if (!mbar_wait_warp(&empty[s], ph, abort_flag)) { ok = false; break; }
+        if (!e8_wait(&empty[s], ph, abort_flag)) { ok = false; break; }
         if (elect_lane()) {
           mbar_expect_tx(&full[s], W_BYTES + A_BYTES);
           tma_load_2d(s_w + s * W_BYTES, &map_w, &full[s], (kb_lo + kb) * E8_BK, e * N + n0);
@@ -197,11 +197,11 @@ gemm_e4m3_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
     int role = 0;
     for (int tile = first; tile < num_tiles && !role; tile += step, t++) {
       const uint32_t buf = t & 1;
-      if (!mbar_wait_warp(&acc_empty[buf], ((t >> 1) & 1) ^ 1, abort_flag)) { role = 54; break; }
+      if (!e8_wait(&acc_empty[buf], ((t >> 1) & 1) ^ 1, abort_flag)) { role = 54; break; }
       tc_fence_after();
       const uint32_t d_tmem = tmem_acc + buf * MP;
       for (int kb = 0; kb < my_nk; kb++) {
-        if (!mbar_wait_warp(&full[s], ph, abort_flag)) { role = 52; break; }
+        if (!e8_wait(&full[s], ph, abort_flag)) { role = 52; break; }
         tc_fence_after();
         if (elect_lane()) {
           const uint64_t dw = w_desc + (uint64_t)(s * (W_BYTES / 16)), da = a_desc + (uint64_t)(s * (A_BYTES / 16));
@@ -229,7 +229,7 @@ gemm_e4m3_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
       const int rows = min(MP, m_end - m0);
       if (tid < rows) sa_s[buf][tid] = sa[m0 + tid];
       if (my_nk > 0) {
-        const bool ok = mbar_wait_warp(&acc_full[buf], (t >> 1) & 1, abort_flag);
+        const bool ok = e8_wait(&acc_full[buf], (t >> 1) & 1, abort_flag);
         if (!ok) {
           if (lane == 0) atomicExch(status, 53);
           gave_up = true;
@@ -278,15 +278,12 @@ gemm_e4m3_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
   tc_fence_before();
   __syncthreads();
   if (abort_s) {      // a role gave up: the copies asked for land and the products end before the block does (else every one has been waited for)
-    auto passed = [](uint64_t* bar, int phase) {
-      for (int n = 0; n < 1 << 16 && !mbar_try_wait(bar, phase & 1); n++) {}
-    };
     if (threadIdx.x == 0) {
-      for (int i = max(sent_s - STAGES, 0); i < sent_s; i++) passed(&full[i % STAGES], i / STAGES);
+      for (int i = max(sent_s - STAGES, 0); i < sent_s; i++) e8_passed(&full[i % STAGES], i / STAGES);
     } else if (warp == 1) {
       if (elect_lane()) {
         umma_commit(&drained);
-        passed(&drained, 0);
+        e8_passed(&drained, 0);
       }
       __syncwarp();
     }

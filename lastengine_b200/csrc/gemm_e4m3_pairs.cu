@@ -130,6 +130,14 @@ gemm_e4m3_pairs_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
     n0 = nt * 256;
   };
 
+  // a role that gives up says so to both blocks, whose roles then leave at their next wait
+  auto gives_up = [&](int code) {
+    if (lane == 0) {
+      atomicExch(status, code);
+      asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(e8_map_to_rank(smem_u32(&abort_s), rank ^ 1)), "r"(1) : "memory");
+    }
+  };
+
   if (warp == 0) {
     const uint32_t full0 = e8_map_to_rank(smem_u32(&full[0]), 0);
     uint32_t s = 0, ph = 1;
@@ -141,7 +149,7 @@ gemm_e4m3_pairs_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
       const int w0 = e * N + n0 + 128 * (int)rank;
       int kk = n0 / 256 * 5 % nk;      // tiles that share rows of A start at different k
       for (int kb = 0; kb < nk; kb++) {
-        if (!mbar_wait_warp(&empty[s], ph, abort_flag)) { ok = false; break; }
+        if (!e8_wait(&empty[s], ph, abort_flag)) { ok = false; break; }
         if (elect_lane()) {
           if (rank == 0) mbar_expect_tx(&full[s], 4 * HALF);
           pair_load_2d(s_a + s * HALF, &map_a, full0 + s * 8, kk * E8_BK, m0);
@@ -153,10 +161,8 @@ gemm_e4m3_pairs_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
         if (++s == STAGES) s = 0, ph ^= 1;
       }
     }
-    if (lane == 0) {
-      sent_s = sent;
-      if (!ok) atomicExch(status, 61);
-    }
+    if (lane == 0) sent_s = sent;
+    if (!ok) gives_up(61);
   } else if (warp == 1) {
     if (rank == 0) {
       const uint64_t a_desc = make_desc(smem_u32(s_a)), w_desc = make_desc(smem_u32(s_w));
@@ -164,11 +170,11 @@ gemm_e4m3_pairs_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
       int gave_up = 0;
       for (int tile = pair; tile < num_tiles && !gave_up; tile += n_pairs, t++) {
         const uint32_t buf = t & 1;
-        if (!mbar_wait_warp(&acc_empty[buf], ((t >> 1) & 1) ^ 1, abort_flag)) { gave_up = 64; break; }
+        if (!e8_wait(&acc_empty[buf], ((t >> 1) & 1) ^ 1, abort_flag)) { gave_up = 64; break; }
         tc_fence_after();
         const uint32_t d_tmem = tmem_acc + buf * 256;
         for (int kb = 0; kb < nk; kb++) {
-          if (!mbar_wait_warp(&full[s], ph, abort_flag)) { gave_up = 62; break; }
+          if (!e8_wait(&full[s], ph, abort_flag)) { gave_up = 62; break; }
           tc_fence_after();
           if (elect_lane()) {
             const uint64_t da = a_desc + (uint64_t)(s * (HALF / 16)), dw = w_desc + (uint64_t)(s * (HALF / 16));
@@ -181,7 +187,7 @@ gemm_e4m3_pairs_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
           if (++s == STAGES) s = 0, ph ^= 1;
         }
       }
-      if (gave_up && lane == 0) atomicExch(status, gave_up);
+      if (gave_up) gives_up(gave_up);
     }
   } else {
     const int quad = warp & 3, half = (warp - 2) >> 2;      // rows 32 quad, columns 128 half
@@ -205,9 +211,9 @@ gemm_e4m3_pairs_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
       const float sam = row0 + lane < m_end ? sa[row0 + lane] : 0.f;
       // (the other buffer may still be read: a tile has one barrier, so nobody is two tiles ahead; the warps leave together)
       if (!e8_all<256>(!gave_up)) break;
-      const bool ok = mbar_wait_warp(&acc_full[buf], (t >> 1) & 1, abort_flag);
+      const bool ok = e8_wait(&acc_full[buf], (t >> 1) & 1, abort_flag);
       if (!ok) {
-        if (lane == 0) atomicExch(status, 63);
+        gives_up(63);
         gave_up = true;
         continue;
       }
@@ -326,15 +332,12 @@ gemm_e4m3_pairs_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
   e8_cluster_sync();      // both blocks are through: nobody frees tensor memory or leaves while the other may still use it
   const bool left = abort_s | remote_int(e8_map_to_rank(smem_u32(&abort_s), rank ^ 1));
   if (left) {      // the copies asked for land and the products end first (else every one has been waited for)
-    auto passed = [](uint64_t* bar, int phase) {
-      for (int n = 0; n < 1 << 16 && !mbar_try_wait(bar, phase & 1); n++) {}
-    };
     if (rank == 0 && threadIdx.x == 0) {
-      for (int i = max(sent_s - STAGES, 0); i < sent_s; i++) passed(&full[i % STAGES], i / STAGES);
+      for (int i = max(sent_s - STAGES, 0); i < sent_s; i++) e8_passed(&full[i % STAGES], i / STAGES);
     } else if (rank == 0 && warp == 1) {
       if (elect_lane()) {
         pair_commit(&drained);
-        passed(&drained, 0);
+        e8_passed(&drained, 0);
       }
     }
     __syncthreads();
