@@ -171,7 +171,7 @@ def cmd_generate(a) -> int:
     from . import Engine, SamplingParams
     prompts = [parse_ids(p) for p in a.prompt_ids]
     need = sum(-(-(len(p) + a.max_new_tokens) // 64) * 64 for p in prompts)
-    kw = dict(dtype=a.dtype, max_tokens=max(need, 64), max_seqs=len(prompts))
+    kw = dict(dtype=a.dtype, max_tokens=max(need, 64), max_seqs=len(prompts), ffn_dtype=a.ffn_dtype)
     if a.model:
         eng = Engine.from_pretrained(a.model, **kw)
     elif a.config:
@@ -259,6 +259,7 @@ def build_parser() -> argparse.ArgumentParser:
     p.add_argument("--seed", type=int, default=None)
     p.add_argument("--stop-token-id", type=int, action="append", default=None,
                    help="ends a request (not emitted); default: the model's eos_token_id")
+    p.add_argument("--ffn-dtype", choices=["e4m3"], default=None, help="matrices of feed-forwards and experts in 8 bits")
     common(p)
     p.set_defaults(fn=cmd_generate)
 

@@ -53,9 +53,14 @@ class EngineOptions:
     use_graphs: bool = True            # decode steps of `generate` as captured CUDA graphs
     seed: int | None = None            # sampling seed for calls whose SamplingParams name none
     device: str = "cuda:0"
+    ffn_dtype: str | None = None       # "e4m3": matrices of feed-forwards and experts in 8 bits (None: in `dtype`)
 
     def __post_init__(self):
-        resolve_dtype(self.dtype)
+        dtype = resolve_dtype(self.dtype)
+        if self.ffn_dtype not in (None, "e4m3"):
+            raise ValueError(f"unknown feed-forward dtype '{self.ffn_dtype}' (e4m3, or None for the engine's dtype)")
+        if self.ffn_dtype is not None and dtype != torch.bfloat16:
+            raise ValueError(f"feed-forwards in {self.ffn_dtype} go with a bfloat16 engine, not {self.dtype}")
         if self.max_tokens < 1 or (self.max_seqs is not None and self.max_seqs < 1) or self.max_batch_tokens < 0:
             raise ValueError(f"engine options out of range: {self}")
 
@@ -89,7 +94,7 @@ class Engine:
         self.dtype = resolve_dtype(dtype)
         self.plan = plan
         self.workspace = Workspace(dev)
-        self.env = BuildEnv(device=dev, dtype=self.dtype, workspace=self.workspace)
+        self.env = BuildEnv(device=dev, dtype=self.dtype, workspace=self.workspace, ffn_e4m3=opt.ffn_dtype == "e4m3")
         self.model = Model(plan, self.env)
         self.max_tokens = int(max_tokens)
         self.cache = Cache(self.model.cache_specs(), max_tokens=self.max_tokens, max_seqs=max_seqs,

@@ -237,6 +237,7 @@ class BuildEnv:
     split_in: Any = None
     split_out: Any = None
     next_block_norm: Any = None        # the norm that reads the residual after this block (set by the model)
+    ffn_e4m3: bool = False             # feed-forwards and experts keep their matrices in 8 bits (with bfloat16)
 
     def take_split_in(self):
         s, self.split_in = self.split_in, None
@@ -296,6 +297,8 @@ class Mixer(Part):
 
 
 class FeedForward(Part):
+    reads_e4m3 = False     # True: forward() takes its rows in 8 bits too (parts.ffn.EightBitRows), as a norm may leave them
+
     def forward(self, h, out, accumulate, batch, env) -> None:
         raise NotImplementedError
 

@@ -24,6 +24,7 @@ import torch
 
 from ..ops import kernels
 from ..registry import BLOCKS
+from .ffn import eight_bit_room
 
 
 @BLOCKS.register("pre_norm_residual")
@@ -62,14 +63,18 @@ class PreNormResidualBlock:
         env.split_out = sp
         return sp
 
-    def _normed(self, norm, x, pending, env):
+    def _normed(self, norm, x, pending, env, reader=None):
         """norm(x) as the next part's input: the split's values (the part scales its first product),
-        or the norm kernel's result."""
+        or the norm kernel's result, in 8 bits for a `reader` that takes them."""
         env.split_in = env.split_out = None   # nothing is left over from a part that did not take its offer (or raised)
         if pending is not None and pending.filled and pending.weight is norm.weight:
             env.split_in = pending
             return pending.values
         M, D = x.shape
+        if getattr(reader, "reads_e4m3", False) and getattr(norm, "splittable", False):
+            h = eight_bit_room(env.workspace, "block.h8", M, D)
+            kernels.rmsnorm_e4m3(h.values, h.scale, x, norm.weight, norm.eps)
+            return h
         h = env.workspace.get("block.h", (M, D), env.dtype)
         kernels.guarded(norm.forward)(h, x)
         return h
@@ -90,7 +95,7 @@ class PreNormResidualBlock:
             kernels.guarded(self.mixer.forward)(h, t, False, batch, cache, env)
             kernels.guarded(self.post_mixer_norm.forward)(x, t, add=True)
         env.split_in = None
-        h = self._normed(self.ffn_norm, x, mid, env)
+        h = self._normed(self.ffn_norm, x, mid, env, self.ffn)
         if self.post_ffn_norm is None:
             nxt = env.next_block_norm
             last = None

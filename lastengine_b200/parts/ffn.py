@@ -11,8 +11,14 @@ the lower index; the bias chooses, it does not weigh); weight s_e, divided by th
 chosen when norm_topk, times the scaling factor; f = sum_e weight_e * expert_e(h).  The
 reference's own lfm3 has no experts (src/dense.rs:187-191); its other architecture routes by
 softmax and adds a shared expert (src/cpu_ref.rs:239-263), which this is not.
+
+In 8 bits (`BuildEnv.ffn_e4m3`, bfloat16 models): the matrices are kept as rows of e4m3 numbers with a scale each, and what they
+multiply is brought to that form row by row: the block's norm leaves it so for a dense feed-forward (`reads_e4m3`), experts' rows are
+brought to 8 bits as they are gathered, and the activation's results before the last product.  Routers, biases and norms stay as they are.
 """
 from __future__ import annotations
+
+from typing import NamedTuple
 
 import torch
 
@@ -29,6 +35,36 @@ def fuse_gate_up(w1: torch.Tensor, w3: torch.Tensor, interleave: bool) -> torch.
     g = w1.reshape(F_ // 16, 16, D)
     u = w3.reshape(F_ // 16, 16, D)
     return torch.stack([g, u], dim=1).reshape(2 * F_, D).contiguous()
+
+
+class EightBitRows(NamedTuple):
+    """Rows of 8-bit numbers and their scales, as ops.kernels.linear_e4m3 takes them."""
+    values: torch.Tensor      # [rows, K] e4m3
+    scale: torch.Tensor       # [rows] float
+
+
+def eight_bit_room(ws, name: str, rows: int, K: int) -> EightBitRows:
+    """Scratch for such rows, 16 bytes (or a multiple of that) apart."""
+    v = ws.get(name, (rows, -(-K // 16) * 16), kernels.E4M3)
+    return EightBitRows(v if v.shape[1] == K else v[:, :K], ws.get(name + ".scale", (rows,), torch.float32))
+
+
+def eight_bit_weights(w: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """Weights [..., N, K] in 8 bits and the scales [..., N] of their rows."""
+    *lead, K = w.shape
+    n = w.numel() // K
+    q, scale = kernels.e4m3_rows(n, K, device=w.device), torch.empty(n, dtype=torch.float32, device=w.device)
+    kernels.quantize_e4m3(q, scale, w.reshape(n, K))
+    return q.unflatten(0, lead), scale.view(lead)
+
+
+def _eight(h, ws, name: str) -> EightBitRows:
+    """h in 8 bits: as the block's norm left it, or brought to them here."""
+    if isinstance(h, EightBitRows):
+        return h
+    r = eight_bit_room(ws, name, *h.shape)
+    kernels.quantize_e4m3(r.values, r.scale, h)
+    return r
 
 
 _ACTIVATIONS = {"silu": kernels.SILU, "gelu_tanh": kernels.GELU_TANH, "clamped_sigmoid": kernels.CLAMPED_SIGMOID}
@@ -54,7 +90,7 @@ class SwiGLU(FeedForward):
         self.act = _ACTIVATIONS[activation]
         self.limit, self.alpha = float(limit), float(alpha)
         self.n_gate, self.n_up, self.n_down = (str(n) for n in names)
-        self.w13 = self.w2 = None
+        self.w13 = self.w2 = self.s13 = self.s2 = None
         self.fused = False
 
     def tensors(self) -> dict[str, TensorSpec]:
@@ -65,14 +101,34 @@ class SwiGLU(FeedForward):
     def load(self, tensors, env: BuildEnv) -> None:
         # the gated epilogue with this part's activation (None: the activation has no fused form)
         self.epilogue = kernels.gated_epilogue(self.act, self.limit, self.alpha)
-        self.fused = (not env.is_float32) and self.F % 16 == 0 and self.D % 8 == 0 and self.epilogue is not None
+        self.fused = (not env.is_float32) and self.F % 16 == 0 and (self.D % 8 == 0 or env.ffn_e4m3) and self.epilogue is not None
         self.w13 = fuse_gate_up(tensors[self.n_gate], tensors[self.n_up], self.fused)
         self.w2 = tensors[self.n_down].contiguous()
+        if env.ffn_e4m3:
+            self.w13, self.s13 = eight_bit_weights(self.w13)
+            self.w2, self.s2 = eight_bit_weights(self.w2)
+            self.split_norm, self.reads_e4m3 = False, True
 
     def split_reader_weight(self):
         return self.w13
 
+    def _forward_eight(self, h, out, accumulate, env) -> None:
+        ws = env.workspace
+        h = _eight(h, ws, "ffn.h8")
+        M = h.values.shape[0]
+        a = ws.get("ffn.a", (M, self.F), env.dtype)
+        if self.fused:
+            kernels.linear_e4m3(a, *h, self.w13, self.s13, self.epilogue)
+        else:
+            gu = ws.get("ffn.gu", (M, 2 * self.F), torch.float32)
+            kernels.linear_e4m3(gu, *h, self.w13, self.s13)
+            kernels.gated_act(a, gu, self.act, self.limit, self.alpha)
+        kernels.linear_e4m3(out, *_eight(a, ws, "ffn.a8"), self.w2, self.s2, kernels.ACCUMULATE if accumulate else kernels.STORE)
+
     def forward(self, h, out, accumulate, batch, env) -> None:
+        if self.s13 is not None:
+            self._forward_eight(h, out, accumulate, env)
+            return
         M = h.shape[0]
         ws = env.workspace
         scale, emit = env.take_split_in(), env.take_split_out()
@@ -104,7 +160,7 @@ class DenseFeedForward(FeedForward):
         self.D, self.F = int(hidden_size), int(intermediate_size)
         self.act = kernels.PLAIN_ACTIVATIONS[activation]
         self.n_up, self.n_down = (str(n) for n in names)
-        self.w1 = self.w2 = None
+        self.w1 = self.w2 = self.s1 = self.s2 = None
 
     def tensors(self) -> dict[str, TensorSpec]:
         return {self.n_up: TensorSpec((self.F, self.D), MATRIX), self.n_down: TensorSpec((self.D, self.F), MATRIX)}
@@ -112,10 +168,20 @@ class DenseFeedForward(FeedForward):
     def load(self, tensors, env: BuildEnv) -> None:
         self.w1 = tensors[self.n_up].contiguous()
         self.w2 = tensors[self.n_down].contiguous()
+        if env.ffn_e4m3:
+            self.w1, self.s1 = eight_bit_weights(self.w1)
+            self.w2, self.s2 = eight_bit_weights(self.w2)
+            self.reads_e4m3 = True
 
     def forward(self, h, out, accumulate, batch, env) -> None:
-        M = h.shape[0]
         ws = env.workspace
+        if self.s1 is not None:
+            h = _eight(h, ws, "ffn.h8")
+            a = ws.get("ffn.a", (h.values.shape[0], self.F), env.dtype)
+            kernels.linear_e4m3(a, *h, self.w1, self.s1, kernels.plain_act_epilogue(self.act))
+            kernels.linear_e4m3(out, *_eight(a, ws, "ffn.a8"), self.w2, self.s2, kernels.ACCUMULATE if accumulate else kernels.STORE)
+            return
+        M = h.shape[0]
         a = ws.get("ffn.a", (M, self.F), env.dtype)
         if kernels.takes_plain_act(h, self.w1):
             # the product applies the activation to its float sums before it stores
@@ -192,7 +258,7 @@ class SigmoidTopKMoE(FeedForward):
                   "up": "experts.{e}.w3.weight", "down": "experts.{e}.w2.weight"}
         self.n.update({"shared_gate": "shared.gate", "shared_up": "shared.up", "shared_down": "shared.down"})
         self.n.update(names or {})
-        self.router_w = self.router_b = self.w13 = self.w2 = None
+        self.router_w = self.router_b = self.w13 = self.w2 = self.s13 = self.s2 = None
         self.fused = False
         self.shared = None
         if shared_size:
@@ -223,14 +289,21 @@ class SigmoidTopKMoE(FeedForward):
             self.epilogue, self.fused = None, False
             self.w13 = torch.stack([tensors[n["up"].format(e=e)] for e in range(self.E)]).contiguous()
             self.w2 = torch.stack([tensors[n["down"].format(e=e)] for e in range(self.E)]).contiguous()
+            self._to_eight(env)
             return
         self.epilogue = kernels.gated_epilogue(self.act, self.limit, self.alpha)
-        self.fused = (not env.is_float32) and self.Fe % 16 == 0 and self.D % 8 == 0 and self.epilogue is not None
+        self.fused = (not env.is_float32) and self.Fe % 16 == 0 and (self.D % 8 == 0 or env.ffn_e4m3) and self.epilogue is not None
         self.w13 = torch.stack([fuse_gate_up(tensors[n["gate"].format(e=e)], tensors[n["up"].format(e=e)],
                                              self.fused) for e in range(self.E)]).contiguous()
         self.w2 = torch.stack([tensors[n["down"].format(e=e)] for e in range(self.E)]).contiguous()
+        self._to_eight(env)
         if self.shared is not None:
             self.shared.load(tensors, env)
+
+    def _to_eight(self, env: BuildEnv) -> None:
+        if env.ffn_e4m3:
+            self.w13, self.s13 = eight_bit_weights(self.w13)
+            self.w2, self.s2 = eight_bit_weights(self.w2)
 
     def flops_per_row(self) -> int:
         # the router, k experts of three matrices, and the shared expert
@@ -257,6 +330,15 @@ class SigmoidTopKMoE(FeedForward):
         offsets = ws.get("moe.offsets", (self.E + 1,), torch.int32)
         sorted_pair = ws.get("moe.sorted", (P,), torch.int32)
         pair_row = ws.get("moe.rows", (P,), torch.int32)
+        if self.s13 is not None:
+            self._experts_eight(h, ids, wts, offsets, sorted_pair, pair_row, out, accumulate, env)
+        else:
+            self._experts(h, ids, wts, offsets, sorted_pair, pair_row, out, accumulate, env)
+        if self.shared is not None:
+            kernels.guarded(self.shared.forward)(h, out, True, batch, env)
+
+    def _experts(self, h, ids, wts, offsets, sorted_pair, pair_row, out, accumulate, env) -> None:
+        ws, P = env.workspace, ids.numel()
         xs = ws.get("moe.xs", (P, self.D), env.dtype)
         kernels.moe_align_gather(offsets, sorted_pair, pair_row, xs, ids, h, self.E, weights=wts if self.weight_input else None)
         a = ws.get("moe.a", (P, self.Fe), env.dtype)
@@ -278,5 +360,21 @@ class SigmoidTopKMoE(FeedForward):
         ys = ws.get("moe.ys", (P, self.D), torch.float32)
         kernels.linear(ys, a, self.w2, group_offsets=offsets, rows_hint=P)
         kernels.moe_combine(out, ys, pair_row, None if self.weight_input else wts, accumulate, k=self.k)
-        if self.shared is not None:
-            kernels.guarded(self.shared.forward)(h, out, True, batch, env)
+
+    def _experts_eight(self, h, ids, wts, offsets, sorted_pair, pair_row, out, accumulate, env) -> None:
+        ws, P = env.workspace, ids.numel()
+        kernels.moe_align(offsets, sorted_pair, pair_row, ids, self.E)
+        xs = eight_bit_room(ws, "moe.x8", P, self.D)
+        kernels.quantize_e4m3(xs.values, xs.scale, h, rows=sorted_pair, div=self.k, weights=wts if self.weight_input else None)
+        a = ws.get("moe.a", (P, self.Fe), env.dtype)
+        if not self.gated:
+            kernels.linear_e4m3(a, *xs, self.w13, self.s13, kernels.plain_act_epilogue(self.act), group_offsets=offsets)
+        elif self.fused:
+            kernels.linear_e4m3(a, *xs, self.w13, self.s13, self.epilogue, group_offsets=offsets)
+        else:
+            gu = ws.get("moe.gu", (P, 2 * self.Fe), torch.float32)
+            kernels.linear_e4m3(gu, *xs, self.w13, self.s13, group_offsets=offsets)
+            kernels.gated_act(a, gu, self.act, self.limit, self.alpha)
+        ys = ws.get("moe.ys", (P, self.D), torch.float32)
+        kernels.linear_e4m3(ys, *_eight(a, ws, "moe.a8"), self.w2, self.s2, group_offsets=offsets)
+        kernels.moe_combine(out, ys, pair_row, None if self.weight_input else wts, accumulate, k=self.k)
