@@ -80,6 +80,11 @@ gemm_e4m3_pairs_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
   const int m_tiles = (M + 255) / 256, n_tiles = (N + 255) / 256;
   int num_tiles = m_tiles * n_tiles;
 
+  if (threadIdx.x == 64) {
+    tma_prefetch_map(&map_a);
+    tma_prefetch_map(&map_w);
+    if (tma_c) tma_prefetch_map(&map_c);
+  }
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; s++) {
       mbar_init(&full[s], 1);      // the first block announces the bytes of both
