@@ -3,37 +3,42 @@
 
 namespace {
 
-// Which kernel takes a product of `groups` times about `rows` rows.
+// Which kernel takes a product of `groups` times about `rows` rows: the one that is through first, by what either takes (us).
 //
-// The weights-first kernel takes them in tiles of 128 columns by the fewest rows (16 to 128) with which there are at most four tiles of
-// rows and at most two tiles an SM (else as many rows as there are, up to 128), and cuts K over up to eight blocks while that
-// leaves no SM with more than two, or with more than 4/3 eighths.  The pairs of SMs take 256 x 256.  Which is ahead goes by what either takes:
-//   weights first  2.7 + c (b (0.2 + 0.0014 rows) + 0.055 rows') us (+ 1.5 for a cluster): c the blocks an SM goes through, b its stages
-//                  of 128 numbers of k, rows' those a block finishes
-//   pairs          2.8 + w (0.31 b + 3) us: w the tiles a pair goes through
-// Fitted to 90 products of 40 to 3,000 rows, 64 to 24,000 columns and K of 128 to 12,000; over these, 117 more and 103 grouped ones (2 to
-// 128 experts, 0.1 to 512 rows each) the choice takes 1.5% more time than the best form of each.  Where it turns: 96 rows x
-// 2,048 x 2,048 weights first 6.1 us, pairs 10.4; 512 rows x 16,384 x 2,048 36.8 and 17.4.
+// weights first (tiles of 128 columns by 16 to 128 rows; `slices` blocks share a tile's K, all of them on the SMs at once: two an SM, one with
+// 128 rows), c blocks an SM, b stages of 128 numbers of k a block:
+//   2.1 + b max(0.21 + 0.0012 rows, c (0.29 + 0.0007 rows) where c > 1) + max(c, 1) rows' (0.05 / slices + 0.037 in a cluster) + 1 for a cluster
+//   (rows' those of a tile that there are)
+// pairs of SMs (tiles of 256 x 256), w of them a pair:
+//   3.5 + w (0.34 b + 2.4)
+// Fitted to 110 products of 1 to 2,000 rows, 64 to 24,000 columns and K of 128 to 12,000, each in every form that it has; over these and 58
+// grouped ones (2 to 128 experts of 0.5 to 400 rows) the choice takes 1.5% more time than the best form of each.  Where it turns: 96 rows
+// x 2,048 x 2,048 weights first 6.1 us, pairs 10.4; 512 rows x 16,384 x 2,048 36.8 and 17.4.
 struct Form {
   bool pairs;
   int rows, slices;      // of the weights-first kernel
 };
 
 Form form_of(int groups, int rows, int N, int K) {
-  const int sms = sm_count(), nk = ceil_div(K, E8_BK), n_tiles = ceil_div(N, 128);
-  Form f{false, 16, 1};
-  for (; f.rows <= 128; f.rows *= 2)
-    if (ceil_div(rows, f.rows) <= 4 && (long long)groups * ceil_div(rows, f.rows) * n_tiles <= 2 * sms) break;
-  if (f.rows > 128)
-    for (f.rows = 16; f.rows < 128 && f.rows < rows; f.rows *= 2) {}
-  const long long tiles = (long long)groups * ceil_div(rows, f.rows) * n_tiles;
-  while (f.slices < 8 && tiles * f.slices * 2 <= (f.slices < 4 ? 2 * sms : sms * 4 / 3) && nk >= 4 * f.slices) f.slices *= 2;
-  if (rows < 48) return f;
-  const double each = (double)tiles * f.slices / sms, finished = rows < f.rows ? rows : f.rows;
-  const double few = 2.7 + (each > 1 ? each : 1) * (ceil_div(nk, f.slices) * (0.2 + 0.0014 * f.rows) + 0.055 * finished * (f.slices == 1 ? 1 : 1.0 / f.slices + 0.2)) + (f.slices > 1 ? 1.5 : 0);
-  const long long turns = ((long long)groups * ceil_div(rows, 256) * ceil_div(N, 256) + sms / 2 - 1) / (sms / 2);
-  f.pairs = 2.8 + turns * (0.31 * nk + 3) < few;
-  return f;
+  const int sms = sm_count(), nk = ceil_div(K, E8_BK);
+  Form best{false, 16, 1};
+  double least = 1e30;
+  for (int mp = 16; mp <= 128; mp *= 2) {
+    if ((mp > 16 && mp >= 2 * rows) || (mp < 128 && ceil_div(rows, mp) > 8)) continue;
+    const long long tiles = (long long)groups * ceil_div(rows, mp) * ceil_div(N, 128);
+    const double there = rows < mp ? rows : mp;
+    for (int s = 1; s <= 8; s *= 2) {
+      if (s > 1 && (tiles * s > (mp < 128 ? 2 * sms : sms) || nk < 2 * s)) break;
+      const double c = (double)tiles * s / sms, one = 0.21 + 0.0012 * mp, shared = c > 1 ? c * (0.29 + 0.0007 * mp) : 0;
+      const double us = 2.1 + ceil_div(nk, s) * (one > shared ? one : shared) + (c > 1 ? c : 1) * there * (0.05 / s + (s > 1 ? 0.037 : 0)) + (s > 1 ? 1 : 0);
+      if (us < least) least = us, best = Form{false, mp, s};
+    }
+  }
+  if (rows < 40) return best;
+  const int pairs = sms / 2 > 0 ? sms / 2 : 1;
+  const long long turns = ((long long)groups * ceil_div(rows, 256) * ceil_div(N, 256) + pairs - 1) / pairs;
+  best.pairs = 3.5 + turns * (0.34 * nk + 2.4) < least;
+  return best;
 }
 
 // One packed argument, numbers of 64 bits in this order (see row_e4m3.cu).

@@ -9,9 +9,9 @@
 // Otherwise the blocks walk the tiles, with two accumulators, so that loads go on under the epilogue.
 //
 // Roles: warp 0 asks for the tiles of W and A (TMA, 128 numbers of k a stage), warp 1 issues the products, warps 2-5 take the sums out of
-// tensor memory, where a lane has a row of W, and turn them in shared memory: a warp then finishes a row of A at a time, a lane four
-// neighbouring columns, so that the results of a tile's row leave in one store.  (Finished as they come out of tensor memory, a lane a
-// column, the unrolled epilogues of all rows were more code than time: 100 rows x 2,048 x 2,048 in 16 tiles 52.9 us.)
+// tensor memory, where a lane has a row of W, and apply the epilogue: a warp stores 32 neighbouring columns of a row of A.  (Turned in
+// shared memory first, 16 rows at a time between two barriers, so that a lane has four columns: FEW_TURNED.)  The epilogue is
+// looked at once for 32 rows: looked at for each, the unrolled code was more than the time.
 //
 // Every wait is bounded: a role that gives up sets the status word and all leave; the block stays until the copies asked for have
 // landed and its products are done.
@@ -37,7 +37,7 @@ gemm_e4m3_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
   __shared__ uint64_t full[STAGES], empty[STAGES], acc_full[2], acc_empty[2], parts_full, drained;
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_s, sent_s, parts_s;
-  __shared__ float sa_s[2][MP];
+  __shared__ float sa_s[2][MP];      // (rows beyond a tile's last: anything, not used)
   __shared__ E8Groups groups;
   volatile int* abort_flag = &abort_s;
 
@@ -133,14 +133,12 @@ gemm_e4m3_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
         z[u] = make_float4(0.f, 0.f, 0.f, 0.f);
         if (r >= i1) continue;
         z[u] = *reinterpret_cast<const float4*>(at);
-        if (CLUSTER) {
 #pragma unroll
-          for (int k = 1; k < 8; k++)
-            if (k < used) {
-              const float4 v = *reinterpret_cast<const float4*>(at + k * apart);
-              z[u].x += v.x, z[u].y += v.y, z[u].z += v.z, z[u].w += v.w;
-            }
-        }
+        for (int k = 1; k < 8; k++)
+          if (k < used) {
+            const float4 v = *reinterpret_cast<const float4*>(at + k * apart);
+            z[u].x += v.x, z[u].y += v.y, z[u].z += v.z, z[u].w += v.w;
+          }
         const float f = sa_t[r];
         z[u].x *= f * swn.x, z[u].y *= f * swn.y, z[u].z *= f * swn.z, z[u].w *= f * swn.w;
       }
@@ -232,12 +230,13 @@ gemm_e4m3_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
       int m0, m_end, n0, e;
       place(tile, m0, m_end, n0, e);
       const uint32_t buf = t & 1, tm = tmem_acc + ((uint32_t)(quad * 32) << 16) + buf * MP;
-      const int n = n0 + lane * 4;
       const float* sw_e = sw + (size_t)e * N;
-      const float4 swn = make_float4(n < N ? sw_e[n] : 0.f, n + 1 < N ? sw_e[n + 1] : 0.f, n + 2 < N ? sw_e[n + 2] : 0.f, n + 3 < N ? sw_e[n + 3] : 0.f);
       const int rows = min(MP, m_end - m0);
       if (tid < rows) sa_s[buf][tid] = sa[m0 + tid];
-      if (CLUSTER) asm volatile("bar.sync 1, 128;" ::: "memory");      // (without a cluster the warps meet below)
+      const int n = CLUSTER ? n0 + lane * 4 : n0 + n_loc;
+      const float4 swn = make_float4(n < N ? sw_e[n] : 0.f, CLUSTER && n + 1 < N ? sw_e[n + 1] : 0.f, CLUSTER && n + 2 < N ? sw_e[n + 2] : 0.f, CLUSTER && n + 3 < N ? sw_e[n + 3] : 0.f);
+      // (the other buffer may still be read: a tile has one barrier, so nobody is two tiles ahead; the warps leave together)
+      if (!e8_all<128>(!gave_up)) break;
       if (my_nk > 0) {
         const bool ok = e8_wait(&acc_full[buf], (t >> 1) & 1, abort_flag);
         if (!ok) {
@@ -274,26 +273,56 @@ gemm_e4m3_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
         }
         break;
       }
-      // the sums of the next 16 rows, [row][column]
-      auto turn = [&](int c0) {
-        uint32_t v[16];
-        tmem_ld16(tm + (uint32_t)c0, v);
-        tmem_ld_wait();
-#pragma unroll
-        for (int i = 0; i < 16; i++) part[i * 128 + n_loc] = __uint_as_float(v[i]);
-      };
-      if (!e8_all<128>(!gave_up)) break;      // (the four warps leave together: they meet again below)
+      if (gave_up) continue;
+      constexpr int R = MP < 32 ? MP : 32;      // rows at a time
 #pragma unroll 1
-      for (int c0 = 0; c0 < rows; c0 += 16) {
-        turn(c0);
-        if (c0 + 16 >= rows) {      // all sums are out of tensor memory: the accumulator is free
+      for (int c0 = 0; c0 < rows; c0 += R) {
+        uint32_t v[32];
+        if (R == 32) tmem_ld32(tm + (uint32_t)c0, v);
+        else tmem_ld16(tm + (uint32_t)c0, v);
+        TC* const c = C + (m0 + c0) * ldc + n;
+        float z[R];
+        if (epilogue == 1) {
+#pragma unroll
+          for (int i = 0; i < R; i++) z[i] = n < N && c0 + i < rows ? to_f32(c[i * ldc]) : 0.f;
+        }
+        tmem_ld_wait();
+        if (c0 + R >= rows) {      // all sums are out of tensor memory: the accumulator is free
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(&acc_empty[buf]);
         }
-        asm volatile("bar.sync 1, 128;" ::: "memory");
-        finish(c0, min(c0 + 16, rows), c0, n0, swn, sa_s[buf], s_part, 1, 0, m0);
-        asm volatile("bar.sync 1, 128;" ::: "memory");
+        const float* f = sa_s[buf] + c0;
+        if (epilogue == 1) {
+#pragma unroll
+          for (int i = 0; i < R; i++) z[i] += __uint_as_float(v[i]) * f[i] * swn.x;
+        } else {
+#pragma unroll
+          for (int i = 0; i < R; i++) z[i] = __uint_as_float(v[i]) * f[i] * swn.x;
+        }
+        if (epilogue == 2) {      // lanes 0-15 hold 16 gate columns, lanes 16-31 their up columns
+          TC* const o = C + (m0 + c0) * ldc + 16 * (n >> 5) + lane;
+#pragma unroll
+          for (int h = 0; h < R; h += 16) {
+            float up[16];
+#pragma unroll
+            for (int i = 0; i < 16; i++) up[i] = __shfl_down_sync(0xffffffffu, z[h + i], 16);
+            gate_all<TC, 16>(z + h, up, act);
+          }
+          if (lane < 16 && n < N)
+#pragma unroll
+            for (int i = 0; i < R; i++)
+              if (c0 + i < rows) o[i * ldc] = from_f32<TC>(z[i]);
+        } else {
+          if (sizeof(TC) == 2 && epilogue == 0 && LEB_PLAIN_ACT_OK(act, epilogue)) {
+#pragma unroll
+            for (int i = 0; i < R; i++) z[i] = plain_act(z[i], act);
+          }
+          if (n < N)
+#pragma unroll
+            for (int i = 0; i < R; i++)
+              if (c0 + i < rows) c[i * ldc] = from_f32<TC>(z[i]);
+        }
       }
     }
   }
@@ -331,7 +360,7 @@ namespace {
 
 template <typename TC, int MP, int STAGES, int PER_SM, bool GROUPED, bool CLUSTER>
 int launch_few(const E8Product& p, int n_slices, cudaStream_t st) {
-  constexpr size_t smem = (size_t)STAGES * (128 + MP) * E8_BK + (CLUSTER ? MP : 16) * 512 + 1024;
+  constexpr size_t smem = (size_t)STAGES * (128 + MP) * E8_BK + (CLUSTER ? MP * 512 : 0) + 1024;
   auto kern = gemm_e4m3_few_kernel<TC, MP, STAGES, PER_SM, GROUPED, CLUSTER>;
   cudaError_t e = leb_allow_smem<gemm_e4m3_few_kernel<TC, MP, STAGES, PER_SM, GROUPED, CLUSTER>, (int)smem>();
   if (e != cudaSuccess) return leb_fail("leb_linear_e4m3: shared memory %zu: %s", smem, cudaGetErrorString(e));
@@ -371,7 +400,7 @@ int launch_few_rows(const E8Product& p, int mp, int n_slices, cudaStream_t st) {
     if (mp == 64) return launch_few<TC, 64, 3, 2, GROUPED, true>(p, n_slices, st);
     return launch_few<TC, 128, 4, 1, GROUPED, true>(p, n_slices, st);
   }
-  if (mp == 16) return launch_few<TC, 16, 5, 2, GROUPED, false>(p, 1, st);
+  if (mp == 16) return launch_few<TC, 16, 6, 2, GROUPED, false>(p, 1, st);
   if (mp == 32) return launch_few<TC, 32, 5, 2, GROUPED, false>(p, 1, st);
   if (mp == 64) return launch_few<TC, 64, 4, 2, GROUPED, false>(p, 1, st);
   return launch_few<TC, 128, 3, 2, GROUPED, false>(p, 1, st);
