@@ -36,9 +36,14 @@ __device__ __forceinline__ uint32_t e8_map_to_rank(uint32_t smem_addr, uint32_t 
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_addr), "r"(rank));
   return a;
 }
-// A value's way to another block's shared memory, its four bytes counted on a barrier there.
-__device__ __forceinline__ void e8_send(uint32_t cluster_addr, uint32_t value, uint32_t bar_cluster_addr) {
-  asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.b32 [%0], %1, [%2];" ::"r"(cluster_addr), "r"(value), "r"(bar_cluster_addr) : "memory");
+// Values' way to another block's shared memory, their bytes counted on a barrier there.
+__device__ __forceinline__ void e8_send4(uint32_t cluster_addr, const uint32_t* v, uint32_t bar_cluster_addr) {
+  asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [%0], {%1, %2, %3, %4}, [%5];"
+               ::"r"(cluster_addr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(bar_cluster_addr) : "memory");
+}
+__device__ __forceinline__ void e8_send2(uint32_t cluster_addr, const uint32_t* v, uint32_t bar_cluster_addr) {
+  asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v2.b32 [%0], {%1, %2}, [%3];"
+               ::"r"(cluster_addr), "r"(v[0]), "r"(v[1]), "r"(bar_cluster_addr) : "memory");
 }
 __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t* v) {
   asm volatile(

@@ -15,6 +15,8 @@
 //
 // Every wait is bounded: a role that gives up sets the status word and all leave; the block stays until the copies asked for have
 // landed and its products are done.
+#include <type_traits>
+
 #include "e4m3_tc.cuh"
 
 #define FEW_THREADS 192
@@ -102,75 +104,49 @@ gemm_e4m3_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
       m_end = M;
     }
   };
-  // Rows [i0, i1) of a tile, this lane's four columns: the sums of all `used` slices (apart bytes from one to the next; row row0's first),
-  // scaled, through the epilogue.  All lanes call.
-  auto finish = [&](int i0, int i1, int row0, int n0, float4 swn, const float* sa_t, const uint8_t* sums, int used, int apart, int m0) {
-    const int n = n0 + lane * 4;
-    const bool vec = ldc % 4 == 0 && ((uintptr_t)C & (sizeof(TC) * 4 - 1)) == 0 && n + 3 < N;
-    constexpr int U = MP >= 64 ? 4 : 2;      // rows at a time
-#pragma unroll 1
-    for (int i = i0 + (warp & 3); i < i1; i += 4 * U) {
-      float4 z[U], old[U];
+  // In a cluster: V of the rows that this block finishes from its row r on (`there` of them are there; c0: the first in C), this lane's column: the
+  // sums of all `used` slices, scaled, through the epilogue.  All lanes of a warp call.
+  const int share = CLUSTER ? MP / n_slices : 1, units = share / 4, used = (nk + per - 1) / per;
+  // where four rows (unit u) of column n lie: columns side by side
+  auto place_of = [&](int k, int n, int u) { return ((k * units + u) * 128 + n) * 4; };
+  auto finish = [&](auto rows_at_a_time, int r, int there, int n_loc, int n, float swn, const float* sa_t, TC* c0) {
+    constexpr int V = decltype(rows_at_a_time)::value;
+    const float* part = reinterpret_cast<const float*>(s_part);
+    float z[V], old[V];
+    TC* const c = c0 + r * ldc;
 #pragma unroll
-      for (int u = 0; u < U; u++) {
-        const int r = i + 4 * u;
-        old[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (epilogue == 1 && r < i1) {
-          const TC* c = C + (m0 + r) * ldc + n;
-          if (vec) old[u] = load4(c);
-          else {
-            if (n < N) old[u].x = to_f32(c[0]);
-            if (n + 1 < N) old[u].y = to_f32(c[1]);
-            if (n + 2 < N) old[u].z = to_f32(c[2]);
-            if (n + 3 < N) old[u].w = to_f32(c[3]);
-          }
+    for (int i = 0; i < V; i++) z[i] = 0.f, old[i] = epilogue == 1 && n < N && r + i < there ? to_f32(c[i * ldc + n]) : 0.f;
+#pragma unroll
+    for (int k = 0; k < 8; k++)
+      if (k < used) {
+        if (V == 4) {
+          const float4 f = *reinterpret_cast<const float4*>(part + place_of(k, n_loc, r >> 2));
+          z[0] += f.x, z[1] += f.y, z[2 % V] += f.z, z[3 % V] += f.w;
+        } else {
+          const float2 f = *reinterpret_cast<const float2*>(part + (k * 128 + n_loc) * share);
+          z[0] += f.x, z[1] += f.y;
         }
       }
 #pragma unroll
-      for (int u = 0; u < U; u++) {
-        const int r = i + 4 * u;
-        const uint8_t* at = sums + (r - row0) * 512 + lane * 16;
-        z[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (r >= i1) continue;
-        z[u] = *reinterpret_cast<const float4*>(at);
+    for (int i = 0; i < V; i++) z[i] = z[i] * sa_t[r + i] * swn + old[i];
+    if (epilogue == 2) {      // lanes 0-15 hold 16 gate columns, lanes 16-31 their up columns
+      float up[V];
 #pragma unroll
-        for (int k = 1; k < 8; k++)
-          if (k < used) {
-            const float4 v = *reinterpret_cast<const float4*>(at + k * apart);
-            z[u].x += v.x, z[u].y += v.y, z[u].z += v.z, z[u].w += v.w;
-          }
-        const float f = sa_t[r];
-        z[u].x *= f * swn.x, z[u].y *= f * swn.y, z[u].z *= f * swn.z, z[u].w *= f * swn.w;
+      for (int i = 0; i < V; i++) up[i] = __shfl_down_sync(0xffffffffu, z[i], 16);
+      gate_all<TC, V>(z, up, act);
+      if (lane < 16 && n < N)
+#pragma unroll
+        for (int i = 0; i < V; i++)
+          if (r + i < there) c[i * ldc + 16 * (n >> 5) + lane] = from_f32<TC>(z[i]);
+    } else {
+      if (sizeof(TC) == 2 && epilogue == 0 && LEB_PLAIN_ACT_OK(act, epilogue)) {
+#pragma unroll
+        for (int i = 0; i < V; i++) z[i] = plain_act(z[i], act);
       }
-      if (epilogue == 2) {      // of eight lanes four hold 16 gate columns, four their up columns
-        float g[4 * U], up[4 * U];
+      if (n < N)
 #pragma unroll
-        for (int u = 0; u < U; u++) g[4 * u] = z[u].x, g[4 * u + 1] = z[u].y, g[4 * u + 2] = z[u].z, g[4 * u + 3] = z[u].w;
-#pragma unroll
-        for (int k = 0; k < 4 * U; k++) up[k] = __shfl_down_sync(0xffffffffu, g[k], 4);
-        gate_all<TC, 4 * U>(g, up, act);
-#pragma unroll
-        for (int u = 0; u < U; u++) z[u] = make_float4(g[4 * u], g[4 * u + 1], g[4 * u + 2], g[4 * u + 3]);
-      } else if (epilogue == 0 && sizeof(TC) == 2 && LEB_PLAIN_ACT_OK(act, epilogue)) {
-#pragma unroll
-        for (int u = 0; u < U; u++) z[u] = make_float4(plain_act(z[u].x, act), plain_act(z[u].y, act), plain_act(z[u].z, act), plain_act(z[u].w, act));
-      }
-#pragma unroll
-      for (int u = 0; u < U; u++) {
-        const int r = i + 4 * u;
-        if (r >= i1) break;
-        if (epilogue == 1) z[u].x += old[u].x, z[u].y += old[u].y, z[u].z += old[u].z, z[u].w += old[u].w;
-        const bool mine = epilogue != 2 || (lane & 4) == 0;
-        TC* c = C + (m0 + r) * ldc + (epilogue == 2 ? (n >> 5) * 16 + (n & 15) : n);
-        if (!mine) continue;
-        if (vec) store4(c, z[u]);
-        else {
-          if (n < N) c[0] = from_f32<TC>(z[u].x);
-          if (n + 1 < N) c[1] = from_f32<TC>(z[u].y);
-          if (n + 2 < N) c[2] = from_f32<TC>(z[u].z);
-          if (n + 3 < N) c[3] = from_f32<TC>(z[u].w);
-        }
-      }
+        for (int i = 0; i < V; i++)
+          if (r + i < there) c[i * ldc + n] = from_f32<TC>(z[i]);
     }
   };
 
@@ -230,11 +206,10 @@ gemm_e4m3_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
       int m0, m_end, n0, e;
       place(tile, m0, m_end, n0, e);
       const uint32_t buf = t & 1, tm = tmem_acc + ((uint32_t)(quad * 32) << 16) + buf * MP;
-      const float* sw_e = sw + (size_t)e * N;
       const int rows = min(MP, m_end - m0);
       if (tid < rows) sa_s[buf][tid] = sa[m0 + tid];
-      const int n = CLUSTER ? n0 + lane * 4 : n0 + n_loc;
-      const float4 swn = make_float4(n < N ? sw_e[n] : 0.f, CLUSTER && n + 1 < N ? sw_e[n + 1] : 0.f, CLUSTER && n + 2 < N ? sw_e[n + 2] : 0.f, CLUSTER && n + 3 < N ? sw_e[n + 3] : 0.f);
+      const int n = n0 + n_loc;
+      const float swn = n < N ? sw[(size_t)e * N + n] : 0.f;
       // (the other buffer may still be read: a tile has one barrier, so nobody is two tiles ahead; the warps leave together)
       if (!e8_all<128>(!gave_up)) break;
       if (my_nk > 0) {
@@ -246,9 +221,10 @@ gemm_e4m3_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
         tc_fence_after();
       }
       if (CLUSTER) {      // one tile
-        const int share = MP / n_slices, shift = __ffs(share) - 1, used = (nk + per - 1) / per, own = min((slice + 1) * share, rows) - slice * share;
+        // V rows of a column at a time (those behind the tile's last are sent with them, and not used)
+        const int V = share >= 4 ? 4 : 2, shift = __ffs(share) - 1, own = min(share, rows - slice * share);
         if (tid == 0 && own > 0) {
-          mbar_expect_tx(&parts_full, (uint32_t)(used * own * 512));
+          mbar_expect_tx(&parts_full, (uint32_t)(used * ((own + V - 1) / V * V) * 512));
           parts_s = 1;
         }
         asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");      // the others' barriers exist
@@ -258,10 +234,18 @@ gemm_e4m3_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
             uint32_t v[16];
             tmem_ld16(tm + (uint32_t)c0, v);      // (after a wait that gave up: anything; what the others wait for is sent all the same)
             tmem_ld_wait();
+            if (V == 4) {
 #pragma unroll
-            for (int i = 0; i < 16; i++) {
-              const int row = c0 + i, owner = row >> shift;
-              if (row < rows) e8_send(e8_map_to_rank(smem_u32(part + (slice * share + (row & (share - 1))) * 128 + n_loc), (uint32_t)owner), v[i], e8_map_to_rank(smem_u32(&parts_full), (uint32_t)owner));
+              for (int i = 0; i < 16; i += 4) {
+                const uint32_t owner = (uint32_t)(c0 + i) >> shift;
+                if (c0 + i < rows) e8_send4(e8_map_to_rank(smem_u32(part + place_of(slice, n_loc, ((c0 + i) & (share - 1)) >> 2)), owner), v + i, e8_map_to_rank(smem_u32(&parts_full), owner));
+              }
+            } else {
+#pragma unroll
+              for (int i = 0; i < 16; i += 2) {
+                const uint32_t owner = (uint32_t)(c0 + i) >> 1;
+                if (c0 + i < rows) e8_send2(e8_map_to_rank(smem_u32(part + (slice * 128 + n_loc) * 2), owner), v + i, e8_map_to_rank(smem_u32(&parts_full), owner));
+              }
             }
           }
         __syncwarp();
@@ -269,7 +253,14 @@ gemm_e4m3_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
         met = true;
         if (own > 0) {
           if (!e8_wait(&parts_full, 0, abort_flag) && lane == 0) atomicExch(status, 55);
-          finish(slice * share, slice * share + own, slice * share, n0, swn, sa_s[buf], s_part, used, share * 512, m0);
+          const float* const sa_t = sa_s[buf] + slice * share;
+          TC* const c0 = C + (m0 + slice * share) * ldc;
+          if (V == 4) {
+#pragma unroll 2
+            for (int r = 0; r < own; r += 4) finish(std::integral_constant<int, 4>{}, r, own, n_loc, n, swn, sa_t, c0);
+          } else {
+            finish(std::integral_constant<int, 2>{}, 0, own, n_loc, n, swn, sa_t, c0);
+          }
         }
         break;
       }
@@ -295,10 +286,10 @@ gemm_e4m3_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
         const float* f = sa_s[buf] + c0;
         if (epilogue == 1) {
 #pragma unroll
-          for (int i = 0; i < R; i++) z[i] += __uint_as_float(v[i]) * f[i] * swn.x;
+          for (int i = 0; i < R; i++) z[i] += __uint_as_float(v[i]) * f[i] * swn;
         } else {
 #pragma unroll
-          for (int i = 0; i < R; i++) z[i] = __uint_as_float(v[i]) * f[i] * swn.x;
+          for (int i = 0; i < R; i++) z[i] = __uint_as_float(v[i]) * f[i] * swn;
         }
         if (epilogue == 2) {      // lanes 0-15 hold 16 gate columns, lanes 16-31 their up columns
           TC* const o = C + (m0 + c0) * ldc + 16 * (n >> 5) + lane;
