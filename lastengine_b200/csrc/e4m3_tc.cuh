@@ -178,6 +178,10 @@ struct E8Product {
   long long w_group_stride;
   int* status;
 };
+// Stages of 128 numbers of k that a block of the weights-first kernel holds: what shared memory has room for with two blocks an SM (one for
+// clusters of 128 rows), beside the sums that a cluster's blocks send one another.
+constexpr int few_stages(int rows, bool cluster) { return cluster ? (rows == 16 ? 5 : rows == 64 ? 3 : 4) : rows == 16 ? 6 : rows == 32 ? 5 : rows == 64 ? 4 : 3; }
+
 int leb_gemm_e4m3_any(const E8Product& p, cudaStream_t st);
 int leb_gemm_e4m3_few(const E8Product& p, int mp, int n_slices, cudaStream_t st);
 int leb_gemm_e4m3_pairs(const E8Product& p, cudaStream_t st);

@@ -382,19 +382,17 @@ int launch_few(const E8Product& p, int n_slices, cudaStream_t st) {
   return 0;
 }
 
-// Stages and blocks an SM: what shared memory holds, beside the sums that a cluster's blocks send one another.
+template <typename TC, int MP, bool GROUPED>
+int launch_few_rows(const E8Product& p, int n_slices, cudaStream_t st) {
+  if (n_slices > 1) return launch_few<TC, MP, few_stages(MP, true), MP == 128 ? 1 : 2, GROUPED, true>(p, n_slices, st);
+  return launch_few<TC, MP, few_stages(MP, false), 2, GROUPED, false>(p, 1, st);
+}
 template <typename TC, bool GROUPED>
 int launch_few_rows(const E8Product& p, int mp, int n_slices, cudaStream_t st) {
-  if (n_slices > 1) {
-    if (mp == 16) return launch_few<TC, 16, 5, 2, GROUPED, true>(p, n_slices, st);
-    if (mp == 32) return launch_few<TC, 32, 4, 2, GROUPED, true>(p, n_slices, st);
-    if (mp == 64) return launch_few<TC, 64, 3, 2, GROUPED, true>(p, n_slices, st);
-    return launch_few<TC, 128, 4, 1, GROUPED, true>(p, n_slices, st);
-  }
-  if (mp == 16) return launch_few<TC, 16, 6, 2, GROUPED, false>(p, 1, st);
-  if (mp == 32) return launch_few<TC, 32, 5, 2, GROUPED, false>(p, 1, st);
-  if (mp == 64) return launch_few<TC, 64, 4, 2, GROUPED, false>(p, 1, st);
-  return launch_few<TC, 128, 3, 2, GROUPED, false>(p, 1, st);
+  if (mp == 16) return launch_few_rows<TC, 16, GROUPED>(p, n_slices, st);
+  if (mp == 32) return launch_few_rows<TC, 32, GROUPED>(p, n_slices, st);
+  if (mp == 64) return launch_few_rows<TC, 64, GROUPED>(p, n_slices, st);
+  return launch_few_rows<TC, 128, GROUPED>(p, n_slices, st);
 }
 
 }  // namespace
