@@ -20,8 +20,8 @@ struct Form {
   int rows, slices;      // of the weights-first kernel
 };
 
-Form form_of(int groups, int rows, int N, int K) {
-  const int sms = sm_count(), nk = ceil_div(K, E8_BK);
+Form form_of(int groups, int rows, int N, int K, int sms) {
+  const int nk = ceil_div(K, E8_BK);
   Form best{false, 16, 1};
   double least = 1e30;
   for (int mp = 16; mp <= 128; mp *= 2) {
@@ -49,6 +49,12 @@ struct LinearArgs {
 
 }  // namespace
 
+// The form that takes a product of so many groups of about so many rows on a device of `sms` SMs: 0 pairs, else rows of a tile | slices of K << 16.
+LEB_API int leb_linear_e4m3_form(int groups, int rows, int N, int K, int sms) {
+  const Form f = form_of(groups, rows, N, K, sms);
+  return f.pairs ? 0 : f.rows | f.slices << 16;
+}
+
 // C [M, N] (or [M, N / 2] gated; rows ldc apart) (+)= the product of A [M, K] with scales sa [M] and W [N, K] with scales sw [N]; with offsets
 // [n_groups + 1] (on the device) rows [offsets[e], offsets[e + 1]) with W[e], sw[e], experts w_group_stride apart, and rows beyond the last
 // offset left as they are.  epilogue: 0 store, 1 add into float C, 2 gated, an activation above it as in the bfloat16 products.
@@ -69,6 +75,6 @@ LEB_API int leb_linear_e4m3(const void* packed, cudaStream_t st) {
                    (!p.offsets || ((p.n_groups == 1 || p.w_group_stride == N * p.ldw) && p.n_groups <= E8_MAX_GROUPS && a.N * a.n_groups < MOST));
   if (!tma) return leb_gemm_e4m3_any(p, st);
   const int groups = p.offsets ? min(p.n_groups, M) : 1;
-  const Form f = form_of(groups, ceil_div(M, groups), N, K);
+  const Form f = form_of(groups, ceil_div(M, groups), N, K, sm_count());
   return f.pairs ? leb_gemm_e4m3_pairs(p, st) : leb_gemm_e4m3_few(p, f.rows, f.slices, st);
 }

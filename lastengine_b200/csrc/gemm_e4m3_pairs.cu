@@ -363,9 +363,10 @@ int launch_pairs(const E8Product& p, cudaStream_t st) {
   CUtensorMap ma, mw;
   if (e8_tensor_map(&ma, p.A, p.M, p.K, p.lda, 128)) return 1;
   if (e8_tensor_map(&mw, p.W, (long long)p.N * (p.offsets ? p.n_groups : 1), p.K, p.ldw, 128)) return 1;
-  // results as the copies of the epilogue see them: 32 rows by 64 bytes, turned as the lanes leave them
+  // results as the copies of the epilogue see them: 32 rows by 64 bytes, turned as the lanes leave them.  (A copy leaves out what lies beyond C in
+  // steps of 16 bytes: rows that end inside such a step are the lanes' to store.)
   const int n_out = (p.epilogue & 255) == 2 ? p.N / 2 : p.N, size = sizeof(TC);
-  const int tma_c = p.ldc * size % 16 == 0 && ((uintptr_t)p.C & 15) == 0 && p.ldc >= n_out;
+  const int tma_c = (long long)n_out * size % 16 == 0 && p.ldc * size % 16 == 0 && ((uintptr_t)p.C & 15) == 0 && p.ldc >= n_out;
   CUtensorMap mc = ma;
   if (tma_c) {
     cuuint64_t dims[2] = {(cuuint64_t)n_out, (cuuint64_t)p.M}, strides[1] = {(cuuint64_t)p.ldc * size};

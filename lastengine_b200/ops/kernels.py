@@ -293,6 +293,7 @@ def _declare(L) -> None:
         "leb_quantize_e4m3": [ctypes.c_char_p, P],
         "leb_rmsnorm_e4m3": [ctypes.c_char_p, P],
         "leb_linear_e4m3": [ctypes.c_char_p, P],
+        "leb_linear_e4m3_form": [I, I, I, I, I],
         "leb_moe_router": [P, P, P, I, P, P, I, I, I, I, I, F, I, P],
         "leb_moe_align": [P, P, P, P, I, I, P],
         "leb_moe_align_gather": [P, P, P, P, I, P, P, P, I, I, I, I, P],

@@ -145,3 +145,24 @@ def test_a_refusal_of_the_library_is_raised(monkeypatch):
     for epilogue, out in ((3, torch.zeros(4, 64)), (K.ACCUMULATE | (1 << 8), torch.zeros(4, 64)), (K.plain_act_epilogue(0), torch.zeros(4, 64)), (K.SWIGLU | (9 << 8), torch.zeros(4, 32))):
         with pytest.raises(K.KernelError, match="epilogue"):
             linear(out, epilogue=epilogue)
+
+
+def test_every_product_has_a_form():
+    """Over all sizes, on devices of any number of SMs: pairs for many rows only, else tiles no wider than the rows need, K cut only where every
+    block has two stages and all blocks are on the SMs at once."""
+    import random
+    rng = random.Random(3)
+    seen = set()
+    for _ in range(20000):
+        g, r, N, K_ = (int(2 ** rng.uniform(0, top)) for top in (7, 12, 16, 14))
+        sms = rng.choice([1, 2, 74, 148, 148, 148, 160])
+        form = K.lib().leb_linear_e4m3_form(g, r, N, K_, sms)
+        if form == 0:
+            assert r >= 40
+            continue
+        rows, slices = form & 0xffff, form >> 16
+        assert rows in (16, 32, 64, 128) and slices in (1, 2, 4, 8) and (rows == 16 or rows < 2 * r)
+        blocks = g * -(-r // rows) * -(-N // 128) * slices
+        assert slices == 1 or (blocks <= (1 if rows == 128 else 2) * sms and -(-K_ // 128) >= 2 * slices)
+        seen.add(form)
+    assert len(seen) == 16

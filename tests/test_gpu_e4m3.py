@@ -326,6 +326,73 @@ def test_grouped_is_exact_on_whole_numbers(counts, N, K_, apart):
     K().check_device_status()
 
 
+# (groups, rows of each, columns, K) by the form that takes them on 148 SMs (0: pairs; else rows of a tile and slices of K)
+FORMS = {
+    (128, 1): (1, 573, 150, 200), (128, 2): (1, 65, 5425, 1429), (128, 4): (1, 516, 159, 1179), (128, 8): (1, 538, 153, 1966),
+    (16, 1): (1, 1, 151, 211), (16, 2): (1, 1, 9690, 1157), (16, 4): (1, 1, 151, 913), (16, 8): (1, 1, 154, 1921),
+    (32, 1): (1, 131, 153, 200), (32, 2): (1, 18, 9837, 2523), (32, 4): (1, 141, 150, 920), (32, 8): (1, 17, 646, 2082),
+    (64, 1): (1, 257, 155, 204), (64, 2): (1, 33, 9573, 5002), (64, 4): (1, 287, 150, 1316), (64, 8): (1, 261, 161, 1933), 0: (1, 195, 12125, 205), "0, results that copies take": (1, 195, 12128, 208),
+}
+GROUPED_FORMS = {
+    (128, 1): (3, 534, 145, 214), (128, 2): (34, 66, 162, 919), (128, 4): (9, 71, 154, 1819), (128, 8): (5, 67, 180, 2360),
+    (16, 1): (2, 1, 167, 203), (16, 2): (39, 1, 150, 1220), (16, 4): (2, 1, 145, 897), (16, 8): (2, 1, 148, 1987),
+    (32, 1): (22, 17, 141, 238), (32, 2): (41, 17, 147, 3612), (32, 4): (9, 17, 142, 932), (32, 8): (3, 17, 169, 2461),
+    (64, 1): (2, 302, 143, 237), (64, 2): (39, 33, 142, 6819), (64, 4): (12, 33, 159, 1799), (64, 8): (6, 36, 155, 3156), 0: (60, 167, 146, 220), "0, results that copies take": (60, 167, 160, 224),
+}
+
+
+@pytest.mark.parametrize("grouped", [False, True])
+@pytest.mark.parametrize("form", FORMS, ids=str)
+def test_every_form_is_exact_on_whole_numbers(form, grouped):
+    """Each kernel, tile and way to cut K, at sizes that nothing divides: stored, added, gated, activated, in both types, rows that TMA stores
+    and rows that it does not."""
+    E, r, N, K_ = (GROUPED_FORMS if grouped else FORMS)[form]
+    sms = K().sm_count()
+    got = K().lib().leb_linear_e4m3_form(E, r, N, K_, sms)
+    if sms == 148:
+        assert got == (form[0] | form[1] << 16 if type(form) is tuple else 0)
+    M = E * r
+    counts = [r] * E
+    if grouped and E > 2:              # as many rows in all, shared out unevenly
+        counts[0], counts[1], counts[-1] = 0, counts[1] + (r + 1) // 2, counts[-1] + r // 2
+    off = torch.tensor([sum(counts[:e]) for e in range(E + 1)], dtype=torch.int32, device=DEV) if grouped else None
+    apart = -(-K_ // 16) * 16
+    x, xv = whole_numbers(M, K_, 1, apart)
+    w, wv = whole_numbers(E * N, K_, 2, apart)
+    sx, sw = powers(M, 4).to(DEV), powers(E * N, 3).to(DEV)
+    xd, wd = xv.to(DEV) * sx.double()[:, None], wv.to(DEV) * sw.double()[:, None]
+    z = torch.cat([xd[sum(counts[:e]):sum(counts[:e + 1])] @ wd[e * N:(e + 1) * N].T for e in range(E)]) if grouped else xd @ wd.T
+    args = (x, sx, torch.as_strided(w, (E, N, K_), (N * apart, apart, 1)), sw.view(E, N)) if grouped else (x, sx, w, sw)
+    for ldc in (-(-N // 8) * 8, N):
+        out, whole = room(M, N, ldc, F32, 5)
+        K().linear_e4m3(out, *args, group_offsets=off)
+        assert torch.equal(out.double(), z)
+        K().linear_e4m3(out, *args, K().ACCUMULATE, group_offsets=off)
+        assert torch.equal(out.double(), 2 * z) and bool((between(whole, M, N, ldc) == 5).all())
+        out, whole = room(M, N, ldc, BF16, 5)
+        K().linear_e4m3(out, *args, group_offsets=off)
+        assert torch.equal(out, z.float().to(BF16)) and bool((between(whole, M, N, ldc) == 5).all())
+        K().linear_e4m3(out, *args, K().plain_act_epilogue(K().PLAIN_ACTIVATIONS["relu_squared"]), group_offsets=off)
+        # (a square of up to 2^21 is rounded to float once, and to bfloat16)
+        want = z.clamp(min=0) ** 2
+        assert bool(((out.double() - want).abs() <= (2.0 ** -8 + 2.0 ** -24) * 1.01 * want).all())
+    n = N // 32 * 32                   # gated: whole blocks of 32 rows of every expert's weights
+    w3 = torch.as_strided(w, (E, n, K_), (n * apart, apart, 1)) if grouped else w[:n]
+    wv3 = wv.to(DEV).reshape(-1)[:E * n * K_].view(E, n, K_)
+    s3 = sw[:E * n] / 1024
+    z3 = torch.cat([xd[sum(counts[:e]):sum(counts[:e + 1])] @ (wv3[e] * s3[e * n:(e + 1) * n].double()[:, None]).T for e in range(E)]) if grouped else xd @ (wv3[0] * s3.double()[:, None]).T
+    want, b = P.gated(z3, "silu"), z3.reshape(M, -1, 2, 16)
+    size = (b[:, :, 0].abs() * b[:, :, 1].abs()).reshape(M, -1)
+    for dtype in (F32, BF16):
+        for ldc in (n // 2, n // 2 + 1):
+            out, whole = room(M, n // 2, ldc, dtype, 5)
+            K().linear_e4m3(out, x, sx, w3, s3.view(E, n) if grouped else s3, K().gated_epilogue(K().SILU), group_offsets=off)
+            half = 2.0 ** -8 if dtype is BF16 else 2.0 ** -24
+            assert bool(((out.double() - want).abs() <= half * 1.01 * want.abs() + 2.0 ** -19 * size + 1e-30).all())
+            assert bool((between(whole, M, n // 2, ldc) == 5).all())
+    K().check_device_status()
+
+
 @pytest.mark.parametrize("pitch", [16, 1])
 def test_offsets_that_are_not_in_order_touch_nothing_else(pitch):
     """Offsets that fall, are negative or go beyond the rows: some rows get some expert's numbers, nothing beyond out is written."""
