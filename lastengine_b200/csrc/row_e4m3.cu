@@ -61,7 +61,7 @@ __device__ __forceinline__ long long source_row(const int* rows, int p, int div,
 template <typename T, int V>
 struct Some {
   T v[V];
-  __device__ __forceinline__ void load(const T* p, int n) {
+  __device__ __forceinline__ void load(const T* p, int n, bool = false) {
 #pragma unroll
     for (int i = 0; i < V; i++) v[i] = i < n ? p[i] : from_f32<T>(0.f);
   }
@@ -73,12 +73,18 @@ struct Some {
   }
   __device__ __forceinline__ float at(int i) const { return to_f32(v[i]); }
 };
+// Sixteen bytes that nobody reads again, past L1.
+__device__ __forceinline__ float4 load4_once(const float* p) {
+  float4 v;
+  asm volatile("ld.global.L1::no_allocate.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "l"(p) : "memory");
+  return v;
+}
 template <>
 struct Some<float, 8> {
   float v[8];
-  __device__ __forceinline__ void load(const float* p, int n) {
+  __device__ __forceinline__ void load(const float* p, int n, bool once = false) {
     if (n >= 8) {
-      const float4 a = load4(p), b = load4(p + 4);
+      const float4 a = once ? load4_once(p) : load4(p), b = once ? load4_once(p + 4) : load4(p + 4);
       v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
     } else {
 #pragma unroll
@@ -96,7 +102,7 @@ struct Some<float, 8> {
 template <>
 struct Some<bf16, 8> {      // two numbers a word
   uint32_t u[4];
-  __device__ __forceinline__ void load(const bf16* p, int n) {
+  __device__ __forceinline__ void load(const bf16* p, int n, bool = false) {
     if (n >= 8) {
       const uint4 r = *reinterpret_cast<const uint4*>(p);
       u[0] = r.x, u[1] = r.y, u[2] = r.z, u[3] = r.w;
@@ -155,7 +161,7 @@ __global__ void __launch_bounds__(512) quantize_kernel(uint8_t* __restrict__ q, 
   Some<TX, V> v[C];
   if (CH > 0) {
 #pragma unroll
-    for (int c = 0; c < C; c++) v[c].load(xi + (tid + c * T) * V, width - (tid + c * T) * V);
+    for (int c = 0; c < C; c++) v[c].load(xi + (tid + c * T) * V, width - (tid + c * T) * V, true);
 #pragma unroll
     for (int c = 0; c < C; c++) top = max(top, v[c].top());
   } else {
@@ -257,7 +263,7 @@ __global__ void __launch_bounds__(512) rmsnorm_e4m3_kernel(uint8_t* __restrict__
 
 // How rows of D numbers are shared out: GO(V, CH, ROWS, blocks, threads).  Few rows: many threads a row, whose loads are one trip to memory.
 // Many rows: few threads a row with many loads each, so that threads seldom wait for one another (8,191 bfloat16 rows of 8,192:
-// 512 threads with two pieces 54 us, FEWER_US).  CH_MANY pieces a thread at most then; four numbers a piece where rows begin anywhere.
+// 512 threads with two pieces 54 us, 128 with eight 32).  CH_MANY pieces a thread at most then; four numbers a piece where rows begin anywhere.
 #define MANY_ROWS 1024
 #define ROW_SHAPES(wide, fours, D, rows, CH_MANY)                                          \
   if (wide && D <= 256) GO(8, 1, 8, ceil_div(rows, 8), 256);                               \
@@ -273,6 +279,10 @@ __global__ void __launch_bounds__(512) rmsnorm_e4m3_kernel(uint8_t* __restrict__
   else if (wide && D <= 8192) GO(8, 2, 1, rows, 512);                                      \
   else if (wide && D <= 16384) GO(8, 4, 1, rows, 512);                                     \
   else if (fours && D <= 512) GO(4, 4, 8, ceil_div(rows, 8), 256);                         \
+  else if (fours && rows >= MANY_ROWS && D <= 1024) GO(4, 8, 8, ceil_div(rows, 8), 256);   \
+  else if (fours && rows >= MANY_ROWS && D <= 2048) GO(4, 8, 1, rows, 64);                 \
+  else if (fours && rows >= MANY_ROWS && D <= 4096) GO(4, 8, 1, rows, 128);                \
+  else if (fours && rows >= MANY_ROWS && D <= 8192) GO(4, 8, 1, rows, 256);                \
   else if (fours && D <= 2048) GO(4, 4, 1, rows, 128);                                     \
   else if (fours && D <= 4096) GO(4, 4, 1, rows, 256);                                     \
   else if (fours && D <= 8192) GO(4, 4, 1, rows, 512);                                     \
