@@ -5,16 +5,16 @@ namespace {
 
 // Which kernel takes a product of `groups` times about `rows` rows: the one that is through first, by what either takes (us).
 //
-// weights first (tiles of 128 columns by 16 to 128 rows; s blocks share a tile's K, all of them on the SMs at once: two an SM, one with 128
-// rows, and clusters of eight only where no part of the chip has to take more of them than fit), c blocks an SM, b stages of 128 numbers of
-// k a block, `held` of them on their way at a time:
-//   2.2 + b max((0.95 + 1.2 min(c, 2)) / held, c (0.215 + 0.0003 rows) where c > 1) + max(c, 1) rows' (0.0175 / s + 0.028 in a cluster)
-//       + 0.4 for a cluster      (rows' those of a tile that there are)
+// weights first (tiles of 128 columns by 16 to 128 rows; s blocks share a tile's K, all of them on the SMs at once, clusters of eight only
+// where no part of the chip has to take more of them than fit), c blocks an SM, b stages of 128 numbers of k a block, `held` of them on
+// their way at a time:
+//   2.4 + b max((0.8 + 1.4 min(c, 2)) / held, 0.18 + 0.0004 rows, c (0.25 + 0.0005 rows) where c > 1)
+//       + max(c, 1) rows' (0.016 / s + 0.024 in a cluster) + 0.38 for a cluster      (rows' those of a tile that there are)
 // pairs of SMs (tiles of 256 x 256), w of them a pair:
-//   3.5 + w (0.34 b + 2.4)
-// Fitted to 110 products of 1 to 2,000 rows, 64 to 24,000 columns and K of 128 to 12,000, each in every form that it has; over these and 58
-// grouped ones (2 to 128 experts of 0.5 to 400 rows) the choice takes 1.8% more time than the best form of each.  Where it turns: 61 rows
-// x 2,048 x 2,048 weights first 5.8 us, pairs 10.3; 512 rows x 16,384 x 2,048 23 and 17.4.
+//   2.9 + w (0.34 b + 2.6)
+// Fitted to 203 products of 1 to 2,500 rows, 64 to 24,000 columns and K of 128 to 12,000, each in every form that it has; over these and 58
+// grouped ones (2 to 128 experts of 0.5 to 400 rows) the choice takes 2.5% more time than the best form of each.  Where it turns: 61 rows
+// x 2,048 x 2,048 weights first 5.8 us, pairs 10.3; 512 rows x 16,384 x 2,048 23 and 16.2.
 struct Form {
   bool pairs;
   int rows, slices;      // of the weights-first kernel
@@ -25,20 +25,23 @@ Form form_of(int groups, int rows, int N, int K, int sms) {
   Form best{false, 16, 1};
   double least = 1e30;
   for (int mp = 16; mp <= 128; mp *= 2) {
-    if ((mp > 16 && mp >= 2 * rows) || (mp < 128 && ceil_div(rows, mp) > 8)) continue;
+    if ((mp > 16 && mp >= 2 * rows) || (mp == 16 && rows > 128) || (mp == 32 && rows > 768)) continue;
     const long long tiles = (long long)groups * ceil_div(rows, mp) * ceil_div(N, 128);
     const double there = rows < mp ? rows : mp;
     for (int s = 1; s <= 8; s *= 2) {
-      if (s > 1 && (tiles * s > (mp == 128 ? sms : s == 8 ? sms * 13 / 8 : 2 * sms) || nk < 2 * s)) break;
-      const double c = (double)tiles * s / sms, alone = (0.95 + 1.2 * (c < 2 ? c : 2)) / few_stages(mp, s > 1), shared = c > 1 ? c * (0.215 + 0.0003 * mp) : 0;
-      const double us = 2.2 + ceil_div(nk, s) * (alone > shared ? alone : shared) + (c > 1 ? c : 1) * there * (0.0175 / s + (s > 1 ? 0.028 : 0)) + (s > 1 ? 0.4 : 0);
+      if (s > 1 && (mp == 128 || tiles * s > (s == 8 ? sms * 13 / 8 : 2 * sms) || nk < 2 * s)) break;
+      const double c = (double)tiles * s / sms, alone = (0.8 + 1.4 * (c < 2 ? c : 2)) / few_stages(mp, s > 1, tiles <= sms);
+      double stage = 0.18 + 0.0004 * mp;
+      if (alone > stage) stage = alone;
+      if (c > 1 && c * (0.25 + 0.0005 * mp) > stage) stage = c * (0.25 + 0.0005 * mp);
+      const double us = 2.4 + ceil_div(nk, s) * stage + (c > 1 ? c : 1) * there * (0.016 / s + (s > 1 ? 0.024 : 0)) + (s > 1 ? 0.38 : 0);
       if (us < least) least = us, best = Form{false, mp, s};
     }
   }
   if (rows < 40) return best;
   const int pairs = sms / 2 > 0 ? sms / 2 : 1;
   const long long turns = ((long long)groups * ceil_div(rows, 256) * ceil_div(N, 256) + pairs - 1) / pairs;
-  best.pairs = 3.5 + turns * (0.34 * nk + 2.4) < least;
+  best.pairs = 2.9 + turns * (0.34 * nk + 2.6) < least;
   return best;
 }
 

@@ -382,23 +382,29 @@ int launch_few(const E8Product& p, int n_slices, cudaStream_t st) {
   return 0;
 }
 
-template <typename TC, int MP, bool GROUPED>
-int launch_few_rows(const E8Product& p, int n_slices, cudaStream_t st) {
-  if (n_slices > 1) return launch_few<TC, MP, few_stages(MP, true), MP == 128 ? 1 : 2, GROUPED, true>(p, n_slices, st);
-  return launch_few<TC, MP, few_stages(MP, false), 2, GROUPED, false>(p, 1, st);
+template <typename TC, int MP, bool GROUPED, bool CLUSTER, bool FEW_TILES>
+int launch_few_form(const E8Product& p, int n_slices, cudaStream_t st) {
+  return launch_few<TC, MP, few_stages(MP, CLUSTER, FEW_TILES), few_alone(MP, CLUSTER, FEW_TILES) ? 1 : 2, GROUPED, CLUSTER>(p, n_slices, st);
 }
 template <typename TC, bool GROUPED>
-int launch_few_rows(const E8Product& p, int mp, int n_slices, cudaStream_t st) {
-  if (mp == 16) return launch_few_rows<TC, 16, GROUPED>(p, n_slices, st);
-  if (mp == 32) return launch_few_rows<TC, 32, GROUPED>(p, n_slices, st);
-  if (mp == 64) return launch_few_rows<TC, 64, GROUPED>(p, n_slices, st);
-  return launch_few_rows<TC, 128, GROUPED>(p, n_slices, st);
+int launch_few_rows(const E8Product& p, int mp, int n_slices, bool few_tiles, cudaStream_t st) {
+  if (n_slices > 1) {
+    if (mp == 16) return launch_few_form<TC, 16, GROUPED, true, false>(p, n_slices, st);
+    if (mp == 32) return launch_few_form<TC, 32, GROUPED, true, false>(p, n_slices, st);
+    return launch_few_form<TC, 64, GROUPED, true, false>(p, n_slices, st);
+  }
+  if (mp == 16) return launch_few_form<TC, 16, GROUPED, false, false>(p, 1, st);
+  if (mp == 32) return launch_few_form<TC, 32, GROUPED, false, false>(p, 1, st);
+  if (mp == 128) return launch_few_form<TC, 128, GROUPED, false, false>(p, 1, st);
+  return few_tiles ? launch_few_form<TC, 64, GROUPED, false, true>(p, 1, st) : launch_few_form<TC, 64, GROUPED, false, false>(p, 1, st);
 }
 
 }  // namespace
 
-// mp: 16, 32, 64 or 128 rows of A a tile; n_slices: 1, 2, 4 or 8 blocks that share a tile's K.
+// mp: 16, 32, 64 or 128 rows of A a tile; n_slices: 1, 2, 4 or 8 blocks that share a tile's K (1 with 128 rows).
 int leb_gemm_e4m3_few(const E8Product& p, int mp, int n_slices, cudaStream_t st) {
-  if (p.c_dtype == LEB_F32) return p.offsets ? launch_few_rows<float, true>(p, mp, n_slices, st) : launch_few_rows<float, false>(p, mp, n_slices, st);
-  return p.offsets ? launch_few_rows<bf16, true>(p, mp, n_slices, st) : launch_few_rows<bf16, false>(p, mp, n_slices, st);
+  const int groups = p.offsets ? min(p.n_groups, p.M) : 1;
+  const bool few_tiles = (long long)groups * ceil_div(ceil_div(p.M, groups), mp) * ceil_div(p.N, 128) <= sm_count();
+  if (p.c_dtype == LEB_F32) return p.offsets ? launch_few_rows<float, true>(p, mp, n_slices, few_tiles, st) : launch_few_rows<float, false>(p, mp, n_slices, few_tiles, st);
+  return p.offsets ? launch_few_rows<bf16, true>(p, mp, n_slices, few_tiles, st) : launch_few_rows<bf16, false>(p, mp, n_slices, few_tiles, st);
 }
