@@ -278,13 +278,14 @@ __global__ void __launch_bounds__(512) rmsnorm_e4m3_kernel(uint8_t* __restrict__
   else if (wide && D <= 4096) GO(8, 1, 1, rows, 512);                                      \
   else if (wide && D <= 8192) GO(8, 2, 1, rows, 512);                                      \
   else if (wide && D <= 16384) GO(8, 4, 1, rows, 512);                                     \
-  else if (fours && D <= 512) GO(4, 4, 8, ceil_div(rows, 8), 256);                         \
+  else if (fours && rows >= MANY_ROWS && D <= 512) GO(4, 4, 8, ceil_div(rows, 8), 256);    \
   else if (fours && rows >= MANY_ROWS && D <= 1024) GO(4, 8, 8, ceil_div(rows, 8), 256);   \
   else if (fours && rows >= MANY_ROWS && D <= 2048) GO(4, 8, 1, rows, 64);                 \
   else if (fours && rows >= MANY_ROWS && D <= 4096) GO(4, 8, 1, rows, 128);                \
   else if (fours && rows >= MANY_ROWS && D <= 8192) GO(4, 8, 1, rows, 256);                \
-  else if (fours && D <= 2048) GO(4, 4, 1, rows, 128);                                     \
-  else if (fours && D <= 4096) GO(4, 4, 1, rows, 256);                                     \
+  else if (fours && D <= 512) GO(4, 1, 1, rows, 128);                                      \
+  else if (fours && D <= 2048) GO(4, 1, 1, rows, 512);                                     \
+  else if (fours && D <= 4096) GO(4, 2, 1, rows, 512);                                     \
   else if (fours && D <= 8192) GO(4, 4, 1, rows, 512);                                     \
   else if (fours && D <= 16384) GO(4, 8, 1, rows, 512);                                    \
   else if (D <= 4096) GO(1, 8, 1, rows, 512);                                              \

@@ -2274,6 +2274,7 @@ def e4m3_rows(*shape: int, device=None) -> torch.Tensor:
 _PACK_QUANTIZE, _PACK_NORM, _PACK_LINEAR = (struct.Struct(f).pack for f in ("12q", "11qd", "17q"))
 
 
+# A call costs the host some 7 us, more than half of it Python: what is checked on the way is written out, what is wrong is said apart.
 def _not_here(name: str, **tensors: torch.Tensor | None) -> None:
     """Raises if a tensor of a call is not on the current device, which the call launches on."""
     for what, t in tensors.items():
@@ -2285,19 +2286,18 @@ def _not_here(name: str, **tensors: torch.Tensor | None) -> None:
             raise KernelError(f"{name}.{what}: tensor is on {t.device}, the current device is cuda:{here}")
 
 
-def _vector(name: str, t: torch.Tensor, dtype: torch.dtype, shape: tuple) -> None:
-    if t.dtype is not dtype or t.shape != shape or not t.is_contiguous():
-        raise KernelError(f"{name}: expected contiguous {dtype} {shape}, got {t.dtype} {tuple(t.shape)}")
+def _not_vector(name: str, t: torch.Tensor, dtype: torch.dtype, shape: tuple) -> None:
+    raise KernelError(f"{name}: expected contiguous {dtype} {shape}, got {t.dtype} {tuple(t.shape)}")
 
 
 def _pitch(name: str, t: torch.Tensor, shape: tuple, written: bool = False) -> int:
     """How far the rows of a matrix of neighbouring numbers (or of each of a stack of them) lie apart; rows that are written do not overlap."""
     if t.shape != shape:
         raise KernelError(f"{name}: expected {shape}, got {tuple(t.shape)}")
-    *_, step, inner = t.stride()
-    K = shape[-1]
-    if inner != 1 and K > 1:
-        raise KernelError(f"{name}: the numbers of a row must be neighbours, they are {inner} apart")
+    stride, K = t.stride(), shape[-1]
+    step = stride[-2]
+    if stride[-1] != 1 and K > 1:
+        raise KernelError(f"{name}: the numbers of a row must be neighbours, they are {stride[-1]} apart")
     if shape[-2] <= 1:      # (where a row behind the only one would lie)
         return -(-K // 16) * 16
     if written and step < K:
@@ -2310,6 +2310,10 @@ def _stream_on(device: int) -> int:
     return _raw_stream(device) if _raw_stream is not None else _stream()
 
 
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device      # (asked with a CUDA tensor at hand)
+_FLOAT, _INT32 = torch.float32, torch.int32
+
+
 def quantize_e4m3(out: torch.Tensor, scale: torch.Tensor, x: torch.Tensor, rows: torch.Tensor | None = None, div: int = 1,
                   weights: torch.Tensor | None = None) -> None:
     """Rows of x [M, K] (float or bfloat16) in 8 bits: out [P, K] = round(448 x / a) and scale [P] = a / 448 (float) with
@@ -2317,7 +2321,7 @@ def quantize_e4m3(out: torch.Tensor, scale: torch.Tensor, x: torch.Tensor, rows:
     `weights` (float) its scale is multiplied by weights[rows[p]].  A row of x with a number that is not finite, and one that
     `rows` does not find in x, gets numbers and a scale that are NaN.  Numbers are rounded to the nearest, ties to even."""
     here = x.get_device()
-    if (here < 0 or out.get_device() != here or scale.get_device() != here or here != torch.cuda.current_device()
+    if (here < 0 or out.get_device() != here or scale.get_device() != here or here != _current_device()
             or (rows is not None and (rows.get_device() != here or (weights is not None and weights.get_device() != here)))):
         _not_here("quantize_e4m3", out=out, scale=scale, x=x, rows=rows, weights=weights)
     if x.dim() != 2 or out.dim() != 2 or out.dtype is not E4M3:
@@ -2325,9 +2329,11 @@ def quantize_e4m3(out: torch.Tensor, scale: torch.Tensor, x: torch.Tensor, rows:
     M, K = x.shape
     P_ = out.shape[0]
     ldx, ldq = _pitch("quantize_e4m3.x", x, (M, K)), _pitch("quantize_e4m3.out", out, (P_, K), True)
-    _vector("quantize_e4m3.scale", scale, torch.float32, (P_,))
+    if scale.dtype is not _FLOAT or scale.shape != (P_,) or not scale.is_contiguous():
+        _not_vector("quantize_e4m3.scale", scale, _FLOAT, (P_,))
     if rows is not None:
-        _vector("quantize_e4m3.rows", rows, torch.int32, (P_,))
+        if rows.dtype is not _INT32 or rows.shape != (P_,) or not rows.is_contiguous():
+            _not_vector("quantize_e4m3.rows", rows, _INT32, (P_,))
         if div < 1:
             raise KernelError(f"quantize_e4m3: div is {div}, at least 1 is wanted")
         if weights is not None and (weights.dtype != torch.float32 or not weights.is_contiguous() or weights.numel() < M * div):
@@ -2351,7 +2357,7 @@ def rmsnorm_e4m3(out: torch.Tensor, scale: torch.Tensor, x: torch.Tensor, w: tor
     or bfloat16, contiguous) the launch also leaves there the normed rows r g, for readers that want more than 8 bits (a router).
     A row with a number that is not finite (or squares whose sum is not) gets numbers and a scale that are NaN."""
     here = x.get_device()
-    if (here < 0 or out.get_device() != here or scale.get_device() != here or w.get_device() != here or here != torch.cuda.current_device()
+    if (here < 0 or out.get_device() != here or scale.get_device() != here or w.get_device() != here or here != _current_device()
             or (y is not None and y.get_device() != here) or (h is not None and h.get_device() != here)):
         _not_here("rmsnorm_e4m3", out=out, scale=scale, x=x, w=w, y=y, h=h)
     if x.dim() != 2 or x.dtype is not torch.float32 or not x.is_contiguous():
@@ -2360,8 +2366,10 @@ def rmsnorm_e4m3(out: torch.Tensor, scale: torch.Tensor, x: torch.Tensor, w: tor
         raise KernelError(f"rmsnorm_e4m3.out: expected rows of {E4M3}, got {out.dtype} {tuple(out.shape)}")
     M, D = shape = x.shape
     ldq = _pitch("rmsnorm_e4m3.out", out, shape, True)
-    _vector("rmsnorm_e4m3.scale", scale, torch.float32, (M,))
-    _vector("rmsnorm_e4m3.w", w, torch.float32, (D,))
+    if scale.dtype is not _FLOAT or scale.shape != (M,) or not scale.is_contiguous():
+        _not_vector("rmsnorm_e4m3.scale", scale, _FLOAT, (M,))
+    if w.dtype is not _FLOAT or w.shape != (D,) or not w.is_contiguous():
+        _not_vector("rmsnorm_e4m3.w", w, _FLOAT, (D,))
     yd = hd = F32
     if y is not None:
         yd = _DT.get(y.dtype, -1)
@@ -2392,7 +2400,7 @@ def linear_e4m3(out: torch.Tensor, x: torch.Tensor, x_scale: torch.Tensor, w: to
     depend, in their last bits, on how many rows the call has."""
     here = x.get_device()
     if (here < 0 or out.get_device() != here or x_scale.get_device() != here or w.get_device() != here or w_scale.get_device() != here
-            or here != torch.cuda.current_device() or (group_offsets is not None and group_offsets.get_device() != here)):
+            or here != _current_device() or (group_offsets is not None and group_offsets.get_device() != here)):
         _not_here("linear_e4m3", out=out, x=x, x_scale=x_scale, w=w, w_scale=w_scale, group_offsets=group_offsets)
     if x.dtype is not E4M3 or w.dtype is not E4M3 or x.dim() != 2 or out.dim() != 2:
         raise KernelError(f"linear_e4m3: expected matrices and operands of {E4M3}, got out {tuple(out.shape)}, x {x.dtype} {tuple(x.shape)}, w {w.dtype}")
@@ -2406,11 +2414,14 @@ def linear_e4m3(out: torch.Tensor, x: torch.Tensor, x_scale: torch.Tensor, w: to
         if w.dim() != 3:
             raise KernelError(f"linear_e4m3: w is {tuple(w.shape)} for groups of rows")
         E, N = w.shape[:2]
-        _vector("linear_e4m3.group_offsets", group_offsets, torch.int32, (E + 1,))
+        if group_offsets.dtype is not _INT32 or group_offsets.shape != (E + 1,) or not group_offsets.is_contiguous():
+            _not_vector("linear_e4m3.group_offsets", group_offsets, _INT32, (E + 1,))
         ldw, scales, offsets = _pitch("linear_e4m3.w", w, (E, N, K)), (E, N), group_offsets.data_ptr()
         stride = w.stride(0) if E > 1 else N * ldw
-    _vector("linear_e4m3.w_scale", w_scale, torch.float32, scales)
-    _vector("linear_e4m3.x_scale", x_scale, torch.float32, (M,))
+    if w_scale.dtype is not _FLOAT or w_scale.shape != scales or not w_scale.is_contiguous():
+        _not_vector("linear_e4m3.w_scale", w_scale, _FLOAT, scales)
+    if x_scale.dtype is not _FLOAT or x_scale.shape != (M,) or not x_scale.is_contiguous():
+        _not_vector("linear_e4m3.x_scale", x_scale, _FLOAT, (M,))
     gated = (epilogue & 255) == SWIGLU
     if gated and N % 32:
         raise KernelError(f"linear_e4m3: gate and up rows come in blocks of 16 each, w has {N} rows")
