@@ -98,7 +98,8 @@ __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 
-// Rows grouped by expert: the offsets, held to the rows that there are, and the running count of tiles of `tile_rows` rows.
+// Rows grouped by expert: the offsets, and the running count of tiles of `tile_rows` rows.  Offsets are held to the rows that there are, and to
+// begin where the experts before have ended: whatever they hold, a row has one expert at most and no tile lies elsewhere.
 struct E8Groups {
   int off[E8_MAX_GROUPS + 1];      // first row of every expert
   int end[E8_MAX_GROUPS];          // behind its last
@@ -106,30 +107,48 @@ struct E8Groups {
 };
 // All threads of the block; the offsets have been written by now.  Two barriers.
 __device__ __forceinline__ void e8_count_groups(E8Groups& g, const int* __restrict__ offsets, int n_groups, int M, int tile_rows, int n_tiles) {
+  constexpr int EACH = E8_MAX_GROUPS / 32;      // experts a lane
   for (int e = threadIdx.x; e < n_groups; e += blockDim.x) {
-    const int lo = min(max(offsets[e], 0), M), hi = min(max(offsets[e + 1], lo), M);
-    g.off[e] = lo;
-    g.end[e] = hi;
+    g.off[e] = min(max(offsets[e], 0), M);
+    g.end[e] = min(max(offsets[e + 1], 0), M);
   }
   __syncthreads();
-  if (threadIdx.x < 32) {      // eight experts a lane
-    int n[E8_MAX_GROUPS / 32], sum = 0;
+  if (threadIdx.x < 32) {
+    const int lane = threadIdx.x;
+    int last = 0;      // the furthest end of the experts before this lane's
+    for (int i = 0; i < EACH; i++)
+      if (lane * EACH + i < n_groups) last = max(last, g.end[lane * EACH + i]);
 #pragma unroll
-    for (int i = 0; i < E8_MAX_GROUPS / 32; i++) {
-      const int e = threadIdx.x * (E8_MAX_GROUPS / 32) + i;
-      n[i] = e < n_groups ? (g.end[e] - g.off[e] + tile_rows - 1) / tile_rows * n_tiles : 0;
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, last, o);
+      if (lane >= o) last = max(last, v);
+    }
+    last = __shfl_up_sync(0xffffffffu, last, 1);
+    if (lane == 0) last = 0;
+    int n[EACH], sum = 0;
+#pragma unroll
+    for (int i = 0; i < EACH; i++) {
+      const int e = lane * EACH + i;
+      n[i] = 0;
+      if (e < n_groups) {
+        const int lo = max(g.off[e], last), hi = max(g.end[e], lo);
+        last = max(last, g.end[e]);
+        g.off[e] = lo;
+        g.end[e] = hi;
+        n[i] = (hi - lo + tile_rows - 1) / tile_rows * n_tiles;
+      }
       sum += n[i];
     }
     int before = sum;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int v = __shfl_up_sync(0xffffffffu, before, o);
-      if ((int)threadIdx.x >= o) before += v;
+      if (lane >= o) before += v;
     }
     before -= sum;
 #pragma unroll
-    for (int i = 0; i < E8_MAX_GROUPS / 32; i++) {
-      const int e = threadIdx.x * (E8_MAX_GROUPS / 32) + i;
+    for (int i = 0; i < EACH; i++) {
+      const int e = lane * EACH + i;
       if (e < n_groups) g.cum[e] = before;
       before += n[i];
       if (e == n_groups - 1) g.cum[n_groups] = before;

@@ -16,9 +16,16 @@ __global__ void __launch_bounds__(256) gemm_e4m3_any_kernel(TC* __restrict__ C, 
   epilogue &= 255;
   pdl_wait();
   int lo = 0, hi = M;
-  if (offsets) {      // rows [offsets[e], offsets[e + 1]) go with expert e's weights (whatever the offsets hold, no row beyond the M is touched)
+  if (offsets) {      // rows [offsets[e], offsets[e + 1]) go with expert e's weights, from where the experts before have ended on (whatever the offsets hold)
     const int e = blockIdx.x / m_tiles;
-    lo = max(offsets[e], 0);
+    __shared__ int ends[8];
+    int last = 0;
+    for (int i = threadIdx.x + 1; i <= e; i += 256) last = max(last, min(offsets[i], M));
+    last = __reduce_max_sync(0xffffffffu, last);
+    if ((threadIdx.x & 31) == 0) ends[threadIdx.x >> 5] = last;
+    __syncthreads();
+    for (int i = 0; i < 8; i++) last = max(last, ends[i]);
+    lo = max(min(offsets[e], M), last);
     hi = min(offsets[e + 1], M);
     W += e * w_group_stride;
     sw += (size_t)e * N;

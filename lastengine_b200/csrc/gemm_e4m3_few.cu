@@ -362,7 +362,7 @@ int launch_few(const E8Product& p, int n_slices, cudaStream_t st) {
   const long long m_tiles = p.M / MP + (GROUPED ? min(p.n_groups, p.M) : (p.M % MP != 0)), tiles = m_tiles * ceil_div(p.N, 128);
   long long clusters = tiles;
   if (n_slices == 1 && tiles > (long long)sm_count() * PER_SM) clusters = (long long)sm_count() * PER_SM;
-  if (clusters * n_slices >= 1LL << 31) return leb_fail("leb_linear_e4m3: %lld tiles", tiles);
+  if (tiles >= 1LL << 30 || clusters * n_slices >= 1LL << 31) return leb_fail("leb_linear_e4m3: %lld tiles", tiles);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(clusters * n_slices));
   cfg.blockDim = dim3(FEW_THREADS);

@@ -376,6 +376,7 @@ int launch_pairs(const E8Product& p, cudaStream_t st) {
     if (r != CUDA_SUCCESS) return leb_fail("leb_linear_e4m3: cuTensorMapEncodeTiled failed (%d) for the results [%d,%d] rows %lld apart", (int)r, p.M, n_out, p.ldc);
   }
   const long long m_tiles = p.M / 256 + (GROUPED ? min(p.n_groups, p.M) : (p.M % 256 != 0)), tiles = m_tiles * ceil_div(p.N, 256);
+  if (tiles >= 1LL << 30) return leb_fail("leb_linear_e4m3: %lld tiles", tiles);
   const long long pairs = tiles < sm_count() / 2 ? tiles : sm_count() / 2;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(2 * pairs));

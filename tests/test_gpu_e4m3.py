@@ -398,16 +398,22 @@ def test_every_form_is_exact_on_whole_numbers(form, grouped):
 
 @pytest.mark.parametrize("pitch", [16, 1])
 def test_offsets_that_are_not_in_order_touch_nothing_else(pitch):
-    """Offsets that fall, are negative or go beyond the rows: some rows get some expert's numbers, nothing beyond out is written."""
-    E, N, K_, M = 4, 96, 64, 50
+    """Offsets that fall, are negative or go beyond the rows: a row gets numbers of an expert or stays, nothing beyond out is written."""
+    E, N, K_ = 4, 96, 64
     apart = 64 if pitch == 16 else 65
-    x, xv = whole_numbers(M, K_, 1, apart)
-    w = torch.as_strided(whole_numbers(E * N, K_, 2, apart)[0], (E, N, K_), (N * apart, apart, 1))
-    one, sw = torch.ones(M, device=DEV), torch.ones(E, N, device=DEV)
-    for off in ([0, 40, 10, 60, 2 ** 31 - 1], [-5, 10, 20, 30, 40], [50, 40, 30, 20, 10], [-2 ** 31, 2 ** 31 - 1, 0, 0, 0]):
-        out, whole = room(M, N, N + 3, F32, 5)
-        K().linear_e4m3(out, x, one, w, sw, group_offsets=torch.tensor(off, dtype=torch.int32, device=DEV))
-        assert bool((between(whole, M, N, N + 3) == 5).all())
+    for M, k in ((50, 1), (3000, 60)):
+        x, xv = whole_numbers(M, K_, 1, apart)
+        wq, wv = whole_numbers(E * N, K_, 2, apart)
+        w = torch.as_strided(wq, (E, N, K_), (N * apart, apart, 1))
+        one, sw = torch.ones(M, device=DEV), torch.ones(E, N, device=DEV)
+        z = torch.stack([xv @ wv[e * N:(e + 1) * N].T for e in range(E)]).to(DEV)
+        for off in ([0, 40, 10, 60, 2 ** 31 - 1], [-5, 10, 20, 30, 40], [50, 40, 30, 20, 10], [-2 ** 31, 2 ** 31 - 1, 0, 0, 0], [0, 50, 0, 50, 0]):
+            off = [o * k if abs(o) < 1000 else o for o in off]
+            out, whole = room(M, N, N + 3, F32, 0.5)
+            K().linear_e4m3(out, x, one, w, sw, group_offsets=torch.tensor(off, dtype=torch.int32, device=DEV))
+            assert bool((between(whole, M, N, N + 3) == 0.5).all())
+            row_is = torch.stack([(out.double() == z[e]).all(1) for e in range(E)] + [(out == 0.5).all(1)]).any(0)
+            assert bool(row_is.all())
     K().check_device_status()
 
 
