@@ -1,7 +1,7 @@
 // 8-bit matrix product on tcgen05 with the weights as the 128-row operand: C[m, n] (+)= (sum_k A[m, k] W[n, k]) sa[m] sw[n], dense or
 // with rows grouped by expert.
 //
-// With few rows the product is bound by reading W, so a tile is 128 rows of W by MP rows of A (16 to 256) and the accumulator in
+// With few rows the product is bound by reading W, so a tile is 128 rows of W by MP rows of A (16 to 128) and the accumulator in
 // tensor memory is the transposed tile.  Where there are fewer tiles than SMs a cluster of up to eight blocks shares a tile: each
 // takes a part of K, sends its sums of every row to the block that finishes the row (st.async into its shared memory, counted there on a
 // barrier), and finishes its share of the rows, adding up in the blocks' order.  (With the sums left where they were made, read by
@@ -20,22 +20,22 @@
 #include "e4m3_tc.cuh"
 
 #define FEW_THREADS 192
-#ifndef FEW_AHEAD
+// Stages of W that a block asks L2 for ahead of its wait for the kernel before.  One row x 16,384 x 2,048: 8.9 us with none, 8.2 with 3,
+// 8.5 with 5, 9.6 with all 16, which are in the way of what the kernel before still loads; x 4,096 x 4,096: 6.5, 6.4, 6.1, 6.2.
 #define FEW_AHEAD 5
-#endif
 
 template <typename TC, int MP, int STAGES, int PER_SM, bool GROUPED, bool CLUSTER>
 __global__ void __launch_bounds__(FEW_THREADS, PER_SM)
 gemm_e4m3_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_a, TC* __restrict__ C,
                      const float* __restrict__ sa, const float* __restrict__ sw, int M, int N, int K, long long ldc, int epilogue, int n_slices,
-                     const int* __restrict__ offsets, int n_groups, int ahead, int* __restrict__ status) {
+                     const int* __restrict__ offsets, int n_groups, int* __restrict__ status) {
   constexpr int W_BYTES = 128 * E8_BK, A_BYTES = MP * E8_BK;
   constexpr uint32_t TMEM_COLS = 2 * MP < 32 ? 32 : 2 * MP;
   const int act = epilogue >> 8;
   epilogue &= 255;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-  uint8_t *s_w = smem, *s_a = smem + STAGES * W_BYTES, *s_part = s_a + STAGES * A_BYTES;      // part: the sums that are being finished
+  uint8_t *s_w = smem, *s_a = smem + STAGES * W_BYTES, *s_part = s_a + STAGES * A_BYTES;      // part: the sums that a cluster's blocks have sent
   __shared__ uint64_t full[STAGES], empty[STAGES], acc_full[2], acc_empty[2], parts_full, drained;
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_s, sent_s, parts_s;
@@ -81,7 +81,7 @@ gemm_e4m3_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
   if (CLUSTER) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");      // this block's barriers exist (waited for before sums are sent)
   pdl_trigger();      // (not before tensor memory is this block's: the next kernel's blocks may hold theirs while they wait for this one)
   if (!GROUPED && warp == 0 && first < num_tiles && elect_lane())      // the first tile's weights, on their way to L2 while the kernel before ends
-    for (int i = 0; i < min(my_nk, ahead); i++) tma_prefetch_2d(&map_w, (kb_lo + i) * E8_BK, first / m_tiles * 128);
+    for (int i = 0; i < min(my_nk, FEW_AHEAD); i++) tma_prefetch_2d(&map_w, (kb_lo + i) * E8_BK, first / m_tiles * 128);
   __syncwarp();
   pdl_wait();
   if (GROUPED) {
@@ -376,7 +376,7 @@ int launch_few(const E8Product& p, int n_slices, cudaStream_t st) {
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = g_leb_pdl ? 2 : 1;
-  e = cudaLaunchKernelEx(&cfg, kern, mw, ma, (TC*)p.C, p.sa, p.sw, p.M, p.N, p.K, p.ldc, p.epilogue, n_slices, p.offsets, p.n_groups, FEW_AHEAD, p.status);
+  e = cudaLaunchKernelEx(&cfg, kern, mw, ma, (TC*)p.C, p.sa, p.sw, p.M, p.N, p.K, p.ldc, p.epilogue, n_slices, p.offsets, p.n_groups, p.status);
   if (e != cudaSuccess) return leb_fail("leb_linear_e4m3: %s", cudaGetErrorString(e));
   LEB_CHECK_LAUNCH("leb_linear_e4m3");
   return 0;

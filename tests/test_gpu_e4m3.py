@@ -435,6 +435,31 @@ def test_weights_made_right_before():
     assert float((outs[5].cpu().double() - z).norm() / z.norm()) < 2.0 ** -20
 
 
+def test_places_beyond_32_bits():
+    """Results, rows and 8-bit numbers of more than 2^31 numbers: the last rows are where they belong, and right."""
+    M, N, K_ = 33000, 66016, 64
+    x, xv = whole_numbers(M, K_, 1)
+    w, wv = whole_numbers(N, K_, 2)
+    out = torch.zeros(M, N, dtype=BF16, device=DEV)
+    K().linear_e4m3(out, x, torch.ones(M, device=DEV), w, torch.ones(N, device=DEV))
+    at = [0, 1, 16383, 32767, 32768, M - 1]
+    assert torch.equal(out[at].double().cpu(), (xv[at] @ wv.T).float().to(BF16).double())
+    q, s = K().e4m3_rows(M, N, device=DEV), torch.zeros(M, device=DEV)
+    K().quantize_e4m3(q, s, out)
+    check_rows(q[at], s[at], out[at].cpu())
+    del out, q
+    M, D = 265000, 8192
+    xs = torch.ones(M, D, device=DEV)
+    xs[at] = gen(len(at), D, seed=3).to(DEV)
+    xs[-1] = gen(D, seed=4).to(DEV)
+    at.append(M - 1)
+    keep = xs[at].cpu()
+    q, s = K().e4m3_rows(M, D, device=DEV), torch.zeros(M, device=DEV)
+    K().rmsnorm_e4m3(q, s, xs, torch.ones(D, device=DEV), 1e-5)
+    r = 1 / torch.sqrt((keep.double() ** 2).mean(1) + 1e-5)
+    check_rows(q[at], s[at], keep, r, 2.0 ** -24 * ((D / 32 + 16) / 2 + 6))
+
+
 # ---- together --------------------------------------------------------------------------------------------------------
 def test_a_feed_forward_in_8_bits():
     """norm -> gate and up -> rows -> down into the stream, as a layer runs them; captured and replayed, and on a stream of its own."""
