@@ -263,47 +263,73 @@ __global__ void __launch_bounds__(512) rmsnorm_e4m3_kernel(uint8_t* __restrict__
 
 // How rows of D numbers are shared out: GO(V, CH, ROWS, blocks, threads).  Few rows: many threads a row, whose loads are one trip to memory.
 // Many rows: few threads a row with many loads each, so that threads seldom wait for one another (8,191 bfloat16 rows of 8,192:
-// 512 threads with two pieces 54 us, 128 with eight 32).  CH_MANY pieces a thread at most then; four numbers a piece where rows begin anywhere.
+// 512 threads with two pieces 54 us, 128 with eight 32).
 #define MANY_ROWS 1024
-#define ROW_SHAPES(wide, fours, D, rows, CH_MANY)                                          \
-  if (wide && D <= 256) GO(8, 1, 8, ceil_div(rows, 8), 256);                               \
-  else if (wide && D <= 512) GO(8, 2, 8, ceil_div(rows, 8), 256);                          \
-  else if (wide && rows >= MANY_ROWS && D <= 1024) GO(8, 4, 8, ceil_div(rows, 8), 256);    \
-  else if (wide && rows >= MANY_ROWS && D <= 256 * CH_MANY) GO(8, CH_MANY, 8, ceil_div(rows, 8), 256); \
-  else if (wide && rows >= MANY_ROWS && D <= 512 * CH_MANY) GO(8, CH_MANY, 1, rows, 64);   \
-  else if (wide && rows >= MANY_ROWS && D <= 1024 * CH_MANY) GO(8, CH_MANY, 1, rows, 128); \
-  else if (wide && rows >= MANY_ROWS && D <= 2048 * CH_MANY) GO(8, CH_MANY, 1, rows, 256); \
-  else if (wide && D <= 1024) GO(8, 1, 1, rows, 128);                                      \
+#define FEW_ROW_SHAPES(wide, fours, D, rows)                                               \
+  if (wide && D <= 1024) GO(8, 1, 1, rows, 128);                                           \
   else if (wide && D <= 2048) GO(8, 1, 1, rows, 256);                                      \
   else if (wide && D <= 4096) GO(8, 1, 1, rows, 512);                                      \
   else if (wide && D <= 8192) GO(8, 2, 1, rows, 512);                                      \
   else if (wide && D <= 16384) GO(8, 4, 1, rows, 512);                                     \
-  else if (fours && rows >= MANY_ROWS && D <= 512) GO(4, 4, 8, ceil_div(rows, 8), 256);    \
-  else if (fours && rows >= MANY_ROWS && D <= 1024) GO(4, 8, 8, ceil_div(rows, 8), 256);   \
-  else if (fours && rows >= MANY_ROWS && D <= 2048) GO(4, 8, 1, rows, 64);                 \
-  else if (fours && rows >= MANY_ROWS && D <= 4096) GO(4, 8, 1, rows, 128);                \
-  else if (fours && rows >= MANY_ROWS && D <= 8192) GO(4, 8, 1, rows, 256);                \
   else if (fours && D <= 512) GO(4, 1, 1, rows, 128);                                      \
+  else if (fours && D <= 1024) GO(4, 1, 1, rows, 256);                                     \
   else if (fours && D <= 2048) GO(4, 1, 1, rows, 512);                                     \
   else if (fours && D <= 4096) GO(4, 2, 1, rows, 512);                                     \
   else if (fours && D <= 8192) GO(4, 4, 1, rows, 512);                                     \
   else if (fours && D <= 16384) GO(4, 8, 1, rows, 512);                                    \
   else if (D <= 4096) GO(1, 8, 1, rows, 512);                                              \
   else GO(1, 0, 1, rows, 512);
+#define QUANTIZE_SHAPES(wide, fours, D, rows)                                              \
+  if (wide && D <= 256) GO(8, 1, 8, ceil_div(rows, 8), 256);                               \
+  else if (wide && D <= 512) GO(8, 2, 8, ceil_div(rows, 8), 256);                          \
+  else if (rows < MANY_ROWS) { FEW_ROW_SHAPES(wide, fours, D, rows) }                      \
+  else if (wide && D <= 1024) GO(8, 4, 8, ceil_div(rows, 8), 256);                         \
+  else if (wide && D <= 2048) GO(8, 8, 8, ceil_div(rows, 8), 256);                         \
+  else if (wide && D <= 4096) GO(8, 8, 1, rows, 64);                                       \
+  else if (wide && D <= 8192) GO(8, 8, 1, rows, 128);                                      \
+  else if (wide && D <= 16384) GO(8, 8, 1, rows, 256);                                     \
+  else if (!wide && fours && D <= 512) GO(4, 4, 8, ceil_div(rows, 8), 256);                \
+  else if (!wide && fours && D <= 1024) GO(4, 8, 8, ceil_div(rows, 8), 256);               \
+  else if (!wide && fours && D <= 2048) GO(4, 8, 1, rows, 64);                             \
+  else if (!wide && fours && D <= 4096) GO(4, 8, 1, rows, 128);                            \
+  else if (!wide && fours && D <= 8192) GO(4, 8, 1, rows, 256);                            \
+  else { FEW_ROW_SHAPES(wide, fours, D, rows) }
+// The norm holds its weights beside the row, and what is added: two pieces a thread (2,048 rows of 2,048 with a bfloat16 addition: four pieces
+// 13.3 us, two 10.7; 16,000 rows 59.3 and 56.1, without the addition 31.3 and 29.5; 2,048 rows of 1,001 with it: a warp a row 12.2, four 7.5).
+// Short rows without an addition have little to load: a warp takes one (16,000 rows of 1,024: 15.6 us, two warps 18.9; with the addition
+// 31.8 and 30.0).
+#define NORM_SHAPES(wide, fours, adds, D, rows)                                            \
+  if (wide && D <= 256) GO(8, 1, 8, ceil_div(rows, 8), 256);                               \
+  else if (wide && D <= 512) GO(8, 2, 8, ceil_div(rows, 8), 256);                          \
+  else if (rows < MANY_ROWS) { FEW_ROW_SHAPES(wide, fours, D, rows) }                      \
+  else if (wide && D <= 1024 && !adds) GO(8, 4, 8, ceil_div(rows, 8), 256);                \
+  else if (wide && D <= 1024) GO(8, 2, 1, rows, 64);                                       \
+  else if (wide && D <= 2048) GO(8, 2, 1, rows, 128);                                      \
+  else if (wide && D <= 4096) GO(8, 2, 1, rows, 256);                                      \
+  else if (!wide && fours && D <= 512 && !adds) GO(4, 4, 8, ceil_div(rows, 8), 256);       \
+  else if (!wide && fours && D <= 512) GO(4, 1, 1, rows, 128);                             \
+  else if (!wide && fours && D <= 1024 && !adds) GO(4, 4, 1, rows, 64);                    \
+  else if (!wide && fours && D <= 1024) GO(4, 2, 1, rows, 128);                            \
+  else if (!wide && fours && D <= 2048 && !adds) GO(4, 4, 1, rows, 128);                   \
+  else if (!wide && fours && D <= 2048) GO(4, 2, 1, rows, 256);                            \
+  else if (!wide && fours && D <= 4096) GO(4, 4, 1, rows, 256);                            \
+  else if (!wide && fours && D <= 8192) GO(4, 8, 1, rows, 256);                            \
+  else { FEW_ROW_SHAPES(wide, fours, D, rows) }
 
 template <typename TX>
 void launch_quantize(bool wide, bool fours, uint8_t* q, float* scale, const TX* x, const int* rows, const float* weights, int div, int P, int M, int D,
                      long long ldx, long long ldq, cudaStream_t st) {
 #define GO(V, CH, ROWS, blocks, threads) \
   leb_launch(quantize_kernel<TX, V, CH, ROWS>, dim3(blocks), dim3(threads), 0, st, q, scale, x, rows, weights, div, P, M, D, ldx, ldq)
-  ROW_SHAPES(wide, fours, D, P, 8)
+  QUANTIZE_SHAPES(wide, fours, D, P)
 #undef GO
 }
 template <typename TY>
 void launch_norm(bool wide, bool fours, uint8_t* q, float* scale, float* x, const float* w, const TY* y, void* h, int h_dtype, int M, int D, float eps, long long ldq, cudaStream_t st) {
 #define GO(V, CH, ROWS, blocks, threads) \
   leb_launch(rmsnorm_e4m3_kernel<TY, V, CH, ROWS>, dim3(blocks), dim3(threads), 0, st, q, scale, x, w, y, h, h_dtype, M, D, eps, ldq)
-  ROW_SHAPES(wide, fours, D, M, 4)
+  const bool adds = y != nullptr;
+  NORM_SHAPES(wide, fours, adds, D, M)
 #undef GO
 }
 

@@ -162,6 +162,32 @@ def test_rmsnorm(y_dtype, M, D):
             assert bool(((h.cpu().double() - want).abs() <= (bound + step) * 1.01 * want.abs() + 1e-45).all())
 
 
+@pytest.mark.parametrize("D", [250, 256, 501, 512, 1000, 1001, 1999, 2048, 3999, 4000, 6001, 8192, 8200, 12000, 16390])
+def test_many_rows(D):
+    """Rows enough to be shared out in the other way, few threads a row: the last block's are part of one."""
+    M = 1029
+    x, w, y = gen(M, D, seed=1, scale=2.0), 1 + 0.2 * gen(D, seed=2), gen(M, D, seed=3, dtype=BF16)
+    for pitch in (-(-D // 16) * 16, D + 3):
+        for t in (x, y):
+            q, whole = room(M, D, pitch, E4M3, 77)
+            s = torch.empty(M, device=DEV)
+            K().quantize_e4m3(q, s, t.to(DEV))
+            check_rows(q, s, t)
+            assert bool((between(whole, M, D, pitch) == 77).all())
+        for added in (None, y, y.float()):
+            q, whole = room(M, D, pitch, E4M3, 77)
+            s, xd, h = torch.empty(M, device=DEV), x.to(DEV), torch.empty(M, D, device=DEV)
+            K().rmsnorm_e4m3(q, s, xd, w.to(DEV), 1e-5, y=None if added is None else added.to(DEV), h=h)
+            new = x if added is None else x + y.float()
+            assert torch.equal(xd.cpu(), new)
+            r = 1 / torch.sqrt((new.double() ** 2).mean(1) + 1e-5)
+            bound = 2.0 ** -24 * ((D / 32 + 16) / 2 + 6)                 # (as above)
+            check_rows(q, s, new * w, r, bound)
+            want = (new * w).double() * r[:, None]
+            assert bool(((h.cpu().double() - want).abs() <= bound * 1.01 * want.abs() + 1e-45).all())
+            assert bool((between(whole, M, D, pitch) == 77).all())
+
+
 def test_no_rows():
     q, s = K().e4m3_rows(0, 64, device=DEV), torch.empty(0, device=DEV)
     K().quantize_e4m3(q, s, torch.empty(0, 64, device=DEV))
