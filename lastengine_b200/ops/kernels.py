@@ -2396,7 +2396,7 @@ def linear_e4m3(out: torch.Tensor, x: torch.Tensor, x_scale: torch.Tensor, w: to
     `out` is bfloat16 or float.  `epilogue`: STORE, ACCUMULATE (out is the float residual), a gated epilogue (`gated_epilogue`: rows of w
     interleaved in blocks of 16 gate and 16 up rows, out has N/2 columns) or, for a bfloat16 out, a plain activation's
     (`plain_act_epilogue`); activations see the scaled sums.  Every size from one on and rows any number of bytes apart are taken;
-    operands whose rows begin on 16 bytes (`e4m3_rows`) go to the tensor cores.  A row's numbers depend on no other row's; they do
+    operands whose rows begin on 16 bytes (`e4m3_rows`) go to the tensor cores, others (of at most 4 million columns) do not.  A row's numbers depend on no other row's; they do
     depend, in their last bits, on how many rows the call has."""
     here = x.get_device()
     if (here < 0 or out.get_device() != here or x_scale.get_device() != here or w.get_device() != here or w_scale.get_device() != here
