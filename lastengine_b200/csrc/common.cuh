@@ -75,6 +75,18 @@ struct LebPlainLaunches {
   explicit LebPlainLaunches(bool turn_off) : saved(g_leb_pdl), off(turn_off) { if (off) g_leb_pdl = 0; }
   ~LebPlainLaunches() { if (off) g_leb_pdl = saved; }
 };
+// The smaller and the larger of two numbers; NaN where either is (fminf and fmaxf give the other one, so that a clamp would make a number of
+// what is none).  One instruction each, as theirs.
+__device__ __forceinline__ float min_or_nan(float a, float b) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float max_or_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
 // silu(g) * u.  The bfloat16 products' epilogues take 2^x and the reciprocal from the special
 // function unit (relative error about 1e-6, far below the rounding of the bfloat16 they store):
 // with exact expf and division an epilogue of a few warps is bound by its instructions.
@@ -95,8 +107,8 @@ template <typename T>
 __device__ __forceinline__ float gate_mul(float g, float u, int act) {
   if ((act & 255) == 2) {
     const float lim = __uint_as_float(((unsigned)act >> 8) << 16);
-    g = fminf(g, lim);
-    u = fminf(fmaxf(u, -lim), lim);
+    g = min_or_nan(g, lim);
+    u = min_or_nan(max_or_nan(u, -lim), lim);
     if (sizeof(T) == 2) return __fdividef(g, 1.0f + __expf(-1.702f * g)) * (u + 1.0f);
     return g / (1.0f + expf(-1.702f * g)) * (u + 1.0f);
   }
@@ -118,7 +130,7 @@ __device__ __forceinline__ float gate_mul(float g, float u, int act) {
 __device__ __forceinline__ float plain_act(float z, int act) {
   const int a = act - LEB_PLAIN_ACT_BASE;
   if (a == 0) return 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
-  if (a == 1) { const float t = fmaxf(z, 0.f); return t * t; }
+  if (a == 1) { const float t = max_or_nan(z, 0.f); return t * t; }
   if (a == 2) return 0.5f * z * (1.0f + tanhf(0.7978845608028654f * (z + 0.044715f * z * z * z)));
   return z / (1.0f + expf(-z));
 }

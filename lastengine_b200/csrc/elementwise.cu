@@ -280,8 +280,8 @@ __global__ void gated_act_kernel(TO* __restrict__ a, const TI* __restrict__ gu, 
   float u = to_f32(gu[m * 2 * F + F + j]);
   float r;
   if (act == 2) {        // clamped: g' = min(g, limit), u' = clamp(u, -limit, limit); g' sigmoid(alpha g') (u' + 1)
-    g = fminf(g, limit);
-    u = fminf(fmaxf(u, -limit), limit);
+    g = min_or_nan(g, limit);
+    u = min_or_nan(max_or_nan(u, -limit), limit);
     r = g / (1.0f + expf(-alpha * g)) * (u + 1.0f);
   } else {
     r = act == 1 ? gelu_tanh_f(g) * u : g / (1.0f + expf(-g)) * u;
@@ -584,7 +584,7 @@ __global__ void activation_kernel(TO* __restrict__ a, const float* __restrict__ 
   const float z = x[m * ldx + j];
   float r;
   if (act == 0) r = 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
-  else if (act == 1) { const float t = fmaxf(z, 0.f); r = t * t; }
+  else if (act == 1) { const float t = max_or_nan(z, 0.f); r = t * t; }
   else if (act == 2) r = gelu_tanh_f(z);
   else r = z / (1.0f + expf(-z));
   a[i] = from_f32<TO>(r);
