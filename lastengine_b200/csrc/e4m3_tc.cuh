@@ -78,8 +78,7 @@ __device__ __forceinline__ bool e8_all(bool ok) {
       : "memory");
   return all != 0;
 }
-// A block that gave up stays until copies that it asked for have landed: a phase's end, or some milliseconds (copies land within microseconds;
-// a phase that a partner's copies belong to may never end).
+// A block that gave up stays until copies that it asked for have landed: a phase's end, or some milliseconds (copies land within microseconds).
 __device__ __forceinline__ void e8_passed(uint64_t* bar, int phase) {
   for (int n = 0; n < 1 << 14; n++) {
     uint32_t ok;
@@ -93,6 +92,25 @@ __device__ __forceinline__ void e8_passed(uint64_t* bar, int phase) {
     if (ok) return;
     __nanosleep(64);
   }
+}
+// A pair that gives up stops its two producers anywhere: the first block has announced the bytes of both on its barriers, and asked for its own half, in
+// `own` stages, the other block has asked for its half in `theirs`, and either may be ahead by as many stages as there were free ones.  A
+// phase ends once its bytes have been announced and have landed, so a stage that only one of them came to is settled by hand: the
+// bytes `theirs` is ahead by have yet to be announced, those that it never asked for are taken off.  Then each phase from the
+// first that may be open (all before it were consumed, or the stage could not have been asked for again) ends when, and not before, all
+// copies asked for in it have landed.
+__host__ __device__ inline int e8_first_out(int own, int theirs, int stages) {
+  const int most = own > theirs ? own : theirs;
+  return most > stages ? most - stages : 0;
+}
+// Bytes to announce in stage i (negative: to take off); `half`: one block's.
+__host__ __device__ inline int e8_owed(int i, int own, int theirs, int half) {
+  if (i >= own && i < theirs) return half;
+  return i < own && i >= theirs ? -half : 0;
+}
+// Takes bytes that nobody will send off a barrier's count.
+__device__ __forceinline__ void mbar_complete_tx(uint64_t* bar, uint32_t bytes) {
+  asm volatile("mbarrier.complete_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
 }
 __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");

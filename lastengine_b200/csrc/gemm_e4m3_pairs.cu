@@ -10,8 +10,8 @@
 //
 // Roles: warp 0 asks for tiles, warp 1 issues products, warps 2-9 are the epilogue.  Tiles are dealt in bands of PAIRS_BAND row
 // tiles, down a band's rows first, so that the blocks that run together share few slabs of operands in L2.
-// Every wait is bounded: a role that gives up sets the status word and all leave; both blocks stay until the copies asked for have landed and
-// the products are done.
+// Every wait is bounded: a role that gives up sets the status word and all leave; both blocks stay until the copies that either asked for
+// have landed and the products are done.
 #include "e4m3_tc.cuh"
 
 #define PAIRS_THREADS 320
@@ -338,12 +338,20 @@ gemm_e4m3_pairs_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
   const bool left = abort_s | remote_int(e8_map_to_rank(smem_u32(&abort_s), rank ^ 1));
   if (left) {      // the copies asked for land and the products end first (else every one has been waited for)
     if (rank == 0 && threadIdx.x == 0) {
-      for (int i = max(sent_s - STAGES, 0); i < sent_s; i++) e8_passed(&full[i % STAGES], i / STAGES);
-    } else if (rank == 0 && warp == 1) {
+      const int theirs = remote_int(e8_map_to_rank(smem_u32(&sent_s), 1));
+      const int begin = e8_first_out(sent_s, theirs, STAGES), end = max(sent_s, theirs);
+      for (int i = begin; i < end; i++) {
+        const int owed = e8_owed(i, sent_s, theirs, 2 * HALF);
+        if (owed > 0) mbar_expect_tx(&full[i % STAGES], (uint32_t)owed);
+        if (owed < 0) mbar_complete_tx(&full[i % STAGES], (uint32_t)-owed);
+      }
+      for (int i = begin; i < end; i++) e8_passed(&full[i % STAGES], i / STAGES);
+    } else if (warp == 1) {
       if (elect_lane()) {
-        pair_commit(&drained);
+        if (rank == 0) pair_commit(&drained);
         e8_passed(&drained, 0);
       }
+      __syncwarp();
     }
     __syncthreads();
   }
