@@ -30,8 +30,9 @@ __global__ void __launch_bounds__(256) gemm_e4m3_any_kernel(TC* __restrict__ C, 
     W += e * w_group_stride;
     sw += (size_t)e * N;
   }
-  const int m0 = lo + (int)(blockIdx.x % m_tiles) * 64, n0 = blockIdx.y * 64;
-  if (m0 >= hi) return;
+  const long long at = lo + (long long)(blockIdx.x % m_tiles) * 64;      // (an expert has blocks for all rows: beyond 2^31 where there are many)
+  if (at >= hi) return;
+  const int m0 = (int)at, n0 = blockIdx.y * 64;
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4, kk = threadIdx.x & 31, row8 = threadIdx.x >> 5;
   float acc[4][4] = {};
   for (int k0 = 0; k0 < K; k0 += 32) {
