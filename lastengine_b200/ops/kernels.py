@@ -110,18 +110,20 @@ class _OwnModules(dict):
 _own_module = _OwnModules()
 
 
-def guarded(method):
-    """A part's method as a forward pass calls it (all of its calls of parts go through here).  The library's own parts touch their
-    operands through this module alone, which launches what waits in a chain first; other code (a part registered from
-    elsewhere, a method wrapped or replaced on a class or an object) may use torch on them, so whatever waits is launched
-    before it runs, and its own products are launched at their call.  Judged at every call: parts change after a model is built."""
-    if not _chain.open:
-        return method
+def own(method) -> bool:
+    """Whether a part's method is the library's own, on an object of a class of the library: not one registered from elsewhere, nor wrapped or
+    replaced on a class or an object.  Judged at every call: parts change after a model is built."""
     if type(method) is types.MethodType and _own_module[type(method.__self__).__module__]:
         f = method.__func__
-        if type(f) is types.FunctionType and _own_module[f.__globals__["__name__"]]:
-            return method
-    return functools.partial(_apart, method)
+        return type(f) is types.FunctionType and _own_module[f.__globals__["__name__"]]
+    return False
+
+
+def guarded(method):
+    """A part's method as a forward pass calls it (all of its calls of parts go through here).  The library's own parts touch their
+    operands through this module alone, which launches what waits in a chain first; other code (see `own`) may use torch on them, so
+    whatever waits is launched before it runs, and its own products are launched at their call."""
+    return method if not _chain.open or own(method) else functools.partial(_apart, method)
 
 
 def _apart(method, *args, **kwargs):

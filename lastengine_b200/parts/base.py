@@ -297,7 +297,8 @@ class Mixer(Part):
 
 
 class FeedForward(Part):
-    reads_e4m3 = False     # True: forward() takes its rows in 8 bits too (parts.ffn.EightBitRows), as a norm may leave them
+    reads_e4m3 = False     # True: forward() takes its rows in 8 bits too (parts.ffn.EightBitRows), as a norm may leave them; a class from
+    #                        elsewhere says so where it defines forward()
 
     def forward(self, h, out, accumulate, batch, env) -> None:
         raise NotImplementedError

@@ -24,7 +24,7 @@ import torch
 
 from ..ops import kernels
 from ..registry import BLOCKS
-from .ffn import eight_bit_room
+from .ffn import eight_bit_room, takes_eight_bit_rows
 
 
 @BLOCKS.register("pre_norm_residual")
@@ -65,13 +65,14 @@ class PreNormResidualBlock:
 
     def _normed(self, norm, x, pending, env, reader=None):
         """norm(x) as the next part's input: the split's values (the part scales its first product),
-        or the norm kernel's result, in 8 bits for a `reader` that takes them."""
+        or the norm kernel's result, in 8 bits for a `reader` that takes them.  A norm whose `forward` is not the library's own (a class
+        from elsewhere, a wrapped method) is called as ever."""
         env.split_in = env.split_out = None   # nothing is left over from a part that did not take its offer (or raised)
         if pending is not None and pending.filled and pending.weight is norm.weight:
             env.split_in = pending
             return pending.values
         M, D = x.shape
-        if getattr(reader, "reads_e4m3", False) and getattr(norm, "splittable", False):
+        if reader is not None and takes_eight_bit_rows(reader) and getattr(norm, "splittable", False) and kernels.own(norm.forward):
             h = eight_bit_room(env.workspace, "block.h8", M, D)
             kernels.rmsnorm_e4m3(h.values, h.scale, x, norm.weight, norm.eps)
             return h

@@ -58,6 +58,17 @@ def eight_bit_weights(w: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     return q.unflatten(0, lead), scale.view(lead)
 
 
+def takes_eight_bit_rows(part) -> bool:
+    """Whether a block may hand `part` its rows in 8 bits: the library's own `forward` where the part says so, that of a class from
+    elsewhere where the class that defines it says so.  A subclass's `forward` and a wrapped one get tensors, whatever they inherit."""
+    if not getattr(part, "reads_e4m3", False):
+        return False
+    if kernels.own(part.forward):
+        return True
+    f = getattr(part.forward, "__func__", None)
+    return any(c.__dict__.get("forward") is f and c.__dict__.get("reads_e4m3", False) for c in type(part).__mro__ if f is not None)
+
+
 def _eight(h, ws, name: str) -> EightBitRows:
     """h in 8 bits: as the block's norm left it, or brought to them here."""
     if isinstance(h, EightBitRows):
