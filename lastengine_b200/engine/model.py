@@ -6,6 +6,8 @@ benchmark all go through it.
 """
 from __future__ import annotations
 
+import warnings
+
 import torch
 
 from .. import parts as _parts  # noqa: F401  (registers the built-in parts)
@@ -122,6 +124,10 @@ class Model:
                 if name in tensors:
                     own[rel] = tensors[name]
             part.load(own, self.env)
+        if self.env.ffn_e4m3:
+            left = sorted({type(b.ffn).__name__ for b in self.blocks if getattr(b, "ffn", None) is not None and not getattr(b.ffn, "in_e4m3", False)})
+            if left:
+                warnings.warn(f"feed-forwards in 8 bits were asked for; {', '.join(left)} did not bring its matrices to them and runs in {self.env.dtype}")
         self.stream_tables = {n: tensors[n].contiguous() for n in self.plan.stream_tables if n in tensors}
         self.stream_matrices = {n: tensors[n].contiguous() for n in self.plan.stream_matrices if n in tensors}
         if getattr(self.head, "tied", False):

@@ -299,6 +299,7 @@ class Mixer(Part):
 class FeedForward(Part):
     reads_e4m3 = False     # True: forward() takes its rows in 8 bits too (parts.ffn.EightBitRows), as a norm may leave them; a class from
     #                        elsewhere says so where it defines forward()
+    in_e4m3 = False        # set by load(): the matrices are kept in 8 bits, as env.ffn_e4m3 asks
 
     def forward(self, h, out, accumulate, batch, env) -> None:
         raise NotImplementedError

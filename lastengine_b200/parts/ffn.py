@@ -118,7 +118,7 @@ class SwiGLU(FeedForward):
         if env.ffn_e4m3:
             self.w13, self.s13 = eight_bit_weights(self.w13)
             self.w2, self.s2 = eight_bit_weights(self.w2)
-            self.split_norm, self.reads_e4m3 = False, True
+            self.split_norm, self.reads_e4m3, self.in_e4m3 = False, True, True
 
     def split_reader_weight(self):
         return self.w13
@@ -182,7 +182,7 @@ class DenseFeedForward(FeedForward):
         if env.ffn_e4m3:
             self.w1, self.s1 = eight_bit_weights(self.w1)
             self.w2, self.s2 = eight_bit_weights(self.w2)
-            self.reads_e4m3 = True
+            self.reads_e4m3 = self.in_e4m3 = True
 
     def forward(self, h, out, accumulate, batch, env) -> None:
         ws = env.workspace
@@ -315,6 +315,7 @@ class SigmoidTopKMoE(FeedForward):
         if env.ffn_e4m3:
             self.w13, self.s13 = eight_bit_weights(self.w13)
             self.w2, self.s2 = eight_bit_weights(self.w2)
+            self.in_e4m3 = True
 
     def flops_per_row(self) -> int:
         # the router, k experts of three matrices, and the shared expert

@@ -116,3 +116,44 @@ def test_a_part_without_the_attribute(launched):
     e = env()
     part = types.SimpleNamespace(forward=lambda *a: None)
     assert isinstance(handed(part, norm.RMSNorm(64, 1e-5), e), torch.Tensor)
+
+
+def model(e, kind):
+    """A model of four layers whose second feed-forward is `kind`, on the host."""
+    import dataclasses
+    from lastengine_b200 import registry
+    from lastengine_b200.engine.model import Model
+    from tiny_configs import TINY_A
+    plan = registry.plan_from_config(TINY_A)
+    ls = plan.layers[1]
+    plan.layers[1] = dataclasses.replace(ls, ffn=dataclasses.replace(ls.ffn, kind=kind))
+    m = Model(plan, e)
+    m.load({n: torch.zeros(s.concrete_shape()) for n, s in m.tensor_specs().items()})
+    return m
+
+
+class StaysInBfloat16(ffn.SwiGLU):
+    def load(self, tensors, env):
+        self.w13, self.w2 = ffn.fuse_gate_up(tensors[self.n_gate], tensors[self.n_up], False), tensors[self.n_down]
+
+
+@pytest.fixture
+def registered():
+    from lastengine_b200.registry import FEED_FORWARDS
+    FEED_FORWARDS.register("stays_in_bfloat16", replace=True)(StaysInBfloat16)
+    yield "stays_in_bfloat16"
+    FEED_FORWARDS.unregister("stays_in_bfloat16")
+
+
+def test_a_part_that_stays_in_bfloat16_is_named(launched, registered):
+    with pytest.warns(UserWarning, match="StaysInBfloat16 did not bring its matrices"):
+        m = model(env(), registered)
+    assert [b.ffn.in_e4m3 for b in m.blocks] == [True, False, True, True]
+
+
+@pytest.mark.parametrize("asked", [True, False])
+def test_nothing_is_said_where_there_is_nothing_to_say(asked, launched, registered, recwarn):
+    e = env()
+    e.ffn_e4m3 = asked
+    m = model(e, "swiglu" if asked else registered)
+    assert not recwarn.list and [b.ffn.in_e4m3 for b in m.blocks] == [asked] * 4
