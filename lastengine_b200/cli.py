@@ -168,14 +168,17 @@ def cmd_probe(a) -> int:
 
 
 def cmd_generate(a) -> int:
-    from . import Engine, SamplingParams
+    from . import Engine, EngineOptions, SamplingParams
     prompts = [parse_ids(p) for p in a.prompt_ids]
     need = sum(-(-(len(p) + a.max_new_tokens) // 64) * 64 for p in prompts)
-    kw = dict(dtype=a.dtype, max_tokens=max(need, 64), max_seqs=len(prompts), ffn_dtype=a.ffn_dtype)
+    try:
+        options = EngineOptions(dtype=a.dtype, max_tokens=max(need, 64), max_seqs=len(prompts), ffn_dtype=a.ffn_dtype)
+    except ValueError as e:
+        raise SystemExit(f"lastengine generate: {e}")
     if a.model:
-        eng = Engine.from_pretrained(a.model, **kw)
+        eng = Engine.from_pretrained(a.model, options)
     elif a.config:
-        eng = Engine.from_config(a.config, seed=a.random_seed, **kw)
+        eng = Engine.from_config(a.config, seed=a.random_seed, options=options)
     else:
         raise SystemExit("lastengine generate: give --model DIR, or --config JSON with --random-seed")
     sp = SamplingParams(temperature=a.temperature, top_p=a.top_p, top_k=a.top_k, min_p=a.min_p,
