@@ -863,6 +863,8 @@ def main() -> int:
     ap.add_argument("--compare", default="", choices=["", "zekivik", "lenesun", "kisilix", "tevilix", "zafilix", "nolapel"],
                     help="instead of the default run: prefill and decode of that design at a few layer sizes beside "
                          "the closest other design at equal sizes, with every kernel's time (prints its own JSON line)")
+    ap.add_argument("--ffn-dtype", default=None, choices=["e4m3"],
+                    help="instead of the default run: feed-forwards and experts in 8 bits (the line says so; without roofline.kernels)")
     args = ap.parse_args()
 
     if args.compare:
@@ -894,7 +896,7 @@ def main() -> int:
     max_b = max(args.batch, 1 if args.skip_points else 64)
     t0 = time.time()
     eng = Engine.from_config(cfg, seed=0, dtype="bfloat16", max_tokens=max_b * (args.context + 64) + 4096,
-                             max_seqs=max_b + 8)
+                             max_seqs=max_b + 8, ffn_dtype=args.ffn_dtype)
     nums = model_numbers(eng)
     from lastengine_b200.config import Lfm3Config
     tc = Lfm3Config.from_dict(cfg)
@@ -962,7 +964,7 @@ def main() -> int:
         print(f"[bench] e2e b{args.batch}: {e2e['value']:.1f} tok/s over {e2e['decode_steps']} steps "
               f"({e2e['first_steps_value']:.1f} over the first {E2E_FIRST_STEPS})", file=sys.stderr)
     per_kernel = None
-    if not args.no_per_kernel:
+    if not args.no_per_kernel and args.ffn_dtype is None:
         per_kernel = time_kernels(eng, nums, args.batch, args.context, pk, rng)
     clocks.stop()
 
@@ -989,6 +991,9 @@ def main() -> int:
     }
     if e2e is not None:
         line["e2e"] = e2e
+    if args.ffn_dtype is not None:
+        line["metric"] += f", feed-forwards in {args.ffn_dtype}"
+        line["dtype"] = f"bf16, feed-forwards and experts {args.ffn_dtype}"
     print(json.dumps(line))
     return 0
 

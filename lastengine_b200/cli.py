@@ -34,11 +34,11 @@ def parse_ids(text: str) -> list[int]:
         raise SystemExit(f"lastengine: prompts are token ids here, got '{text}'") from None
 
 
-def _engine(path: str, dtype: str, ctx: int, n_seqs: int = 1):
+def _engine(path: str, dtype: str, ctx: int, n_seqs: int = 1, ffn_dtype: str | None = None):
     from . import Engine
     page = 64
     per = -(-(ctx + 1) // page) * page
-    return Engine.from_pretrained(path, dtype=dtype, max_tokens=per * n_seqs, max_seqs=max(n_seqs, 1))
+    return Engine.from_pretrained(path, dtype=dtype, max_tokens=per * n_seqs, max_seqs=max(n_seqs, 1), ffn_dtype=ffn_dtype)
 
 
 def _logprobs(logits):
@@ -88,12 +88,13 @@ def cmd_tf_dump(a) -> int:
 def cmd_dense_cmp(a) -> int:
     """The reference's dense-cmp (src/main.rs:138-158) compares its CPU forward with its GPU forward
     token by token; here the true 32-bit path stands where the CPU stood and the bfloat16 path is
-    the one under test.  Both follow the 32-bit path's greedy tokens."""
+    the one under test, with `--ffn-dtype` its feed-forwards and experts in that.  Both follow the 32-bit
+    path's greedy tokens."""
     import time
     import torch
     ids = parse_ids(a.prompt)
     exact = _engine(a.path, "float32", a.ctx)
-    fast = _engine(a.path, "bfloat16", a.ctx)
+    fast = _engine(a.path, "bfloat16", a.ctx, ffn_dtype=a.ffn_dtype)
     se, sf = exact.new_sequence(), fast.new_sequence()
     le = _logprobs(exact.step([se], [ids], "last", check=True))[0].clone()
     t0 = time.perf_counter()
@@ -206,7 +207,7 @@ def cmd_init(a) -> int:
 def cmd_replay(a) -> int:
     exe = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "bin", "trace_run")
     os.execv(sys.executable, [sys.executable, exe, "--model", a.model, "--dtype", a.dtype, "--out", a.out,
-                              "--max-tokens", str(a.max_tokens)])
+                              "--max-tokens", str(a.max_tokens)] + (["--ffn-dtype", a.ffn_dtype] if a.ffn_dtype else []))
     return 0
 
 
@@ -217,6 +218,9 @@ def build_parser() -> argparse.ArgumentParser:
     def common(p, dtype_default="bfloat16"):
         p.add_argument("--dtype", default=dtype_default, choices=["bfloat16", "float32"])
         p.add_argument("--ctx", type=int, default=4096, help="context length (tokens per sequence)")
+
+    def ffn_dtype(p):
+        p.add_argument("--ffn-dtype", choices=["e4m3"], default=None, help="matrices of feed-forwards and experts in 8 bits")
 
     p = sub.add_parser("gpu", help="top-N next-token logprobs + a 32-token greedy decode")
     p.add_argument("path")
@@ -237,6 +241,7 @@ def build_parser() -> argparse.ArgumentParser:
     p.add_argument("prompt")
     p.add_argument("n", nargs="?", type=int, default=32)
     p.add_argument("--ctx", type=int, default=4096)
+    ffn_dtype(p)
     p.set_defaults(fn=cmd_dense_cmp)
 
     p = sub.add_parser("inspect", help="print the model folder's configuration and tensors")
@@ -262,7 +267,7 @@ def build_parser() -> argparse.ArgumentParser:
     p.add_argument("--seed", type=int, default=None)
     p.add_argument("--stop-token-id", type=int, action="append", default=None,
                    help="ends a request (not emitted); default: the model's eos_token_id")
-    p.add_argument("--ffn-dtype", choices=["e4m3"], default=None, help="matrices of feed-forwards and experts in 8 bits")
+    ffn_dtype(p)
     common(p)
     p.set_defaults(fn=cmd_generate)
 
@@ -279,6 +284,7 @@ def build_parser() -> argparse.ArgumentParser:
     p.add_argument("--dtype", required=True, choices=["bfloat16", "float32"])
     p.add_argument("--out", required=True)
     p.add_argument("--max-tokens", type=int, required=True)
+    ffn_dtype(p)
     p.set_defaults(fn=cmd_replay)
     return ap
 
