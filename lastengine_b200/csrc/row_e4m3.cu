@@ -8,7 +8,8 @@
 //
 // Bound by memory: a float row is read and a quarter of its bytes written.  A thread keeps its numbers in registers between the sums and the
 // rounding, so a row is read once, with all loads out before the first is used: eight neighbours at a time where rows begin on 16 bytes,
-// single numbers (four of a thread side by side, so that they are written as one word) otherwise; rows of more than 16,384 are read twice.  The largest
+// single numbers (four of a thread side by side, so that they are written as one word) otherwise; rows of more than 16,384 are read twice, a number
+// at a time (2,048 bfloat16 rows of 28,672: 151 us, 27 by their bytes).  The largest
 // |g| is taken over the bits (for numbers without a sign they order as the numbers do, infinity and NaN on top).
 #include "e4m3_common.cuh"
 
@@ -297,7 +298,8 @@ __global__ void __launch_bounds__(512) rmsnorm_e4m3_kernel(uint8_t* __restrict__
 // The norm holds its weights beside the row, and what is added: two pieces a thread (2,048 rows of 2,048 with a bfloat16 addition: four pieces
 // 13.3 us, two 10.7; 16,000 rows 59.3 and 56.1, without the addition 31.3 and 29.5; 2,048 rows of 1,001 with it: a warp a row 12.2, four 7.5).
 // Short rows without an addition have little to load: a warp takes one (16,000 rows of 1,024: 15.6 us, two warps 18.9; with the addition
-// 31.8 and 30.0).
+// 31.8 and 30.0).  Chosen with the addition; without it two sizes lose to twice as many pieces a thread: 16,000 x 1,001 22.5 us (20.0),
+// 8,191 x 4,096 33.7 (32.4).  Wider rows off 16 bytes have no other shape to compare with: 8,191 x 6,001 87 us, 4,096 x 12,001 109 (38 either by their bytes).
 #define NORM_SHAPES(wide, fours, adds, D, rows)                                            \
   if (wide && D <= 256) GO(8, 1, 8, ceil_div(rows, 8), 256);                               \
   else if (wide && D <= 512) GO(8, 2, 8, ceil_div(rows, 8), 256);                          \

@@ -2321,7 +2321,8 @@ def quantize_e4m3(out: torch.Tensor, scale: torch.Tensor, x: torch.Tensor, rows:
     """Rows of x [M, K] (float or bfloat16) in 8 bits: out [P, K] = round(448 x / a) and scale [P] = a / 448 (float) with
     a = max(max |x|, 2^-100), the row's largest magnitude.  `rows` (int32 [P]): row p is x[rows[p] // div] (P = M without), and with
     `weights` (float) its scale is multiplied by weights[rows[p]].  A row of x with a number that is not finite, and one that
-    `rows` does not find in x, gets numbers and a scale that are NaN.  Numbers are rounded to the nearest, ties to even."""
+    `rows` does not find in x, gets numbers and a scale that are NaN.  Numbers are rounded to the nearest, ties to even, of the float product of x and
+    the float quotient 448 / a: what lies within 2^-22 of a middle may go either way.  Rows of more than 16,384 numbers are read twice, a number at a time."""
     here = x.get_device()
     if (here < 0 or out.get_device() != here or scale.get_device() != here or here != _current_device()
             or (rows is not None and (rows.get_device() != here or (weights is not None and weights.get_device() != here)))):
@@ -2397,9 +2398,10 @@ def linear_e4m3(out: torch.Tensor, x: torch.Tensor, x_scale: torch.Tensor, w: to
     [group_offsets[e], group_offsets[e + 1]) of x and out go with expert e, and rows of out behind the last offset stay as they are.
     `out` is bfloat16 or float.  `epilogue`: STORE, ACCUMULATE (out is the float residual), a gated epilogue (`gated_epilogue`: rows of w
     interleaved in blocks of 16 gate and 16 up rows, out has N/2 columns) or, for a bfloat16 out, a plain activation's
-    (`plain_act_epilogue`); activations see the scaled sums.  Every size from one on and rows any number of bytes apart are taken;
-    operands whose rows begin on 16 bytes (`e4m3_rows`) go to the tensor cores, others (of at most 4 million columns) do not.  A row's numbers depend on no other row's; they do
-    depend, in their last bits, on how many rows the call has."""
+    (`plain_act_epilogue`); activations see the scaled sums, and what is NaN stays so.  Every size from one on and rows any number of bytes apart are
+    taken.  Operands whose rows begin on 16 bytes and lie a multiple of 16 bytes apart (`e4m3_rows`; a contiguous K of 1,000 does not) go to the tensor cores, of at
+    most 256 experts that lie behind one another without gaps.  Others (of at most 4 million columns) take 13 to 70 times as long.  A row's numbers
+    depend on no other row's; they do depend, in their last bits, on how many rows the call has."""
     here = x.get_device()
     if (here < 0 or out.get_device() != here or x_scale.get_device() != here or w.get_device() != here or w_scale.get_device() != here
             or here != _current_device() or (group_offsets is not None and group_offsets.get_device() != here)):
